@@ -219,6 +219,83 @@ void p1a_set_prefill_staging_limit(size_t bytes);
  * takes all scratch from the caller (src/fast/attn_fold.cuh:25-26). */
 int p1a_warmup_prefill(int T, int p0, int Hq, int Hkv, int D, void *stream);
 
+/*
+ * ---- Sequences in bounded caches: chunks of several sequences, windows, attention weights, eviction (no counterparts in the reference) ----
+ *
+ * Which rows a call has, whose they are and what they see. Row t of q / out belongs to sequence s when row0[s] <= t < row0[s + 1], and stands at
+ * cache position p = pos0[s] + t - row0[s]; it sees the positions j <= p with j > p - window or j < n_sink. Rows of no sequence - those behind
+ * row0[n_seq] - are left as they are; a row whose position is negative or not below the descriptor's n_ctx sees nothing: its result is 0, its
+ * log-sum-exp -inf. Sequence s reads the page table pt + rtab[s]; without rtab (or without pt) there is one sequence.
+ * row0 and pos0 are read on the device when the kernels run; the other fields are the host's. A pair of row0 that runs backwards is an empty
+ * sequence, rows past T or past max_rows of a sequence are not looked at. Page-table entries of positions that no row sees are never read, nor
+ * is memory behind them: a page that has left the window may be given away.
+ */
+#define P1A_ROWS_F32  0
+#define P1A_ROWS_BF16 1
+typedef struct p1a_rows {
+    int32_t T;               /* rows of q, out, gate, lse */
+    int32_t n_seq;
+    int32_t max_rows;        /* the most rows a sequence has in this call (0: T) */
+    int32_t max_n;           /* the most positions a sequence holds, the new rows included (0: the descriptor's n_ctx). Results do not depend on it
+                                beyond the order of sums: it chooses how the work is dealt out */
+    const int32_t * row0;    /* device [n_seq + 1]; NULL: T / n_seq rows each */
+    const int32_t * pos0;    /* device [n_seq]; NULL: p0 for the only sequence */
+    int32_t p0;
+    int32_t window;          /* 0: every position up to the row's own */
+    int32_t n_sink;          /* first positions that stay visible (means something with a window) */
+} p1a_rows;
+
+/*
+ * Attention of the rows' q [T][Hq][D] over the cache (which already holds their own positions): out [T][Hq][D], and where lse != NULL
+ * lse [T][Hq] f32 = log of the sum of exp(scale * q . k) over what the row sees. gate [T][Hq*D] f32 (or NULL): out *= 1 / (1 + exp(-gate)).
+ * q_type / out_type: P1A_ROWS_F32 or P1A_ROWS_BF16 (rounded once, at the end). From single tokens of many sequences to whole prompts.
+ * Precision: where a result is f32 (out, or lse is asked for) q, the probabilities and quantized K / V enter the f16 products as two halves each and
+ * results are within 1e-5 (relative L2) of exact ones; with bf16 results they enter rounded to f16 once. K and V values of magnitude 65504 and more
+ * are beyond the products' range, as in p1a_attn_prefill. A key whose V holds an infinity or NaN reaches rows of the same sequence in the same call
+ * that do not see it; keys that no row sees reach nothing.
+ * D = 64, 128 or 256; Hq / Hkv up to 64; 16-byte aligned q, out and gate; f16 caches: 16-byte aligned bases and page strides, q8_0: 4-byte aligned,
+ * q4_0: 2-byte aligned; pages of any length.
+ * A call of few rows is split over its keys and its partials merged by a second launch; they live in `scratch` (256-byte aligned, at least
+ * p1a_attn_chunk_scratch_bytes) or, with NULL or less, in the library's buffers of (device, stream), under the rules of p1a_attn_prefill's: nothing is
+ * allocated during stream capture (P1A_E_SCRATCH: make one eager call first, or bring scratch), graphs captured on one stream share them - replay
+ * such graphs one behind the other, or bring scratch for each. Result bits depend on the call's host numbers and the device, not on scratch.
+ */
+int p1a_attn_chunk(const void *q, int q_type, const p1a_kv *c, void *out, int out_type, const float *gate, float *lse, const p1a_rows *rows,
+                   int Hq, float scale, void *scratch, size_t scratch_bytes, void *stream);
+/* bytes of partials such a call has (0: none) */
+size_t p1a_attn_chunk_scratch_bytes(const p1a_kv *c, const p1a_rows *rows, int Hq);
+
+/*
+ * Attention weight per cache position: mass [n_seq][Hkv][ld] f32 (row s, h starting at (s * Hkv + h) * ld),
+ *     mass[s][h][j] += sum over the rows t of sequence s and the q heads i of kv head h of exp(scale * q[t][i] . K[j][h] - lse[t][i])
+ * over the positions j < ld that row t sees; lse [T][Hq] as p1a_attn_chunk leaves it (a row with lse = -inf adds nothing). Entries that no row
+ * sees are left as they are. f32 accuracy whatever the cache; every entry is summed by one wave in a fixed order: the same bits every time. Shapes and
+ * alignment as for p1a_attn_chunk. Nothing is allocated.
+ */
+int p1a_attn_mass(const void *q, int q_type, const p1a_kv *c, const float *lse, float *mass, int ld, const p1a_rows *rows, int Hq, float scale,
+                  void *stream);
+
+/*
+ * Which positions of a cache stay: per sequence s and kv head the first n_sink of its n positions, the last n_recent, and of those between the
+ * budget - n_sink - n_recent of the largest mass (ties: the lowest position; a NaN counts as less than everything). keep [n_seq][Hkv][budget]
+ * int32 gets them in ascending order; where n <= budget all n of them, and -1 behind. n_dev [n_seq] (device; cut to 0 ... ld) or NULL: n for every
+ * sequence. n_sink + n_recent <= budget <= 2^20.
+ */
+int p1a_evict_select(const float *mass, int ld, int n_seq, int Hkv, const int32_t *n_dev, int n, int budget, int n_sink, int n_recent,
+                     int32_t *keep, void *stream);
+
+/*
+ * Moves the kept rows to the front, in place: position k of kv head h of sequence s becomes what position keep[s][h][k] was, K and V, for every k
+ * with keep[s][h][k] > k (ascending lists as p1a_evict_select leaves them; entries that are negative, not above their own index or not below the
+ * descriptor's n_ctx move nothing). Heads keep different positions: behind the call a cache position is a slot, not a token's place, and rows still
+ * carry the rotation of their tokens' places. New tokens are appended at the next slot with their true positions as rotary ones (p1a_attn_prep:
+ * p0 >= 0, or p1a_attn_prep_mrope with sect = s0 = 1 for rows of several sequences). Positions from `budget` on are as they were.
+ * mass, mass_out [n_seq][Hkv][ld] (or both NULL): mass_out[s][h][k] = mass[s][h][keep[s][h][k]] for entries kept, 0 from there up to ld; mass_out ==
+ * mass is allowed, partial overlap is not. Sequences (their page-table rows) must not share pages.
+ * Alignment: 2 bytes for every cache type (the move uses the widest that rows, bases and page strides have in common).
+ */
+int p1a_kv_compact(const p1a_kv *c, const int32_t *keep, int n_seq, int budget, const float *mass, float *mass_out, int ld, void *stream);
+
 /* Standalone sigmoid gate x[i] *= 1 / (1 + exp(-g[i])). Replaces k::sigmoid_mul, src/kernels.cu:85-93. */
 int p1a_sigmoid_mul(float *x, const float *g, size_t n, void *stream);
 

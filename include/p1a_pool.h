@@ -80,6 +80,9 @@ int p1a_seq_advance(p1a_pool * p, int id, const int32_t * toks, int T);
 /* rollback (tp_model.cu:3159-3170): of the last step's T rows keep the first n_keep; later KV rows are simply overwritten */
 int p1a_seq_rollback(p1a_pool * p, int id, int T, int n_keep);
 int p1a_seq_truncate(p1a_pool * p, int id, int n);             /* :3544-3559 */
+/* after p1a_kv_compact on every layer: the sequence holds its first n_keep slots, the pages behind them are given back. Slots are no longer the
+ * places of tokens, so its tokens read -1 from then on (what was in flight is waited for, as in p1a_seq_truncate). No counterpart in the reference. */
+int p1a_seq_evict(p1a_pool * p, int id, int n_keep);
 int p1a_seq_fork(p1a_pool * p, int src, int n);                /* :3572-3603 -> id of the copy holding positions 0..n-1 */
 int p1a_seq_offload(p1a_pool * p, int id);                     /* :3435-3490 */
 int p1a_seq_restore(p1a_pool * p, int id);                     /* :3492-3496 */

@@ -12,6 +12,7 @@ KV_F16, KV_Q4_0, KV_Q8_0 = 1, 2, 8
 EXPORTS = [
     "p1a_kv_row_bytes", "p1a_kv_append", "p1a_kv_fill_random", "p1a_attn_prep", "p1a_attn_prep_mrope", "p1a_attn_decode", "p1a_attn_decode_a16", "p1a_attn_decode_noalloc", "p1a_a16_bytes", "p1a_ew_quant", "p1a_attn_prefill", "p1a_attn_prefill_scratch_bytes", "p1a_attn_prefill_key_splits", "p1a_attn_prefill_call_splits",
     "p1a_sigmoid_mul", "p1a_warmup", "p1a_get_nsplit", "p1a_set_nsplit", "p1a_reload_env", "p1a_warmup_prefill", "p1a_set_prefill_staging_limit", "p1a_bench_decode_split_only", "p1a_bench_stream_read", "p1a_release", "p1a_last_error",
+    "p1a_attn_chunk", "p1a_attn_chunk_scratch_bytes", "p1a_attn_mass", "p1a_evict_select", "p1a_kv_compact", "p1a_seq_evict",
     "p1a_version", "p1a_decode_scratch_bytes", "p1a_decode_footprint_bytes", "p1a_numerics_id",
     # include/p1a_pool.h
     "p1a_pool_create", "p1a_pool_destroy", "p1a_pool_n_pages", "p1a_pool_free_pages", "p1a_pool_max_pages", "p1a_pool_page_bytes",
@@ -32,6 +33,13 @@ class p1a_kv(ctypes.Structure):
         ("type", ctypes.c_uint32), ("n_ctx", ctypes.c_int32), ("Hkv", ctypes.c_int32), ("D", ctypes.c_int32),
         ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("pt", ctypes.c_void_p), ("rtab", ctypes.c_void_p),
         ("psh", ctypes.c_int32), ("pstride", ctypes.c_size_t),
+    ]
+
+
+class p1a_rows(ctypes.Structure):
+    _fields_ = [
+        ("T", ctypes.c_int32), ("n_seq", ctypes.c_int32), ("max_rows", ctypes.c_int32), ("max_n", ctypes.c_int32),
+        ("row0", ctypes.c_void_p), ("pos0", ctypes.c_void_p), ("p0", ctypes.c_int32), ("window", ctypes.c_int32), ("n_sink", ctypes.c_int32),
     ]
 
 
@@ -107,6 +115,17 @@ def lib():
     L.p1a_attn_prefill.argtypes = [vp, kvp, vp, vp, i32, i32, i32, f32, vp, sz, vp]
     L.p1a_attn_prefill_scratch_bytes.restype = sz
     L.p1a_attn_prefill_scratch_bytes.argtypes = [i32, i32, i32, i32, i32]
+    rp = ctypes.POINTER(p1a_rows)
+    L.p1a_attn_chunk.restype = i32
+    L.p1a_attn_chunk.argtypes = [vp, i32, kvp, vp, i32, vp, vp, rp, i32, f32, vp, sz, vp]
+    L.p1a_attn_chunk_scratch_bytes.restype = sz
+    L.p1a_attn_chunk_scratch_bytes.argtypes = [kvp, rp, i32]
+    L.p1a_attn_mass.restype = i32
+    L.p1a_attn_mass.argtypes = [vp, i32, kvp, vp, vp, i32, rp, i32, f32, vp]
+    L.p1a_evict_select.restype = i32
+    L.p1a_evict_select.argtypes = [vp, i32, i32, i32, vp, i32, i32, i32, i32, vp, vp]
+    L.p1a_kv_compact.restype = i32
+    L.p1a_kv_compact.argtypes = [kvp, vp, i32, i32, vp, vp, i32, vp]
     L.p1a_kv_fill_random.restype = i32
     L.p1a_kv_fill_random.argtypes = [kvp, i32, i32, ctypes.c_uint32, vp]
     L.p1a_attn_prefill_key_splits.restype = i32
@@ -165,7 +184,7 @@ def lib():
     for name in ("p1a_seq_free", "p1a_seq_len", "p1a_seq_resident", "p1a_seq_pages", "p1a_seq_offload", "p1a_seq_restore"):
         getattr(L, name).restype = i32
         getattr(L, name).argtypes = [pp, i32]
-    for name in ("p1a_seq_ensure_pages", "p1a_seq_truncate", "p1a_seq_fork", "p1a_seq_restore_prefix"):
+    for name in ("p1a_seq_ensure_pages", "p1a_seq_truncate", "p1a_seq_evict", "p1a_seq_fork", "p1a_seq_restore_prefix"):
         getattr(L, name).restype = i32
         getattr(L, name).argtypes = [pp, i32, i32]
     L.p1a_seq_host_bytes.restype = sz
@@ -355,6 +374,64 @@ def attn_prefill(q, c, out, T, p0, Hq, scale, gate=None, scratch=None):
     _check((_call or _calls()).prefill(q, c, out, gate, T, p0, Hq, scale, scratch, nbytes), "attn_prefill")
 
 
+class Rows:
+    """Which rows a call over bounded caches has, whose they are and what they see (include/p1a_attn.h, p1a_rows): T rows of n_seq sequences, sequence s
+    having row0[s] .. row0[s + 1] - 1 (int32 on the device; None: T / n_seq each), the first of them at position pos0[s] (int32 on the device; None: p0).
+    max_rows, max_n: the most rows and positions of a sequence, where the host knows them. One object serves every layer of a step."""
+
+    def __init__(self, T, n_seq=1, row0=None, pos0=None, p0=0, max_rows=0, max_n=0, window=0, n_sink=0):
+        self._keep = (row0, pos0)
+        self._st = p1a_rows(T, n_seq, max_rows, max_n, _ptr(row0), _ptr(pos0), p0, window, n_sink)
+        self._ref = ctypes.byref(self._st)
+
+
+_row_types = {}
+
+
+def _row_type(t):
+    """P1A_ROWS_* of a tensor"""
+    r = _row_types.get(t.dtype)
+    if r is None:
+        import torch
+        _row_types.update({torch.float32: 0, torch.bfloat16: 1})
+        r = _row_types.get(t.dtype)
+        if r is None:
+            raise P1AError(f"rows are float32 or bfloat16, not {t.dtype}")
+    return r
+
+
+def attn_chunk(q, c, out, rows, Hq, scale, gate=None, lse=None, scratch=None):
+    """Attention of the new tokens of several sequences, windows and sinks among what `rows` says: q, out [T][Hq][D] float32 or bfloat16, gate [T][Hq*D] and
+    lse [T][Hq] float32 or None."""
+    nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    _check(lib().p1a_attn_chunk(_ptr(q), _row_type(q), ctypes.byref(c.struct()), _ptr(out), _row_type(out), _ptr(gate), _ptr(lse), rows._ref, Hq, scale,
+                                _ptr(scratch), nbytes, _stream()), "attn_chunk")
+
+
+def chunk_scratch_bytes(c, rows, Hq):
+    return int(lib().p1a_attn_chunk_scratch_bytes(ctypes.byref(c.struct()), rows._ref, Hq))
+
+
+def attn_mass(q, c, lse, mass, rows, Hq, scale):
+    """Adds the attention weight that the rows give to every cache position to mass [n_seq][Hkv][ld] float32; lse as attn_chunk leaves it."""
+    _check(lib().p1a_attn_mass(_ptr(q), _row_type(q), ctypes.byref(c.struct()), _ptr(lse), _ptr(mass), mass.shape[-1], rows._ref, Hq, scale, _stream()), "attn_mass")
+
+
+def evict_select(mass, n, keep, n_sink=0, n_recent=0):
+    """The positions that stay, ascending: keep [n_seq][Hkv][budget] int32 of mass [n_seq][Hkv][ld] float32; n: positions held, a number or int32 [n_seq] on
+    the device."""
+    n_dev, n_host = (None, n) if isinstance(n, int) else (_ptr(n), 0)
+    _check(lib().p1a_evict_select(_ptr(mass), mass.shape[-1], mass.shape[0], mass.shape[1], n_dev, n_host, keep.shape[-1], n_sink, n_recent, _ptr(keep), _stream()),
+           "evict_select")
+
+
+def kv_compact(c, keep, mass=None, mass_out=None):
+    """Moves the rows that keep [n_seq][Hkv][budget] lists to the front of the sequences' pages, in place, and the totals with them (mass_out: mass itself, or
+    another tensor of its shape)."""
+    _check(lib().p1a_kv_compact(ctypes.byref(c.struct()), _ptr(keep), keep.shape[0], keep.shape[-1], _ptr(mass), _ptr(mass_out), 0 if mass is None else mass.shape[-1],
+                                _stream()), "kv_compact")
+
+
 def sigmoid_mul(x, g):
     _check(lib().p1a_sigmoid_mul(_ptr(x), _ptr(g), x.numel(), _stream()), "sigmoid_mul")
 
@@ -509,6 +586,10 @@ class Pool:
 
     def seq_truncate(self, seq, n):
         self._rc(lib().p1a_seq_truncate(self._p, seq, n), "seq_truncate")
+
+    def seq_evict(self, seq, n_keep):
+        """after kv_compact on every layer: the sequence holds n_keep slots, the pages behind them are free"""
+        self._rc(lib().p1a_seq_evict(self._p, seq, n_keep), "seq_evict")
 
     def seq_fork(self, src, n):
         return self._rc(lib().p1a_seq_fork(self._p, src, n), "seq_fork")

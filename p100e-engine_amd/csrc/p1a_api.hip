@@ -1,7 +1,9 @@
 // extern "C" layer of the paged-KV attention library: argument validation (refusals launch nothing), split-K
 // scratch ownership per (device, stream), split-count bookkeeping. All device work lives in the other .hip files.
 #include "p1a_common.hpp"
+#include "p1a_tiles.hpp"
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -217,6 +219,37 @@ int decode_call(const float * q, const p1a_kv * c, float * out, const float * ga
     return launch_decode(*c, a, s);
 }
 
+
+// the rows of a call over bounded caches, checked: what the kernels take (`max_n`: the most positions a sequence may hold)
+int rows_ok(const p1a_kv * c, const p1a_rows * r, int Hq, const char * who, rows_view & R, int & max_n) {
+    if (!kv_ok(c, who)) return P1A_E_ARG;
+    if (!r || r->T < 0 || r->n_seq < 0 || r->max_rows < 0 || r->max_n < 0 || r->window < 0 || r->n_sink < 0 || c->n_ctx < 0) { set_error("%s: no rows, or a negative count among them", who); return P1A_E_ARG; }
+    if (!r->pos0 && r->n_seq > 1) { set_error("%s: %d sequences need positions in device memory", who, r->n_seq); return P1A_E_ARG; }
+    if (r->n_seq > 1 && (!c->pt || !c->rtab)) { set_error("%s: %d sequences need a page table and a row table", who, r->n_seq); return P1A_E_ARG; }
+    if (!r->row0 && r->n_seq > 0 && r->T % r->n_seq) { set_error("%s: %d rows do not divide among %d sequences", who, r->T, r->n_seq); return P1A_E_ARG; }
+    if ((c->D != 64 && c->D != 128 && c->D != 256) || Hq < c->Hkv || Hq % c->Hkv || Hq / c->Hkv > 64 || r->n_seq > 65535 || c->Hkv > 4096 || (long long) r->T * Hq > 1 << 30) {
+        set_error("%s: unsupported shape (D=%d Hq=%d Hkv=%d T=%d n_seq=%d)", who, c->D, Hq, c->Hkv, r->T, r->n_seq);
+        return P1A_E_SHAPE;
+    }
+    const uintptr_t al = c->type == P1A_KV_F16 ? 15 : c->type == P1A_KV_Q8_0 ? 3 : 1;
+    if ((((uintptr_t) c->k | (uintptr_t) c->v) & al) || (c->pt && (c->pstride & al))) { set_error("%s: cache base / page stride must be %d-byte aligned", who, (int) al + 1); return P1A_E_SHAPE; }
+    R.row0 = r->row0; R.pos0 = r->pos0; R.T = r->T; R.n_seq = r->n_seq; R.p0 = r->p0;
+    R.per = r->row0 || !r->n_seq ? 0 : r->T / r->n_seq;
+    R.max_rows = r->max_rows && r->max_rows < r->T ? r->max_rows : r->T;
+    if (!r->row0 && R.per < R.max_rows) R.max_rows = R.per;
+    R.window = r->window ? r->window : INT32_MAX;
+    R.n_sink = r->window ? r->n_sink : 0;
+    R.n_ctx = c->n_ctx;
+    max_n = r->max_n && r->max_n < c->n_ctx ? r->max_n : c->n_ctx;
+    if (!r->pos0) max_n = (int) std::max(1LL, std::min<long long>(max_n, (long long) r->p0 + r->T));
+    return P1A_OK;
+}
+bool rows_type_ok(int type, const char * who) {
+    if (type == P1A_ROWS_F32 || type == P1A_ROWS_BF16) return true;
+    set_error("%s: unknown type of rows %d", who, type);
+    return false;
+}
+
 }   // namespace
 
 bool split_scratch(hipStream_t s, size_t bytes_o, size_t bytes_ml, float *& o, float *& ml) {
@@ -398,6 +431,70 @@ int p1a_attn_prefill(const float * q, const p1a_kv * c, float * out, const float
     if (Hq < c->Hkv || Hq % c->Hkv) { set_error("p1a_attn_prefill: unsupported shape (Hq=%d Hkv=%d)", Hq, c->Hkv); return P1A_E_SHAPE; }
     if ((((uintptr_t) q | (uintptr_t) out | (uintptr_t) gate) & 15)) { set_error("p1a_attn_prefill: q/out/gate must be 16-byte aligned"); return P1A_E_SHAPE; }
     return launch_prefill(*c, q, out, gate, T, p0, Hq, scale, scratch, scratch_bytes, (hipStream_t) stream);
+}
+
+int p1a_attn_chunk(const void * q, int q_type, const p1a_kv * c, void * out, int out_type, const float * gate, float * lse, const p1a_rows * rows,
+                   int Hq, float scale, void * scratch, size_t scratch_bytes, void * stream) {
+    static const char * const who = "p1a_attn_chunk";
+    chunk_args a;
+    const int rc = rows_ok(c, rows, Hq, who, a.R, a.max_n);
+    if (rc != P1A_OK) return rc;
+    if (!q || !out || !rows_type_ok(q_type, who) || !rows_type_ok(out_type, who)) { if (!q || !out) set_error("%s: null q/out", who); return P1A_E_ARG; }
+    if (((uintptr_t) q | (uintptr_t) out | (uintptr_t) gate) & 15 || (uintptr_t) lse & 3) { set_error("%s: q/out/gate must be 16-byte aligned, lse 4-byte", who); return P1A_E_SHAPE; }
+    if (!rows->T || !rows->n_seq) return P1A_OK;
+    a.q = q; a.out = out; a.gate = gate; a.lse = lse; a.q_bf16 = q_type == P1A_ROWS_BF16; a.out_bf16 = out_type == P1A_ROWS_BF16;
+    a.Hq = Hq; a.scale = scale; a.scratch = scratch; a.scratch_bytes = scratch_bytes;
+    return launch_chunk(*c, a, (hipStream_t) stream);
+}
+
+size_t p1a_attn_chunk_scratch_bytes(const p1a_kv * c, const p1a_rows * rows, int Hq) {
+    rows_view R;
+    int max_n;
+    if (rows_ok(c, rows, Hq, "p1a_attn_chunk_scratch_bytes", R, max_n) != P1A_OK || !rows->T || !rows->n_seq) return 0;
+    const size_t n = (size_t) R.T * Hq, k = (size_t) chunk_splits(*c, R, Hq, max_n, cu_count());
+    return k > 1 ? ((n * k * 8 + 255) & ~(size_t) 255) + n * k * c->D * 4 : 0;
+}
+
+int p1a_attn_mass(const void * q, int q_type, const p1a_kv * c, const float * lse, float * mass, int ld, const p1a_rows * rows, int Hq, float scale,
+                  void * stream) {
+    static const char * const who = "p1a_attn_mass";
+    rows_view R;
+    int max_n;
+    const int rc = rows_ok(c, rows, Hq, who, R, max_n);
+    if (rc != P1A_OK) return rc;
+    if (!q || !lse || !mass || ld < 0) { set_error("%s: null q / lse / mass or negative ld", who); return P1A_E_ARG; }
+    if (!rows_type_ok(q_type, who)) return P1A_E_ARG;
+    if (((uintptr_t) q & 15) || (((uintptr_t) lse | (uintptr_t) mass) & 3)) { set_error("%s: q must be 16-byte aligned, lse and mass 4-byte", who); return P1A_E_SHAPE; }
+    if (!rows->T || !rows->n_seq || !ld) return P1A_OK;
+    return launch_mass(*c, q, q_type == P1A_ROWS_BF16, lse, mass, ld, R, Hq, scale, max_n, (hipStream_t) stream);
+}
+
+int p1a_evict_select(const float * mass, int ld, int n_seq, int Hkv, const int32_t * n_dev, int n, int budget, int n_sink, int n_recent,
+                     int32_t * keep, void * stream) {
+    static const char * const who = "p1a_evict_select";
+    if (!mass || !keep || ld < 0 || n_seq < 0 || Hkv < 1 || n_sink < 0 || n_recent < 0 || (!n_dev && n < 0)) { set_error("%s: null argument or a negative count", who); return P1A_E_ARG; }
+    if (budget < 0 || budget > 1 << 20 || (long long) n_sink + n_recent > budget || n_seq > 65535 || Hkv > 4096) {
+        set_error("%s: budget=%d must hold n_sink=%d and n_recent=%d and be at most 2^20", who, budget, n_sink, n_recent);
+        return P1A_E_SHAPE;
+    }
+    if (((uintptr_t) mass | (uintptr_t) keep) & 3) { set_error("%s: mass and keep must be 4-byte aligned", who); return P1A_E_SHAPE; }
+    if (!n_seq || !budget) return P1A_OK;
+    return launch_evict_select(mass, ld, n_seq, Hkv, n_dev, n, budget, n_sink, n_recent, keep, (hipStream_t) stream);
+}
+
+int p1a_kv_compact(const p1a_kv * c, const int32_t * keep, int n_seq, int budget, const float * mass, float * mass_out, int ld, void * stream) {
+    static const char * const who = "p1a_kv_compact";
+    if (!kv_ok(c, who)) return P1A_E_ARG;
+    if (!keep || n_seq < 0 || budget < 0 || !mass != !mass_out || (mass && ld < 0) || c->n_ctx < 0) { set_error("%s: null keep, a negative count, or one of mass and mass_out alone", who); return P1A_E_ARG; }
+    if (n_seq > 1 && (!c->pt || !c->rtab)) { set_error("%s: %d sequences need a page table and a row table", who, n_seq); return P1A_E_ARG; }
+    if (budget > 1 << 20 || n_seq > 65535 || c->Hkv > 4096) { set_error("%s: unsupported shape (budget=%d n_seq=%d Hkv=%d)", who, budget, n_seq, c->Hkv); return P1A_E_SHAPE; }
+    if ((((uintptr_t) c->k | (uintptr_t) c->v) & 1) || (c->pt && (c->pstride & 1)) || (((uintptr_t) keep | (uintptr_t) mass | (uintptr_t) mass_out) & 3)) {
+        set_error("%s: cache base and page stride must be 2-byte aligned, keep and mass 4-byte", who);
+        return P1A_E_SHAPE;
+    }
+    if (mass && mass != mass_out && mass < mass_out + (size_t) n_seq * c->Hkv * ld && mass_out < mass + (size_t) n_seq * c->Hkv * ld) { set_error("%s: mass and mass_out overlap in part", who); return P1A_E_ARG; }
+    if (!n_seq || (!budget && !mass)) return P1A_OK;
+    return launch_kv_compact(*c, keep, n_seq, budget, mass, mass_out, ld, (hipStream_t) stream);
 }
 
 int p1a_sigmoid_mul(float * x, const float * g, size_t n, void * stream) {

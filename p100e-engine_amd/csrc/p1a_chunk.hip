@@ -1,0 +1,398 @@
+// Attention of the new tokens of several sequences over their paged caches - from one token each to whole prompts, ragged, with a sliding window and
+// first positions that stay visible - for gfx950.
+//
+// Work: a block is 128 consecutive rows of one sequence and kv head (row r: token r / GQA under q head r % GQA of the group); a workgroup of four
+// waves owns one, wave w the 32 rows from 32 w on, and walks the tiles of keys that any of its rows sees: the sinks' and the window's. Calls of few
+// blocks deal a block's tiles to several workgroups, whose partials a second kernel merges.
+// Arithmetic: S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_32x32x16_f16, sums in fp32, one pass with a running reference r of every row:
+// P = exp2(scale log2 e S - r), O and l are sums over P and rescaled when the row's maximum comes out of [r + 8 - inf, r + 14]. Where results are f32, q and P
+// are two f16 halves (EXACT) and quantized K and V two planes (p1a_tiles.hpp): 2 products for f16 caches, 3 for quantized ones (low times low is 2^-22
+// of the result and left out). P runs up to 2^14, so its low halves end 2^-38 below the largest weight.
+#include "p1a_tiles.hpp"
+
+#include <algorithm>
+#include <atomic>
+
+namespace p1a {
+namespace {
+
+constexpr int BM = 128, NTHR = 256;
+constexpr float HEAD = 8.f, STEP = 6.f;                       // log2 of P at the row's maximum: HEAD when the reference moves, at most HEAD + STEP
+
+struct chunk_params {
+    const void * q;
+    void * out;
+    const float * gate;
+    float * lse;
+    const char * kc;
+    const char * vc;
+    kv_view pg;
+    rows_view R;
+    int Hq, Hkv, GQA;
+    uint32_t gqa_magic;    // floor(2^32 / GQA) (2^32 - 1 for GQA = 1)
+    float factor, sign;    // scores are factor * (sign q . k), in log2 units; factor > 0
+    int q_bf16, out_bf16;
+    int nks;               // workgroups of a block
+    float * part_o;        // [T * Hq][nks][D], relative to r
+    float * part_ml;       // [T * Hq][nks][2]: r, l
+};
+
+template <uint32_t KT, int D, bool EXACT> struct chunk_cfg {
+    static constexpr int NPL = group_planes(KT, EXACT);
+    static constexpr int BN = NPL == 2 && D >= 128 ? 32 : 64; // keys of a tile: 64 KB and less of LDS for K and V
+    static constexpr int NG = BN / 16, G_B = NPL * plane_bytes(D), STAGE_B = 2 * NG * G_B;
+};
+
+__device__ __forceinline__ float gate_of(float g) { return 1.0f / (1.0f + expf(-g)); }
+// four results of a row, at element i of out
+__device__ __forceinline__ void put4(void * out, bool bf16, size_t i, f4 v) {
+    if (!bf16) *(__attribute__((address_space(1))) f4 *) ((__attribute__((address_space(1))) char *) out + 4 * i) = v;
+    else *(__attribute__((address_space(1))) u2w *) ((__attribute__((address_space(1))) char *) out + 2 * i) =
+        u2w{bf16_of(v[0]) | bf16_of(v[1]) << 16, bf16_of(v[2]) | bf16_of(v[3]) << 16};
+}
+
+template <uint32_t KT, int D, bool EXACT>
+__global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_params P) {
+    using C = chunk_cfg<KT, D, EXACT>;
+    using G = group<KT, D, C::NPL>;
+    constexpr int BN = C::BN, NG = C::NG, G_B = C::G_B, PL_B = plane_bytes(D), NPL = C::NPL;
+    constexpr int NKS = D / 16, NDT = D / 32, NH = BN / 32, NQ = EXACT ? 2 : 1;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, g = lane >> 5;
+    // kv heads side by side (their XCDs), then the splits of a block, then blocks
+    const int item = blockIdx.x / P.Hkv, hk = blockIdx.x - item * P.Hkv, bi = item / P.nks, ksp = item - bi * P.nks;
+    item_at at;
+    if (!find_item(P.R, bi, P.GQA, BM, lane, at)) return;
+    const int nrows = at.v.count * P.GQA, row0 = (at.of - 1 - at.index) * BM;   // (the blocks that see most first)
+    const int wrow0 = row0 + 32 * wave, wrows = min(32, nrows - wrow0);
+    auto tok_of = [&](int r) {                                // (the multiplication is at most one short)
+        const int t = (int) __umulhi((uint32_t) r, P.gqa_magic);
+        return r - t * P.GQA >= P.GQA ? t + 1 : t;
+    };
+    auto row_index = [&](int r) { const int t = tok_of(r); return (size_t) (at.v.first + t) * P.Hq + (size_t) hk * P.GQA + (r - t * P.GQA); };
+    const bool live = c < wrows;
+    const int my_row = wrow0 + min(c, max(wrows, 1) - 1), my_tok = tok_of(min(my_row, nrows - 1));
+    int my_pos = at.v.pos0 + my_tok;
+    if (!live || my_pos < 0 || my_pos >= P.R.n_ctx) my_pos = -1;   // sees nothing
+    const size_t my_index = row_index(min(my_row, nrows - 1));
+
+    const span sp = span_of<BN>(P.R, at.v.pos0 + tok_of(row0), at.v.pos0 + tok_of(min(row0 + BM, nrows) - 1));
+    const int tps = (sp.nt + P.nks - 1) / P.nks, ta = min(ksp * tps, sp.nt), tb = min(ta + tps, sp.nt);
+    // positions that every row of the wave sees: up to all_hi, from all_lo on (rows stand at consecutive positions; none where one of them sees nothing)
+    const int all_hi = __builtin_amdgcn_readlane(my_pos, 0), last_pos = __builtin_amdgcn_readlane(my_pos, max(wrows, 1) - 1);
+    const int all_lo = all_hi < 0 || last_pos < 0 ? INT32_MAX : P.R.window == INT32_MAX ? 0 : max(last_pos - P.R.window + 1, 0);
+
+    // ---- where rows of the cache are ----
+    const int32_t * const ptab = P.pg.pt ? P.pg.pt + (P.pg.rtab ? P.pg.rtab[at.seq] : 0) : nullptr;
+    const size_t head_off = (size_t) hk * head_bytes(KT, D);
+    // BN = 64: wave w fills group w of K and V; 32: groups 0 and 1 of K (waves 0, 1) and of V (waves 2, 3)
+    constexpr bool BOTH = BN == 64;
+    const int grp = BOTH ? wave : wave & 1, my_key = 16 * grp + G::key(lane);
+    const bool my_v = !BOTH && wave >= 2;
+    auto pos_of = [&](int tile) { return seen_or_near<BN>(sp, tile * BN, tile * BN + my_key); };
+    auto page_of = [&](int tile) { return ptab ? ptab[pos_of(tile) >> P.pg.psh] : 0; };
+    auto row_of = [&](int tile, int page) {
+        const int j = pos_of(tile);
+        return head_off + (ptab ? (size_t) page * P.pg.pstride + (size_t) (j & ((1 << P.pg.psh) - 1)) * P.pg.rowb : (size_t) j * P.pg.rowb);
+    };
+    auto k_groups = [&](int st) { return lds + st * C::STAGE_B; };
+    auto v_groups = [&](int st) { return lds + st * C::STAGE_B + NG * G_B; };
+
+    int page = ta < tb ? page_of(sp.tile(ta)) : 0;
+
+    // ---- Q^T operands: lane (row c, half g) holds dims 16 ks + 8 g .. + 7 ----
+    h8 qf[NQ][NKS];
+    float factor = P.factor;
+    {
+        f4 x[NKS][2];
+        float most = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                x[ks][e] = q4_at(P.q, P.q_bf16, my_index * D + 16 * ks + 8 * g + 4 * e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(x[ks][e][i]));
+            }
+        const int ex = row_exponent(max_swap32(most));
+        factor = ldexpf(factor, ex);
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float y = live ? ldexpf(x[ks][e >> 2][e & 3] * P.sign, -ex) : 0.f;
+                qf[0][ks][e] = (half_t) y;
+                if constexpr (EXACT) qf[NQ - 1][ks][e] = (half_t) (y - (float) (half_t) y);
+            }
+    }
+
+    f16x o[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    float ref = MINUS_INF, l = 0.f;
+
+    const k_frag kf(lane, G_B);
+    const v_frag vf(lane);
+
+    // ---- one tile ----
+    auto compute = [&](int st, int tile) {
+        const int k0 = tile * BN;
+        f16x s[NH];
+#pragma unroll
+        for (int u = 0; u < NH; ++u) {
+            const char * kg = k_groups(st) + 2 * u * G_B;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks) {
+                const h8 a = kf.read(kg, ks);
+                s[u] = mfma32(a, qf[0][ks], s[u]);
+                if constexpr (EXACT) s[u] = mfma32(a, qf[NQ - 1][ks], s[u]);
+                if constexpr (NPL == 2) s[u] = mfma32(kf.read(kg + PL_B, ks), qf[0][ks], s[u]);
+            }
+        }
+        if (!(k0 + BN - 1 <= all_hi && k0 >= all_lo)) {
+            const int hi = my_pos - k0, lo = max(hi, 0) - P.R.window, sk = P.R.n_sink - k0;
+#pragma unroll
+            for (int u = 0; u < NH; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const int j = 32 * u + mfma_row(i, g);
+                    s[u][i] = j <= hi && (j > lo || j < sk) ? s[u][i] : MINUS_INF;
+                }
+        }
+        float mx = MINUS_INF;
+#pragma unroll
+        for (int u = 0; u < NH; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
+        mx = max_swap32(mx) * factor;
+        const bool fresh = ref == MINUS_INF, move = mx > (fresh ? MINUS_INF : ref + (HEAD + STEP));
+        if (__any(move)) {
+            const float to = move ? mx - HEAD : ref, alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(ref - to);   // (fresh: nothing accumulated)
+            ref = to;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
+        }
+        const float nr = ref == MINUS_INF ? 0.f : -ref;       // (a row that has seen nothing: exp2(-inf))
+        h8 pb[NQ][2 * NH];
+        float ls[2] = {0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < NH; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(s[u][i], factor, nr));
+                ls[i & 1] += p;
+                const half_t h = (half_t) p;
+                pb[0][2 * u + (i >> 3)][i & 7] = h;
+                if constexpr (EXACT) pb[NQ - 1][2 * u + (i >> 3)][i & 7] = (half_t) (p - (float) h);
+            }
+        l += ls[0] + ls[1];
+#pragma unroll
+        for (int ps = 0; ps < NG; ++ps) {
+            const char * vg = v_groups(st) + ps * G_B;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt) {
+                const h8 a = vf.read(vg, dt);
+                o[dt] = mfma32(a, pb[0][ps], o[dt]);
+                if constexpr (EXACT) o[dt] = mfma32(a, pb[NQ - 1][ps], o[dt]);
+                if constexpr (NPL == 2) o[dt] = mfma32(vf.read(vg + PL_B, dt), pb[0][ps], o[dt]);
+            }
+        }
+    };
+
+    // ---- the walk: tile i + 1 is on its way while tile i is worked on; its page-table entries were asked for a tile ahead ----
+    auto run = [&](auto && fetch, auto && put) {
+        if (ta >= tb) return;
+        fetch(0, sp.tile(ta), page);
+        put(0);
+        page = ta + 1 < tb ? page_of(sp.tile(ta + 1)) : 0;
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        for (int i = ta, st = 0; i < tb; ++i, st ^= 1) {
+            const bool more = i + 1 < tb;
+            if (more) fetch(st ^ 1, sp.tile(i + 1), page);
+            if (i + 2 < tb) page = page_of(sp.tile(i + 2));
+            if (wrows > 0) compute(st, sp.tile(i));
+            if (more) put(st ^ 1);
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        }
+    };
+    if constexpr (G::DIRECT) {
+        run([&](int st, int tile, int pg) {
+            const size_t row = row_of(tile, pg);
+            G::load((gbytes) P.kc + row, k_groups(st) + grp * G_B, lane);
+            G::load((gbytes) P.vc + row, v_groups(st) + grp * G_B, lane);
+        }, [](int) {});
+    } else {
+        typename G::raw ra, rb;
+        run([&](int, int tile, int pg) {
+            const size_t row = row_of(tile, pg);
+            G::load(ra, (my_v ? (gbytes) P.vc : (gbytes) P.kc) + row, lane);
+            if constexpr (BOTH) G::load(rb, (gbytes) P.vc + row, lane);
+        }, [&](int st) {
+            G::store(ra, (my_v ? v_groups(st) : k_groups(st)) + grp * G_B, lane);
+            if constexpr (BOTH) G::store(rb, v_groups(st) + grp * G_B, lane);
+        });
+    }
+
+    // ---- results: lane (row c, half g) holds dims 32 dt + 8 (i / 4) + 4 g + i % 4 ----
+    l += __shfl_xor(l, 32);
+    if (!live) return;
+    if (P.nks > 1) {
+        float * ml = P.part_ml + (my_index * P.nks + ksp) * 2;
+        if (g == 0) { ml[0] = ref; ml[1] = l; }
+        if (ref == MINUS_INF) return;                         // (nothing seen: the merge does not look at it)
+        float * po = P.part_o + (my_index * P.nks + ksp) * D;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<f4 *>(po + 32 * dt + 8 * q + 4 * g) = f4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
+        return;
+    }
+    const float inv = ref == MINUS_INF ? 0.f : 1.0f / l;
+    if (P.lse && g == 0) P.lse[my_index] = ref == MINUS_INF ? MINUS_INF : (ref + log2f(l)) * LN2;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const size_t e = my_index * D + 32 * dt + 8 * q + 4 * g;
+            f4 v = f4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]} * inv;
+            if (P.gate) {
+                const f4 gt = *reinterpret_cast<const f4 *>(P.gate + e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] *= gate_of(gt[i]);
+            }
+            put4(P.out, P.out_bf16, e, v);
+        }
+}
+
+// Partials of a row -> its result: 256 / (D / 4) rows a workgroup, four dims a thread
+struct chunk_merge_params {
+    rows_view R;
+    const float * part_o, * part_ml, * gate;
+    void * out;
+    float * lse;
+    int Hq, D, nks, out_bf16;
+};
+__global__ void __launch_bounds__(NTHR) chunk_merge_k(const chunk_merge_params P) {
+    const int tpr = P.D >> 2, sub = threadIdx.x / tpr, d = 4 * (threadIdx.x - sub * tpr);
+    const long long row = (long long) blockIdx.x * (NTHR / tpr) + sub;
+    if (row >= (long long) P.R.T * P.Hq) return;
+    if (P.R.row0) {                                           // the last sequence that starts at or ahead of the row's token
+        const int t = (int) (row / P.Hq);
+        int a = 0, b = P.R.n_seq;
+        while (b - a > 1) {
+            const int m = (a + b) >> 1;
+            if (P.R.row0[m] <= t) a = m; else b = m;
+        }
+        const seq_view v = seq_of(P.R, a);
+        if (t < v.first || t >= v.first + v.count) return;    // (nobody's: left as it is)
+    }
+    const float2 * ml = reinterpret_cast<const float2 *>(P.part_ml) + row * P.nks;
+    float M = MINUS_INF;
+    for (int k = 0; k < P.nks; ++k) M = fmaxf(M, ml[k].x);
+    f4 acc = {0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    for (int k = 0; k < P.nks; ++k) {
+        const float2 p = ml[k];
+        if (p.x == MINUS_INF) continue;
+        const float w = __builtin_amdgcn_exp2f(p.x - M);
+        l += p.y * w;
+        acc += *reinterpret_cast<const f4 *>(P.part_o + (row * P.nks + k) * P.D + d) * w;
+    }
+    if (P.lse && d == 0) P.lse[row] = M == MINUS_INF ? MINUS_INF : (M + log2f(l)) * LN2;
+    f4 v = acc * (M == MINUS_INF ? 0.f : 1.0f / l);
+    const size_t e = (size_t) row * P.D + d;
+    if (P.gate) {
+        const f4 gt = *reinterpret_cast<const f4 *>(P.gate + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] *= gate_of(gt[i]);
+    }
+    put4(P.out, P.out_bf16, e, v);
+}
+
+template <uint32_t KT, int D, bool EXACT> int launch_cfg(const chunk_params & P, unsigned grid, hipStream_t s) {
+    constexpr int lds = 2 * chunk_cfg<KT, D, EXACT>::STAGE_B;
+    // (the attribute belongs to the function on ONE device: remembered per device, set again on another)
+    static std::atomic<uint32_t> attr_set{0};
+    int dev = 0;
+    (void) hipGetDevice(&dev);
+    const uint32_t bit = 1u << (dev & 31);
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
+        if (hipFuncSetAttribute((const void *) chunk_k<KT, D, EXACT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+            (void) hipGetLastError();
+            set_error("p1a_attn_chunk: cannot reserve %d bytes of LDS", lds);
+            return P1A_E_LAUNCH;
+        }
+        attr_set.fetch_or(bit, std::memory_order_release);
+    }
+    chunk_k<KT, D, EXACT><<<grid, NTHR, lds, s>>>(P);
+    return launched();
+}
+template <uint32_t KT, int D> int launch_d(const chunk_params & P, bool exact, unsigned grid, hipStream_t s) {
+    return exact ? launch_cfg<KT, D, true>(P, grid, s) : launch_cfg<KT, D, false>(P, grid, s);
+}
+template <uint32_t KT> int launch_kt(const chunk_params & P, int D, bool exact, unsigned grid, hipStream_t s) {
+    return D == 256 ? launch_d<KT, 256>(P, exact, grid, s) : D == 128 ? launch_d<KT, 128>(P, exact, grid, s) : launch_d<KT, 64>(P, exact, grid, s);
+}
+
+// the most blocks the rows can make
+long long block_bound(const rows_view & R, int GQA) {
+    const long long each = ((long long) R.max_rows * GQA + BM - 1) / BM * R.n_seq;
+    return R.row0 ? std::min(each, (long long) R.T * GQA / BM + R.n_seq) : each;
+}
+
+}   // namespace
+
+// Workgroups of a block, from the call's host numbers and the device: the count that minimises rounds of workgroups x (tiles of a workgroup + 3 for
+// its set-up and results), and 3 for a merge
+int chunk_splits(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus) {
+    const int GQA = Hq / c.Hkv, BN = 64;
+    const long long units = block_bound(R, GQA) * c.Hkv, slots = (long long) std::max(cus, 1) * (c.D <= 128 ? 2 : 1);
+    const long long keys = R.window == INT32_MAX ? max_n : std::min<long long>(max_n, (long long) R.window + std::min(R.max_rows, BM / GQA + 1) + R.n_sink);
+    const long long nt = std::max<long long>(keys / BN, 1);
+    auto cost = [&](long long k) { return (units * k + slots - 1) / slots * ((nt + k - 1) / k + 3) + (k > 1 ? 3 : 0); };
+    long long best = 1;
+    for (long long k = 2; k <= 64 && k <= nt; ++k) if (cost(k) < cost(best)) best = k;
+    return (int) best;
+}
+
+int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
+    chunk_params P;
+    P.q = a.q; P.out = a.out; P.gate = a.gate; P.lse = a.lse;
+    P.kc = (const char *) c.k; P.vc = (const char *) c.v; P.pg = view_of(c); P.R = a.R;
+    P.Hq = a.Hq; P.Hkv = c.Hkv; P.GQA = a.Hq / c.Hkv;
+    P.gqa_magic = (uint32_t) (P.GQA == 1 ? (1ull << 32) - 1 : (1ull << 32) / (unsigned) P.GQA);
+    P.factor = a.scale == 0.f ? 1.f : (a.scale < 0 ? -a.scale : a.scale) * LOG2E;
+    P.sign = a.scale == 0.f ? 0.f : a.scale < 0 ? -1.f : 1.f;
+    P.q_bf16 = a.q_bf16; P.out_bf16 = a.out_bf16;
+    P.nks = chunk_splits(c, a.R, a.Hq, a.max_n, cu_count());
+    P.part_o = P.part_ml = nullptr;
+    const size_t rows = (size_t) a.R.T * a.Hq;
+    if (P.nks > 1) {
+        const size_t bm = (rows * P.nks * 8 + 255) & ~(size_t) 255, bo = rows * P.nks * c.D * 4;
+        if (a.scratch && !((uintptr_t) a.scratch & 255) && a.scratch_bytes >= bm + bo) {
+            P.part_ml = (float *) a.scratch;
+            P.part_o = (float *) ((char *) a.scratch + bm);
+        } else if (!split_scratch(s, bo, bm, P.part_o, P.part_ml)) return P1A_E_SCRATCH;
+    }
+    const long long grid = block_bound(a.R, P.GQA) * P.nks * c.Hkv;
+    if (grid > 0x7fffffffLL) { set_error("p1a_attn_chunk: too many rows for one call"); return P1A_E_SHAPE; }
+    const bool exact = !a.out_bf16 || a.lse;
+    const int rc = c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, exact, (unsigned) grid, s)
+                 : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, exact, (unsigned) grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, exact, (unsigned) grid, s);
+    if (rc != P1A_OK || P.nks == 1) return rc;
+    const chunk_merge_params M{a.R, P.part_o, P.part_ml, a.gate, a.out, a.lse, a.Hq, c.D, P.nks, a.out_bf16};
+    const size_t per = NTHR / (c.D / 4);
+    chunk_merge_k<<<(unsigned) ((rows + per - 1) / per), NTHR, 0, s>>>(M);
+    return launched();
+}
+
+}   // namespace p1a

@@ -384,6 +384,13 @@ int p1a_seq_truncate(p1a_pool * p, int id, int n) {
     return P1A_OK;
 }
 
+int p1a_seq_evict(p1a_pool * p, int id, int n_keep) {
+    const int rc = p1a_seq_truncate(p, id, n_keep);
+    if (rc != P1A_OK) return rc;
+    for (int32_t & t : p->get(id)->toks) t = -1;
+    return P1A_OK;
+}
+
 int p1a_seq_fork(p1a_pool * p, int src, int n) {
     if (!p) return P1A_E_ARG;
     {

@@ -1,0 +1,268 @@
+// What the kernels over bounded caches share (internal header): whose a call's rows are and what they see, and tiles of 16 keys in LDS.
+#pragma once
+#include "p1a_common.hpp"
+
+namespace p1a {
+
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float MINUS_INF = -__builtin_inff();
+
+// ---- rows of several sequences (p1a_rows as the kernels take it) ----
+struct rows_view {
+    const int32_t * row0, * pos0;
+    int T, n_seq, max_rows, per, p0;   // per: rows of a sequence without row0
+    int window, n_sink;                // window: INT32_MAX for none (n_sink 0 then)
+    int n_ctx;
+};
+struct seq_view { int first, count, pos0; };   // rows first .. first + count - 1, the first of them at position pos0
+// (whatever the device arrays hold: rows inside 0 .. T, positions where adding a row to one does not overflow)
+__device__ __forceinline__ seq_view seq_of(const rows_view & R, int s) {
+    seq_view v;
+    v.first = R.row0 ? min(max(R.row0[s], 0), R.T) : s * R.per;
+    v.count = min(R.row0 ? max(min(R.row0[s + 1], R.T) - v.first, 0) : R.per, R.max_rows);
+    v.pos0 = min(max(R.pos0 ? R.pos0[s] : R.p0, -(1 << 30)), R.n_ctx);
+    return v;
+}
+// Item b of a list that holds ceil(count * mul / unit) items of each sequence, in order: whose it is, and which of them; false: there are fewer.
+// Every lane of the wave calls, with the same b.
+struct item_at { int seq, index, of; seq_view v; };
+__device__ __forceinline__ bool find_item(const rows_view & R, int b, int mul, int unit, int lane, item_at & at) {
+    if (!R.row0) {
+        at.of = (R.max_rows * mul + unit - 1) / unit;          // (max_rows is at most per)
+        at.seq = b / at.of;
+        at.index = b - at.seq * at.of;
+        if (at.seq >= R.n_seq) return false;
+        at.v = seq_of(R, at.seq);
+        return true;
+    }
+    for (int s0 = 0; s0 < R.n_seq; s0 += 64) {
+        const int s = s0 + lane;
+        const int n = s < R.n_seq ? (int) (((long long) seq_of(R, s).count * mul + unit - 1) / unit) : 0;
+        int u = n;                                             // sums over the lanes up to this one
+        u += __builtin_amdgcn_update_dpp(0, u, 0x111, 0xf, 0xf, true);
+        u += __builtin_amdgcn_update_dpp(0, u, 0x112, 0xf, 0xf, true);
+        u += __builtin_amdgcn_update_dpp(0, u, 0x114, 0xf, 0xf, true);
+        u += __builtin_amdgcn_update_dpp(0, u, 0x118, 0xf, 0xf, true);
+        u += __builtin_amdgcn_update_dpp(0, u, 0x142, 0xa, 0xf, false);
+        u += __builtin_amdgcn_update_dpp(0, u, 0x143, 0xc, 0xf, false);
+        const unsigned long long behind = __ballot(u > b);
+        if (behind) {
+            const int l = __builtin_ctzll(behind);
+            at.seq = s0 + l;
+            at.of = __builtin_amdgcn_readlane(n, l);
+            at.index = b - (__builtin_amdgcn_readlane(u, l) - at.of);
+            at.v = seq_of(R, at.seq);
+            return true;
+        }
+        b -= __builtin_amdgcn_readlane(u, 63);
+    }
+    return false;
+}
+
+// The positions that rows at pmin .. pmax of one sequence see, in tiles of BN: the sinks' tiles, then the window's
+struct span {
+    int pmax, lo, ns;                  // visible: lo .. pmax and 0 .. ns - 1
+    int nst, tw0, nt;                  // tiles of sinks, first tile of the window, all tiles (0: nothing is seen)
+    __device__ __forceinline__ int tile(int i) const { return i < nst ? i : tw0 + (i - nst); }
+};
+template <int BN> __device__ __forceinline__ span span_of(const rows_view & R, int pmin, int pmax) {
+    span s;
+    pmin = max(pmin, 0);
+    s.pmax = min(pmax, R.n_ctx - 1);
+    s.lo = R.window == INT32_MAX ? 0 : max(pmin - R.window + 1, 0);
+    s.ns = max(min(R.n_sink, s.pmax + 1), 0);
+    s.nst = (s.ns + BN - 1) / BN;
+    s.tw0 = max(s.lo / BN, s.nst);
+    s.nt = pmin > s.pmax ? 0 : s.nst + max(s.pmax / BN - s.tw0 + 1, 0);
+    return s;
+}
+// Position j of the tile that starts at k0 or, where nothing sees j, one of the tile that is seen: its row is fetched in its place, so that no
+// page-table entry and no memory behind one is read that the call may not know
+template <int BN> __device__ __forceinline__ int seen_or_near(const span & s, int k0, int j) {
+    if (j > s.pmax) return s.pmax;
+    if (j < s.lo && j >= s.ns) return k0 + BN > s.lo ? s.lo : s.ns - 1;
+    return j;
+}
+
+// ---- rows of q as operands: two halves whose sum is the f32 value ----
+// A row is brought below 1 by a power of two first (its inverse goes into the factor of the scores), so that the low halves do not end where f16 does.
+// (Not above 2^100: the factor stays a number above zero.)
+__device__ __forceinline__ int row_exponent(float most) { return most > 0.f && most < __builtin_inff() ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0; }
+
+// ---- tiles of 16 keys in LDS ----
+// A group is 16 keys of one kv head as f16, in one plane or - where a quantized value has to keep all its 18 bits - two, whose sum it is. A plane
+// is cut into blocks of 1 KB, four 16-byte chunks (32 dims) of the 16 keys: chunk x of key k lies in block x / 4 at (x % 4) * 256 + (k ^ 4 (x % 4)) * 16. A
+// block is what one global_load_lds_dwordx4 moves (64 lanes x 16 bytes to consecutive LDS), 64 bytes of each of 16 rows; a lane's key is the same in every
+// block, so it needs one page-table entry and one address a tile, whatever the pages' length. The operand of S^T = K Q^T reads 16 keys of a chunk, 256 bytes
+// on end; the transposing read of V^T takes 4 keys of the four chunks of a block, which the exclusive or puts side by side in the banks.
+typedef const __attribute__((address_space(1))) char * gbytes;
+template <typename T> __device__ __forceinline__ T gload(gbytes p) { return *(const __attribute__((address_space(1))) T *) p; }
+typedef u4 u4_a4 __attribute__((aligned(4)));
+typedef u4 u4_a2 __attribute__((aligned(2)));
+typedef unsigned u2w __attribute__((ext_vector_type(2)));
+typedef u2w u2_a4 __attribute__((aligned(4)));
+
+constexpr int group_planes(uint32_t kt, bool exact) { return exact && kt != P1A_KV_F16 ? 2 : 1; }
+constexpr int plane_bytes(int D) { return 16 * 2 * D; }
+
+__device__ __forceinline__ uint32_t lds_at(const char * p) { return (uint32_t) (size_t) (const __attribute__((address_space(3))) char *) p; }
+__device__ __forceinline__ int chunk_at(int key, int x) { return (x >> 2) * 1024 + (x & 3) * 256 + ((key ^ (4 * (x & 3))) * 16); }
+
+// 4 codes in the bytes of w (biased so that byte - off is the code) times d: rounded to f16, and what the rounding left (exact: the product is a
+// multiple of 2^-24 of at most 18 bits)
+template <int NPL> __device__ __forceinline__ void times4(uint32_t w, float off, h2 d, uint32_t * hi, uint32_t * lo) {
+    const h2 o = {(half_t) off, (half_t) off};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const h2 c = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, k ? 0x04030402u : 0x04010400u)) - o;
+        const h2 p = c * d;
+        hi[k] = __builtin_bit_cast(uint32_t, p);
+        if constexpr (NPL == 2) lo[k] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, d, -p));
+    }
+}
+
+// A wave's part in filling one group: every lane stands for one key (row) of it
+template <uint32_t KT, int D, int NPL> struct group;
+
+template <int D, int NPL> struct group<P1A_KV_F16, D, NPL> {
+    static constexpr bool DIRECT = true;
+    static __device__ __forceinline__ int key(int lane) { return (lane & 15) ^ (4 * (lane >> 4)); }
+    // straight to LDS: complete when vmcnt says so
+    static __device__ __forceinline__ void load(gbytes row, char * to, int lane) {
+        gbytes p = row + (lane >> 4) * 16;
+        const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(to));
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j)
+            asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(p + 64 * j), "s"(at), "i"(1024 * j) : "memory", "m0", "scc");
+    }
+};
+
+template <int D, int NPL> struct group<P1A_KV_Q8_0, D, NPL> {
+    static constexpr bool DIRECT = false;
+    static constexpr int NJ = D / 64, NB = D / 32;            // loads of 16 codes a lane; blocks of a row
+    struct raw { u4 w[NJ]; uint32_t d[NB / 2]; };
+    static __device__ __forceinline__ int key(int lane) { return lane & 15; }
+    static __device__ __forceinline__ void load(raw & r, gbytes row, int lane) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) r.w[j] = gload<u4_a4>(row + 2 * NB + (4 * j + (lane >> 4)) * 16);
+        if constexpr (NB == 8) { const u4 t = gload<u4_a4>(row); r.d[0] = t[0]; r.d[1] = t[1]; r.d[2] = t[2]; r.d[3] = t[3]; }
+        else if constexpr (NB == 4) { const u2w t = gload<u2_a4>(row); r.d[0] = t[0]; r.d[1] = t[1]; }
+        else r.d[0] = gload<uint32_t>(row);
+    }
+    static __device__ __forceinline__ void store(const raw & r, char * to, int lane) {
+        const int q = lane >> 4, k = lane & 15;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {                        // codes of part 4 j + q: block 2 j + q / 2, chunks 8 j + 2 q and the next
+            const uint32_t s = q & 2 ? r.d[j] >> 16 : r.d[j] & 0xffff;
+            const h2 d = __builtin_bit_cast(h2, s | (s << 16));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                u4 hi, lo;
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) times4<NPL>(r.w[j][2 * x + e] ^ 0x80808080u, 1152.f, d, h + 2 * e, l + 2 * e);
+                hi = u4{h[0], h[1], h[2], h[3]};
+                char * at = to + chunk_at(k, 8 * j + 2 * q + x);
+                *reinterpret_cast<u4 *>(at) = hi;
+                if constexpr (NPL == 2) { lo = u4{l[0], l[1], l[2], l[3]}; *reinterpret_cast<u4 *>(at + plane_bytes(D)) = lo; }
+            }
+        }
+    }
+};
+
+template <int D, int NPL> struct group<P1A_KV_Q4_0, D, NPL> {
+    static constexpr bool DIRECT = false;
+    static constexpr int NB = D / 32, NJ = (NB + 3) / 4;      // blocks of a row; of a lane
+    struct raw { u4 w[NJ]; uint32_t d[NJ]; };
+    static __device__ __forceinline__ int key(int lane) { return lane & 15; }
+    static __device__ __forceinline__ void load(raw & r, gbytes row, int lane) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const gbytes b = row + min(4 * j + (lane >> 4), NB - 1) * 18;
+            r.d[j] = gload<uint16_t>(b);
+            r.w[j] = gload<u4_a2>(b + 2);
+        }
+    }
+    static __device__ __forceinline__ void store(const raw & r, char * to, int lane) {
+        const int k = lane & 15;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int b = 4 * j + (lane >> 4);
+            if (NB % 4 && b >= NB) break;
+            const h2 d = __builtin_bit_cast(h2, r.d[j] | (r.d[j] << 16));
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {                     // values 8 x ..: bytes 8 (x & 1) .., low nibbles, then high ones
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t w = r.w[j][2 * (x & 1) + e];
+                    times4<NPL>((x & 2 ? w >> 4 : w) & 0x0f0f0f0fu, 1032.f, d, h + 2 * e, l + 2 * e);
+                }
+                char * at = to + chunk_at(k, 4 * b + x);
+                *reinterpret_cast<u4 *>(at) = u4{h[0], h[1], h[2], h[3]};
+                if constexpr (NPL == 2) *reinterpret_cast<u4 *>(at + plane_bytes(D)) = u4{l[0], l[1], l[2], l[3]};
+            }
+        }
+    }
+};
+
+// The 32 keys of groups 2 u and 2 u + 1 as rows of a 32 x 16 operand: lane (row c, half g) reads chunk 2 ks + g of key c in step ks. base: what of
+// the address depends on the lane, for even and odd steps
+struct k_frag {
+    int base[2];
+    __device__ __forceinline__ k_frag(int lane, int group_bytes) {
+        const int c = lane & 31, g = lane >> 5;
+#pragma unroll
+        for (int o = 0; o < 2; ++o) base[o] = (c >> 4) * group_bytes + chunk_at(c & 15, 2 * o + g);
+    }
+    __device__ __forceinline__ h8 read(const char * groups, int ks) const { return *reinterpret_cast<const h8 *>(groups + base[ks & 1] + (ks >> 1) * 1024); }
+};
+// V^T as a 32 x 16 operand: lane (row c: dim 32 dt + c, half g) gets keys 4 g .. 4 g + 3 and 8 + 4 g .. of one group - the order in which the result
+// of S^T holds its 16 keys
+struct v_frag {
+    int base[2];
+    __device__ __forceinline__ v_frag(int lane) {
+        const int g = lane >> 5, i16 = lane & 15, kk = i16 >> 2, jq = i16 & 3, x = 2 * ((lane >> 4) & 1) + (jq >> 1);
+#pragma unroll
+        for (int o = 0; o < 2; ++o) base[o] = chunk_at(4 * g + kk + 8 * o, x) + (jq & 1) * 8;
+    }
+    __device__ __forceinline__ h8 read(const char * grp, int dt) const {
+        const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4 __attribute__((address_space(3))) *) (grp + base[0] + dt * 1024));
+        const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4 __attribute__((address_space(3))) *) (grp + base[1] + dt * 1024));
+        const h4 a = __builtin_bit_cast(h4, lo), b = __builtin_bit_cast(h4, hi);
+        return h8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    }
+};
+
+__device__ __forceinline__ f16x mfma32(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+// row of value i of a lane (half g) of a 32 x 32 result
+__device__ __forceinline__ constexpr int mfma_row(int i, int g) { return 8 * (i >> 2) + 4 * g + (i & 3); }
+
+// 4 consecutive values of a row of q, as f32
+__device__ __forceinline__ f4 q4_at(const void * q, bool bf16, size_t i) {
+    if (!bf16) return *(const __attribute__((address_space(1))) f4 *) ((gbytes) q + 4 * i);
+    const u2w w = *(const __attribute__((address_space(1))) u2w *) ((gbytes) q + 2 * i);
+    return f4{__builtin_bit_cast(float, w[0] << 16), __builtin_bit_cast(float, w[0] & 0xffff0000u), __builtin_bit_cast(float, w[1] << 16), __builtin_bit_cast(float, w[1] & 0xffff0000u)};
+}
+// f32 -> bf16, to nearest, ties to even (a NaN stays one)
+__device__ __forceinline__ uint32_t bf16_of(float x) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    return x == x ? (u + 0x7fffu + ((u >> 16) & 1)) >> 16 : 0x7fc0u;
+}
+
+// host side (p1a_api.hip)
+struct chunk_args {
+    const void * q; void * out; const float * gate; float * lse;
+    bool q_bf16, out_bf16;
+    rows_view R;
+    int Hq, max_n;
+    float scale;
+    void * scratch; size_t scratch_bytes;
+};
+int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s);
+int chunk_splits(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus);
+int launch_mass(const p1a_kv & c, const void * q, bool q_bf16, const float * lse, float * mass, int ld, const rows_view & R, int Hq, float scale, int max_n, hipStream_t s);
+int launch_evict_select(const float * mass, int ld, int n_seq, int Hkv, const int32_t * n_dev, int n, int budget, int n_sink, int n_recent, int32_t * keep, hipStream_t s);
+int launch_kv_compact(const p1a_kv & c, const int32_t * keep, int n_seq, int budget, const float * mass, float * mass_out, int ld, hipStream_t s);
+
+}   // namespace p1a
