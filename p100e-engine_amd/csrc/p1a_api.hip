@@ -451,7 +451,7 @@ size_t p1a_attn_chunk_scratch_bytes(const p1a_kv * c, const p1a_rows * rows, int
     rows_view R;
     int max_n;
     if (rows_ok(c, rows, Hq, "p1a_attn_chunk_scratch_bytes", R, max_n) != P1A_OK || !rows->T || !rows->n_seq) return 0;
-    const size_t n = (size_t) R.T * Hq, k = (size_t) chunk_splits(*c, R, Hq, max_n, cu_count());
+    const size_t n = (size_t) R.T * Hq, k = (size_t) plan_chunk(*c, R, Hq, max_n, cu_count()).nks;
     return k > 1 ? ((n * k * 8 + 255) & ~(size_t) 255) + n * k * c->D * 4 : 0;
 }
 

@@ -17,39 +17,12 @@ namespace p1a {
 namespace {
 
 constexpr int BM = 128, NTHR = 256;
-constexpr float HEAD = 8.f, STEP = 6.f;                       // log2 of P at the row's maximum: HEAD when the reference moves, at most HEAD + STEP
-
-struct chunk_params {
-    const void * q;
-    void * out;
-    const float * gate;
-    float * lse;
-    const char * kc;
-    const char * vc;
-    kv_view pg;
-    rows_view R;
-    int Hq, Hkv, GQA;
-    uint32_t gqa_magic;    // floor(2^32 / GQA) (2^32 - 1 for GQA = 1)
-    float factor, sign;    // scores are factor * (sign q . k), in log2 units; factor > 0
-    int q_bf16, out_bf16;
-    int nks;               // workgroups of a block
-    float * part_o;        // [T * Hq][nks][D], relative to r
-    float * part_ml;       // [T * Hq][nks][2]: r, l
-};
 
 template <uint32_t KT, int D, bool EXACT> struct chunk_cfg {
     static constexpr int NPL = group_planes(KT, EXACT);
     static constexpr int BN = NPL == 2 && D >= 128 ? 32 : 64; // keys of a tile: 64 KB and less of LDS for K and V
     static constexpr int NG = BN / 16, G_B = NPL * plane_bytes(D), STAGE_B = 2 * NG * G_B;
 };
-
-__device__ __forceinline__ float gate_of(float g) { return 1.0f / (1.0f + expf(-g)); }
-// four results of a row, at element i of out
-__device__ __forceinline__ void put4(void * out, bool bf16, size_t i, f4 v) {
-    if (!bf16) *(__attribute__((address_space(1))) f4 *) ((__attribute__((address_space(1))) char *) out + 4 * i) = v;
-    else *(__attribute__((address_space(1))) u2w *) ((__attribute__((address_space(1))) char *) out + 2 * i) =
-        u2w{bf16_of(v[0]) | bf16_of(v[1]) << 16, bf16_of(v[2]) | bf16_of(v[3]) << 16};
-}
 
 template <uint32_t KT, int D, bool EXACT>
 __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_params P) {
@@ -351,17 +324,23 @@ long long block_bound(const rows_view & R, int GQA) {
 
 }   // namespace
 
-// Workgroups of a block, from the call's host numbers and the device: the count that minimises rounds of workgroups x (tiles of a workgroup + 3 for
-// its set-up and results), and 3 for a merge
-int chunk_splits(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus) {
-    const int GQA = Hq / c.Hkv, BN = 64;
-    const long long units = block_bound(R, GQA) * c.Hkv, slots = (long long) std::max(cus, 1) * (c.D <= 128 ? 2 : 1);
+// How a call is dealt out, from its host numbers and the device. Up to 32 rows of a sequence under a kv head take the kernel of p1a_step.hip. The
+// number of workgroups that share a block's keys minimises rounds of workgroups x (steps of a workgroup + 3 for its set-up and results) and 3 for a merge; a
+// step is 64 keys for blocks of rows and 128 for few rows.
+chunk_plan plan_chunk(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus) {
+    const int GQA = Hq / c.Hkv;
+    chunk_plan pl;
+    pl.few = (long long) R.max_rows * GQA <= 32 ? (R.max_rows * GQA + 15) / 16 : 0;
+    const int step = pl.few ? 128 : 64;
+    const bool two = c.D <= 128 || (pl.few && c.type != P1A_KV_F16 && pl.few == 1);   // two workgroups to a compute unit
+    const long long units = (pl.few ? R.n_seq : block_bound(R, GQA)) * c.Hkv, slots = (long long) std::max(cus, 1) * (two ? 2 : 1);
     const long long keys = R.window == INT32_MAX ? max_n : std::min<long long>(max_n, (long long) R.window + std::min(R.max_rows, BM / GQA + 1) + R.n_sink);
-    const long long nt = std::max<long long>(keys / BN, 1);
+    const long long nt = std::max<long long>((keys + step - 1) / step, 1);
     auto cost = [&](long long k) { return (units * k + slots - 1) / slots * ((nt + k - 1) / k + 3) + (k > 1 ? 3 : 0); };
     long long best = 1;
     for (long long k = 2; k <= 64 && k <= nt; ++k) if (cost(k) < cost(best)) best = k;
-    return (int) best;
+    pl.nks = (int) best;
+    return pl;
 }
 
 int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
@@ -373,7 +352,8 @@ int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
     P.factor = a.scale == 0.f ? 1.f : (a.scale < 0 ? -a.scale : a.scale) * LOG2E;
     P.sign = a.scale == 0.f ? 0.f : a.scale < 0 ? -1.f : 1.f;
     P.q_bf16 = a.q_bf16; P.out_bf16 = a.out_bf16;
-    P.nks = chunk_splits(c, a.R, a.Hq, a.max_n, cu_count());
+    const chunk_plan pl = plan_chunk(c, a.R, a.Hq, a.max_n, cu_count());
+    P.nks = pl.nks;
     P.part_o = P.part_ml = nullptr;
     const size_t rows = (size_t) a.R.T * a.Hq;
     if (P.nks > 1) {
@@ -386,7 +366,7 @@ int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
     const long long grid = block_bound(a.R, P.GQA) * P.nks * c.Hkv;
     if (grid > 0x7fffffffLL) { set_error("p1a_attn_chunk: too many rows for one call"); return P1A_E_SHAPE; }
     const bool exact = !a.out_bf16 || a.lse;
-    const int rc = c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, exact, (unsigned) grid, s)
+    const int rc = pl.few ? launch_step(c, P, pl.few, exact, s) : c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, exact, (unsigned) grid, s)
                  : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, exact, (unsigned) grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, exact, (unsigned) grid, s);
     if (rc != P1A_OK || P.nks == 1) return rc;
     const chunk_merge_params M{a.R, P.part_o, P.part_ml, a.gate, a.out, a.lse, a.Hq, c.D, P.nks, a.out_bf16};

@@ -1,0 +1,360 @@
+// Attention of few rows a sequence - single tokens, drafts to verify - over bounded caches: p1a_attn_chunk where a sequence's rows under a kv head are at
+// most 32, and so one or two tiles of 16 columns.
+//
+// Work: a workgroup of four waves owns a sequence's rows under one kv head and a share of their keys (nks shares); each wave walks tiles of 32 keys of its
+// own, 4 apart, nothing is shared and nothing waited for until the waves' results are folded at the end. (p1a_chunk.hip's blocks, whose waves
+// share tiles and split rows, would leave three waves of four idle here.)
+// Arithmetic: S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16. K is read straight into the operand; codes of quantized caches stay whole numbers,
+// exact in f16. K's scales multiply the fp32 result of a block; V's multiply P (fp32) ahead of the product, P d being what is cut into f16 halves. q and
+// P (P d) are two halves where results are f32, one where they are bf16 (EXACT). d enters as d / 2^E with E the largest exponent of a scale so far
+// - O is counted in 2^E - so that halves of P d do not end where f16 does.
+// V goes through LDS (16 keys of a dim lie in 16 rows): f16 straight there, two tiles a wave, codes through registers. While a tile's weights
+// and results are worked out the next one is on its way; its page-table entries were asked for ahead of the scores.
+// What bounds it: reading K and V.
+#include "p1a_tiles.hpp"
+
+#include <atomic>
+
+namespace p1a {
+namespace {
+
+constexpr int NW = 4, NTHR = NW * 64, PC = 8;                 // waves; columns folded at a time
+
+template <uint32_t KT, int D> struct step_cfg {
+    static constexpr bool F16 = KT == P1A_KV_F16;
+    static constexpr int VT_B = 2 * plane_bytes(D);           // 32 keys of V
+    static constexpr int V_B = (F16 ? 2 : 1) * VT_B;
+    static constexpr int TAB = keys16<KT, D>::TAB;
+    static constexpr int WAVE_B = V_B + 4 * TAB * 4;          // and the scales of 2 x 16 keys of K and V
+    static_assert(PC * (D + 4) * 4 <= V_B, "folded columns fit where V was");
+};
+
+template <uint32_t KT, int D, int NT, bool EXACT>
+__global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2) ? 1 : 2) step_k(const chunk_params P) {
+    using C = step_cfg<KT, D>;
+    using K = keys16<KT, D>;
+    using G = group<KT, D, C::F16 ? 1 : 0>;
+    constexpr bool F16 = C::F16;
+    constexpr int NB = D / 32, NDT = D / 16, NQ = EXACT ? 2 : 1, PL_B = plane_bytes(D);
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ float ml[NW][2][16 * NT];
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    // the kv heads of a sequence's share, whose rows have cache lines in common, on one XCD
+    const int xcd = blockIdx.x & 7, jx = blockIdx.x >> 3, hk = jx % P.Hkv, unit = jx / P.Hkv * 8 + xcd, seq = unit / P.nks, ksp = unit - seq * P.nks;
+    if (seq >= P.R.n_seq) return;
+    const seq_view sv = seq_of(P.R, seq);
+    const int R = min(sv.count * P.GQA, 16 * NT);
+    if (R < 1) return;
+    auto tok_of = [&](int r) {
+        const int t = (int) __umulhi((uint32_t) r, P.gqa_magic);
+        return r - t * P.GQA >= P.GQA ? t + 1 : t;
+    };
+    auto row_index = [&](int r) { const int t = tok_of(r); return (size_t) (sv.first + t) * P.Hq + (size_t) hk * P.GQA + (r - t * P.GQA); };
+    const span sp = span_of<32>(P.R, sv.pos0, sv.pos0 + sv.count - 1);
+    const int tps = ((sp.nt + P.nks - 1) / P.nks + NW - 1) / NW * NW, ta = min(ksp * tps, sp.nt), tb = min(ta + tps, sp.nt);
+    // positions that all rows see
+    const bool odd = sv.pos0 < 0 || sv.pos0 + sv.count > P.R.n_ctx;
+    const int all_hi = odd ? -1 : sv.pos0, all_lo = P.R.window == INT32_MAX ? 0 : sp.pmax - P.R.window + 1;
+
+    const int32_t * const ptab = P.pg.pt ? P.pg.pt + (P.pg.rtab ? P.pg.rtab[seq] : 0) : nullptr;
+    const size_t head_off = (size_t) hk * head_bytes(KT, D);
+    char * const mine = lds + wave * C::WAVE_B;
+    float * const tk = reinterpret_cast<float *>(mine + C::V_B), * const tv = tk + 2 * C::TAB;
+
+    auto pos_of = [&](int tile, int x) { return seen_or_near<32>(sp, tile * 32, tile * 32 + 16 * x + c); };
+    struct pages { int p[2]; };
+    auto pages_of = [&](int tile) {
+        pages r;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) r.p[x] = ptab ? ptab[pos_of(tile, x) >> P.pg.psh] : 0;
+        return r;
+    };
+    struct where { size_t off[2]; };                          // the rows of this lane's keys
+    auto where_is = [&](int tile, const pages & e) {
+        where r;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int j = pos_of(tile, x);
+            r.off[x] = head_off + (ptab ? (size_t) e.p[x] * P.pg.pstride + (size_t) (j & ((1 << P.pg.psh) - 1)) * P.pg.rowb : (size_t) j * P.pg.rowb);
+        }
+        return r;
+    };
+    typename K::raw kr[2];
+    typename K::scales vs[2];
+    struct none {};
+    typename std::conditional<F16, none, typename group<F16 ? P1A_KV_Q8_0 : KT, D, 0>::raw>::type vr[2];
+    auto ask_k = [&](const where & w) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) K::load(kr[x], (gbytes) P.kc + w.off[x], g);
+    };
+    auto ask_v = [&](const where & w, int st) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            if constexpr (F16) {                              // (this lane's part of the direct load belongs to another key)
+                const size_t off = __shfl((unsigned long long) w.off[x], G::key(lane));
+                G::load((gbytes) P.vc + off, mine + st * C::VT_B + x * PL_B, lane);
+            } else {
+                G::load(vr[x], (gbytes) P.vc + w.off[x], lane);
+                K::load_scales(vs[x], (gbytes) P.vc + w.off[x], g);
+            }
+        }
+    };
+
+    int i = ta + wave;
+    where at;
+    if (i < tb) {
+        at = where_is(sp.tile(i), pages_of(sp.tile(i)));
+        if constexpr (F16) ask_v(at, 0);
+        ask_k(at);
+    }
+
+    // ---- Q^T: columns 16 n + c ----
+    h8 qf[NT][NQ][NB];
+    float factor[NT];
+    int pos[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const int r = 16 * n + c, rr = min(r, R - 1);
+        factor[n] = ldexpf(P.factor, q_columns<KT, D, NQ>(P.q, P.q_bf16, row_index(rr), P.sign, g, qf[n]));
+        pos[n] = sv.pos0 + tok_of(rr);
+        if (pos[n] < 0 || pos[n] >= P.R.n_ctx) pos[n] = -1;   // sees nothing
+        __builtin_amdgcn_sched_barrier(0);
+    }
+
+    if constexpr (!F16) { if (i < tb) ask_v(at, 0); }         // (not ahead of Q: registers)
+
+    f4 o[NT][NDT];
+    float ref[NT], l[NT];
+    int E = -40;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        ref[n] = MINUS_INF;
+        l[n] = 0.f;
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) o[n][dt] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    int vbase[2];                                             // V^T operand: dims 16 dt + lane % 16, keys 4 g .. of a group; for even and odd dt
+    {
+        const int kk = c >> 2, jq = c & 3;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) vbase[e] = chunk_at(4 * g + kk, 2 * e + (jq >> 1)) + (jq & 1) * 8;
+    }
+    auto v_read = [&](const char * grp, int dt) {
+        return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4 __attribute__((address_space(3))) *) (grp + vbase[dt & 1] + (dt >> 1) * 1024)));
+    };
+
+    for (int st = 0; i < tb; i += NW, st ^= 1) {
+        const int k0 = sp.tile(i) * 32;
+        const bool more = i + NW < tb;
+        pages pg;
+        if (more) pg = pages_of(sp.tile(i + NW));
+        // ---- V's codes and the scales into LDS ----
+        if constexpr (!F16) {
+            float dm = 0.f;
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int y = 0; y < K::NSC; ++y) dm = fmaxf(dm, fabsf(K::scale(vs[x], y)));
+            dm = wave_max(dm);
+            const int e = __builtin_amdgcn_readfirstlane(dm > 0.f && dm < __builtin_inff() ? __builtin_amdgcn_frexp_expf(dm) : E);
+            if (e > E) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) o[n][dt][y] = ldexpf(o[n][dt][y], E - e);
+                E = e;
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                K::put(tk + x * C::TAB, kr[x].d, c, g);
+                K::put(tv + x * C::TAB, vs[x], c, g, -E);
+                G::store(vr[x], mine + x * PL_B, lane);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+        // ---- S^T ----
+        f4 s[2][NT];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) K::template scores<NT, NQ>(kr[x], qf, tk + x * C::TAB, g, s[x]);
+        // (V of this tile was asked for ahead of its K)
+        if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (more) {
+            const where at = where_is(sp.tile(i + NW), pg);
+            ask_v(at, st ^ 1);
+            ask_k(at);
+        }
+        // ---- softmax ----
+        if (!(k0 + 31 <= all_hi && k0 >= all_lo)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int hi = pos[n] - k0, lo = max(hi, 0) - P.R.window, sk = P.R.n_sink - k0;
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int j = 16 * x + 4 * g + e;
+                        s[x][n][e] = j <= hi && (j > lo || j < sk) ? s[x][n][e] : MINUS_INF;
+                    }
+            }
+        }
+        float p[NT][8];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            float mx = MINUS_INF;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = fmaxf(mx, s[e >> 2][n][e & 3]);
+            mx = max_swap32(max_swap16(mx)) * factor[n];
+            const bool fresh = ref[n] == MINUS_INF, move = mx > (fresh ? MINUS_INF : ref[n] + (HEAD + STEP));
+            if (__any(move)) {
+                const float to = move ? mx - HEAD : ref[n], alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(ref[n] - to);
+                ref[n] = to;
+                l[n] *= alpha;
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) o[n][dt] *= alpha;
+            }
+            const float nr = ref[n] == MINUS_INF ? 0.f : -ref[n];
+            float sum = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                p[n][e] = __builtin_amdgcn_exp2f(fmaf(s[e >> 2][n][e & 3], factor[n], nr));
+                sum += p[n][e];
+            }
+            l[n] += sum;
+        }
+        // ---- O^T += V^T (P d) ----
+        const char * const vt = mine + (F16 ? st * C::VT_B : 0);
+        h8 pb[NT][NQ];
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            f4 d[2];
+            if constexpr (!F16) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) d[x] = *reinterpret_cast<const f4 *>(tv + x * C::TAB + b * 16 + 4 * g);
+            }
+            if (!F16 || b == 0) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        const float w = F16 ? p[n][e] : p[n][e] * d[e >> 2][e & 3];
+                        pb[n][0][e] = (half_t) w;
+                        if constexpr (EXACT) pb[n][NQ - 1][e] = (half_t) (w - (float) (half_t) w);
+                    }
+                if constexpr (!F16 && D == 256) __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll
+            for (int dt = 2 * b; dt < 2 * b + 2; ++dt) {
+                const h4 a0 = v_read(vt, dt), a1 = v_read(vt + PL_B, dt);
+                const h8 a = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < NQ; ++k) o[n][dt] = mfma16(a, pb[n][k], o[n][dt]);
+            }
+        }
+    }
+
+    // ---- fold the waves, in wave order ----
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        l[n] += __shfl_xor(l[n], 16);
+        l[n] += __shfl_xor(l[n], 32);
+        if (g == 0) { ml[wave][0][16 * n + c] = ref[n]; ml[wave][1][16 * n + c] = l[n]; }
+    }
+    float * const parked = reinterpret_cast<float *>(mine);
+    constexpr int OS = D + 4, D4 = D / 4;
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int half = 0; half < 16; half += PC) {
+            const int h0 = 16 * n + half, he = min(h0 + PC, R);
+            if (h0 >= R) break;
+            if (h0) __syncthreads();
+            if (c >= half && c < half + PC) {
+#pragma unroll
+                for (int dt = 0; dt < NDT; ++dt) {
+                    f4 v = o[n][dt];
+                    if constexpr (!F16) {
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) v[y] = ldexpf(v[y], E);
+                    }
+                    *reinterpret_cast<f4 *>(parked + (c - half) * OS + 16 * dt + 4 * g) = v;
+                }
+            }
+            __syncthreads();
+            for (int t = tid; t < (he - h0) * D4; t += NTHR) {
+                const int cc = t / D4, d = 4 * (t - cc * D4), col = h0 + cc;
+                float m[NW], M = MINUS_INF, lt = 0.f;
+                f4 a[NW], acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    a[w] = *reinterpret_cast<const f4 *>(reinterpret_cast<const float *>(lds + w * C::WAVE_B) + cc * OS + d);
+                    m[w] = ml[w][0][col];
+                    M = fmaxf(M, m[w]);
+                }
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const float f = m[w] == MINUS_INF ? 0.f : __builtin_amdgcn_exp2f(m[w] - M);
+                    lt += ml[w][1][col] * f;
+                    acc += a[w] * f;
+                }
+                const size_t row = row_index(col);
+                if (P.nks > 1) {
+                    if (d == 0) {
+                        float * pm = P.part_ml + (row * P.nks + ksp) * 2;
+                        pm[0] = M;
+                        pm[1] = lt;
+                    }
+                    if (M != MINUS_INF) *reinterpret_cast<f4 *>(P.part_o + (row * P.nks + ksp) * D + d) = acc;
+                    continue;
+                }
+                if (P.lse && d == 0) P.lse[row] = M == MINUS_INF ? MINUS_INF : (M + log2f(lt)) * LN2;
+                f4 v = acc * (M == MINUS_INF ? 0.f : 1.0f / lt);
+                if (P.gate) {
+                    const f4 gt = *reinterpret_cast<const f4 *>(P.gate + row * D + d);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) v[y] *= gate_of(gt[y]);
+                }
+                put4(P.out, P.out_bf16, row * D + d, v);
+            }
+        }
+}
+
+template <uint32_t KT, int D, int NT, bool EXACT> int launch_cfg(const chunk_params & P, unsigned grid, hipStream_t s) {
+    constexpr int lds = NW * step_cfg<KT, D>::WAVE_B;
+    static std::atomic<uint32_t> attr_set{0};
+    int dev = 0;
+    (void) hipGetDevice(&dev);
+    const uint32_t bit = 1u << (dev & 31);
+    if (!(attr_set.load(std::memory_order_acquire) & bit)) {
+        if (hipFuncSetAttribute((const void *) step_k<KT, D, NT, EXACT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+            (void) hipGetLastError();
+            set_error("p1a_attn_chunk: cannot reserve %d bytes of LDS", lds);
+            return P1A_E_LAUNCH;
+        }
+        attr_set.fetch_or(bit, std::memory_order_release);
+    }
+    step_k<KT, D, NT, EXACT><<<grid, NTHR, lds, s>>>(P);
+    return launched();
+}
+template <uint32_t KT, int D> int launch_d(const chunk_params & P, int NT, bool exact, unsigned grid, hipStream_t s) {
+    if (NT == 1) return exact ? launch_cfg<KT, D, 1, true>(P, grid, s) : launch_cfg<KT, D, 1, false>(P, grid, s);
+    return exact ? launch_cfg<KT, D, 2, true>(P, grid, s) : launch_cfg<KT, D, 2, false>(P, grid, s);
+}
+template <uint32_t KT> int launch_kt(const chunk_params & P, int D, int NT, bool exact, unsigned grid, hipStream_t s) {
+    return D == 256 ? launch_d<KT, 256>(P, NT, exact, grid, s) : D == 128 ? launch_d<KT, 128>(P, NT, exact, grid, s) : launch_d<KT, 64>(P, NT, exact, grid, s);
+}
+
+}   // namespace
+
+int launch_step(const p1a_kv & c, const chunk_params & P, int NT, bool exact, hipStream_t s) {
+    const long long units = (long long) P.R.n_seq * P.nks, grid = (units + 7) / 8 * 8 * c.Hkv;
+    if (grid > 0x7fffffffLL) { set_error("p1a_attn_chunk: too many rows for one call"); return P1A_E_SHAPE; }
+    return c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, NT, exact, (unsigned) grid, s)
+         : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, NT, exact, (unsigned) grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, NT, exact, (unsigned) grid, s);
+}
+
+}   // namespace p1a

@@ -2,6 +2,8 @@
 #pragma once
 #include "p1a_common.hpp"
 
+#include <type_traits>
+
 namespace p1a {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
@@ -110,15 +112,23 @@ __device__ __forceinline__ int chunk_at(int key, int x) { return (x >> 2) * 1024
 
 // 4 codes in the bytes of w (biased so that byte - off is the code) times d: rounded to f16, and what the rounding left (exact: the product is a
 // multiple of 2^-24 of at most 18 bits)
+// NPL = 0: the code itself.
 template <int NPL> __device__ __forceinline__ void times4(uint32_t w, float off, h2 d, uint32_t * hi, uint32_t * lo) {
     const h2 o = {(half_t) off, (half_t) off};
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
         const h2 c = __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, k ? 0x04030402u : 0x04010400u)) - o;
-        const h2 p = c * d;
+        const h2 p = NPL == 0 ? c : c * d;
         hi[k] = __builtin_bit_cast(uint32_t, p);
         if constexpr (NPL == 2) lo[k] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c, d, -p));
     }
+}
+
+// ... the codes alone
+__device__ __forceinline__ void codes4(uint32_t w, float off, uint32_t * c) {
+    const h2 o = {(half_t) off, (half_t) off};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) c[k] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, __builtin_amdgcn_perm(0x64646464u, w, k ? 0x04030402u : 0x04010400u)) - o);
 }
 
 // A wave's part in filling one group: every lane stands for one key (row) of it
@@ -235,6 +245,7 @@ struct v_frag {
 };
 
 __device__ __forceinline__ f16x mfma32(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f4 mfma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 // row of value i of a lane (half g) of a 32 x 32 result
 __device__ __forceinline__ constexpr int mfma_row(int i, int g) { return 8 * (i >> 2) + 4 * g + (i & 3); }
 
@@ -250,6 +261,144 @@ __device__ __forceinline__ uint32_t bf16_of(float x) {
     return x == x ? (u + 0x7fffu + ((u >> 16) & 1)) >> 16 : 0x7fc0u;
 }
 
+// ---- 16 keys straight from memory as the rows of a 16 x 32 operand ----
+// Lane (key c = lane % 16, group g = lane / 16) reads the 8 values of each 32-dim block that it feeds to the products: 16, 8 or 4 bytes, 64, 32 or 16 on
+// end for a key. Codes enter as the whole numbers they are (exact in f16); a block's scale multiplies its fp32 result, from a table in LDS that
+// turns scales by key into scales by result (lane group g holds keys 4 g ..).
+template <uint32_t KT, int D> struct keys16 {
+    static constexpr bool F16 = KT == P1A_KV_F16, Q8 = KT == P1A_KV_Q8_0;
+    static constexpr int NB = D / 32, NSC = (NB + 3) / 4, SC = Q8 ? 2 : 18;   // blocks; scales a lane fetches; their distance
+    static constexpr int TAB = F16 ? 0 : NB * 16;             // floats of the table
+    typedef uint32_t u1_a2 __attribute__((aligned(2)));
+    static constexpr bool PAIRS = Q8 && NB == 8;              // two scales side by side in one load
+    struct scales { uint16_t s[F16 || PAIRS ? 1 : NSC]; uint32_t two; };
+    // the block of a lane's scale x (lanes without a block of their own repeat the last one)
+    static __device__ __forceinline__ int block(int x, int g) { return PAIRS ? 2 * g + x : min(4 * x + g, NB - 1); }
+    struct raw {
+        u4 w[F16 ? NB : 1];
+        u2w w8[Q8 ? NB : 1];
+        uint32_t w4[!F16 && !Q8 ? NB : 1];
+        scales d;
+    };
+    // dims of the 8 slots of lane group g in a block: two runs of four
+    static __device__ __forceinline__ int dims(int g, int half) { return F16 || Q8 ? 8 * g + 4 * half : 4 * g + 16 * half; }
+    static __device__ __forceinline__ void load_scales(scales & r, gbytes row, int g) {
+        if constexpr (PAIRS) r.two = gload<uint32_t>(row + 4 * g);
+        else if constexpr (!F16) {
+#pragma unroll
+            for (int x = 0; x < NSC; ++x) r.s[x] = gload<uint16_t>(row + block(x, g) * SC);
+        }
+    }
+    static __device__ __forceinline__ void load(raw & r, gbytes row, int g) {
+        load_scales(r.d, row, g);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            if constexpr (F16) r.w[b] = gload<u4>(row + 64 * b + 16 * g);
+            else if constexpr (Q8) r.w8[b] = gload<u2_a4>(row + 2 * NB + 32 * b + 8 * g);
+            else r.w4[b] = gload<u1_a2>(row + 18 * b + 2 + 4 * g);
+        }
+    }
+    static __device__ __forceinline__ float scale(const scales & r, int x) { return (float) (PAIRS ? __builtin_bit_cast(h2, r.two)[x & 1] : __builtin_bit_cast(half_t, r.s[PAIRS ? 0 : x])); }
+    static __device__ __forceinline__ void put(float * table, const scales & r, int c, int g, int shift = 0) {
+        if constexpr (!F16) {
+#pragma unroll
+            for (int x = 0; x < NSC; ++x) table[block(x, g) * 16 + c] = ldexpf(scale(r, x), shift);
+        }
+    }
+    static __device__ __forceinline__ h8 operand(const raw & r, int b) {
+        if constexpr (F16) return __builtin_bit_cast(h8, r.w[b]);
+        else {
+            uint32_t a[4];
+            if constexpr (Q8) {
+                codes4(r.w8[b][0] ^ 0x80808080u, 1152.f, a);
+                codes4(r.w8[b][1] ^ 0x80808080u, 1152.f, a + 2);
+            } else {
+                codes4(r.w4[b] & 0x0f0f0f0fu, 1032.f, a);
+                codes4((r.w4[b] >> 4) & 0x0f0f0f0fu, 1032.f, a + 2);
+            }
+            return __builtin_bit_cast(h8, u4{a[0], a[1], a[2], a[3]});
+        }
+    }
+    // S^T of the 16 keys and NT tiles of 16 columns: value i of lane (column c, group g) is key 4 g + i
+    template <int NT, int NQ> static __device__ __forceinline__ void scores(const raw & r, const h8 (&q)[NT][NQ][NB], const float * table, int g, f4 (&s)[NT]) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const h8 a = operand(r, b);
+            f4 d;
+            if constexpr (!F16) d = *reinterpret_cast<const f4 *>(table + b * 16 + 4 * g);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                f4 t = F16 ? s[n] : f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < NQ; ++k) t = mfma16(a, q[n][k][b], t);
+                if constexpr (F16) s[n] = t;
+                else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[n][i] = fmaf(t[i], d[i], s[n][i]);
+                    asm volatile("" : "+v"(s[n]));            // (here: put off behind the next branch, every block's t and d would stay in registers)
+                }
+            }
+        }
+    }
+};
+// 16 columns of q for it: lane (column c, group g). Returns the factor's exponent (the same in the column's four lanes)
+template <uint32_t KT, int D, int NQ> __device__ __forceinline__ int q_columns(const void * q, bool bf16, size_t row, float sign, int g, h8 (&qf)[NQ][D / 32]) {
+    constexpr int NB = D / 32;
+    f4 x[NB][2];
+    auto fetch = [&](auto as_bf16) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) x[b][e] = q4_at(q, as_bf16, row * D + 32 * b + keys16<KT, D>::dims(g, e));
+    };
+    if (bf16) fetch(std::true_type{});
+    else fetch(std::false_type{});
+    float most = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[b][e >> 2][e & 3]));
+    const int ex = row_exponent(max_swap32(max_swap16(most)));
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float y = ldexpf(x[b][e >> 2][e & 3] * sign, -ex);
+            qf[0][b][e] = (half_t) y;
+            if constexpr (NQ == 2) qf[NQ - 1][b][e] = (half_t) (y - (float) (half_t) y);
+        }
+    return ex;
+}
+
+// ---- attention of chunks: what its kernels share ----
+constexpr float HEAD = 8.f, STEP = 6.f;                       // log2 of P at the row's maximum: HEAD when the reference moves, at most HEAD + STEP
+struct chunk_params {
+    const void * q;
+    void * out;
+    const float * gate;
+    float * lse;
+    const char * kc;
+    const char * vc;
+    kv_view pg;
+    rows_view R;
+    int Hq, Hkv, GQA;
+    uint32_t gqa_magic;    // floor(2^32 / GQA) (2^32 - 1 for GQA = 1)
+    float factor, sign;    // scores are factor * (sign q . k), in log2 units; factor > 0
+    int q_bf16, out_bf16;
+    int nks;               // workgroups of a block
+    float * part_o;        // [T * Hq][nks][D], relative to r
+    float * part_ml;       // [T * Hq][nks][2]: r, l
+};
+__device__ __forceinline__ float gate_of(float g) { return 1.0f / (1.0f + expf(-g)); }
+// four results of a row, at element i of out
+__device__ __forceinline__ void put4(void * out, bool bf16, size_t i, f4 v) {
+    if (!bf16) *(__attribute__((address_space(1))) f4 *) ((__attribute__((address_space(1))) char *) out + 4 * i) = v;
+    else *(__attribute__((address_space(1))) u2w *) ((__attribute__((address_space(1))) char *) out + 2 * i) =
+        u2w{bf16_of(v[0]) | bf16_of(v[1]) << 16, bf16_of(v[2]) | bf16_of(v[3]) << 16};
+}
+
 // host side (p1a_api.hip)
 struct chunk_args {
     const void * q; void * out; const float * gate; float * lse;
@@ -260,7 +409,9 @@ struct chunk_args {
     void * scratch; size_t scratch_bytes;
 };
 int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s);
-int chunk_splits(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus);
+struct chunk_plan { int few, nks; };   // few: tiles of 16 columns that hold a sequence's rows (p1a_step.hip), or 0; workgroups that share the keys
+chunk_plan plan_chunk(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus);
+int launch_step(const p1a_kv & c, const chunk_params & P, int NT, bool exact, hipStream_t s);
 int launch_mass(const p1a_kv & c, const void * q, bool q_bf16, const float * lse, float * mass, int ld, const rows_view & R, int Hq, float scale, int max_n, hipStream_t s);
 int launch_evict_select(const float * mass, int ld, int n_seq, int Hkv, const int32_t * n_dev, int n, int budget, int n_sink, int n_recent, int32_t * keep, hipStream_t s);
 int launch_kv_compact(const p1a_kv & c, const int32_t * keep, int n_seq, int budget, const float * mass, float * mass_out, int ld, hipStream_t s);
