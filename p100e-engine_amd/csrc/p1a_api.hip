@@ -451,8 +451,8 @@ size_t p1a_attn_chunk_scratch_bytes(const p1a_kv * c, const p1a_rows * rows, int
     rows_view R;
     int max_n;
     if (rows_ok(c, rows, Hq, "p1a_attn_chunk_scratch_bytes", R, max_n) != P1A_OK || !rows->T || !rows->n_seq) return 0;
-    const size_t n = (size_t) R.T * Hq, k = (size_t) plan_chunk(*c, R, Hq, max_n, cu_count()).nks;
-    return k > 1 ? ((n * k * 8 + 255) & ~(size_t) 255) + n * k * c->D * 4 : 0;
+    const chunk_plan pl = plan_chunk(*c, R, Hq, max_n, cu_count());
+    return pl.bytes_n + pl.bytes_ml + pl.bytes_o;
 }
 
 int p1a_attn_mass(const void * q, int q_type, const p1a_kv * c, const float * lse, float * mass, int ld, const p1a_rows * rows, int Hq, float scale,

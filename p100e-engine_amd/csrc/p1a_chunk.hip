@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
     const int all_lo = all_hi < 0 || last_pos < 0 ? INT32_MAX : P.R.window == INT32_MAX ? 0 : max(last_pos - P.R.window + 1, 0);
 
     // ---- where rows of the cache are ----
-    const int32_t * const ptab = P.pg.pt ? P.pg.pt + (P.pg.rtab ? P.pg.rtab[at.seq] : 0) : nullptr;
+    const int32_t * const ptab = P.pg.pt ? P.pg.pt + (P.pg.rtab ? sload_i32(P.pg.rtab + at.seq) : 0) : nullptr;
     const size_t head_off = (size_t) hk * head_bytes(KT, D);
     // BN = 64: wave w fills group w of K and V; 32: groups 0 and 1 of K (waves 0, 1) and of V (waves 2, 3)
     constexpr bool BOTH = BN == 64;
@@ -253,27 +253,36 @@ struct chunk_merge_params {
     void * out;
     float * lse;
     int Hq, D, nks, out_bf16;
+    const int * part_n;    // few rows: partials that each sequence has (1: its rows are finished), or null: nks
 };
 __global__ void __launch_bounds__(NTHR) chunk_merge_k(const chunk_merge_params P) {
     const int tpr = P.D >> 2, sub = threadIdx.x / tpr, d = 4 * (threadIdx.x - sub * tpr);
     const long long row = (long long) blockIdx.x * (NTHR / tpr) + sub;
     if (row >= (long long) P.R.T * P.Hq) return;
+    const int t = (int) (row / P.Hq);
+    int a = 0, n = P.nks;
     if (P.R.row0) {                                           // the last sequence that starts at or ahead of the row's token
-        const int t = (int) (row / P.Hq);
-        int a = 0, b = P.R.n_seq;
+        int b = P.R.n_seq;
         while (b - a > 1) {
             const int m = (a + b) >> 1;
             if (P.R.row0[m] <= t) a = m; else b = m;
         }
         const seq_view v = seq_of(P.R, a);
         if (t < v.first || t >= v.first + v.count) return;    // (nobody's: left as it is)
+    } else {
+        a = t / P.R.per;
+        if (t - a * P.R.per >= P.R.max_rows) return;
+    }
+    if (P.part_n) {
+        n = min(P.part_n[a], P.nks);
+        if (n < 2) return;
     }
     const float2 * ml = reinterpret_cast<const float2 *>(P.part_ml) + row * P.nks;
     float M = MINUS_INF;
-    for (int k = 0; k < P.nks; ++k) M = fmaxf(M, ml[k].x);
+    for (int k = 0; k < n; ++k) M = fmaxf(M, ml[k].x);
     f4 acc = {0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
-    for (int k = 0; k < P.nks; ++k) {
+    for (int k = 0; k < n; ++k) {
         const float2 p = ml[k];
         if (p.x == MINUS_INF) continue;
         const float w = __builtin_amdgcn_exp2f(p.x - M);
@@ -324,22 +333,41 @@ long long block_bound(const rows_view & R, int GQA) {
 
 }   // namespace
 
-// How a call is dealt out, from its host numbers and the device. Up to 32 rows of a sequence under a kv head take the kernel of p1a_step.hip. The
-// number of workgroups that share a block's keys minimises rounds of workgroups x (steps of a workgroup + 3 for its set-up and results) and 3 for a merge; a
-// step is 64 keys for blocks of rows and 128 for few rows.
+// How a call is dealt out, from its host numbers and the device. Up to 32 rows of a sequence under a kv head take the kernel of p1a_step.hip.
+//   blocks of rows: the number of workgroups that share a block's keys minimises rounds of workgroups x (64-key tiles of a workgroup + 3 for its set-up and
+//     results), and 3 for a merge.
+//   few rows: as many runs of 128-key steps as there are places for workgroups, unless one for each sequence takes no longer than a run, its
+//     set-up (3), a second sequence's (2) and the merge (3). Partials stay within 64 MB: fewer runs to a sequence where there are many rows.
 chunk_plan plan_chunk(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus) {
     const int GQA = Hq / c.Hkv;
-    chunk_plan pl;
+    chunk_plan pl{};
     pl.few = (long long) R.max_rows * GQA <= 32 ? (R.max_rows * GQA + 15) / 16 : 0;
+    pl.runs = R.n_seq;
     const int step = pl.few ? 128 : 64;
-    const bool two = c.D <= 128 || (pl.few && c.type != P1A_KV_F16 && pl.few == 1);   // two workgroups to a compute unit
+    const bool two = c.D <= 128 || (pl.few == 1 && c.type != P1A_KV_F16);   // two workgroups to a compute unit
     const long long units = (pl.few ? R.n_seq : block_bound(R, GQA)) * c.Hkv, slots = (long long) std::max(cus, 1) * (two ? 2 : 1);
     const long long keys = R.window == INT32_MAX ? max_n : std::min<long long>(max_n, (long long) R.window + std::min(R.max_rows, BM / GQA + 1) + R.n_sink);
     const long long nt = std::max<long long>((keys + step - 1) / step, 1);
-    auto cost = [&](long long k) { return (units * k + slots - 1) / slots * ((nt + k - 1) / k + 3) + (k > 1 ? 3 : 0); };
-    long long best = 1;
-    for (long long k = 2; k <= 64 && k <= nt; ++k) if (cost(k) < cost(best)) best = k;
-    pl.nks = (int) best;
+    const size_t rows = (size_t) R.T * Hq, row_bytes = (size_t) c.D * 4 + 8;
+    if (pl.few) {
+        pl.nks = 1;
+        const long long runs = std::min(std::max(slots / c.Hkv, 1LL), R.n_seq * nt), per = (R.n_seq * nt + runs - 1) / runs;
+        const long long most = std::min({64LL, runs, nt + 1, std::max(2LL, (64LL << 20) / (long long) (rows * row_bytes))});
+        if (most > 1 && (units + slots - 1) / slots * (nt + 3) > std::max(per, (nt + most - 2) / (most - 1)) + 8) {
+            pl.runs = (int) runs;
+            pl.nks = (int) most;
+        }
+    } else {
+        auto cost = [&](long long k) { return (units * k + slots - 1) / slots * ((nt + k - 1) / k + 3) + (k > 1 ? 3 : 0); };
+        long long best = 1;
+        for (long long k = 2; k <= 64 && k <= nt; ++k) if (cost(k) < cost(best)) best = k;
+        pl.nks = (int) best;
+    }
+    if (pl.nks > 1) {
+        pl.bytes_n = pl.few ? ((size_t) R.n_seq * 4 + 255) & ~(size_t) 255 : 0;
+        pl.bytes_ml = (rows * pl.nks * 8 + 255) & ~(size_t) 255;
+        pl.bytes_o = rows * pl.nks * c.D * 4;
+    }
     return pl;
 }
 
@@ -353,15 +381,20 @@ int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
     P.sign = a.scale == 0.f ? 0.f : a.scale < 0 ? -1.f : 1.f;
     P.q_bf16 = a.q_bf16; P.out_bf16 = a.out_bf16;
     const chunk_plan pl = plan_chunk(c, a.R, a.Hq, a.max_n, cu_count());
-    P.nks = pl.nks;
-    P.part_o = P.part_ml = nullptr;
+    P.nks = pl.nks; P.runs = pl.runs;
+    P.part_o = P.part_ml = nullptr; P.part_n = nullptr;
     const size_t rows = (size_t) a.R.T * a.Hq;
     if (P.nks > 1) {
-        const size_t bm = (rows * P.nks * 8 + 255) & ~(size_t) 255, bo = rows * P.nks * c.D * 4;
-        if (a.scratch && !((uintptr_t) a.scratch & 255) && a.scratch_bytes >= bm + bo) {
-            P.part_ml = (float *) a.scratch;
-            P.part_o = (float *) ((char *) a.scratch + bm);
-        } else if (!split_scratch(s, bo, bm, P.part_o, P.part_ml)) return P1A_E_SCRATCH;
+        if (a.scratch && !((uintptr_t) a.scratch & 255) && a.scratch_bytes >= pl.bytes_n + pl.bytes_ml + pl.bytes_o) {
+            P.part_n = (int *) a.scratch;
+            P.part_ml = (float *) ((char *) a.scratch + pl.bytes_n);
+            P.part_o = (float *) ((char *) a.scratch + pl.bytes_n + pl.bytes_ml);
+        } else {
+            float * first;
+            if (!split_scratch(s, pl.bytes_o, pl.bytes_n + pl.bytes_ml, P.part_o, first)) return P1A_E_SCRATCH;
+            P.part_n = (int *) first;
+            P.part_ml = (float *) ((char *) first + pl.bytes_n);
+        }
     }
     const long long grid = block_bound(a.R, P.GQA) * P.nks * c.Hkv;
     if (grid > 0x7fffffffLL) { set_error("p1a_attn_chunk: too many rows for one call"); return P1A_E_SHAPE; }
@@ -369,7 +402,7 @@ int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
     const int rc = pl.few ? launch_step(c, P, pl.few, exact, s) : c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, exact, (unsigned) grid, s)
                  : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, exact, (unsigned) grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, exact, (unsigned) grid, s);
     if (rc != P1A_OK || P.nks == 1) return rc;
-    const chunk_merge_params M{a.R, P.part_o, P.part_ml, a.gate, a.out, a.lse, a.Hq, c.D, P.nks, a.out_bf16};
+    const chunk_merge_params M{a.R, P.part_o, P.part_ml, a.gate, a.out, a.lse, a.Hq, c.D, P.nks, a.out_bf16, pl.few ? P.part_n : nullptr};
     const size_t per = NTHR / (c.D / 4);
     chunk_merge_k<<<(unsigned) ((rows + per - 1) / per), NTHR, 0, s>>>(M);
     return launched();

@@ -47,10 +47,10 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) mass_k(const mass_para
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, g = lane >> 5;
     const int hk = blockIdx.x % P.Hkv, bx = blockIdx.x / P.Hkv, seq = blockIdx.y;
-    const seq_view sv = seq_of(P.R, seq);
+    const seq_view sv = seq_of<true>(P.R, seq);
     if (sv.count < 1) return;
     const span sp = span_of<32>(P.R, sv.pos0, sv.pos0 + sv.count - 1);   // tiles of 32 keys: a wave's NU are consecutive ones of the list
-    const int32_t * const ptab = P.pg.pt ? P.pg.pt + (P.pg.rtab ? P.pg.rtab[seq] : 0) : nullptr;
+    const int32_t * const ptab = P.pg.pt ? P.pg.pt + (P.pg.rtab ? sload_i32(P.pg.rtab + seq) : 0) : nullptr;
     const size_t head_off = (size_t) hk * head_bytes(KT, D);
     const int nrows = sv.count * P.GQA;
     auto tok_of = [&](int r) {

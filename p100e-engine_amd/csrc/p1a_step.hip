@@ -1,9 +1,11 @@
 // Attention of few rows a sequence - single tokens, drafts to verify - over bounded caches: p1a_attn_chunk where a sequence's rows under a kv head are at
 // most 32, and so one or two tiles of 16 columns.
 //
-// Work: a workgroup of four waves owns a sequence's rows under one kv head and a share of their keys (nks shares); each wave walks tiles of 32 keys of its
-// own, 4 apart, nothing is shared and nothing waited for until the waves' results are folded at the end. (p1a_chunk.hip's blocks, whose waves
-// share tiles and split rows, would leave three waves of four idle here.)
+// Work: steps of 128 keys, counted through over the sequences of a kv head; a workgroup of four waves takes a run of them, as long as every other
+// workgroup's - a sequence's end, the next one and its beginning, if need be. (Equal shares of every sequence: 32 sequences of 300 ... 32768 keys through a window
+// of 4096 left a third of the device idle at the end.) Within a sequence each wave walks tiles of 32 keys of its own, 4 apart; nothing is
+// shared and nothing waited for until the waves' results are folded. A sequence that lies in one run is finished there, the others' partials are
+// merged by chunk_merge_k. (p1a_chunk.hip's blocks, whose waves share tiles and split rows, would leave three waves of four idle here.)
 // Arithmetic: S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16. K is read straight into the operand; codes of quantized caches stay whole numbers,
 // exact in f16. K's scales multiply the fp32 result of a block; V's multiply P (fp32) ahead of the product, P d being what is cut into f16 halves. q and
 // P (P d) are two halves where results are f32, one where they are bf16 (EXACT). d enters as d / 2^E with E the largest exponent of a scale so far
@@ -20,47 +22,103 @@ namespace {
 
 constexpr int NW = 4, NTHR = NW * 64, PC = 8;                 // waves; columns folded at a time
 
-template <uint32_t KT, int D> struct step_cfg {
+template <uint32_t KT, int D, int NT, bool EXACT> struct step_cfg {
     static constexpr bool F16 = KT == P1A_KV_F16;
     static constexpr int VT_B = 2 * plane_bytes(D);           // 32 keys of V
     static constexpr int V_B = (F16 ? 2 : 1) * VT_B;
     static constexpr int TAB = keys16<KT, D>::TAB;
     static constexpr int WAVE_B = V_B + 4 * TAB * 4;          // and the scales of 2 x 16 keys of K and V
+    // (the low halves of q, where registers do not hold them: the same for every wave, each writes all of them)
+    static constexpr bool QL = !F16 && EXACT && NT * D >= 256;
+    static constexpr int ML_B = NW * 2 * 16 * NT * 4, LDS = NW * WAVE_B + (QL ? NT * D * 32 : 0) + (4 * TAB * 4 >= ML_B ? 0 : ML_B);
+    static constexpr int ML_AT = 4 * TAB * 4 >= ML_B ? V_B : LDS - ML_B;      // (the first wave's scales are done with by then)
     static_assert(PC * (D + 4) * 4 <= V_B, "folded columns fit where V was");
 };
 
 template <uint32_t KT, int D, int NT, bool EXACT>
 __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2) ? 1 : 2) step_k(const chunk_params P) {
-    using C = step_cfg<KT, D>;
+    using C = step_cfg<KT, D, NT, EXACT>;
     using K = keys16<KT, D>;
     using G = group<KT, D, C::F16 ? 1 : 0>;
     constexpr bool F16 = C::F16;
     constexpr int NB = D / 32, NDT = D / 16, NQ = EXACT ? 2 : 1, PL_B = plane_bytes(D);
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    __shared__ float ml[NW][2][16 * NT];
 
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    // the kv heads of a sequence's share, whose rows have cache lines in common, on one XCD
-    const int xcd = blockIdx.x & 7, jx = blockIdx.x >> 3, hk = jx % P.Hkv, unit = jx / P.Hkv * 8 + xcd, seq = unit / P.nks, ksp = unit - seq * P.nks;
-    if (seq >= P.R.n_seq) return;
-    const seq_view sv = seq_of(P.R, seq);
-    const int R = min(sv.count * P.GQA, 16 * NT);
-    if (R < 1) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // the kv heads of a run of steps, whose rows have cache lines in common, on one XCD
+    const int xcd = blockIdx.x & 7, jx = blockIdx.x >> 3, hk = jx % P.Hkv, run = jx / P.Hkv * 8 + xcd;
+    if (run >= P.runs) return;
     auto tok_of = [&](int r) {
         const int t = (int) __umulhi((uint32_t) r, P.gqa_magic);
         return r - t * P.GQA >= P.GQA ? t + 1 : t;
     };
+    auto span_of_rows = [&](const seq_view & v) { return span_of<32>(P.R, v.pos0, v.pos0 + v.count - 1); };
+    // ---- this workgroup's steps: first .. end - 1 of all sequences' ----
+    // lane i of a wave counts the steps of sequence s0 + i; a sequence with rows has one at least (its rows' results)
+    auto steps_of = [&](int s) {
+        if (s >= P.R.n_seq) return 0;
+        const seq_view v = seq_of(P.R, s);
+        return v.count < 1 ? 0 : max((span_of_rows(v).nt + NW - 1) / NW, 1);
+    };
+    const int steps64 = steps_of(threadIdx.x & 63);                       // of the first 64
+    int first, end, per = 1 << 30;
+    if (P.nks > 1) {
+        int n = 0, most = 0;
+        for (int s0 = 0; s0 < P.R.n_seq; s0 += 64) {
+            const int x = s0 ? steps_of(s0 + (threadIdx.x & 63)) : steps64;
+            n += __builtin_amdgcn_readlane(lanes_up_to(x), 63);
+            most = max(most, x);
+        }
+        most = (int) wave_max((float) most);                  // (2^24 steps at most: exact)
+        most = rfl(most);
+        per = max((n + P.runs - 1) / P.runs, (most + P.nks - 2) / (P.nks - 1));   // (no sequence in more than nks runs)
+        first = run * per;
+        end = min(first + per, n);
+        if (first >= end) return;
+    } else {                                                  // a sequence each
+        first = 0;
+        end = steps_of(run);
+        if (end < 1) return;
+    }
+    char * const mine = lds + wave * C::WAVE_B;
+    float * const tk = reinterpret_cast<float *>(mine + C::V_B), * const tv = tk + 2 * C::TAB;
+    const size_t head_off = (size_t) hk * head_bytes(KT, D);
+
+  for (int at_step = first; at_step < end;) {
+    // (the lane's number anew for each sequence, and once more for the fold: what follows from it would be worked out ahead of the loop and kept, 40 registers)
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, c = lane & 15, g = lane >> 4;
+    // whose step that is
+    int seq = run, s_first = 0, s_steps = end;
+    if (P.nks > 1) {
+        int base = 0;
+        for (int s0 = 0;; s0 += 64) {                         // (there is one: at_step < n)
+            const int x = s0 ? steps_of(s0 + lane) : steps64, u = base + lanes_up_to(x);
+            const unsigned long long behind = __ballot(u > at_step);
+            if (behind) {
+                const int l = __builtin_ctzll(behind);
+                seq = s0 + l;
+                s_steps = __builtin_amdgcn_readlane(x, l);
+                s_first = __builtin_amdgcn_readlane(u, l) - s_steps;
+                break;
+            }
+            base = __builtin_amdgcn_readlane(u, 63);
+        }
+    }
+    // its runs, which of them this is, and the tiles of this one
+    const int run0 = s_first / per, pieces = P.nks > 1 ? (s_first + s_steps - 1) / per - run0 + 1 : 1, piece = P.nks > 1 ? run - run0 : 0;
+    const seq_view sv = seq_of<true>(P.R, seq);
+    const int R = min(sv.count * P.GQA, 16 * NT);
     auto row_index = [&](int r) { const int t = tok_of(r); return (size_t) (sv.first + t) * P.Hq + (size_t) hk * P.GQA + (r - t * P.GQA); };
-    const span sp = span_of<32>(P.R, sv.pos0, sv.pos0 + sv.count - 1);
-    const int tps = ((sp.nt + P.nks - 1) / P.nks + NW - 1) / NW * NW, ta = min(ksp * tps, sp.nt), tb = min(ta + tps, sp.nt);
+    const span sp = span_of_rows(sv);
+    const int ta = (at_step - s_first) * NW, tb = min((min(end, s_first + s_steps) - s_first) * NW, sp.nt);
+    at_step = s_first + s_steps;
     // positions that all rows see
     const bool odd = sv.pos0 < 0 || sv.pos0 + sv.count > P.R.n_ctx;
     const int all_hi = odd ? -1 : sv.pos0, all_lo = P.R.window == INT32_MAX ? 0 : sp.pmax - P.R.window + 1;
 
-    const int32_t * const ptab = P.pg.pt ? P.pg.pt + (P.pg.rtab ? P.pg.rtab[seq] : 0) : nullptr;
-    const size_t head_off = (size_t) hk * head_bytes(KT, D);
-    char * const mine = lds + wave * C::WAVE_B;
-    float * const tk = reinterpret_cast<float *>(mine + C::V_B), * const tv = tk + 2 * C::TAB;
+    const int32_t * const ptab = P.pg.pt ? P.pg.pt + (P.pg.rtab ? sload_i32(P.pg.rtab + seq) : 0) : nullptr;
 
     auto pos_of = [&](int tile, int x) { return seen_or_near<32>(sp, tile * 32, tile * 32 + 16 * x + c); };
     struct pages { int p[2]; };
@@ -79,6 +137,15 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
             r.off[x] = head_off + (ptab ? (size_t) e.p[x] * P.pg.pstride + (size_t) (j & ((1 << P.pg.psh) - 1)) * P.pg.rowb : (size_t) j * P.pg.rowb);
         }
         return r;
+    };
+    int vbase[2];                                             // V^T operand: dims 16 dt + lane % 16, keys 4 g .. of a group; for even and odd dt
+    {
+        const int kk = c >> 2, jq = c & 3;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) vbase[e] = chunk_at(4 * g + kk, 2 * e + (jq >> 1)) + (jq & 1) * 8;
+    }
+    auto v_read = [&](const char * grp, int dt) {
+        return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4 __attribute__((address_space(3))) *) (grp + vbase[dt & 1] + (dt >> 1) * 1024)));
     };
     typename K::raw kr[2];
     typename K::scales vs[2];
@@ -106,23 +173,36 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
     if (i < tb) {
         at = where_is(sp.tile(i), pages_of(sp.tile(i)));
         if constexpr (F16) ask_v(at, 0);
-        ask_k(at);
+        if constexpr (F16 || NT * D <= 128) ask_k(at);
     }
 
     // ---- Q^T: columns 16 n + c ----
-    h8 qf[NT][NQ][NB];
+    constexpr int NQR = C::QL ? 1 : NQ;                       // halves in registers
+    h8 qf[NT][NQR][NB];
+    char * const ql = lds + NW * C::WAVE_B + lane * 16;
+    auto q_at = [&](int n, int k, int b) { return k < NQR ? qf[n][k < NQR ? k : 0][b] : *reinterpret_cast<const h8 *>(ql + (n * NB + b) * 1024); };
     float factor[NT];
     int pos[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const int r = 16 * n + c, rr = min(r, R - 1);
-        factor[n] = ldexpf(P.factor, q_columns<KT, D, NQ>(P.q, P.q_bf16, row_index(rr), P.sign, g, qf[n]));
+        h8 qq[NQ][NB];
+        factor[n] = ldexpf(P.factor, q_columns<KT, D, NQ>(P.q, P.q_bf16, row_index(rr), P.sign, g, qq));
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+#pragma unroll
+            for (int k = 0; k < NQR; ++k) qf[n][k][b] = qq[k][b];
+            if constexpr (C::QL) *reinterpret_cast<h8 *>(ql + (n * NB + b) * 1024) = qq[NQ - 1][b];
+        }
         pos[n] = sv.pos0 + tok_of(rr);
         if (pos[n] < 0 || pos[n] >= P.R.n_ctx) pos[n] = -1;   // sees nothing
         __builtin_amdgcn_sched_barrier(0);
     }
 
-    if constexpr (!F16) { if (i < tb) ask_v(at, 0); }         // (not ahead of Q: registers)
+    if (i < tb) {                                             // (what registers hold not ahead of Q)
+        if constexpr (!F16) ask_v(at, 0);
+        if constexpr (!F16 && NT * D > 128) ask_k(at);
+    }
 
     f4 o[NT][NDT];
     float ref[NT], l[NT];
@@ -134,16 +214,6 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) o[n][dt] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    int vbase[2];                                             // V^T operand: dims 16 dt + lane % 16, keys 4 g .. of a group; for even and odd dt
-    {
-        const int kk = c >> 2, jq = c & 3;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) vbase[e] = chunk_at(4 * g + kk, 2 * e + (jq >> 1)) + (jq & 1) * 8;
-    }
-    auto v_read = [&](const char * grp, int dt) {
-        return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4 __attribute__((address_space(3))) *) (grp + vbase[dt & 1] + (dt >> 1) * 1024)));
-    };
-
     for (int st = 0; i < tb; i += NW, st ^= 1) {
         const int k0 = sp.tile(i) * 32;
         const bool more = i + NW < tb;
@@ -178,7 +248,7 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
         // ---- S^T ----
         f4 s[2][NT];
 #pragma unroll
-        for (int x = 0; x < 2; ++x) K::template scores<NT, NQ>(kr[x], qf, tk + x * C::TAB, g, s[x]);
+        for (int x = 0; x < 2; ++x) K::template scores<NT, NQ>(kr[x], q_at, tk + x * C::TAB, g, s[x]);
         // (V of this tile was asked for ahead of its K)
         if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (more) {
@@ -258,11 +328,16 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
     }
 
     // ---- fold the waves, in wave order ----
+    {
+    asm volatile("" : "+v"(tid));
+    const int c = tid & 15, g = (tid >> 4) & 3;
+    auto ml = [&](int w, int which, int col) -> float & { return reinterpret_cast<float *>(lds + C::ML_AT)[(w * 2 + which) * 16 * NT + col]; };
+    if constexpr (C::ML_AT < C::WAVE_B) __syncthreads();      // (until the first wave has done with them)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         l[n] += __shfl_xor(l[n], 16);
         l[n] += __shfl_xor(l[n], 32);
-        if (g == 0) { ml[wave][0][16 * n + c] = ref[n]; ml[wave][1][16 * n + c] = l[n]; }
+        if (g == 0) { ml(wave, 0, 16 * n + c) = ref[n]; ml(wave, 1, 16 * n + c) = l[n]; }
     }
     float * const parked = reinterpret_cast<float *>(mine);
     constexpr int OS = D + 4, D4 = D / 4;
@@ -292,23 +367,23 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
 #pragma unroll
                 for (int w = 0; w < NW; ++w) {
                     a[w] = *reinterpret_cast<const f4 *>(reinterpret_cast<const float *>(lds + w * C::WAVE_B) + cc * OS + d);
-                    m[w] = ml[w][0][col];
+                    m[w] = ml(w, 0, col);
                     M = fmaxf(M, m[w]);
                 }
 #pragma unroll
                 for (int w = 0; w < NW; ++w) {
                     const float f = m[w] == MINUS_INF ? 0.f : __builtin_amdgcn_exp2f(m[w] - M);
-                    lt += ml[w][1][col] * f;
+                    lt += ml(w, 1, col) * f;
                     acc += a[w] * f;
                 }
                 const size_t row = row_index(col);
-                if (P.nks > 1) {
+                if (pieces > 1) {
                     if (d == 0) {
-                        float * pm = P.part_ml + (row * P.nks + ksp) * 2;
+                        float * pm = P.part_ml + (row * P.nks + piece) * 2;
                         pm[0] = M;
                         pm[1] = lt;
                     }
-                    if (M != MINUS_INF) *reinterpret_cast<f4 *>(P.part_o + (row * P.nks + ksp) * D + d) = acc;
+                    if (M != MINUS_INF) *reinterpret_cast<f4 *>(P.part_o + (row * P.nks + piece) * D + d) = acc;
                     continue;
                 }
                 if (P.lse && d == 0) P.lse[row] = M == MINUS_INF ? MINUS_INF : (M + log2f(lt)) * LN2;
@@ -321,10 +396,14 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
                 put4(P.out, P.out_bf16, row * D + d, v);
             }
         }
+    }
+    if (P.nks > 1 && piece == 0 && hk == 0 && tid == 0) P.part_n[seq] = pieces;
+    __syncthreads();                                          // (what was folded is read; the next sequence's V goes there)
+  }
 }
 
 template <uint32_t KT, int D, int NT, bool EXACT> int launch_cfg(const chunk_params & P, unsigned grid, hipStream_t s) {
-    constexpr int lds = NW * step_cfg<KT, D>::WAVE_B;
+    constexpr int lds = step_cfg<KT, D, NT, EXACT>::LDS;
     static std::atomic<uint32_t> attr_set{0};
     int dev = 0;
     (void) hipGetDevice(&dev);
@@ -351,7 +430,7 @@ template <uint32_t KT> int launch_kt(const chunk_params & P, int D, int NT, bool
 }   // namespace
 
 int launch_step(const p1a_kv & c, const chunk_params & P, int NT, bool exact, hipStream_t s) {
-    const long long units = (long long) P.R.n_seq * P.nks, grid = (units + 7) / 8 * 8 * c.Hkv;
+    const long long grid = (P.runs + 7LL) / 8 * 8 * c.Hkv;
     if (grid > 0x7fffffffLL) { set_error("p1a_attn_chunk: too many rows for one call"); return P1A_E_SHAPE; }
     return c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, NT, exact, (unsigned) grid, s)
          : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, NT, exact, (unsigned) grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, NT, exact, (unsigned) grid, s);

@@ -18,12 +18,24 @@ struct rows_view {
 };
 struct seq_view { int first, count, pos0; };   // rows first .. first + count - 1, the first of them at position pos0
 // (whatever the device arrays hold: rows inside 0 .. T, positions where adding a row to one does not overflow)
-__device__ __forceinline__ seq_view seq_of(const rows_view & R, int s) {
+// (UNIFORM: every lane asks for the same sequence - scalar loads, and what follows from them stays in scalar registers)
+template <bool UNIFORM = false> __device__ __forceinline__ seq_view seq_of(const rows_view & R, int s) {
+    auto at = [](const int32_t * p) { return UNIFORM ? sload_i32(p) : *p; };
     seq_view v;
-    v.first = R.row0 ? min(max(R.row0[s], 0), R.T) : s * R.per;
-    v.count = min(R.row0 ? max(min(R.row0[s + 1], R.T) - v.first, 0) : R.per, R.max_rows);
-    v.pos0 = min(max(R.pos0 ? R.pos0[s] : R.p0, -(1 << 30)), R.n_ctx);
+    v.first = R.row0 ? min(max(at(R.row0 + s), 0), R.T) : s * R.per;
+    v.count = min(R.row0 ? max(min(at(R.row0 + s + 1), R.T) - v.first, 0) : R.per, R.max_rows);
+    v.pos0 = min(max(R.pos0 ? at(R.pos0 + s) : R.p0, -(1 << 30)), R.n_ctx);
     return v;
+}
+// sums over the lanes up to this one
+__device__ __forceinline__ int lanes_up_to(int u) {
+    u += __builtin_amdgcn_update_dpp(0, u, 0x111, 0xf, 0xf, true);
+    u += __builtin_amdgcn_update_dpp(0, u, 0x112, 0xf, 0xf, true);
+    u += __builtin_amdgcn_update_dpp(0, u, 0x114, 0xf, 0xf, true);
+    u += __builtin_amdgcn_update_dpp(0, u, 0x118, 0xf, 0xf, true);
+    u += __builtin_amdgcn_update_dpp(0, u, 0x142, 0xa, 0xf, false);
+    u += __builtin_amdgcn_update_dpp(0, u, 0x143, 0xc, 0xf, false);
+    return u;
 }
 // Item b of a list that holds ceil(count * mul / unit) items of each sequence, in order: whose it is, and which of them; false: there are fewer.
 // Every lane of the wave calls, with the same b.
@@ -34,26 +46,20 @@ __device__ __forceinline__ bool find_item(const rows_view & R, int b, int mul, i
         at.seq = b / at.of;
         at.index = b - at.seq * at.of;
         if (at.seq >= R.n_seq) return false;
-        at.v = seq_of(R, at.seq);
+        at.v = seq_of<true>(R, at.seq);
         return true;
     }
     for (int s0 = 0; s0 < R.n_seq; s0 += 64) {
         const int s = s0 + lane;
         const int n = s < R.n_seq ? (int) (((long long) seq_of(R, s).count * mul + unit - 1) / unit) : 0;
-        int u = n;                                             // sums over the lanes up to this one
-        u += __builtin_amdgcn_update_dpp(0, u, 0x111, 0xf, 0xf, true);
-        u += __builtin_amdgcn_update_dpp(0, u, 0x112, 0xf, 0xf, true);
-        u += __builtin_amdgcn_update_dpp(0, u, 0x114, 0xf, 0xf, true);
-        u += __builtin_amdgcn_update_dpp(0, u, 0x118, 0xf, 0xf, true);
-        u += __builtin_amdgcn_update_dpp(0, u, 0x142, 0xa, 0xf, false);
-        u += __builtin_amdgcn_update_dpp(0, u, 0x143, 0xc, 0xf, false);
+        const int u = lanes_up_to(n);
         const unsigned long long behind = __ballot(u > b);
         if (behind) {
             const int l = __builtin_ctzll(behind);
             at.seq = s0 + l;
             at.of = __builtin_amdgcn_readlane(n, l);
             at.index = b - (__builtin_amdgcn_readlane(u, l) - at.of);
-            at.v = seq_of(R, at.seq);
+            at.v = seq_of<true>(R, at.seq);
             return true;
         }
         b -= __builtin_amdgcn_readlane(u, 63);
@@ -319,8 +325,8 @@ template <uint32_t KT, int D> struct keys16 {
             return __builtin_bit_cast(h8, u4{a[0], a[1], a[2], a[3]});
         }
     }
-    // S^T of the 16 keys and NT tiles of 16 columns: value i of lane (column c, group g) is key 4 g + i
-    template <int NT, int NQ> static __device__ __forceinline__ void scores(const raw & r, const h8 (&q)[NT][NQ][NB], const float * table, int g, f4 (&s)[NT]) {
+    // S^T of the 16 keys and NT tiles of 16 columns: value i of lane (column c, group g) is key 4 g + i. q(n, k, b): half k of block b of tile n's operand
+    template <int NT, int NQ, class Q> static __device__ __forceinline__ void scores(const raw & r, Q && q, const float * table, int g, f4 (&s)[NT]) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) s[n] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -332,7 +338,7 @@ template <uint32_t KT, int D> struct keys16 {
             for (int n = 0; n < NT; ++n) {
                 f4 t = F16 ? s[n] : f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int k = 0; k < NQ; ++k) t = mfma16(a, q[n][k][b], t);
+                for (int k = 0; k < NQ; ++k) t = mfma16(a, q(n, k, b), t);
                 if constexpr (F16) s[n] = t;
                 else {
 #pragma unroll
@@ -387,7 +393,9 @@ struct chunk_params {
     uint32_t gqa_magic;    // floor(2^32 / GQA) (2^32 - 1 for GQA = 1)
     float factor, sign;    // scores are factor * (sign q . k), in log2 units; factor > 0
     int q_bf16, out_bf16;
-    int nks;               // workgroups of a block
+    int nks;               // partials of a row: workgroups of a block, or the most runs that a sequence of few rows may lie in
+    int runs;              // few rows: workgroups of a kv head
+    int * part_n;          // few rows: [n_seq] runs that the sequence lies in
     float * part_o;        // [T * Hq][nks][D], relative to r
     float * part_ml;       // [T * Hq][nks][2]: r, l
 };
@@ -409,7 +417,11 @@ struct chunk_args {
     void * scratch; size_t scratch_bytes;
 };
 int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s);
-struct chunk_plan { int few, nks; };   // few: tiles of 16 columns that hold a sequence's rows (p1a_step.hip), or 0; workgroups that share the keys
+struct chunk_plan {
+    int few;                           // tiles of 16 columns that hold a sequence's rows under a kv head (p1a_step.hip), or 0
+    int nks, runs;                     // as in chunk_params
+    size_t bytes_n, bytes_ml, bytes_o; // scratch (0: no partials), in this order
+};
 chunk_plan plan_chunk(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus);
 int launch_step(const p1a_kv & c, const chunk_params & P, int NT, bool exact, hipStream_t s);
 int launch_mass(const p1a_kv & c, const void * q, bool q_bf16, const float * lse, float * mass, int ld, const rows_view & R, int Hq, float scale, int max_n, hipStream_t s);
