@@ -91,14 +91,14 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
             }
         const int ex = row_exponent(max_swap32(most));
         factor = ldexpf(factor, ex);
+        const float by = ldexpf(P.sign, -ex);
 #pragma unroll
-        for (int ks = 0; ks < NKS; ++ks)
+        for (int ks = 0; ks < NKS; ++ks) {
+            h8 r[NQ];
+            halves<NQ>([&](int e) { return x[ks][e >> 2][e & 3]; }, [&](int) { return by; }, r);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float y = live ? ldexpf(x[ks][e >> 2][e & 3] * P.sign, -ex) : 0.f;
-                qf[0][ks][e] = (half_t) y;
-                if constexpr (EXACT) qf[NQ - 1][ks][e] = (half_t) (y - (float) (half_t) y);
-            }
+            for (int k = 0; k < NQ; ++k) qf[k][ks] = r[k];
+        }
     }
 
     f16x o[NDT];
@@ -277,17 +277,35 @@ __global__ void __launch_bounds__(NTHR) chunk_merge_k(const chunk_merge_params P
         n = min(P.part_n[a], P.nks);
         if (n < 2) return;
     }
+    // four partials at a time, asked for together
     const float2 * ml = reinterpret_cast<const float2 *>(P.part_ml) + row * P.nks;
-    float M = MINUS_INF;
-    for (int k = 0; k < n; ++k) M = fmaxf(M, ml[k].x);
+    const float * po = P.part_o + row * P.nks * P.D + d;
+    float M = MINUS_INF, l = 0.f;
     f4 acc = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    for (int k = 0; k < n; ++k) {
-        const float2 p = ml[k];
-        if (p.x == MINUS_INF) continue;
-        const float w = __builtin_amdgcn_exp2f(p.x - M);
-        l += p.y * w;
-        acc += *reinterpret_cast<const f4 *>(P.part_o + (row * P.nks + k) * P.D + d) * w;
+    for (int k0 = 0; k0 < n; k0 += 4) {
+        float2 p[4];
+        f4 v[4];
+        float m = M;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int kk = min(k0 + k, n - 1);
+            p[k] = ml[kk];
+            v[k] = *reinterpret_cast<const f4 *>(po + (size_t) kk * P.D);
+            if (k0 + k >= n) p[k].x = MINUS_INF;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = fmaxf(m, p[k].x);
+        const float w0 = M == MINUS_INF ? 0.f : __builtin_amdgcn_exp2f(M - m);
+        l *= w0;
+        acc *= w0;
+        M = m;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (p[k].x == MINUS_INF) continue;                // (it has seen nothing, and written no values)
+            const float w = __builtin_amdgcn_exp2f(p[k].x - M);
+            l += p[k].y * w;
+            acc += v[k] * w;
+        }
     }
     if (P.lse && d == 0) P.lse[row] = M == MINUS_INF ? MINUS_INF : (M + log2f(l)) * LN2;
     f4 v = acc * (M == MINUS_INF ? 0.f : 1.0f / l);

@@ -83,19 +83,15 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) mass_k(const mass_para
         most = fmaxf(most, __shfl_xor(most, 8));
         most = max_swap32(max_swap16(most));
         const int ex = row_exponent(most);
+        const float by = ldexpf(P.sign, -ex);
         char * const to = lds + st * C::Q_B + (qrow >> 4) * PL_B;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            h8 hi, lo;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float y = ldexpf(r.x[j][e >> 2][e & 3] * P.sign, -ex);
-                hi[e] = (half_t) y;
-                lo[e] = (half_t) (y - (float) (half_t) y);
-            }
+            h8 y[2];
+            halves<2>([&](int e) { return r.x[j][e >> 2][e & 3]; }, [&](int) { return by; }, y);
             char * const at = to + chunk_at(qrow & 15, 8 * j + (lane >> 3));
-            *reinterpret_cast<h8 *>(at) = hi;
-            *reinterpret_cast<h8 *>(at + 2 * PL_B) = lo;
+            *reinterpret_cast<h8 *>(at) = y[0];
+            *reinterpret_cast<h8 *>(at + 2 * PL_B) = y[1];
         }
         if (lane < 8) info[st * QR + qrow] = row_info{ldexpf(P.factor, ex), -r.lse * LOG2E, r.pos};
     };

@@ -55,17 +55,24 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
     auto span_of_rows = [&](const seq_view & v) { return span_of<32>(P.R, v.pos0, v.pos0 + v.count - 1); };
     // ---- this workgroup's steps: first .. end - 1 of all sequences' ----
     // lane i of a wave counts the steps of sequence s0 + i; a sequence with rows has one at least (its rows' results)
-    auto steps_of = [&](int s) {
-        if (s >= P.R.n_seq) return 0;
+    struct of_lane { int rows, pos0, table, steps; };          // first row * 64 + rows (there are 2^21 rows at most); where its page-table row begins
+    auto look = [&](int s) {
+        of_lane r{0, 0, 0, 0};
+        if (s >= P.R.n_seq) return r;
         const seq_view v = seq_of(P.R, s);
-        return v.count < 1 ? 0 : max((span_of_rows(v).nt + NW - 1) / NW, 1);
+        r.table = P.pg.pt && P.pg.rtab ? P.pg.rtab[s] : 0;
+        r.rows = v.first << 6 | v.count;
+        r.pos0 = v.pos0;
+        r.steps = v.count < 1 ? 0 : max((span_of_rows(v).nt + NW - 1) / NW, 1);
+        return r;
     };
-    const int steps64 = steps_of(threadIdx.x & 63);                       // of the first 64
-    int first, end, per = 1 << 30;
+    of_lane seen64;                                           // the first 64 (all of them, mostly)
+    int first = 0, end = 1, per = 1 << 30;
     if (P.nks > 1) {
+        seen64 = look(threadIdx.x & 63);
         int n = 0, most = 0;
         for (int s0 = 0; s0 < P.R.n_seq; s0 += 64) {
-            const int x = s0 ? steps_of(s0 + (threadIdx.x & 63)) : steps64;
+            const int x = s0 ? look(s0 + (threadIdx.x & 63)).steps : seen64.steps;
             n += __builtin_amdgcn_readlane(lanes_up_to(x), 63);
             most = max(most, x);
         }
@@ -75,10 +82,6 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
         first = run * per;
         end = min(first + per, n);
         if (first >= end) return;
-    } else {                                                  // a sequence each
-        first = 0;
-        end = steps_of(run);
-        if (end < 1) return;
     }
     char * const mine = lds + wave * C::WAVE_B;
     float * const tk = reinterpret_cast<float *>(mine + C::V_B), * const tv = tk + 2 * C::TAB;
@@ -89,26 +92,36 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
     const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-    // whose step that is
-    int seq = run, s_first = 0, s_steps = end;
+    // whose step that is: its sequence, the sequence's first step and their number
+    int seq = run, s_first = 0, s_steps = 1 << 24, table = 0;
+    seq_view sv;
     if (P.nks > 1) {
         int base = 0;
         for (int s0 = 0;; s0 += 64) {                         // (there is one: at_step < n)
-            const int x = s0 ? steps_of(s0 + lane) : steps64, u = base + lanes_up_to(x);
+            const of_lane x = s0 ? look(s0 + lane) : seen64;
+            const int u = base + lanes_up_to(x.steps);
             const unsigned long long behind = __ballot(u > at_step);
             if (behind) {
-                const int l = __builtin_ctzll(behind);
+                const int l = __builtin_ctzll(behind), rows = __builtin_amdgcn_readlane(x.rows, l);
                 seq = s0 + l;
-                s_steps = __builtin_amdgcn_readlane(x, l);
+                s_steps = __builtin_amdgcn_readlane(x.steps, l);
                 s_first = __builtin_amdgcn_readlane(u, l) - s_steps;
+                sv.first = rows >> 6;
+                sv.count = rows & 63;
+                sv.pos0 = __builtin_amdgcn_readlane(x.pos0, l);
+                table = __builtin_amdgcn_readlane(x.table, l);
                 break;
             }
             base = __builtin_amdgcn_readlane(u, 63);
         }
+    } else {                                                  // a sequence each
+        sv = seq_of<true>(P.R, run);
+        if (P.pg.pt && P.pg.rtab) table = sload_i32(P.pg.rtab + run);
+        if (sv.count < 1) return;
+        end = s_steps;
     }
     // its runs, which of them this is, and the tiles of this one
     const int run0 = s_first / per, pieces = P.nks > 1 ? (s_first + s_steps - 1) / per - run0 + 1 : 1, piece = P.nks > 1 ? run - run0 : 0;
-    const seq_view sv = seq_of<true>(P.R, seq);
     const int R = min(sv.count * P.GQA, 16 * NT);
     auto row_index = [&](int r) { const int t = tok_of(r); return (size_t) (sv.first + t) * P.Hq + (size_t) hk * P.GQA + (r - t * P.GQA); };
     const span sp = span_of_rows(sv);
@@ -118,7 +131,7 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
     const bool odd = sv.pos0 < 0 || sv.pos0 + sv.count > P.R.n_ctx;
     const int all_hi = odd ? -1 : sv.pos0, all_lo = P.R.window == INT32_MAX ? 0 : sp.pmax - P.R.window + 1;
 
-    const int32_t * const ptab = P.pg.pt ? P.pg.pt + (P.pg.rtab ? sload_i32(P.pg.rtab + seq) : 0) : nullptr;
+    const int32_t * const ptab = P.pg.pt ? P.pg.pt + table : nullptr;
 
     auto pos_of = [&](int tile, int x) { return seen_or_near<32>(sp, tile * 32, tile * 32 + 16 * x + c); };
     struct pages { int p[2]; };
@@ -247,8 +260,7 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
         }
         // ---- S^T ----
         f4 s[2][NT];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) K::template scores<NT, NQ>(kr[x], q_at, tk + x * C::TAB, g, s[x]);
+        K::template scores<NT, NQ>(kr, q_at, tk, g, s);
         // (V of this tile was asked for ahead of its K)
         if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (more) {
@@ -296,34 +308,38 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
         }
         // ---- O^T += V^T (P d) ----
         const char * const vt = mine + (F16 ? st * C::VT_B : 0);
+        // (a block's scales and rows of V^T are asked for a block ahead)
+        struct block { f4 d[2]; h4 a[2][2]; };
+        auto read = [&](int b) {
+            block r;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                if constexpr (!F16) r.d[x] = *reinterpret_cast<const f4 *>(tv + x * C::TAB + b * 16 + 4 * g);
+#pragma unroll
+                for (int y = 0; y < 2; ++y) r.a[y][x] = v_read(vt + x * PL_B, 2 * b + y);
+            }
+            return r;
+        };
         h8 pb[NT][NQ];
+        block next = read(0);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            f4 d[2];
-            if constexpr (!F16) {
-#pragma unroll
-                for (int x = 0; x < 2; ++x) d[x] = *reinterpret_cast<const f4 *>(tv + x * C::TAB + b * 16 + 4 * g);
-            }
+            const block now = next;
+            if (b + 1 < NB) next = read(b + 1);
             if (!F16 || b == 0) {
 #pragma unroll
+                for (int n = 0; n < NT; ++n) halves<NQ>([&](int e) { return p[n][e]; }, [&](int e) { return F16 ? 1.f : now.d[e >> 2][e & 3]; }, pb[n]);
+            }
+#pragma unroll
+            for (int k = 0; k < NQ; ++k)
+#pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const float w = F16 ? p[n][e] : p[n][e] * d[e >> 2][e & 3];
-                        pb[n][0][e] = (half_t) w;
-                        if constexpr (EXACT) pb[n][NQ - 1][e] = (half_t) (w - (float) (half_t) w);
+                    for (int y = 0; y < 2; ++y) {
+                        const h4 a0 = now.a[y][0], a1 = now.a[y][1];
+                        o[n][2 * b + y] = mfma16(h8{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]}, pb[n][k], o[n][2 * b + y]);
                     }
-                if constexpr (!F16 && D == 256) __builtin_amdgcn_sched_barrier(0);
-            }
-#pragma unroll
-            for (int dt = 2 * b; dt < 2 * b + 2; ++dt) {
-                const h4 a0 = v_read(vt, dt), a1 = v_read(vt + PL_B, dt);
-                const h8 a = {a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]};
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int k = 0; k < NQ; ++k) o[n][dt] = mfma16(a, pb[n][k], o[n][dt]);
-            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 

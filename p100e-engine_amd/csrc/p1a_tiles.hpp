@@ -97,6 +97,22 @@ template <int BN> __device__ __forceinline__ int seen_or_near(const span & s, in
 // (Not above 2^100: the factor stays a number above zero.)
 __device__ __forceinline__ int row_exponent(float most) { return most > 0.f && most < __builtin_inff() ? max(__builtin_amdgcn_frexp_expf(most), -100) : 0; }
 
+// x(0 .. 7) * y(0 .. 7) in f16 halves: the rounded products, and (NQ = 2) what the rounding left, rounded itself
+typedef float f2w __attribute__((ext_vector_type(2)));
+template <int NQ, class X, class Y> __device__ __forceinline__ void halves(X && x, Y && y, h8 (&out)[NQ]) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const float x0 = x(2 * e), y0 = y(2 * e), x1 = x(2 * e + 1), y1 = y(2 * e + 1);
+        h2 h = __builtin_convertvector(f2w{x0 * y0, x1 * y1}, h2);
+        asm("" : "+v"(h));                                    // (one conversion of both, not one more of each for the rest)
+        hi[e] = __builtin_bit_cast(uint32_t, h);
+        if constexpr (NQ == 2) lo[e] = __builtin_bit_cast(uint32_t, h2{(half_t) fmaf(x0, y0, -(float) h[0]), (half_t) fmaf(x1, y1, -(float) h[1])});
+    }
+    out[0] = __builtin_bit_cast(h8, u4{hi[0], hi[1], hi[2], hi[3]});
+    if constexpr (NQ == 2) out[NQ - 1] = __builtin_bit_cast(h8, u4{lo[0], lo[1], lo[2], lo[3]});
+}
+
 // ---- tiles of 16 keys in LDS ----
 // A group is 16 keys of one kv head as f16, in one plane or - where a quantized value has to keep all its 18 bits - two, whose sum it is. A plane
 // is cut into blocks of 1 KB, four 16-byte chunks (32 dims) of the 16 keys: chunk x of key k lies in block x / 4 at (x % 4) * 256 + (k ^ 4 (x % 4)) * 16. A
@@ -325,27 +341,51 @@ template <uint32_t KT, int D> struct keys16 {
             return __builtin_bit_cast(h8, u4{a[0], a[1], a[2], a[3]});
         }
     }
-    // S^T of the 16 keys and NT tiles of 16 columns: value i of lane (column c, group g) is key 4 g + i. q(n, k, b): half k of block b of tile n's operand
-    template <int NT, int NQ, class Q> static __device__ __forceinline__ void scores(const raw & r, Q && q, const float * table, int g, f4 (&s)[NT]) {
+    // S^T of two times 16 keys and NT tiles of 16 columns: value i of lane (column c, group g) is key 4 g + i. q(n, k, b): half k of block b of tile n's
+    // operand. (Both halves side by side, and a block's scales asked for a block ahead: a product's result and LDS take a hundred clocks and more.)
+    template <int NT, int NQ, class Q> static __device__ __forceinline__ void scores(const raw (&r)[2], Q && q, const float * table, int g, f4 (&s)[2][NT]) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) s[n] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[x][n] = f4{0.f, 0.f, 0.f, 0.f};
+        f4 d[2], dn[2];
+        auto fetch = [&](int b) {
+            if constexpr (!F16) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) dn[x] = *reinterpret_cast<const f4 *>(table + x * TAB + b * 16 + 4 * g);
+            }
+        };
+        fetch(0);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-            const h8 a = operand(r, b);
-            f4 d;
-            if constexpr (!F16) d = *reinterpret_cast<const f4 *>(table + b * 16 + 4 * g);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                f4 t = F16 ? s[n] : f4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int k = 0; k < NQ; ++k) t = mfma16(a, q(n, k, b), t);
-                if constexpr (F16) s[n] = t;
-                else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s[n][i] = fmaf(t[i], d[i], s[n][i]);
-                    asm volatile("" : "+v"(s[n]));            // (here: put off behind the next branch, every block's t and d would stay in registers)
-                }
+            if constexpr (!F16) {
+                d[0] = dn[0];
+                d[1] = dn[1];
+                if (b + 1 < NB) fetch(b + 1);
             }
+            h8 a[2];
+#pragma unroll
+            for (int x = 0; x < 2; ++x) a[x] = operand(r[x], b);
+            f4 t[2][NT];
+#pragma unroll
+            for (int k = 0; k < NQ; ++k)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const h8 qq = q(n, k, b);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) t[x][n] = mfma16(a[x], qq, k ? t[x][n] : F16 ? s[x][n] : f4{0.f, 0.f, 0.f, 0.f});
+                }
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    if constexpr (F16) s[x][n] = t[x][n];
+                    else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[x][n][i] = fmaf(t[x][n][i], d[x][i], s[x][n][i]);
+                        asm volatile("" : "+v"(s[x][n]));     // (here: put off behind the next branch, every block's t and d would stay in registers)
+                    }
+                }
         }
     }
 };
@@ -367,14 +407,14 @@ template <uint32_t KT, int D, int NQ> __device__ __forceinline__ int q_columns(c
 #pragma unroll
         for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[b][e >> 2][e & 3]));
     const int ex = row_exponent(max_swap32(max_swap16(most)));
+    const float by = ldexpf(sign, -ex);
 #pragma unroll
-    for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b) {
+        h8 r[NQ];
+        halves<NQ>([&](int e) { return x[b][e >> 2][e & 3]; }, [&](int) { return by; }, r);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float y = ldexpf(x[b][e >> 2][e & 3] * sign, -ex);
-            qf[0][b][e] = (half_t) y;
-            if constexpr (NQ == 2) qf[NQ - 1][b][e] = (half_t) (y - (float) (half_t) y);
-        }
+        for (int k = 0; k < NQ; ++k) qf[k][b] = r[k];
+    }
     return ex;
 }
 
