@@ -258,7 +258,8 @@ typedef struct p1a_rows {
  * A call of few rows is split over its keys and its partials merged by a second launch; they live in `scratch` (256-byte aligned, at least
  * p1a_attn_chunk_scratch_bytes) or, with NULL or less, in the library's buffers of (device, stream), under the rules of p1a_attn_prefill's: nothing is
  * allocated during stream capture (P1A_E_SCRATCH: make one eager call first, or bring scratch), graphs captured on one stream share them - replay
- * such graphs one behind the other, or bring scratch for each. Result bits depend on the call's host numbers and the device, not on scratch.
+ * such graphs one behind the other, or bring scratch for each. Result bits depend on the call's numbers - the
+ * positions of all its sequences among them, as a call of few rows deals out their keys evenly - and the device, not on scratch.
  */
 int p1a_attn_chunk(const void *q, int q_type, const p1a_kv *c, void *out, int out_type, const float *gate, float *lse, const p1a_rows *rows,
                    int Hq, float scale, void *scratch, size_t scratch_bytes, void *stream);
@@ -269,11 +270,14 @@ size_t p1a_attn_chunk_scratch_bytes(const p1a_kv *c, const p1a_rows *rows, int H
  * Attention weight per cache position: mass [n_seq][Hkv][ld] f32 (row s, h starting at (s * Hkv + h) * ld),
  *     mass[s][h][j] += sum over the rows t of sequence s and the q heads i of kv head h of exp(scale * q[t][i] . K[j][h] - lse[t][i])
  * over the positions j < ld that row t sees; lse [T][Hq] as p1a_attn_chunk leaves it (a row with lse = -inf adds nothing). Entries that no row
- * sees are left as they are. f32 accuracy whatever the cache; every entry is summed by one wave in a fixed order: the same bits every time. Shapes and
- * alignment as for p1a_attn_chunk. Nothing is allocated.
+ * sees are left as they are. f32 accuracy whatever the cache; every entry is summed in a fixed order: the same bits every time. Shapes and
+ * alignment as for p1a_attn_chunk. Calls of many rows over few keys add up partial sums of the size of `mass`, in `scratch` (256-byte aligned, at
+ * least p1a_attn_mass_scratch_bytes) or, with NULL or less, the library's buffers, as p1a_attn_chunk's partials.
  */
 int p1a_attn_mass(const void *q, int q_type, const p1a_kv *c, const float *lse, float *mass, int ld, const p1a_rows *rows, int Hq, float scale,
-                  void *stream);
+                  void *scratch, size_t scratch_bytes, void *stream);
+/* bytes of partial sums such a call has (0: none) */
+size_t p1a_attn_mass_scratch_bytes(const p1a_kv *c, int ld, const p1a_rows *rows, int Hq);
 
 /*
  * Which positions of a cache stay: per sequence s and kv head the first n_sink of its n positions, the last n_recent, and of those between the

@@ -12,7 +12,7 @@ KV_F16, KV_Q4_0, KV_Q8_0 = 1, 2, 8
 EXPORTS = [
     "p1a_kv_row_bytes", "p1a_kv_append", "p1a_kv_fill_random", "p1a_attn_prep", "p1a_attn_prep_mrope", "p1a_attn_decode", "p1a_attn_decode_a16", "p1a_attn_decode_noalloc", "p1a_a16_bytes", "p1a_ew_quant", "p1a_attn_prefill", "p1a_attn_prefill_scratch_bytes", "p1a_attn_prefill_key_splits", "p1a_attn_prefill_call_splits",
     "p1a_sigmoid_mul", "p1a_warmup", "p1a_get_nsplit", "p1a_set_nsplit", "p1a_reload_env", "p1a_warmup_prefill", "p1a_set_prefill_staging_limit", "p1a_bench_decode_split_only", "p1a_bench_stream_read", "p1a_release", "p1a_last_error",
-    "p1a_attn_chunk", "p1a_attn_chunk_scratch_bytes", "p1a_attn_mass", "p1a_evict_select", "p1a_kv_compact", "p1a_seq_evict",
+    "p1a_attn_chunk", "p1a_attn_chunk_scratch_bytes", "p1a_attn_mass", "p1a_attn_mass_scratch_bytes", "p1a_evict_select", "p1a_kv_compact", "p1a_seq_evict",
     "p1a_version", "p1a_decode_scratch_bytes", "p1a_decode_footprint_bytes", "p1a_numerics_id",
     # include/p1a_pool.h
     "p1a_pool_create", "p1a_pool_destroy", "p1a_pool_n_pages", "p1a_pool_free_pages", "p1a_pool_max_pages", "p1a_pool_page_bytes",
@@ -121,7 +121,9 @@ def lib():
     L.p1a_attn_chunk_scratch_bytes.restype = sz
     L.p1a_attn_chunk_scratch_bytes.argtypes = [kvp, rp, i32]
     L.p1a_attn_mass.restype = i32
-    L.p1a_attn_mass.argtypes = [vp, i32, kvp, vp, vp, i32, rp, i32, f32, vp]
+    L.p1a_attn_mass.argtypes = [vp, i32, kvp, vp, vp, i32, rp, i32, f32, vp, sz, vp]
+    L.p1a_attn_mass_scratch_bytes.restype = sz
+    L.p1a_attn_mass_scratch_bytes.argtypes = [kvp, i32, rp, i32]
     L.p1a_evict_select.restype = i32
     L.p1a_evict_select.argtypes = [vp, i32, i32, i32, vp, i32, i32, i32, i32, vp, vp]
     L.p1a_kv_compact.restype = i32
@@ -412,9 +414,15 @@ def chunk_scratch_bytes(c, rows, Hq):
     return int(lib().p1a_attn_chunk_scratch_bytes(ctypes.byref(c.struct()), rows._ref, Hq))
 
 
-def attn_mass(q, c, lse, mass, rows, Hq, scale):
+def attn_mass(q, c, lse, mass, rows, Hq, scale, scratch=None):
     """Adds the attention weight that the rows give to every cache position to mass [n_seq][Hkv][ld] float32; lse as attn_chunk leaves it."""
-    _check(lib().p1a_attn_mass(_ptr(q), _row_type(q), ctypes.byref(c.struct()), _ptr(lse), _ptr(mass), mass.shape[-1], rows._ref, Hq, scale, _stream()), "attn_mass")
+    nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
+    _check(lib().p1a_attn_mass(_ptr(q), _row_type(q), ctypes.byref(c.struct()), _ptr(lse), _ptr(mass), mass.shape[-1], rows._ref, Hq, scale, _ptr(scratch), nbytes,
+                               _stream()), "attn_mass")
+
+
+def mass_scratch_bytes(c, ld, rows, Hq):
+    return int(lib().p1a_attn_mass_scratch_bytes(ctypes.byref(c.struct()), ld, rows._ref, Hq))
 
 
 def evict_select(mass, n, keep, n_sink=0, n_recent=0):

@@ -456,17 +456,24 @@ size_t p1a_attn_chunk_scratch_bytes(const p1a_kv * c, const p1a_rows * rows, int
 }
 
 int p1a_attn_mass(const void * q, int q_type, const p1a_kv * c, const float * lse, float * mass, int ld, const p1a_rows * rows, int Hq, float scale,
-                  void * stream) {
+                  void * scratch, size_t scratch_bytes, void * stream) {
     static const char * const who = "p1a_attn_mass";
-    rows_view R;
-    int max_n;
-    const int rc = rows_ok(c, rows, Hq, who, R, max_n);
+    mass_args a;
+    const int rc = rows_ok(c, rows, Hq, who, a.R, a.max_n);
     if (rc != P1A_OK) return rc;
     if (!q || !lse || !mass || ld < 0) { set_error("%s: null q / lse / mass or negative ld", who); return P1A_E_ARG; }
     if (!rows_type_ok(q_type, who)) return P1A_E_ARG;
     if (((uintptr_t) q & 15) || (((uintptr_t) lse | (uintptr_t) mass) & 3)) { set_error("%s: q must be 16-byte aligned, lse and mass 4-byte", who); return P1A_E_SHAPE; }
     if (!rows->T || !rows->n_seq || !ld) return P1A_OK;
-    return launch_mass(*c, q, q_type == P1A_ROWS_BF16, lse, mass, ld, R, Hq, scale, max_n, (hipStream_t) stream);
+    a.q = q; a.q_bf16 = q_type == P1A_ROWS_BF16; a.lse = lse; a.mass = mass; a.ld = ld; a.Hq = Hq; a.scale = scale; a.scratch = scratch; a.scratch_bytes = scratch_bytes;
+    return launch_mass(*c, a, (hipStream_t) stream);
+}
+
+size_t p1a_attn_mass_scratch_bytes(const p1a_kv * c, int ld, const p1a_rows * rows, int Hq) {
+    rows_view R;
+    int max_n;
+    if (rows_ok(c, rows, Hq, "p1a_attn_mass_scratch_bytes", R, max_n) != P1A_OK || !rows->T || !rows->n_seq || ld < 1) return 0;
+    return plan_mass(*c, R, Hq, max_n, ld, cu_count()).bytes;
 }
 
 int p1a_evict_select(const float * mass, int ld, int n_seq, int Hkv, const int32_t * n_dev, int n, int budget, int n_sink, int n_recent,

@@ -129,12 +129,12 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
             }
         }
         if (!(k0 + BN - 1 <= all_hi && k0 >= all_lo)) {
-            const int hi = my_pos - k0, lo = max(hi, 0) - P.R.window, sk = P.R.n_sink - k0;
+            const int from = k0 + 4 * g, hi = my_pos - from, lo = max(my_pos - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - from;
 #pragma unroll
             for (int u = 0; u < NH; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    const int j = 32 * u + mfma_row(i, g);
+                    const int j = 32 * u + mfma_row(i, 0);    // (and 4 g: a number the comparison holds itself)
                     s[u][i] = j <= hi && (j > lo || j < sk) ? s[u][i] : MINUS_INF;
                 }
         }

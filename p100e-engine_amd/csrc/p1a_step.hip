@@ -52,105 +52,42 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
         const int t = (int) __umulhi((uint32_t) r, P.gqa_magic);
         return r - t * P.GQA >= P.GQA ? t + 1 : t;
     };
-    auto span_of_rows = [&](const seq_view & v) { return span_of<32>(P.R, v.pos0, v.pos0 + v.count - 1); };
-    // ---- this workgroup's steps: first .. end - 1 of all sequences' ----
-    // lane i of a wave counts the steps of sequence s0 + i; a sequence with rows has one at least (its rows' results)
-    struct of_lane { int rows, pos0, table, steps; };          // first row * 64 + rows (there are 2^21 rows at most); where its page-table row begins
-    auto look = [&](int s) {
-        of_lane r{0, 0, 0, 0};
-        if (s >= P.R.n_seq) return r;
-        const seq_view v = seq_of(P.R, s);
-        r.table = P.pg.pt && P.pg.rtab ? P.pg.rtab[s] : 0;
-        r.rows = v.first << 6 | v.count;
-        r.pos0 = v.pos0;
-        r.steps = v.count < 1 ? 0 : max((span_of_rows(v).nt + NW - 1) / NW, 1);
-        return r;
-    };
-    of_lane seen64;                                           // the first 64 (all of them, mostly)
-    int first = 0, end = 1, per = 1 << 30;
-    if (P.nks > 1) {
-        seen64 = look(threadIdx.x & 63);
-        int n = 0, most = 0;
-        for (int s0 = 0; s0 < P.R.n_seq; s0 += 64) {
-            const int x = s0 ? look(s0 + (threadIdx.x & 63)).steps : seen64.steps;
-            n += __builtin_amdgcn_readlane(lanes_up_to(x), 63);
-            most = max(most, x);
-        }
-        most = (int) wave_max((float) most);                  // (2^24 steps at most: exact)
-        most = rfl(most);
-        per = max((n + P.runs - 1) / P.runs, (most + P.nks - 2) / (P.nks - 1));   // (no sequence in more than nks runs)
-        first = run * per;
-        end = min(first + per, n);
-        if (first >= end) return;
-    }
+    step_runs<NW> steps;
+    steps.first = 0;
+    steps.end = 1;
+    steps.per = 1 << 30;
+    if (P.nks > 1 && !steps.begin(P.R, P.pg, run, P.runs, P.nks)) return;
     char * const mine = lds + wave * C::WAVE_B;
     float * const tk = reinterpret_cast<float *>(mine + C::V_B), * const tv = tk + 2 * C::TAB;
     const size_t head_off = (size_t) hk * head_bytes(KT, D);
 
-  for (int at_step = first; at_step < end;) {
+  for (int at_step = steps.first; at_step < steps.end;) {
     // (the lane's number anew for each sequence, and once more for the fold: what follows from it would be worked out ahead of the loop and kept, 40 registers)
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
     const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-    // whose step that is: its sequence, the sequence's first step and their number
-    int seq = run, s_first = 0, s_steps = 1 << 24, table = 0;
-    seq_view sv;
-    if (P.nks > 1) {
-        int base = 0;
-        for (int s0 = 0;; s0 += 64) {                         // (there is one: at_step < n)
-            const of_lane x = s0 ? look(s0 + lane) : seen64;
-            const int u = base + lanes_up_to(x.steps);
-            const unsigned long long behind = __ballot(u > at_step);
-            if (behind) {
-                const int l = __builtin_ctzll(behind), rows = __builtin_amdgcn_readlane(x.rows, l);
-                seq = s0 + l;
-                s_steps = __builtin_amdgcn_readlane(x.steps, l);
-                s_first = __builtin_amdgcn_readlane(u, l) - s_steps;
-                sv.first = rows >> 6;
-                sv.count = rows & 63;
-                sv.pos0 = __builtin_amdgcn_readlane(x.pos0, l);
-                table = __builtin_amdgcn_readlane(x.table, l);
-                break;
-            }
-            base = __builtin_amdgcn_readlane(u, 63);
-        }
-    } else {                                                  // a sequence each
-        sv = seq_of<true>(P.R, run);
-        if (P.pg.pt && P.pg.rtab) table = sload_i32(P.pg.rtab + run);
-        if (sv.count < 1) return;
-        end = s_steps;
+    // whose step that is, and the sequence's runs, which of them this is
+    typename step_runs<NW>::found f;
+    if (P.nks > 1) f = steps.find(P.R, P.pg, at_step, lane);
+    else {                                                    // a sequence each
+        f.seq = run; f.first = 0; f.steps = 1 << 24;
+        f.v = seq_of<true>(P.R, run);
+        f.table = P.pg.pt && P.pg.rtab ? sload_i32(P.pg.rtab + run) : 0;
+        if (f.v.count < 1) return;
     }
-    // its runs, which of them this is, and the tiles of this one
-    const int run0 = s_first / per, pieces = P.nks > 1 ? (s_first + s_steps - 1) / per - run0 + 1 : 1, piece = P.nks > 1 ? run - run0 : 0;
+    const seq_view & sv = f.v;
+    const int run0 = f.first / steps.per, pieces = P.nks > 1 ? (f.first + f.steps - 1) / steps.per - run0 + 1 : 1, piece = P.nks > 1 ? run - run0 : 0;
     const int R = min(sv.count * P.GQA, 16 * NT);
     auto row_index = [&](int r) { const int t = tok_of(r); return (size_t) (sv.first + t) * P.Hq + (size_t) hk * P.GQA + (r - t * P.GQA); };
-    const span sp = span_of_rows(sv);
-    const int ta = (at_step - s_first) * NW, tb = min((min(end, s_first + s_steps) - s_first) * NW, sp.nt);
-    at_step = s_first + s_steps;
+    const span sp = step_runs<NW>::span_of_rows(P.R, sv);
+    const int ta = (at_step - f.first) * NW, tb = P.nks > 1 ? min((min(steps.end, f.first + f.steps) - f.first) * NW, sp.nt) : sp.nt;
+    at_step = f.first + f.steps;
     // positions that all rows see
     const bool odd = sv.pos0 < 0 || sv.pos0 + sv.count > P.R.n_ctx;
     const int all_hi = odd ? -1 : sv.pos0, all_lo = P.R.window == INT32_MAX ? 0 : sp.pmax - P.R.window + 1;
 
-    const int32_t * const ptab = P.pg.pt ? P.pg.pt + table : nullptr;
-
-    auto pos_of = [&](int tile, int x) { return seen_or_near<32>(sp, tile * 32, tile * 32 + 16 * x + c); };
-    struct pages { int p[2]; };
-    auto pages_of = [&](int tile) {
-        pages r;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) r.p[x] = ptab ? ptab[pos_of(tile, x) >> P.pg.psh] : 0;
-        return r;
-    };
-    struct where { size_t off[2]; };                          // the rows of this lane's keys
-    auto where_is = [&](int tile, const pages & e) {
-        where r;
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const int j = pos_of(tile, x);
-            r.off[x] = head_off + (ptab ? (size_t) e.p[x] * P.pg.pstride + (size_t) (j & ((1 << P.pg.psh) - 1)) * P.pg.rowb : (size_t) j * P.pg.rowb);
-        }
-        return r;
-    };
+    const key_rows keys{sp, P.pg, P.pg.pt ? P.pg.pt + f.table : nullptr, head_off, c};
+    using where = key_rows::where;
     int vbase[2];                                             // V^T operand: dims 16 dt + lane % 16, keys 4 g .. of a group; for even and odd dt
     {
         const int kk = c >> 2, jq = c & 3;
@@ -184,7 +121,7 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
     int i = ta + wave;
     where at;
     if (i < tb) {
-        at = where_is(sp.tile(i), pages_of(sp.tile(i)));
+        at = keys.at(sp.tile(i), keys.pages_of(sp.tile(i)));
         if constexpr (F16) ask_v(at, 0);
         if constexpr (F16 || NT * D <= 128) ask_k(at);
     }
@@ -230,8 +167,8 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
     for (int st = 0; i < tb; i += NW, st ^= 1) {
         const int k0 = sp.tile(i) * 32;
         const bool more = i + NW < tb;
-        pages pg;
-        if (more) pg = pages_of(sp.tile(i + NW));
+        key_rows::pages pg;
+        if (more) pg = keys.pages_of(sp.tile(i + NW));
         // ---- V's codes and the scales into LDS ----
         if constexpr (!F16) {
             float dm = 0.f;
@@ -264,7 +201,7 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
         // (V of this tile was asked for ahead of its K)
         if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (more) {
-            const where at = where_is(sp.tile(i + NW), pg);
+            const where at = keys.at(sp.tile(i + NW), pg);
             ask_v(at, st ^ 1);
             ask_k(at);
         }
@@ -272,12 +209,12 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
         if (!(k0 + 31 <= all_hi && k0 >= all_lo)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int hi = pos[n] - k0, lo = max(hi, 0) - P.R.window, sk = P.R.n_sink - k0;
+                const int from = k0 + 4 * g, hi = pos[n] - from, lo = max(pos[n] - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - from;
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        const int j = 16 * x + 4 * g + e;
+                        const int j = 16 * x + e;                // (and 4 g)
                         s[x][n][e] = j <= hi && (j > lo || j < sk) ? s[x][n][e] : MINUS_INF;
                     }
             }
@@ -413,7 +350,7 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
             }
         }
     }
-    if (P.nks > 1 && piece == 0 && hk == 0 && tid == 0) P.part_n[seq] = pieces;
+    if (P.nks > 1 && piece == 0 && hk == 0 && tid == 0) P.part_n[f.seq] = pieces;
     __syncthreads();                                          // (what was folded is read; the next sequence's V goes there)
   }
 }

@@ -418,6 +418,91 @@ template <uint32_t KT, int D, int NQ> __device__ __forceinline__ int q_columns(c
     return ex;
 }
 
+// ---- few rows a sequence: steps of 32 TPS keys, counted through over the sequences, in runs of equal length ----
+// A sequence with rows has one step at least. Lane i of a wave counts for sequence s0 + i and keeps what it found out about the first 64 (all of
+// them, mostly).
+template <int TPS> struct step_runs {
+    struct of_lane { int rows, pos0, table, steps; };          // first row * 64 + rows (there are 2^21 rows at most); where its page-table row begins
+    of_lane first64;
+    int first, end, per;                                      // this run's steps; steps of a run
+    static __device__ __forceinline__ span span_of_rows(const rows_view & R, const seq_view & v) { return span_of<32>(R, v.pos0, v.pos0 + v.count - 1); }
+    static __device__ __forceinline__ of_lane look(const rows_view & R, const kv_view & pg, int s) {
+        of_lane r{0, 0, 0, 0};
+        if (s >= R.n_seq) return r;
+        const seq_view v = seq_of(R, s);
+        r.table = pg.pt && pg.rtab ? pg.rtab[s] : 0;
+        r.rows = v.first << 6 | v.count;
+        r.pos0 = v.pos0;
+        r.steps = v.count < 1 ? 0 : max((span_of_rows(R, v).nt + TPS - 1) / TPS, 1);
+        return r;
+    }
+    // run number `run` of `runs`; no sequence in more than `most_runs` of them. False: there is nothing for it
+    __device__ __forceinline__ bool begin(const rows_view & R, const kv_view & pg, int run, int runs, int most_runs) {
+        const int lane = threadIdx.x & 63;
+        first64 = look(R, pg, lane);
+        int n = 0, most = 0;
+        for (int s0 = 0; s0 < R.n_seq; s0 += 64) {
+            const int x = s0 ? look(R, pg, s0 + lane).steps : first64.steps;
+            n += __builtin_amdgcn_readlane(lanes_up_to(x), 63);
+            most = max(most, x);
+        }
+        most = rfl((int) wave_max((float) most));             // (2^24 steps at most: exact)
+        per = max((n + runs - 1) / runs, (most + most_runs - 2) / (most_runs - 1));
+        first = run * per;
+        end = min(first + per, n);
+        return first < end;
+    }
+    // the sequence that holds step `at` (of begin()'s run), where its steps begin and how many it has
+    struct found { int seq, first, steps, table; seq_view v; };
+    __device__ __forceinline__ found find(const rows_view & R, const kv_view & pg, int at, int lane) const {
+        found f;
+        int base = 0;
+        for (int s0 = 0;; s0 += 64) {
+            const of_lane x = s0 ? look(R, pg, s0 + lane) : first64;
+            const int u = base + lanes_up_to(x.steps);
+            const unsigned long long behind = __ballot(u > at);
+            if (behind) {
+                const int l = __builtin_ctzll(behind), rows = __builtin_amdgcn_readlane(x.rows, l);
+                f.seq = s0 + l;
+                f.steps = __builtin_amdgcn_readlane(x.steps, l);
+                f.first = __builtin_amdgcn_readlane(u, l) - f.steps;
+                f.v.first = rows >> 6;
+                f.v.count = rows & 63;
+                f.v.pos0 = __builtin_amdgcn_readlane(x.pos0, l);
+                f.table = __builtin_amdgcn_readlane(x.table, l);
+                return f;
+            }
+            base = __builtin_amdgcn_readlane(u, 63);
+        }
+    }
+};
+// The rows of a lane's keys: key c of each half of a tile of 32
+struct key_rows {
+    const span & sp;
+    const kv_view & pg;
+    const int32_t * ptab;
+    size_t head_off;
+    int c;
+    struct pages { int p[2]; };
+    struct where { size_t off[2]; };
+    __device__ __forceinline__ int pos(int tile, int x) const { return seen_or_near<32>(sp, tile * 32, tile * 32 + 16 * x + c); }
+    __device__ __forceinline__ pages pages_of(int tile) const {
+        pages r;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) r.p[x] = ptab ? ptab[pos(tile, x) >> pg.psh] : 0;
+        return r;
+    }
+    __device__ __forceinline__ where at(int tile, const pages & e) const {
+        where r;
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int j = pos(tile, x);
+            r.off[x] = head_off + (ptab ? (size_t) e.p[x] * pg.pstride + (size_t) (j & ((1 << pg.psh) - 1)) * pg.rowb : (size_t) j * pg.rowb);
+        }
+        return r;
+    }
+};
+
 // ---- attention of chunks: what its kernels share ----
 constexpr float HEAD = 8.f, STEP = 6.f;                       // log2 of P at the row's maximum: HEAD when the reference moves, at most HEAD + STEP
 struct chunk_params {
@@ -464,7 +549,17 @@ struct chunk_plan {
 };
 chunk_plan plan_chunk(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus);
 int launch_step(const p1a_kv & c, const chunk_params & P, int NT, bool exact, hipStream_t s);
-int launch_mass(const p1a_kv & c, const void * q, bool q_bf16, const float * lse, float * mass, int ld, const rows_view & R, int Hq, float scale, int max_n, hipStream_t s);
+struct mass_args {
+    const void * q; bool q_bf16; const float * lse; float * mass;
+    int ld;
+    rows_view R;
+    int Hq, max_n;
+    float scale;
+    void * scratch; size_t scratch_bytes;
+};
+struct mass_plan { int few, runs, blocks, splits; size_t bytes; };   // (few as in chunk_plan; bytes of scratch)
+mass_plan plan_mass(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int ld, int cus);
+int launch_mass(const p1a_kv & c, const mass_args & a, hipStream_t s);
 int launch_evict_select(const float * mass, int ld, int n_seq, int Hkv, const int32_t * n_dev, int n, int budget, int n_sink, int n_recent, int32_t * keep, hipStream_t s);
 int launch_kv_compact(const p1a_kv & c, const int32_t * keep, int n_seq, int budget, const float * mass, float * mass_out, int ld, hipStream_t s);
 

@@ -40,7 +40,7 @@ def chunk(kv=None, r=None, q=4096, out=4096, gate=None, lse=None, qt=0, ot=0, Hq
 
 def mass(kv=None, r=None, q=4096, lse=4096, m=4096, ld=64, qt=0, Hq=24):
     kv, r = kv or cache(), r or rows()
-    return p1a.lib().p1a_attn_mass(q, qt, ctypes.byref(kv), lse, m, ld, ctypes.byref(r), Hq, 0.1, None)
+    return p1a.lib().p1a_attn_mass(q, qt, ctypes.byref(kv), lse, m, ld, ctypes.byref(r), Hq, 0.1, None, 0, None)
 
 
 def test_no_rows_are_no_work():
@@ -120,12 +120,12 @@ def test_an_evicted_sequence_gives_pages_back():
         pool.seq_evict(1, 0)
 
 
-@pytest.mark.parametrize("source, kernel, builds", [("p1a_chunk.hip", "chunk_k", 18), ("p1a_mass.hip", "mass_k", 9)])
+@pytest.mark.parametrize("source, kernel, builds", [("p1a_chunk.hip", "chunk_k", 18), ("p1a_step.hip", "step_k", 36), ("p1a_mass.hip", "mass_k", 9), ("p1a_mass.hip", "mass_step_k", 18)])
 def test_kernels_fit_their_budget(tmp_path, source, kernel, builds):
     """nothing in memory; two workgroups to a compute unit where heads have 128 dims and fewer"""
     ks = {k: v for k, v in resource_report(tmp_path, source, VGPR_FORM).items() if kernel in k}
     assert len(ks) >= builds, sorted(ks)
     for name, r in ks.items():
-        D = int(re.search(kernel + r"ILj\d+ELi(\d+)E", name).group(1))
+        D = int(re.search(r"ILj\d+ELi(\d+)E", name).group(1))
         assert r.get("VGPRs Spill", 0) == 0 and r.get("ScratchSize", 0) == 0, (name, r)
         assert r["Occupancy"] >= (2 if D <= 128 else 1), (name, r)
