@@ -20,7 +20,8 @@ constexpr int BM = 128, NTHR = 256;
 
 template <uint32_t KT, int D, bool EXACT> struct chunk_cfg {
     static constexpr int NPL = group_planes(KT, EXACT);
-    static constexpr int BN = NPL == 2 && D >= 128 ? 32 : 64; // keys of a tile: 64 KB and less of LDS for K and V
+    // keys of a tile, by what registers hold: scores of this tile and the next, P, and a quantized tile on its way
+    static constexpr int BN = D >= 128 && (EXACT || KT != P1A_KV_F16) ? 32 : 64;
     static constexpr int NG = BN / 16, G_B = NPL * plane_bytes(D), STAGE_B = 2 * NG * G_B;
 };
 
@@ -29,7 +30,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
     using C = chunk_cfg<KT, D, EXACT>;
     using G = group<KT, D, C::NPL>;
     constexpr int BN = C::BN, NG = C::NG, G_B = C::G_B, PL_B = plane_bytes(D), NPL = C::NPL;
-    constexpr int NKS = D / 16, NDT = D / 32, NH = BN / 32, NQ = EXACT ? 2 : 1;
+    constexpr int NKS = D / 16, NDT = D / 32, NH = BN / 32, NQ = EXACT ? 2 : 1, PF_K = NPL == 2 ? 1 : EXACT ? 2 : 4, PF_V = NPL == 2 ? 1 : EXACT ? 2 : 3;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -110,42 +111,47 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
 
     const k_frag kf(lane, G_B);
     const v_frag vf(lane);
+    auto k_read = [&](int st, int k, int pl) { return kf.read(k_groups(st) + 2 * (k / NKS) * G_B + pl * PL_B, k % NKS); };
+    auto v_read = [&](int st, int f, int pl) { return vf.read(v_groups(st) + (f / NDT) * G_B + pl * PL_B, f % NDT); };
 
-    // ---- one tile ----
-    auto compute = [&](int st, int tile) {
-        const int k0 = tile * BN;
-        f16x s[NH];
-#pragma unroll
-        for (int u = 0; u < NH; ++u) {
-            const char * kg = k_groups(st) + 2 * u * G_B;
+    // ---- S^T of one tile: product k of NH * NKS ----
+    auto s_product = [&](f16x (&s)[NH], int k, const h8 (&a)[NPL]) {
+        const int u = k / NKS, ks = k % NKS;
+        if (ks == 0) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-#pragma unroll
-            for (int ks = 0; ks < NKS; ++ks) {
-                const h8 a = kf.read(kg, ks);
-                s[u] = mfma32(a, qf[0][ks], s[u]);
-                if constexpr (EXACT) s[u] = mfma32(a, qf[NQ - 1][ks], s[u]);
-                if constexpr (NPL == 2) s[u] = mfma32(kf.read(kg + PL_B, ks), qf[0][ks], s[u]);
-            }
         }
-        if (!(k0 + BN - 1 <= all_hi && k0 >= all_lo)) {
-            const int from = k0 + 4 * g, hi = my_pos - from, lo = max(my_pos - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - from;
-#pragma unroll
-            for (int u = 0; u < NH; ++u)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const int j = 32 * u + mfma_row(i, 0);    // (and 4 g: a number the comparison holds itself)
-                    s[u][i] = j <= hi && (j > lo || j < sk) ? s[u][i] : MINUS_INF;
-                }
-        }
-        float mx = MINUS_INF;
+        s[u] = mfma32(a[0], qf[0][ks], s[u]);
+        if constexpr (EXACT) s[u] = mfma32(a[0], qf[NQ - 1][ks], s[u]);
+        if constexpr (NPL == 2) s[u] = mfma32(a[NPL - 1], qf[0][ks], s[u]);
+    };
+    // what a row does not see, where a row of the wave does not see all of the tile
+    auto mask = [&](f16x (&s)[NH], int k0) {
+        const int from = k0 + 4 * g, hi = my_pos - from, lo = max(my_pos - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - from;
 #pragma unroll
         for (int u = 0; u < NH; ++u)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) mx = fmaxf(mx, s[u][i]);
-        mx = max_swap32(mx) * factor;
+            for (int i = 0; i < 16; ++i) {
+                const int j = 32 * u + mfma_row(i, 0);        // (and 4 g: a number the comparison holds itself)
+                s[u][i] = j <= hi && (j > lo || j < sk) ? s[u][i] : MINUS_INF;
+            }
+    };
+    auto most_of = [&](const f16x (&s)[NH]) {
+        float m = MINUS_INF;
+#pragma unroll
+        for (int u = 0; u < NH; ++u)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, s[u][i]);
+        return m;
+    };
+    auto whole = [&](int k0) { return k0 + BN - 1 <= all_hi && k0 >= all_lo; };
+    float mx = MINUS_INF;                                     // the row's largest score of the tile in hand
+
+    // ---- a step: P of this tile beside the products S^T of the next one, then O^T beside the next one's maximum. The loads of K two tiles on and V one
+    // tile on are under way meanwhile ----
+    auto step = [&](int st, int next, f16x (&s)[NH], f16x (&sn)[NH], auto && more_loads) {
         const bool fresh = ref == MINUS_INF, move = mx > (fresh ? MINUS_INF : ref + (HEAD + STEP));
-        if (__any(move)) {
+        if (__builtin_expect(__any(move), 0)) {
             const float to = move ? mx - HEAD : ref, alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(ref - to);   // (fresh: nothing accumulated)
             ref = to;
             l *= alpha;
@@ -155,64 +161,134 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
                 for (int i = 0; i < 16; ++i) o[dt][i] *= alpha;
         }
         const float nr = ref == MINUS_INF ? 0.f : -ref;       // (a row that has seen nothing: exp2(-inf))
+        constexpr int NK = NH * NKS, NF = NG * NDT, NV = NH * 16;
         h8 pb[NQ][2 * NH];
         float ls[2] = {0.f, 0.f};
+        // (operands from LDS are asked for a few products ahead, and no further: registers)
+        h8 fr[PF_K][NPL];
 #pragma unroll
-        for (int u = 0; u < NH; ++u)
+        for (int k = 0; k < PF_K; ++k)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(s[u][i], factor, nr));
-                ls[i & 1] += p;
-                const half_t h = (half_t) p;
-                pb[0][2 * u + (i >> 3)][i & 7] = h;
-                if constexpr (EXACT) pb[NQ - 1][2 * u + (i >> 3)][i & 7] = (half_t) (p - (float) h);
+            for (int pl = 0; pl < NPL; ++pl) fr[k][pl] = k_read(st ^ 1, k, pl);
+        more_loads();
+#pragma unroll
+        for (int k = 0; k < NK; ++k) {
+            h8 a[NPL];
+#pragma unroll
+            for (int pl = 0; pl < NPL; ++pl) {
+                a[pl] = fr[k % PF_K][pl];
+                if (k + PF_K < NK) fr[k % PF_K][pl] = k_read(st ^ 1, k + PF_K, pl);
             }
-        l += ls[0] + ls[1];
+            s_product(sn, k, a);
 #pragma unroll
-        for (int ps = 0; ps < NG; ++ps) {
-            const char * vg = v_groups(st) + ps * G_B;
-#pragma unroll
-            for (int dt = 0; dt < NDT; ++dt) {
-                const h8 a = vf.read(vg, dt);
-                o[dt] = mfma32(a, pb[0][ps], o[dt]);
-                if constexpr (EXACT) o[dt] = mfma32(a, pb[NQ - 1][ps], o[dt]);
-                if constexpr (NPL == 2) o[dt] = mfma32(vf.read(vg + PL_B, dt), pb[0][ps], o[dt]);
+            for (int v = k * NV / NK / 2 * 2; v < (k + 1) * NV / NK / 2 * 2; v += 2) {   // pairs of values of P
+                const int u = v >> 4, i = v & 15;
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][i], factor, nr)), p1 = __builtin_amdgcn_exp2f(fmaf(s[u][i + 1], factor, nr));
+                ls[0] += p0;
+                ls[1] += p1;
+                h2 h = __builtin_convertvector(f2w{p0, p1}, h2);
+                asm("" : "+v"(h));
+                pb[0][2 * u + (i >> 3)][i & 7] = h[0];
+                pb[0][2 * u + (i >> 3)][(i & 7) + 1] = h[1];
+                if constexpr (EXACT) {
+                    pb[NQ - 1][2 * u + (i >> 3)][i & 7] = (half_t) (p0 - (float) h[0]);
+                    pb[NQ - 1][2 * u + (i >> 3)][(i & 7) + 1] = (half_t) (p1 - (float) h[1]);
+                }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
+        l += ls[0] + ls[1];
+        h8 fv[PF_V][NPL];
+#pragma unroll
+        for (int f = 0; f < PF_V; ++f)
+#pragma unroll
+            for (int pl = 0; pl < NPL; ++pl) fv[f][pl] = v_read(st, f, pl);
+        mx = MINUS_INF;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            const int ps = f / NDT, dt = f % NDT;
+            h8 a[NPL];
+#pragma unroll
+            for (int pl = 0; pl < NPL; ++pl) {
+                a[pl] = fv[f % PF_V][pl];
+                if (f + PF_V < NF) fv[f % PF_V][pl] = v_read(st, f + PF_V, pl);
+            }
+            o[dt] = mfma32(a[0], pb[0][ps], o[dt]);
+            if constexpr (EXACT) o[dt] = mfma32(a[0], pb[NQ - 1][ps], o[dt]);
+            if constexpr (NPL == 2) o[dt] = mfma32(a[NPL - 1], pb[0][ps], o[dt]);
+#pragma unroll
+            for (int v = f * NV / NF; v < (f + 1) * NV / NF; ++v) mx = fmaxf(mx, sn[v >> 4][v & 15]);
+            asm volatile("" : "+v"(mx));
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        if (__builtin_expect(!whole(next * BN), 0)) {
+            mask(sn, next * BN);
+            mx = most_of(sn);
+        }
+        mx = max_swap32(mx) * factor;
     };
 
-    // ---- the walk: tile i + 1 is on its way while tile i is worked on; its page-table entries were asked for a tile ahead ----
-    auto run = [&](auto && fetch, auto && put) {
+    // ---- the walk. K of tile i and V of tile i - 1 are fetched into stage i & 1 together with nothing else in flight; page-table entries a tile ahead ----
+    constexpr auto done = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    auto run = [&](auto && k_fetch, auto && k_put, auto && v_fetch, auto && v_put) {
         if (ta >= tb) return;
-        fetch(0, sp.tile(ta), page);
-        put(0);
-        page = ta + 1 < tb ? page_of(sp.tile(ta + 1)) : 0;
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        for (int i = ta, st = 0; i < tb; ++i, st ^= 1) {
-            const bool more = i + 1 < tb;
-            if (more) fetch(st ^ 1, sp.tile(i + 1), page);
-            if (i + 2 < tb) page = page_of(sp.tile(i + 2));
-            if (wrows > 0) compute(st, sp.tile(i));
-            if (more) put(st ^ 1);
-            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        auto tile = [&](int i) { return sp.tile(min(i, tb - 1)); };          // (past the last: that one once more, unused)
+        size_t row_v = row_of(tile(ta), page), row_k;
+        page = page_of(tile(ta + 1));
+        k_fetch(0, row_v);
+        k_put(0);
+        row_k = row_of(tile(ta + 1), page);
+        page = page_of(tile(ta + 2));
+        done();
+        k_fetch(1, row_k);
+        v_fetch(0, row_v);
+        f16x sa[NH], sb[NH];
+        if (wrows > 0) {
+#pragma unroll
+            for (int k = 0; k < NH * NKS; ++k) {
+                h8 a[NPL];
+#pragma unroll
+                for (int pl = 0; pl < NPL; ++pl) a[pl] = k_read(0, k, pl);
+                s_product(sa, k, a);
+            }
+            if (!whole(tile(ta) * BN)) mask(sa, tile(ta) * BN);
+            mx = max_swap32(most_of(sa)) * factor;
+        }
+        k_put(1);
+        v_put(0);
+        done();
+        // tile i: K(i + 1) and V(i) are there; K(i + 2) goes where K(i) was, V(i + 1) where V(i - 1) was
+        auto turn = [&](int i, int st, f16x (&s)[NH], f16x (&sn)[NH]) {
+            auto loads = [&] {
+                row_v = row_k;
+                row_k = row_of(tile(i + 2), page);
+                page = page_of(tile(i + 3));
+                k_fetch(st, row_k);
+                v_fetch(st ^ 1, row_v);
+            };
+            if (wrows > 0) step(st, tile(i + 1), s, sn, loads);
+            else loads();
+            k_put(st);
+            v_put(st ^ 1);
+            done();
+        };
+        for (int i = ta;;) {
+            turn(i, 0, sa, sb);
+            if (++i == tb) break;
+            turn(i, 1, sb, sa);
+            if (++i == tb) break;
         }
     };
     if constexpr (G::DIRECT) {
-        run([&](int st, int tile, int pg) {
-            const size_t row = row_of(tile, pg);
-            G::load((gbytes) P.kc + row, k_groups(st) + grp * G_B, lane);
-            G::load((gbytes) P.vc + row, v_groups(st) + grp * G_B, lane);
-        }, [](int) {});
+        auto nothing = [](int) {};
+        run([&](int st, size_t row) { if (BOTH || !my_v) G::load((gbytes) P.kc + row, k_groups(st) + grp * G_B, lane); }, nothing,
+            [&](int st, size_t row) { if (BOTH || my_v) G::load((gbytes) P.vc + row, v_groups(st) + grp * G_B, lane); }, nothing);
     } else {
-        typename G::raw ra, rb;
-        run([&](int, int tile, int pg) {
-            const size_t row = row_of(tile, pg);
-            G::load(ra, (my_v ? (gbytes) P.vc : (gbytes) P.kc) + row, lane);
-            if constexpr (BOTH) G::load(rb, (gbytes) P.vc + row, lane);
-        }, [&](int st) {
-            G::store(ra, (my_v ? v_groups(st) : k_groups(st)) + grp * G_B, lane);
-            if constexpr (BOTH) G::store(rb, v_groups(st) + grp * G_B, lane);
-        });
+        typename G::raw rk, rv;                               // (32-key tiles: a wave has one of the two)
+        run([&](int, size_t row) { if (BOTH || !my_v) G::load(rk, (gbytes) P.kc + row, lane); },
+            [&](int st) { if (BOTH || !my_v) G::store(rk, k_groups(st) + grp * G_B, lane); },
+            [&](int, size_t row) { if (BOTH || my_v) G::load(rv, (gbytes) P.vc + row, lane); },
+            [&](int st) { if (BOTH || my_v) G::store(rv, v_groups(st) + grp * G_B, lane); });
     }
 
     // ---- results: lane (row c, half g) holds dims 32 dt + 8 (i / 4) + 4 g + i % 4 ----
