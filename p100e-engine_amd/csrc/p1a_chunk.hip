@@ -98,7 +98,11 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
             h8 r[NQ];
             halves<NQ>([&](int e) { return x[ks][e >> 2][e & 3]; }, [&](int) { return by; }, r);
 #pragma unroll
-            for (int k = 0; k < NQ; ++k) qf[k][ks] = r[k];
+            for (int k = 0; k < NQ; ++k) {
+                qf[k][ks] = r[k];
+                // (in accumulation registers, where the products read it as it is: what vector instructions work on has the others)
+                if constexpr (D == 256) asm volatile("" : "+a"(qf[k][ks]));
+            }
         }
     }
 
