@@ -115,8 +115,14 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
 
     const k_frag kf(lane, G_B);
     const v_frag vf(lane);
-    auto k_read = [&](int st, int k, int pl) { return kf.read(k_groups(st) + 2 * (k / NKS) * G_B + pl * PL_B, k % NKS); };
-    auto v_read = [&](int st, int f, int pl) { return vf.read(v_groups(st) + (f / NDT) * G_B + pl * PL_B, f % NDT); };
+    // (stage: its place in LDS as a number the compiler does not see through - offsets from it fit the instructions, those from the start do not)
+    auto stage_of = [&](int st) {
+        int at = st * C::STAGE_B;
+        asm volatile("" : "+s"(at));
+        return (const char *) lds + at;
+    };
+    auto k_read = [&](const char * stage, int k, int pl) { return kf.read(stage + 2 * (k / NKS) * G_B + pl * PL_B, k % NKS); };
+    auto v_read = [&](const char * stage, int f, int pl) { return vf.read(stage + NG * G_B + (f / NDT) * G_B + pl * PL_B, f % NDT); };
 
     // ---- S^T of one tile: product k of NH * NKS ----
     auto s_product = [&](f16x (&s)[NH], int k, const h8 (&a)[NPL]) {
@@ -131,7 +137,9 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
     };
     // what a row does not see, where a row of the wave does not see all of the tile
     auto mask = [&](f16x (&s)[NH], int k0) {
-        const int from = k0 + 4 * g, hi = my_pos - from, lo = max(my_pos - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - from;
+        const int from = k0 + 4 * g;
+        int hi = my_pos - from, lo = max(my_pos - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - from;
+        asm volatile("" : "+v"(hi), "+v"(lo), "+v"(sk));      // (or the comparisons would be made ahead of the branch, for every tile)
 #pragma unroll
         for (int u = 0; u < NH; ++u)
 #pragma unroll
@@ -140,12 +148,14 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
                 s[u][i] = j <= hi && (j > lo || j < sk) ? s[u][i] : MINUS_INF;
             }
     };
+    float top = -MINUS_INF;
+    asm volatile("" : "+s"(top));
     auto most_of = [&](const f16x (&s)[NH]) {
         float m = MINUS_INF;
 #pragma unroll
         for (int u = 0; u < NH; ++u)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) m = fmaxf(m, s[u][i]);
+            for (int i = 0; i < 16; ++i) m = larger(m, s[u][i], top);
         return m;
     };
     auto whole = [&](int k0) { return k0 + BN - 1 <= all_hi && k0 >= all_lo; };
@@ -154,6 +164,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
     // ---- a step: P of this tile beside the products S^T of the next one, then O^T beside the next one's maximum. The loads of K two tiles on and V one
     // tile on are under way meanwhile ----
     auto step = [&](int st, int next, f16x (&s)[NH], f16x (&sn)[NH], auto && more_loads) {
+        const char * const here = stage_of(st), * const after = stage_of(st ^ 1);
         const bool fresh = ref == MINUS_INF, move = mx > (fresh ? MINUS_INF : ref + (HEAD + STEP));
         if (__builtin_expect(__any(move), 0)) {
             const float to = move ? mx - HEAD : ref, alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(ref - to);   // (fresh: nothing accumulated)
@@ -173,7 +184,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
 #pragma unroll
         for (int k = 0; k < PF_K; ++k)
 #pragma unroll
-            for (int pl = 0; pl < NPL; ++pl) fr[k][pl] = k_read(st ^ 1, k, pl);
+            for (int pl = 0; pl < NPL; ++pl) fr[k][pl] = k_read(after, k, pl);
         more_loads();
 #pragma unroll
         for (int k = 0; k < NK; ++k) {
@@ -181,7 +192,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
 #pragma unroll
             for (int pl = 0; pl < NPL; ++pl) {
                 a[pl] = fr[k % PF_K][pl];
-                if (k + PF_K < NK) fr[k % PF_K][pl] = k_read(st ^ 1, k + PF_K, pl);
+                if (k + PF_K < NK) fr[k % PF_K][pl] = k_read(after, k + PF_K, pl);
             }
             s_product(sn, k, a);
 #pragma unroll
@@ -190,6 +201,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
                 const float p0 = __builtin_amdgcn_exp2f(fmaf(s[u][i], factor, nr)), p1 = __builtin_amdgcn_exp2f(fmaf(s[u][i + 1], factor, nr));
                 ls[0] += p0;
                 ls[1] += p1;
+                asm volatile("" : "+v"(ls[0]), "+v"(ls[1]));  // (here: put off, all of P would stay in registers)
                 h2 h = __builtin_convertvector(f2w{p0, p1}, h2);
                 asm("" : "+v"(h));
                 pb[0][2 * u + (i >> 3)][i & 7] = h[0];
@@ -206,7 +218,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
 #pragma unroll
         for (int f = 0; f < PF_V; ++f)
 #pragma unroll
-            for (int pl = 0; pl < NPL; ++pl) fv[f][pl] = v_read(st, f, pl);
+            for (int pl = 0; pl < NPL; ++pl) fv[f][pl] = v_read(here, f, pl);
         mx = MINUS_INF;
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
@@ -215,13 +227,13 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
 #pragma unroll
             for (int pl = 0; pl < NPL; ++pl) {
                 a[pl] = fv[f % PF_V][pl];
-                if (f + PF_V < NF) fv[f % PF_V][pl] = v_read(st, f + PF_V, pl);
+                if (f + PF_V < NF) fv[f % PF_V][pl] = v_read(here, f + PF_V, pl);
             }
             o[dt] = mfma32(a[0], pb[0][ps], o[dt]);
             if constexpr (EXACT) o[dt] = mfma32(a[0], pb[NQ - 1][ps], o[dt]);
             if constexpr (NPL == 2) o[dt] = mfma32(a[NPL - 1], pb[0][ps], o[dt]);
 #pragma unroll
-            for (int v = f * NV / NF; v < (f + 1) * NV / NF; ++v) mx = fmaxf(mx, sn[v >> 4][v & 15]);
+            for (int v = f * NV / NF; v < (f + 1) * NV / NF; ++v) mx = larger(mx, sn[v >> 4][v & 15], top);
             asm volatile("" : "+v"(mx));
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -252,7 +264,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
             for (int k = 0; k < NH * NKS; ++k) {
                 h8 a[NPL];
 #pragma unroll
-                for (int pl = 0; pl < NPL; ++pl) a[pl] = k_read(0, k, pl);
+                for (int pl = 0; pl < NPL; ++pl) a[pl] = k_read(lds, k, pl);
                 s_product(sa, k, a);
             }
             if (!whole(tile(ta) * BN)) mask(sa, tile(ta) * BN);

@@ -300,7 +300,9 @@ __global__ void __launch_bounds__(NTHR, 2) mass_k(const mass_params P) {
             for (int u = 0; u < NU; ++u) {
                 const int k0 = tile[u] * 32;
                 if (!__all(my.pos >= k0 + 31 && k0 > my.pos - P.R.window)) {   // (else every row of the 32 sees every key of the tile)
-                    const int at = k0 + 4 * g, hi = my.pos - at, lo = max(my.pos - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - at;
+                    const int at = k0 + 4 * g;
+                    int hi = my.pos - at, lo = max(my.pos - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - at;
+                    asm volatile("" : "+v"(hi), "+v"(lo), "+v"(sk));   // (or the comparisons would be made ahead of the branch, for every tile)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         const int j = mfma_row(i, 0);         // (and 4 g: a number the comparison holds itself)

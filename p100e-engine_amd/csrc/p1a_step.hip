@@ -209,7 +209,9 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
         if (!(k0 + 31 <= all_hi && k0 >= all_lo)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int from = k0 + 4 * g, hi = pos[n] - from, lo = max(pos[n] - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - from;
+                const int from = k0 + 4 * g;
+                int hi = pos[n] - from, lo = max(pos[n] - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - from;
+                asm volatile("" : "+v"(hi), "+v"(lo), "+v"(sk));   // (or the comparisons would be made ahead of the branch, for every tile)
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll

@@ -268,6 +268,8 @@ struct v_frag {
 
 __device__ __forceinline__ f16x mfma32(h8 a, h8 b, f16x c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ f4 mfma16(h8 a, h8 b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+// the larger of two numbers, in one instruction (fmaxf has to make a NaN quiet first). top: infinity, in a register the compiler knows nothing about
+__device__ __forceinline__ float larger(float a, float b, float top) { return __builtin_amdgcn_fmed3f(a, b, top); }
 // row of value i of a lane (half g) of a 32 x 32 result
 __device__ __forceinline__ constexpr int mfma_row(int i, int g) { return 8 * (i >> 2) + 4 * g + (i & 3); }
 
