@@ -74,22 +74,24 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
     auto k_groups = [&](int st) { return lds + st * C::STAGE_B; };
     auto v_groups = [&](int st) { return lds + st * C::STAGE_B + NG * G_B; };
 
-    int page = ta < tb ? page_of(sp.tile(ta)) : 0;
-
     // ---- Q^T operands: lane (row c, half g) holds dims 16 ks + 8 g .. + 7 ----
     h8 qf[NQ][NKS];
     float factor = P.factor;
-    {
+    auto load_q = [&] {
         f4 x[NKS][2];
         float most = 0.f;
+        auto fetch = [&](auto as_bf16) {
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) x[ks][e] = q4_at(P.q, as_bf16, my_index * D + 16 * ks + 8 * g + 4 * e);
+        };
+        if (P.q_bf16) fetch(std::true_type{});
+        else fetch(std::false_type{});
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                x[ks][e] = q4_at(P.q, P.q_bf16, my_index * D + 16 * ks + 8 * g + 4 * e);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(x[ks][e][i]));
-            }
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[ks][e >> 2][e & 3]));
         const int ex = row_exponent(max_swap32(most));
         factor = ldexpf(factor, ex);
         const float by = ldexpf(P.sign, -ex);
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
                 if constexpr (D == 256) asm volatile("" : "+a"(qf[k][ks]));
             }
         }
-    }
+    };
 
     f16x o[NDT];
 #pragma unroll
@@ -161,9 +163,10 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
     auto whole = [&](int k0) { return k0 + BN - 1 <= all_hi && k0 >= all_lo; };
     float mx = MINUS_INF;                                     // the row's largest score of the tile in hand
 
+    constexpr int NPC = (BOTH ? 2 : 1) * G::PIECES;           // loads of a step
     // ---- a step: P of this tile beside the products S^T of the next one, then O^T beside the next one's maximum. The loads of K two tiles on and V one
     // tile on are under way meanwhile ----
-    auto step = [&](int st, int next, f16x (&s)[NH], f16x (&sn)[NH], auto && more_loads) {
+    auto step = [&](int st, int next, f16x (&s)[NH], f16x (&sn)[NH], auto && piece) __attribute__((always_inline)) {
         const char * const here = stage_of(st), * const after = stage_of(st ^ 1);
         const bool fresh = ref == MINUS_INF, move = mx > (fresh ? MINUS_INF : ref + (HEAD + STEP));
         if (__builtin_expect(__any(move), 0)) {
@@ -185,9 +188,8 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
         for (int k = 0; k < PF_K; ++k)
 #pragma unroll
             for (int pl = 0; pl < NPL; ++pl) fr[k][pl] = k_read(after, k, pl);
-        more_loads();
-#pragma unroll
-        for (int k = 0; k < NK; ++k) {
+        static_assert(NPC <= NK);
+        each<NK>([&](auto k) __attribute__((always_inline)) {
             h8 a[NPL];
 #pragma unroll
             for (int pl = 0; pl < NPL; ++pl) {
@@ -195,6 +197,8 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
                 if (k + PF_K < NK) fr[k % PF_K][pl] = k_read(after, k + PF_K, pl);
             }
             s_product(sn, k, a);
+            // (a load now and then: one behind the other they would hold the wave for as long as the compute unit takes for all of them)
+            if constexpr (k * NPC % NK < NPC) piece(std::integral_constant<int, k * NPC / NK>{});
 #pragma unroll
             for (int v = k * NV / NK / 2 * 2; v < (k + 1) * NV / NK / 2 * 2; v += 2) {   // pairs of values of P
                 const int u = v >> 4, i = v & 15;
@@ -212,7 +216,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
                 }
             }
             __builtin_amdgcn_sched_barrier(0);
-        }
+        });
         l += ls[0] + ls[1];
         h8 fv[PF_V][NPL];
 #pragma unroll
@@ -244,20 +248,34 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
         mx = max_swap32(mx) * factor;
     };
 
-    // ---- the walk. K of tile i and V of tile i - 1 are fetched into stage i & 1 together with nothing else in flight; page-table entries a tile ahead ----
-    constexpr auto done = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
-    auto run = [&](auto && k_fetch, auto && k_put, auto && v_fetch, auto && v_put) {
-        if (ta >= tb) return;
+    // ---- the walk. Stage i & 1 holds K of tile i and V of tile i; page-table entries are asked for a tile ahead of the rows ----
+    // 64-key tiles: a wave has its group of K and of V; 32: one of the two
+    typename G::raw rk, rv;
+    const gbytes k_from = (gbytes) (my_v ? P.vc : P.kc), v_from = (gbytes) P.vc;
+    // load y of those of a step: K of its tile + 2 into stage k_st, V of its tile + 1 into the other one
+    auto piece = [&](auto y, int k_st, size_t row_k, size_t row_v) __attribute__((always_inline)) {
+        if constexpr (BOTH && y >= G::PIECES) G::template piece<y - G::PIECES>(rv, v_from + row_v, v_groups(k_st ^ 1) + grp * G_B, lane);
+        else G::template piece<y>(rk, k_from + (my_v ? row_v : row_k), (my_v ? v_groups(k_st ^ 1) : k_groups(k_st)) + grp * G_B, lane);
+    };
+    auto put = [&](int k_st) {                                // (what came through registers)
+        if constexpr (!G::DIRECT) {
+            G::store(rk, (my_v ? v_groups(k_st ^ 1) : k_groups(k_st)) + grp * G_B, lane);
+            if constexpr (BOTH) G::store(rv, v_groups(k_st ^ 1) + grp * G_B, lane);
+        }
+    };
+    auto done = [] { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+    if (ta < tb) {
         auto tile = [&](int i) { return sp.tile(min(i, tb - 1)); };          // (past the last: that one once more, unused)
-        size_t row_v = row_of(tile(ta), page), row_k;
-        page = page_of(tile(ta + 1));
-        k_fetch(0, row_v);
-        k_put(0);
-        row_k = row_of(tile(ta + 1), page);
+        int page = page_of(tile(ta)), page1 = page_of(tile(ta + 1));
+        size_t row_v = row_of(tile(ta), page), row_k = row_of(tile(ta + 1), page1);
         page = page_of(tile(ta + 2));
-        done();
-        k_fetch(1, row_k);
-        v_fetch(0, row_v);
+        // K of the first tile into stage 0 (quantized: and V into stage 1, where nobody looks at it), then K of the second and V of the first
+        each<G::DIRECT ? G::PIECES : NPC>([&](auto y) __attribute__((always_inline)) { piece(y, 0, row_v, row_v); });
+        if constexpr (!G::DIRECT) put(0);
+        each<NPC>([&](auto y) __attribute__((always_inline)) { piece(y, 1, row_k, row_v); });
+        load_q();
+        if constexpr (!G::DIRECT) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else done();
         f16x sa[NH], sb[NH];
         if (wrows > 0) {
 #pragma unroll
@@ -270,22 +288,16 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
             if (!whole(tile(ta) * BN)) mask(sa, tile(ta) * BN);
             mx = max_swap32(most_of(sa)) * factor;
         }
-        k_put(1);
-        v_put(0);
+        put(1);
         done();
         // tile i: K(i + 1) and V(i) are there; K(i + 2) goes where K(i) was, V(i + 1) where V(i - 1) was
-        auto turn = [&](int i, int st, f16x (&s)[NH], f16x (&sn)[NH]) {
-            auto loads = [&] {
-                row_v = row_k;
-                row_k = row_of(tile(i + 2), page);
-                page = page_of(tile(i + 3));
-                k_fetch(st, row_k);
-                v_fetch(st ^ 1, row_v);
-            };
-            if (wrows > 0) step(st, tile(i + 1), s, sn, loads);
-            else loads();
-            k_put(st);
-            v_put(st ^ 1);
+        auto turn = [&](int i, int st, f16x (&s)[NH], f16x (&sn)[NH]) __attribute__((always_inline)) {
+            row_v = row_k;
+            row_k = row_of(tile(i + 2), page);
+            page = page_of(tile(i + 3));
+            if (wrows > 0) step(st, tile(i + 1), s, sn, [&](auto y) __attribute__((always_inline)) { piece(y, st, row_k, row_v); });
+            else each<NPC>([&](auto y) __attribute__((always_inline)) { piece(y, st, row_k, row_v); });
+            put(st);
             done();
         };
         for (int i = ta;;) {
@@ -294,17 +306,6 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
             turn(i, 1, sb, sa);
             if (++i == tb) break;
         }
-    };
-    if constexpr (G::DIRECT) {
-        auto nothing = [](int) {};
-        run([&](int st, size_t row) { if (BOTH || !my_v) G::load((gbytes) P.kc + row, k_groups(st) + grp * G_B, lane); }, nothing,
-            [&](int st, size_t row) { if (BOTH || my_v) G::load((gbytes) P.vc + row, v_groups(st) + grp * G_B, lane); }, nothing);
-    } else {
-        typename G::raw rk, rv;                               // (32-key tiles: a wave has one of the two)
-        run([&](int, size_t row) { if (BOTH || !my_v) G::load(rk, (gbytes) P.kc + row, lane); },
-            [&](int st) { if (BOTH || !my_v) G::store(rk, k_groups(st) + grp * G_B, lane); },
-            [&](int, size_t row) { if (BOTH || my_v) G::load(rv, (gbytes) P.vc + row, lane); },
-            [&](int st) { if (BOTH || my_v) G::store(rv, v_groups(st) + grp * G_B, lane); });
     }
 
     // ---- results: lane (row c, half g) holds dims 32 dt + 8 (i / 4) + 4 g + i % 4 ----

@@ -3,11 +3,16 @@
 #include "p1a_common.hpp"
 
 #include <type_traits>
+#include <utility>
 
 namespace p1a {
 
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float MINUS_INF = -__builtin_inff();
+
+// f(0), f(1) ... f(N - 1), each with its number as a constant
+template <int... I, typename F> __device__ __forceinline__ void each_of(std::integer_sequence<int, I...>, F && f) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, typename F> __device__ __forceinline__ void each(F && f) { each_of(std::make_integer_sequence<int, N>{}, f); }
 
 // ---- rows of several sequences (p1a_rows as the kernels take it) ----
 struct rows_view {
@@ -159,25 +164,31 @@ template <uint32_t KT, int D, int NPL> struct group;
 template <int D, int NPL> struct group<P1A_KV_F16, D, NPL> {
     static constexpr bool DIRECT = true;
     static __device__ __forceinline__ int key(int lane) { return (lane & 15) ^ (4 * (lane >> 4)); }
-    // straight to LDS: complete when vmcnt says so
+    static constexpr int PIECES = D / 32;                     // loads of a group
+    struct raw {};
+    // load j, straight to LDS: complete when vmcnt says so. (The instruction adds its offset to both addresses.)
+    template <int j> static __device__ __forceinline__ void piece(raw &, gbytes row, char * to, int lane) {
+        asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off offset:%3" :: "v"(row + (lane >> 4) * 16), "s"(__builtin_amdgcn_readfirstlane(lds_at(to))), "i"(960 * j), "i"(64 * j)
+                     : "memory", "m0", "scc");
+    }
     static __device__ __forceinline__ void load(gbytes row, char * to, int lane) {
-        gbytes p = row + (lane >> 4) * 16;
-        const uint32_t at = __builtin_amdgcn_readfirstlane(lds_at(to));
-#pragma unroll
-        for (int j = 0; j < D / 32; ++j)
-            asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(p + 64 * j), "s"(at), "i"(1024 * j) : "memory", "m0", "scc");
+        raw r;
+        each<PIECES>([&](auto j) __attribute__((always_inline)) { piece<j>(r, row, to, lane); });
     }
 };
 
 template <int D, int NPL> struct group<P1A_KV_Q8_0, D, NPL> {
     static constexpr bool DIRECT = false;
     static constexpr int NJ = D / 64, NB = D / 32;            // loads of 16 codes a lane; blocks of a row
+    static constexpr int PIECES = NJ + 1;
     struct raw { u4 w[NJ]; uint32_t d[NB / 2]; };
     static __device__ __forceinline__ int key(int lane) { return lane & 15; }
     static __device__ __forceinline__ void load(raw & r, gbytes row, int lane) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) r.w[j] = gload<u4_a4>(row + 2 * NB + (4 * j + (lane >> 4)) * 16);
-        if constexpr (NB == 8) { const u4 t = gload<u4_a4>(row); r.d[0] = t[0]; r.d[1] = t[1]; r.d[2] = t[2]; r.d[3] = t[3]; }
+        each<PIECES>([&](auto j) __attribute__((always_inline)) { piece<j>(r, row, nullptr, lane); });
+    }
+    template <int j> static __device__ __forceinline__ void piece(raw & r, gbytes row, char *, int lane) {
+        if constexpr (j < NJ) r.w[j] = gload<u4_a4>(row + 2 * NB + (4 * j + (lane >> 4)) * 16);
+        else if constexpr (NB == 8) { const u4 t = gload<u4_a4>(row); r.d[0] = t[0]; r.d[1] = t[1]; r.d[2] = t[2]; r.d[3] = t[3]; }
         else if constexpr (NB == 4) { const u2w t = gload<u2_a4>(row); r.d[0] = t[0]; r.d[1] = t[1]; }
         else r.d[0] = gload<uint32_t>(row);
     }
@@ -205,15 +216,16 @@ template <int D, int NPL> struct group<P1A_KV_Q8_0, D, NPL> {
 template <int D, int NPL> struct group<P1A_KV_Q4_0, D, NPL> {
     static constexpr bool DIRECT = false;
     static constexpr int NB = D / 32, NJ = (NB + 3) / 4;      // blocks of a row; of a lane
+    static constexpr int PIECES = NJ;
     struct raw { u4 w[NJ]; uint32_t d[NJ]; };
     static __device__ __forceinline__ int key(int lane) { return lane & 15; }
+    template <int j> static __device__ __forceinline__ void piece(raw & r, gbytes row, char *, int lane) {
+        const gbytes b = row + min(4 * j + (lane >> 4), NB - 1) * 18;
+        r.d[j] = gload<uint16_t>(b);
+        r.w[j] = gload<u4_a2>(b + 2);
+    }
     static __device__ __forceinline__ void load(raw & r, gbytes row, int lane) {
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const gbytes b = row + min(4 * j + (lane >> 4), NB - 1) * 18;
-            r.d[j] = gload<uint16_t>(b);
-            r.w[j] = gload<u4_a2>(b + 2);
-        }
+        each<PIECES>([&](auto j) __attribute__((always_inline)) { piece<j>(r, row, nullptr, lane); });
     }
     static __device__ __forceinline__ void store(const raw & r, char * to, int lane) {
         const int k = lane & 15;
