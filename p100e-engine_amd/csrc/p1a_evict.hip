@@ -6,7 +6,8 @@ namespace {
 
 // ---- which positions stay ----
 // One workgroup per (sequence, kv head): the want-th largest of the positions between the sinks and the last ones by radix selection, 8 bits of the
-// value a pass, then one pass that lists what is above it, and of what equals it the first ones, in order. A thread holds 16 consecutive values of a part
+// value a pass - until what shares the digits so far is wanted as a whole -, then one pass that lists what is above it, and of what equals it the first
+// ones, in order. A thread holds 16 consecutive values of a part
 // of 16384; longer rows are read again for each pass (from L2). Counts go to 32 copies of the histogram, one for every other lane: values of one order of
 // magnitude share their first digit, and additions to one address wait for each other.
 constexpr int STHR = 1024, PER = 16, PART = STHR * PER;
@@ -22,7 +23,7 @@ __global__ void __launch_bounds__(STHR) select_k(const float * mass, int ld, con
     __shared__ uint32_t hist[256 * HS];
     __shared__ uint32_t count[256];
     __shared__ uint32_t wsum[STHR / 64];
-    __shared__ uint32_t found[2];                             // digit, how many of it are still wanted
+    __shared__ uint32_t found[3];                             // digit, how many of it are still wanted, how many there are
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = blockIdx.x, s = blockIdx.y;
     const size_t row = (size_t) s * gridDim.x + h;
     const float * const m = mass + row * ld;
@@ -55,7 +56,7 @@ __global__ void __launch_bounds__(STHR) select_k(const float * mass, int ld, con
             for (int x = 0; x < PER; ++x) key[x] = i0 + x < b ? key_of(m[i0 + x]) : 0u;
         }
     };
-    uint32_t prefix = 0, left = (uint32_t) want;
+    uint32_t prefix = 0, left = (uint32_t) want, low = 0;
     for (int shift = 24; shift >= 0; shift -= 8) {
         for (int i = tid; i < 256 * HS; i += STHR) hist[i] = 0;
         __syncthreads();
@@ -86,7 +87,7 @@ __global__ void __launch_bounds__(STHR) select_k(const float * mass, int ld, con
             if (before < left && left <= upto) {
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    if (before < left && left <= before + c[x]) { found[0] = 255 - 4 * lane - x; found[1] = left - before; }
+                    if (before < left && left <= before + c[x]) { found[0] = 255 - 4 * lane - x; found[1] = left - before; found[2] = c[x]; }
                     before += c[x];
                 }
             }
@@ -94,17 +95,19 @@ __global__ void __launch_bounds__(STHR) select_k(const float * mass, int ld, con
         __syncthreads();
         prefix |= found[0] << shift;
         left = found[1];
+        low = found[2] == left ? prefix : prefix + 1;         // (no value has the largest key)
+        if (low == prefix) break;
         __syncthreads();
     }
-    // above `prefix`: all; equal to it: the first `left`
+    // from `low` on: all; equal to `prefix` below it: the first `left`
     uint32_t gt0 = 0, eq0 = 0;                                // of the parts behind
     for (int part = 0; part < parts; ++part) {
         hold(part);
         const int i0 = a + part * PART + tid * PER, live = b - i0;
-        uint32_t mine = 0;                                    // above, and equal in the upper half
+        uint32_t mine = 0;                                    // from `low` on, and equal in the upper half
 #pragma unroll
         for (int x = 0; x < PER; ++x)
-            if (x < live) mine += key[x] > prefix ? 1u : key[x] == prefix ? 0x10000u : 0u;
+            if (x < live) mine += key[x] >= low ? 1u : key[x] == prefix ? 0x10000u : 0u;
         uint32_t upto = mine;
         for (int d = 1; d < 64; d <<= 1) { const uint32_t y = __shfl_up(upto, d); if (lane >= d) upto += y; }
         if (lane == 63) wsum[wave] = upto;
@@ -115,7 +118,7 @@ __global__ void __launch_bounds__(STHR) select_k(const float * mass, int ld, con
 #pragma unroll
         for (int x = 0; x < PER; ++x) {
             if (x >= live) break;
-            const bool above = key[x] > prefix, equal = key[x] == prefix;
+            const bool above = key[x] >= low, equal = !above && key[x] == prefix;
             if (above || (equal && eq < left)) keep[n_sink + gt + min(eq, left)] = i0 + x;
             gt += above;
             eq += equal;
@@ -182,26 +185,50 @@ template <int W> __global__ void __launch_bounds__(MTHR) move_k(const move_param
     char * const base = (v ? P.vc : P.kc) + (size_t) h * P.hb;
     const int per = 1 << P.per_sh, w = slice * per + (tid & (per - 1)), rpi = MTHR >> P.per_sh;
     const bool mine = w < P.words;
-    for (int k0 = 0; k0 < P.budget; k0 += rpi * DEPTH) {
-        word x[DEPTH];
-        int src[DEPTH];
-        size_t to[DEPTH];
+    // Three things in a row - which position, its page, its bytes - asked for in one go, of three stretches: positions two ahead, pages one
+    auto kept = [&](int (&src)[DEPTH], int k0) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
             const int k = k0 + d * rpi + (tid >> P.per_sh);
             src[d] = mine && k < P.budget ? keep[k] : -1;
-            if (src[d] <= k || src[d] >= P.n_ctx) src[d] = -1;
         }
+    };
+    auto moves = [&](int from, int k) { return from > k && from < P.n_ctx; };
+    auto pages = [&](const int (&src)[DEPTH], int (&fp)[DEPTH], int (&tp)[DEPTH], int k0) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-            if (src[d] < 0) continue;
             const int k = k0 + d * rpi + (tid >> P.per_sh);
-            x[d] = *(gword) (base + kv_off_tab(P.pg, ptab, src[d]) + (size_t) w * W);
-            to[d] = kv_off_tab(P.pg, ptab, k) + (size_t) w * W;
+            const bool go = moves(src[d], k);
+            fp[d] = go && ptab ? ptab[src[d] >> P.pg.psh] : 0;
+            tp[d] = go && ptab ? ptab[k >> P.pg.psh] : 0;
         }
+    };
+    auto where = [&](int j, int page) {
+        return (ptab ? (size_t) page * P.pg.pstride + (size_t) (j & ((1 << P.pg.psh) - 1)) * P.pg.rowb : (size_t) j * P.pg.rowb) + (size_t) w * W;
+    };
+    const int step = rpi * DEPTH;
+    int src[DEPTH], next[DEPTH], fp[DEPTH], tp[DEPTH];
+    kept(src, 0);
+    kept(next, step);
+    pages(src, fp, tp, 0);
+    for (int k0 = 0; k0 < P.budget; k0 += step) {
+        word x[DEPTH];
+        size_t to[DEPTH];
+        bool go[DEPTH];
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+            const int k = k0 + d * rpi + (tid >> P.per_sh);
+            go[d] = moves(src[d], k);
+            if (go[d]) x[d] = *(gword) (base + where(src[d], fp[d]));
+            to[d] = where(k, tp[d]);
+        }
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) src[d] = next[d];
+        pages(src, fp, tp, k0 + step);
+        kept(next, k0 + 2 * step);
         all_fetched();
 #pragma unroll
-        for (int d = 0; d < DEPTH; ++d) if (src[d] >= 0) *(gword) (base + to[d]) = x[d];
+        for (int d = 0; d < DEPTH; ++d) if (go[d]) *(gword) (base + to[d]) = x[d];
     }
 }
 

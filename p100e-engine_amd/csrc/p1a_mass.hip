@@ -141,21 +141,21 @@ __global__ void __launch_bounds__(NTHR, D == 256 && NT == 2 ? 1 : 2) mass_step_k
 }
 
 // ---- many rows ----
+constexpr int MW = 8, MTHR = MW * 64;                         // waves of a workgroup
 template <uint32_t KT, int D> struct mass_cfg {
-    static constexpr int NPL = group_planes(KT, true), NU = NPL == 2 && D == 256 ? 1 : 2, BK = NW * 32 * NU;
+    static constexpr int NPL = group_planes(KT, true), NU = NPL == 2 && D == 256 ? 1 : 2, BK = MW * 32 * NU;
     static constexpr int G_B = NPL * plane_bytes(D);
-    static constexpr int AT_ONCE = NPL == 2 && D == 256 ? 1 : 2;             // groups of 16 keys of a wave on their way to its registers: two workgroups' LDS
-    static constexpr int K_B = NW * AT_ONCE * G_B;
+    static constexpr int AT_ONCE = std::min(2 * NU, 16384 / G_B);            // groups of 16 keys of a wave on their way to its registers: 128 KB of LDS
+    static constexpr int K_B = MW * AT_ONCE * G_B;
     static constexpr int Q_B = 2 * 2 * plane_bytes(D);        // 32 rows in two halves
     static constexpr int ROWS_AT = std::max(K_B, 2 * Q_B), LDS = ROWS_AT + 2 * QR * 12;   // (the rows go where the keys were)
 };
 
 template <uint32_t KT, int D>
-__global__ void __launch_bounds__(NTHR, 2) mass_k(const mass_params P) {
+__global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
     using C = mass_cfg<KT, D>;
     using G = group<KT, D, C::NPL>;
-    constexpr int NPL = C::NPL, NU = C::NU, G_B = C::G_B, PL_B = plane_bytes(D), NKS = D / 16, NJ = D / 64, TB = NW * NU;   // TB: tiles of a block
-    constexpr bool LATE = NU * NPL * D >= 512;                // the next rows are asked for behind half of the weights, not ahead of the products: registers
+    constexpr int NPL = C::NPL, NU = C::NU, G_B = C::G_B, PL_B = plane_bytes(D), NKS = D / 16, NJ = (D + 127) / 128, TB = MW * NU;   // TB: tiles of a block
     extern __shared__ __attribute__((aligned(16))) char lds[];
     struct row_info { float factor, lse; int pos; };
     row_info * const info = reinterpret_cast<row_info *>(lds + C::ROWS_AT);   // [2][QR]
@@ -177,18 +177,18 @@ __global__ void __launch_bounds__(NTHR, 2) mass_k(const mass_params P) {
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));
     const int c = lane & 31, g = lane >> 5;
-    const k_frag qfr(lane, PL_B);
-    // Rows of q as the operand's columns. Wave w brings rows 8 w .. 8 w + 7 of the 32: lane (row lane % 8, chunk 8 j + lane / 8)
-    const int qrow = 8 * wave + (lane & 7);
+    // Rows of q as the operand's columns. Wave w brings rows 4 w .. 4 w + 3 of the 32: lane (row lane % 4, chunk 16 j + lane / 4; heads of 64: twice)
+    auto qrow_of = [&] { return 4 * wave + (lane & 3); };
+    auto qchunk_of = [&] { return (lane >> 2) & (D / 8 - 1); };
     struct rows_raw { f4 x[NJ][2]; float lse; int pos; };
     auto fetch_rows = [&](rows_raw & r, int r0) {
-        const int row = min(r0 + qrow, nrows - 1), t = token_of(P, row);
+        const int qrow = qrow_of(), qchunk = qchunk_of(), row = min(r0 + qrow, nrows - 1), t = token_of(P, row);
         const size_t i = (size_t) (sv.first + t) * P.Hq + (size_t) hk * P.GQA + (row - t * P.GQA);
         auto fetch = [&](auto as_bf16) {
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) r.x[j][e] = q4_at(P.q, as_bf16, i * D + (8 * j + (lane >> 3)) * 8 + 4 * e);
+                for (int e = 0; e < 2; ++e) r.x[j][e] = q4_at(P.q, as_bf16, i * D + (16 * j + qchunk) * 8 + 4 * e);
         };
         if (P.q_bf16) fetch(std::true_type{});
         else fetch(std::false_type{});
@@ -197,11 +197,13 @@ __global__ void __launch_bounds__(NTHR, 2) mass_k(const mass_params P) {
         if (r0 + qrow >= nrows || r.pos < 0 || r.pos >= P.R.n_ctx || r.lse == MINUS_INF) r.pos = -1;   // sees nothing
     };
     auto put_rows = [&](const rows_raw & r, int st) {
+        const int qrow = qrow_of(), qchunk = qchunk_of();
         float most = 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(r.x[j][e >> 2][e & 3]));
+        most = fmaxf(most, __shfl_xor(most, 4));
         most = fmaxf(most, __shfl_xor(most, 8));
         most = max_swap32(max_swap16(most));
         const int ex = row_exponent(most);
@@ -211,45 +213,48 @@ __global__ void __launch_bounds__(NTHR, 2) mass_k(const mass_params P) {
         for (int j = 0; j < NJ; ++j) {
             h8 y[2];
             halves<2>([&](int e) { return r.x[j][e >> 2][e & 3]; }, [&](int) { return by; }, y);
-            char * const at = to + chunk_at(qrow & 15, 8 * j + (lane >> 3));
+            char * const at = to + chunk_at(qrow & 15, 16 * j + qchunk);
             *reinterpret_cast<h8 *>(at) = y[0];
             *reinterpret_cast<h8 *>(at + 2 * PL_B) = y[1];
         }
-        if (lane < 8) info[st * QR + qrow] = row_info{ldexpf(P.factor, ex), -r.lse * LOG2E, r.pos};
+        if (lane < 4) info[st * QR + qrow] = row_info{ldexpf(P.factor, ex), -r.lse * LOG2E, r.pos};
     };
 
-        // ---- this wave's keys, 16 at a time through LDS ----
+        // ---- this wave's keys, AT_ONCE groups of 16 at a time through LDS ----
         h8 kr[NU][NPL][NKS];
         int tile[NU];
+        size_t from[2 * NU];
 #pragma unroll
         for (int u = 0; u < NU; ++u) {
             tile[u] = sp.tile(min(b + wave * NU + u, sp.nt - 1));
-            char * const to = lds + wave * C::AT_ONCE * G_B;
-            const k_frag kf(C::AT_ONCE == 2 ? lane : lane & ~16, G_B);   // (one at a time: row c % 16 of the group that is there)
 #pragma unroll
-            for (int x0 = 0; x0 < 2; x0 += C::AT_ONCE) {
+            for (int x = 0; x < 2; ++x) from[2 * u + x] = head_off + kv_off_tab(P.pg, ptab, seen_or_near<32>(sp, tile[u] * 32, tile[u] * 32 + 16 * x + G::key(lane)));
+        }
+        char * const to = lds + wave * C::AT_ONCE * G_B;
 #pragma unroll
-                for (int x = x0; x < x0 + C::AT_ONCE; ++x) {
-                    const int j = seen_or_near<32>(sp, tile[u] * 32, tile[u] * 32 + 16 * x + G::key(lane));
-                    const size_t row = head_off + kv_off_tab(P.pg, ptab, j);
-                    if constexpr (G::DIRECT) G::load((gbytes) P.kc + row, to + (x - x0) * G_B, lane);
-                    else {
-                        typename G::raw raw;
-                        G::load(raw, (gbytes) P.kc + row, lane);
-                        G::store(raw, to + (x - x0) * G_B, lane);
-                    }
+        for (int x0 = 0; x0 < 2 * NU; x0 += C::AT_ONCE) {
+#pragma unroll
+            for (int x = x0; x < x0 + C::AT_ONCE; ++x) {
+                if constexpr (G::DIRECT) G::load((gbytes) P.kc + from[x], to + (x - x0) * G_B, lane);
+                else {
+                    typename G::raw raw;
+                    G::load(raw, (gbytes) P.kc + from[x], lane);
+                    G::store(raw, to + (x - x0) * G_B, lane);
                 }
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_wave_barrier();
-                if (C::AT_ONCE == 2 || (c >> 4) == x0) {
+            }
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
+            const k_frag kf(C::AT_ONCE > 1 ? lane : lane & ~16, G_B);        // (one at a time: row c % 16 of the group that is there)
+            if (C::AT_ONCE > 1 || (c >> 4) == x0) {
+#pragma unroll
+                for (int u = x0 / 2; u < (x0 + C::AT_ONCE + 1) / 2; ++u)
 #pragma unroll
                     for (int pl = 0; pl < NPL; ++pl)
 #pragma unroll
-                        for (int ks = 0; ks < NKS; ++ks) kr[u][pl][ks] = kf.read(to + pl * PL_B, ks);
-                }
-                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_wave_barrier();
+                        for (int ks = 0; ks < NKS; ++ks) kr[u][pl][ks] = kf.read(to + (2 * u - (C::AT_ONCE > 1 ? x0 : 2 * u)) * G_B + pl * PL_B, ks);
             }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __builtin_amdgcn_wave_barrier();
         }
         float acc[NU][16];
 #pragma unroll
@@ -264,14 +269,22 @@ __global__ void __launch_bounds__(NTHR, 2) mass_k(const mass_params P) {
         const int rb = (rows_end + QR - 1) / QR, per = (max(rb - ra, 0) + P.splits - 1) / P.splits;   // this split's share of them
         int r0 = (ra + split * per) * QR;
         const int r1 = min((ra + (split + 1) * per) * QR, rb * QR);
-        rows_raw rr;
-        if (r0 < r1) fetch_rows(rr, r0);
+        // rows are asked for AHEAD steps before they go to LDS: a step of short heads is over before they have come
+        constexpr int AHEAD = NU * NPL * D < 512 ? 2 : 1;
+        rows_raw ring[AHEAD];
+        if (r0 < r1) {
+            fetch_rows(ring[0], r0);
+            if (AHEAD == 2 && r0 + QR < r1) fetch_rows(ring[AHEAD - 1], r0 + QR);
+        }
         __syncthreads();                                      // (the rows go where the keys were)
-        if (r0 < r1) put_rows(rr, 0);
+        if (r0 < r1) put_rows(ring[0], 0);
         __syncthreads();
-        for (int st = 0; r0 < r1; r0 += QR, st ^= 1) {
+        auto turn = [&](int st, rows_raw & later, rows_raw & next) __attribute__((always_inline)) {
+            if (AHEAD == 1) asm volatile("" : "+v"(lane));   // (anew for each step: registers)
+            const int c = lane & 31, g = lane >> 5;
+            const k_frag qfr(lane, PL_B);
             const bool more = r0 + QR < r1;
-            if (more && !LATE) fetch_rows(rr, r0 + QR);
+            if (r0 + AHEAD * QR < r1) fetch_rows(later, r0 + AHEAD * QR);
             const row_info my = info[st * QR + c];
             f16x s[NU];
 #pragma unroll
@@ -314,13 +327,19 @@ __global__ void __launch_bounds__(NTHR, 2) mass_k(const mass_params P) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) acc[u][i] += __builtin_amdgcn_exp2f(fmaf(s[u][i], my.factor, my.lse));
                 }
-                if (LATE && u == 0) {
-                    __builtin_amdgcn_sched_barrier(0);
-                    if (more) fetch_rows(rr, r0 + QR);
-                }
             }
-            if (more) put_rows(rr, st ^ 1);
+            if (more) put_rows(next, st ^ 1);
             __syncthreads();
+            r0 += QR;
+        };
+        if constexpr (AHEAD == 1) {
+            for (int st = 0; r0 < r1; st ^= 1) turn(st, ring[0], ring[0]);
+        } else {
+            while (r0 < r1) {
+                turn(0, ring[0], ring[1]);
+                if (r0 >= r1) break;
+                turn(1, ring[1], ring[0]);
+            }
         }
         // ---- sums over the 32 rows' lanes; lane i of a half adds value i to its key ----
         asm volatile("" : "+v"(lane));
@@ -369,7 +388,7 @@ template <class F> int launch_big(F kernel, std::atomic<uint32_t> & attr_set, in
         }
         attr_set.fetch_or(bit, std::memory_order_release);
     }
-    kernel<<<grid, NTHR, lds, s>>>(P);
+    kernel<<<grid, MTHR, lds, s>>>(P);
     return launched();
 }
 template <uint32_t KT, int D> int launch_d(const mass_params & P, int few, dim3 grid, hipStream_t s) {
@@ -399,7 +418,7 @@ mass_plan plan_mass(const p1a_kv & c, const rows_view & R, int Hq, int max_n, in
         pl.runs = (int) std::max(1LL, std::min(slots * (c.D == 256 ? 1 : 2) / c.Hkv, R.n_seq * ((keys + 127) / 128)));
         return pl;
     }
-    const int BK = 128 * (planes && c.D == 256 ? 1 : 2);
+    const int BK = MW * 32 * (planes && c.D == 256 ? 1 : 2);
     pl.blocks = (int) std::min<long long>((keys + BK - 1) / BK, 65536 / c.Hkv + 1);
     const long long units = (long long) pl.blocks * c.Hkv * R.n_seq, tiles = ((long long) R.max_rows * GQA + QR - 1) / QR;
     pl.splits = (int) std::max(1LL, std::min({4 * slots / units, tiles / 16, 32LL}));
