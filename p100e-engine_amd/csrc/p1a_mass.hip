@@ -148,7 +148,7 @@ template <uint32_t KT, int D> struct mass_cfg {
     static constexpr int AT_ONCE = std::min(2 * NU, 16384 / G_B);            // groups of 16 keys of a wave on their way to its registers: 128 KB of LDS
     static constexpr int K_B = MW * AT_ONCE * G_B;
     static constexpr int Q_B = 2 * 2 * plane_bytes(D);        // 32 rows in two halves
-    static constexpr int ROWS_AT = std::max(K_B, 2 * Q_B), LDS = ROWS_AT + 2 * QR * 12;   // (the rows go where the keys were)
+    static constexpr int ROWS_AT = std::max(K_B, 4 * Q_B), LDS = ROWS_AT + 4 * QR * 12;   // (the rows go where the keys were)
 };
 
 template <uint32_t KT, int D>
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
     constexpr int NPL = C::NPL, NU = C::NU, G_B = C::G_B, PL_B = plane_bytes(D), NKS = D / 16, NJ = (D + 127) / 128, TB = MW * NU;   // TB: tiles of a block
     extern __shared__ __attribute__((aligned(16))) char lds[];
     struct row_info { float factor, lse; int pos; };
-    row_info * const info = reinterpret_cast<row_info *>(lds + C::ROWS_AT);   // [2][QR]
+    row_info * const info = reinterpret_cast<row_info *>(lds + C::ROWS_AT);   // [4][QR]
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // kv heads side by side, then the splits of a block, then blocks (those of the first keys, which most rows see, ahead)
@@ -269,35 +269,41 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
         const int rb = (rows_end + QR - 1) / QR, per = (max(rb - ra, 0) + P.splits - 1) / P.splits;   // this split's share of them
         int r0 = (ra + split * per) * QR;
         const int r1 = min((ra + (split + 1) * per) * QR, rb * QR);
-        // rows are asked for AHEAD steps before they go to LDS: a step of short heads is over before they have come
+        // Step i reads the rows in place i % 4 and brings those of step i + 2, so that the waves meet after every second step only: one's
+        // products run beside another's exponentials. Rows are asked for AHEAD steps before they go to LDS: a step of short heads is over before they come
         constexpr int AHEAD = NU * NPL * D < 512 ? 2 : 1;
         rows_raw ring[AHEAD];
-        if (r0 < r1) {
-            fetch_rows(ring[0], r0);
-            if (AHEAD == 2 && r0 + QR < r1) fetch_rows(ring[AHEAD - 1], r0 + QR);
-        }
+        if (r0 < r1) fetch_rows(ring[0], r0);
+        if (AHEAD == 2 && r0 + QR < r1) fetch_rows(ring[AHEAD - 1], r0 + QR);
         __syncthreads();                                      // (the rows go where the keys were)
         if (r0 < r1) put_rows(ring[0], 0);
+        if (AHEAD == 1 && r0 + QR < r1) fetch_rows(ring[0], r0 + QR);
+        if (r0 + QR < r1) put_rows(ring[AHEAD - 1], 1);
+        if (AHEAD == 2 && r0 + 2 * QR < r1) fetch_rows(ring[0], r0 + 2 * QR);
         __syncthreads();
         auto turn = [&](int st, rows_raw & later, rows_raw & next) __attribute__((always_inline)) {
             if (AHEAD == 1) asm volatile("" : "+v"(lane));   // (anew for each step: registers)
             const int c = lane & 31, g = lane >> 5;
             const k_frag qfr(lane, PL_B);
-            const bool more = r0 + QR < r1;
-            if (r0 + AHEAD * QR < r1) fetch_rows(later, r0 + AHEAD * QR);
+            const bool more = r0 + 2 * QR < r1;
+            if (r0 + (1 + AHEAD) * QR < r1) fetch_rows(later, r0 + (1 + AHEAD) * QR);
             const row_info my = info[st * QR + c];
             f16x s[NU];
 #pragma unroll
             for (int u = 0; u < NU; ++u)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[u][i] = 0.f;
-            h8 qn[2] = {qfr.read(lds + st * C::Q_B, 0), qfr.read(lds + st * C::Q_B + 2 * PL_B, 0)};
+            const char * const rows = lds + st * C::Q_B;
+            h8 qn[2] = {qfr.read(rows, 0), qfr.read(rows + 2 * PL_B, 0)};
+            bool all[NU];                                     // every row of the 32 sees every key of the tile
+#pragma unroll
+            for (int u = 0; u < NU; ++u) all[u] = __all(my.pos >= tile[u] * 32 + 31 && tile[u] * 32 > my.pos - P.R.window);
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks) {                // (the next step's halves of q on their way, no more: registers)
                 const h8 q0 = qn[0], q1 = qn[1];
                 if (ks + 1 < NKS) {
-                    qn[0] = qfr.read(lds + st * C::Q_B, ks + 1);
-                    qn[1] = qfr.read(lds + st * C::Q_B + 2 * PL_B, ks + 1);
+                    qn[0] = qfr.read(rows, ks + 1);
+                    qn[1] = qfr.read(rows + 2 * PL_B, ks + 1);
                 }
 #pragma unroll
                 for (int u = 0; u < NU; ++u) s[u] = mfma32(kr[u][0][ks], q0, s[u]);
@@ -312,7 +318,7 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
                 const int k0 = tile[u] * 32;
-                if (!__all(my.pos >= k0 + 31 && k0 > my.pos - P.R.window)) {   // (else every row of the 32 sees every key of the tile)
+                if (__builtin_expect(!all[u], 0)) {
                     const int at = k0 + 4 * g;
                     int hi = my.pos - at, lo = max(my.pos - k0, 0) - P.R.window - 4 * g, sk = P.R.n_sink - at;
                     asm volatile("" : "+v"(hi), "+v"(lo), "+v"(sk));   // (or the comparisons would be made ahead of the branch, for every tile)
@@ -328,17 +334,17 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
                     for (int i = 0; i < 16; ++i) acc[u][i] += __builtin_amdgcn_exp2f(fmaf(s[u][i], my.factor, my.lse));
                 }
             }
-            if (more) put_rows(next, st ^ 1);
-            __syncthreads();
+            if (more) put_rows(next, (st + 2) & 3);
             r0 += QR;
+            if (st & 1) __syncthreads();
         };
         if constexpr (AHEAD == 1) {
-            for (int st = 0; r0 < r1; st ^= 1) turn(st, ring[0], ring[0]);
+            for (int st = 0; r0 < r1; st = (st + 1) & 3) turn(st, ring[0], ring[0]);
         } else {
-            while (r0 < r1) {
-                turn(0, ring[0], ring[1]);
+            for (int st = 0; r0 < r1; st = (st + 2) & 3) {
+                turn(st, ring[1], ring[0]);
                 if (r0 >= r1) break;
-                turn(1, ring[1], ring[0]);
+                turn(st + 1, ring[0], ring[1]);
             }
         }
         // ---- sums over the 32 rows' lanes; lane i of a half adds value i to its key ----
