@@ -29,7 +29,7 @@ template <uint32_t KT, int D, int NT, bool EXACT> struct step_cfg {
     static constexpr int TAB = keys16<KT, D>::TAB;
     static constexpr int WAVE_B = V_B + 4 * TAB * 4;          // and the scales of 2 x 16 keys of K and V
     // (the low halves of q, where registers do not hold them: the same for every wave, each writes all of them)
-    static constexpr bool QL = !F16 && EXACT && NT * D >= 256;
+    static constexpr bool QL = EXACT && NT * D >= (F16 ? 512 : 256);
     static constexpr int ML_B = NW * 2 * 16 * NT * 4, LDS = NW * WAVE_B + (QL ? NT * D * 32 : 0) + (4 * TAB * 4 >= ML_B ? 0 : ML_B);
     static constexpr int ML_AT = 4 * TAB * 4 >= ML_B ? V_B : LDS - ML_B;      // (the first wave's scales are done with by then)
     static_assert(PC * (D + 4) * 4 <= V_B, "folded columns fit where V was");
