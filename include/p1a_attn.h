@@ -253,7 +253,7 @@ typedef struct p1a_rows {
  * results are within 1e-5 (relative L2) of exact ones; with bf16 results they enter rounded to f16 once. K and V values of magnitude 65504 and more
  * are beyond the products' range, as in p1a_attn_prefill. A key whose V holds an infinity or NaN reaches rows of the same sequence in the same call
  * that do not see it; keys that no row sees reach nothing.
- * D = 64, 128 or 256; Hq / Hkv up to 64; 16-byte aligned q, out and gate; f16 caches: 16-byte aligned bases and page strides, q8_0: 4-byte aligned,
+ * D = 64, 128 or 256; Hq / Hkv up to 64; T * Hq, n_ctx up to 2^30, n_seq up to 65535, Hkv up to 4096, n_seq * Hkv up to 2^22; 16-byte aligned q, out and gate; f16 caches: 16-byte aligned bases and page strides, q8_0: 4-byte aligned,
  * q4_0: 2-byte aligned; pages of any length.
  * A call of few rows is split over its keys and its partials merged by a second launch; they live in `scratch` (256-byte aligned, at least
  * p1a_attn_chunk_scratch_bytes) or, with NULL or less, in the library's buffers of (device, stream), under the rules of p1a_attn_prefill's: nothing is
@@ -271,7 +271,7 @@ size_t p1a_attn_chunk_scratch_bytes(const p1a_kv *c, const p1a_rows *rows, int H
  *     mass[s][h][j] += sum over the rows t of sequence s and the q heads i of kv head h of exp(scale * q[t][i] . K[j][h] - lse[t][i])
  * over the positions j < ld that row t sees; lse [T][Hq] as p1a_attn_chunk leaves it (a row with lse = -inf adds nothing). Entries that no row
  * sees are left as they are. f32 accuracy whatever the cache; every entry is summed in a fixed order: the same bits every time. Shapes and
- * alignment as for p1a_attn_chunk. Calls of many rows over few keys add up partial sums of the size of `mass`, in `scratch` (256-byte aligned, at
+ * alignment as for p1a_attn_chunk, ld up to 2^30. Calls of many rows over few keys add up partial sums of the size of `mass`, in `scratch` (256-byte aligned, at
  * least p1a_attn_mass_scratch_bytes) or, with NULL or less, the library's buffers, as p1a_attn_chunk's partials.
  */
 int p1a_attn_mass(const void *q, int q_type, const p1a_kv *c, const float *lse, float *mass, int ld, const p1a_rows *rows, int Hq, float scale,
@@ -283,7 +283,7 @@ size_t p1a_attn_mass_scratch_bytes(const p1a_kv *c, int ld, const p1a_rows *rows
  * Which positions of a cache stay: per sequence s and kv head the first n_sink of its n positions, the last n_recent, and of those between the
  * budget - n_sink - n_recent of the largest mass (ties: the lowest position; a NaN counts as less than everything). keep [n_seq][Hkv][budget]
  * int32 gets them in ascending order; where n <= budget all n of them, and -1 behind. n_dev [n_seq] (device; cut to 0 ... ld) or NULL: n for every
- * sequence. n_sink + n_recent <= budget <= 2^20.
+ * sequence. n_sink + n_recent <= budget <= 2^20; n_seq, Hkv, ld up to 65535, 4096, 2^30.
  */
 int p1a_evict_select(const float *mass, int ld, int n_seq, int Hkv, const int32_t *n_dev, int n, int budget, int n_sink, int n_recent,
                      int32_t *keep, void *stream);
@@ -295,7 +295,7 @@ int p1a_evict_select(const float *mass, int ld, int n_seq, int Hkv, const int32_
  * carry the rotation of their tokens' places. New tokens are appended at the next slot with their true positions as rotary ones (p1a_attn_prep:
  * p0 >= 0, or p1a_attn_prep_mrope with sect = s0 = 1 for rows of several sequences). Positions from `budget` on are as they were.
  * mass, mass_out [n_seq][Hkv][ld] (or both NULL): mass_out[s][h][k] = mass[s][h][keep[s][h][k]] for entries kept, 0 from there up to ld; mass_out ==
- * mass is allowed, partial overlap is not. Sequences (their page-table rows) must not share pages.
+ * mass is allowed, partial overlap is not. budget up to 2^20, n_seq * Hkv up to 2^20 / (16-byte pieces of a head's row). Sequences (their page-table rows) must not share pages.
  * Alignment: 2 bytes for every cache type (the move uses the widest that rows, bases and page strides have in common).
  */
 int p1a_kv_compact(const p1a_kv *c, const int32_t *keep, int n_seq, int budget, const float *mass, float *mass_out, int ld, void *stream);

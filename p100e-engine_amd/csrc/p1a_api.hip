@@ -227,8 +227,8 @@ int rows_ok(const p1a_kv * c, const p1a_rows * r, int Hq, const char * who, rows
     if (!r->pos0 && r->n_seq > 1) { set_error("%s: %d sequences need positions in device memory", who, r->n_seq); return P1A_E_ARG; }
     if (r->n_seq > 1 && (!c->pt || !c->rtab)) { set_error("%s: %d sequences need a page table and a row table", who, r->n_seq); return P1A_E_ARG; }
     if (!r->row0 && r->n_seq > 0 && r->T % r->n_seq) { set_error("%s: %d rows do not divide among %d sequences", who, r->T, r->n_seq); return P1A_E_ARG; }
-    if ((c->D != 64 && c->D != 128 && c->D != 256) || Hq < c->Hkv || Hq % c->Hkv || Hq / c->Hkv > 64 || r->n_seq > 65535 || c->Hkv > 4096 || (long long) r->T * Hq > 1 << 30) {
-        set_error("%s: unsupported shape (D=%d Hq=%d Hkv=%d T=%d n_seq=%d)", who, c->D, Hq, c->Hkv, r->T, r->n_seq);
+    if ((c->D != 64 && c->D != 128 && c->D != 256) || Hq < c->Hkv || Hq % c->Hkv || Hq / c->Hkv > 64 || r->n_seq > 65535 || c->Hkv > 4096 || (long long) r->n_seq * c->Hkv > 1 << 22 || (long long) r->T * Hq > 1 << 30 || c->n_ctx > 1 << 30) {
+        set_error("%s: unsupported shape (D=%d Hq=%d Hkv=%d T=%d n_seq=%d n_ctx=%d)", who, c->D, Hq, c->Hkv, r->T, r->n_seq, c->n_ctx);
         return P1A_E_SHAPE;
     }
     const uintptr_t al = c->type == P1A_KV_F16 ? 15 : c->type == P1A_KV_Q8_0 ? 3 : 1;
@@ -463,6 +463,7 @@ int p1a_attn_mass(const void * q, int q_type, const p1a_kv * c, const float * ls
     if (rc != P1A_OK) return rc;
     if (!q || !lse || !mass || ld < 0) { set_error("%s: null q / lse / mass or negative ld", who); return P1A_E_ARG; }
     if (!rows_type_ok(q_type, who)) return P1A_E_ARG;
+    if (ld > 1 << 30) { set_error("%s: unsupported shape (ld=%d)", who, ld); return P1A_E_SHAPE; }
     if (((uintptr_t) q & 15) || (((uintptr_t) lse | (uintptr_t) mass) & 3)) { set_error("%s: q must be 16-byte aligned, lse and mass 4-byte", who); return P1A_E_SHAPE; }
     if (!rows->T || !rows->n_seq || !ld) return P1A_OK;
     a.q = q; a.q_bf16 = q_type == P1A_ROWS_BF16; a.lse = lse; a.mass = mass; a.ld = ld; a.Hq = Hq; a.scale = scale; a.scratch = scratch; a.scratch_bytes = scratch_bytes;
@@ -472,7 +473,7 @@ int p1a_attn_mass(const void * q, int q_type, const p1a_kv * c, const float * ls
 size_t p1a_attn_mass_scratch_bytes(const p1a_kv * c, int ld, const p1a_rows * rows, int Hq) {
     rows_view R;
     int max_n;
-    if (rows_ok(c, rows, Hq, "p1a_attn_mass_scratch_bytes", R, max_n) != P1A_OK || !rows->T || !rows->n_seq || ld < 1) return 0;
+    if (rows_ok(c, rows, Hq, "p1a_attn_mass_scratch_bytes", R, max_n) != P1A_OK || !rows->T || !rows->n_seq || ld < 1 || ld > 1 << 30) return 0;
     return plan_mass(*c, R, Hq, max_n, ld, cu_count()).bytes;
 }
 
@@ -480,8 +481,8 @@ int p1a_evict_select(const float * mass, int ld, int n_seq, int Hkv, const int32
                      int32_t * keep, void * stream) {
     static const char * const who = "p1a_evict_select";
     if (!mass || !keep || ld < 0 || n_seq < 0 || Hkv < 1 || n_sink < 0 || n_recent < 0 || (!n_dev && n < 0)) { set_error("%s: null argument or a negative count", who); return P1A_E_ARG; }
-    if (budget < 0 || budget > 1 << 20 || (long long) n_sink + n_recent > budget || n_seq > 65535 || Hkv > 4096) {
-        set_error("%s: budget=%d must hold n_sink=%d and n_recent=%d and be at most 2^20", who, budget, n_sink, n_recent);
+    if (budget < 0 || budget > 1 << 20 || (long long) n_sink + n_recent > budget || n_seq > 65535 || Hkv > 4096 || ld > 1 << 30) {
+        set_error("%s: budget=%d must hold n_sink=%d and n_recent=%d and be at most 2^20, n_seq=%d, Hkv=%d, ld=%d at most 65535, 4096, 2^30", who, budget, n_sink, n_recent, n_seq, Hkv, ld);
         return P1A_E_SHAPE;
     }
     if (((uintptr_t) mass | (uintptr_t) keep) & 3) { set_error("%s: mass and keep must be 4-byte aligned", who); return P1A_E_SHAPE; }
@@ -494,7 +495,10 @@ int p1a_kv_compact(const p1a_kv * c, const int32_t * keep, int n_seq, int budget
     if (!kv_ok(c, who)) return P1A_E_ARG;
     if (!keep || n_seq < 0 || budget < 0 || !mass != !mass_out || (mass && ld < 0) || c->n_ctx < 0) { set_error("%s: null keep, a negative count, or one of mass and mass_out alone", who); return P1A_E_ARG; }
     if (n_seq > 1 && (!c->pt || !c->rtab)) { set_error("%s: %d sequences need a page table and a row table", who, n_seq); return P1A_E_ARG; }
-    if (budget > 1 << 20 || n_seq > 65535 || c->Hkv > 4096) { set_error("%s: unsupported shape (budget=%d n_seq=%d Hkv=%d)", who, budget, n_seq, c->Hkv); return P1A_E_SHAPE; }
+    if (budget > 1 << 20 || n_seq > 65535 || (long long) n_seq * c->Hkv * ((head_bytes(c->type, c->D) + 15) / 16) > 1 << 20 || (mass && ld > 1 << 30)) {
+        set_error("%s: unsupported shape (budget=%d n_seq=%d Hkv=%d D=%d ld=%d)", who, budget, n_seq, c->Hkv, c->D, ld);
+        return P1A_E_SHAPE;
+    }
     if ((((uintptr_t) c->k | (uintptr_t) c->v) & 1) || (c->pt && (c->pstride & 1)) || (((uintptr_t) keep | (uintptr_t) mass | (uintptr_t) mass_out) & 3)) {
         set_error("%s: cache base and page stride must be 2-byte aligned, keep and mass 4-byte", who);
         return P1A_E_SHAPE;

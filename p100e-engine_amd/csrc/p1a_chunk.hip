@@ -508,7 +508,7 @@ int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
         }
     }
     const long long grid = block_bound(a.R, P.GQA) * P.nks * c.Hkv;
-    if (grid > 0x7fffffffLL) { set_error("p1a_attn_chunk: too many rows for one call"); return P1A_E_SHAPE; }
+    if (grid > 0xffffff) { set_error("p1a_attn_chunk: too many rows for one call"); return P1A_E_SHAPE; }
     const bool exact = !a.out_bf16 || a.lse;
     const int rc = pl.few ? launch_step(c, P, pl.few, exact, s) : c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, exact, (unsigned) grid, s)
                  : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, exact, (unsigned) grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, exact, (unsigned) grid, s);

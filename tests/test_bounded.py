@@ -87,6 +87,20 @@ def test_arguments_refused():
     assert compact(n_seq=0) == 0 and compact(budget=0) == 0
 
 
+def test_sizes_past_the_limits():
+    """positions, totals and grids whose arithmetic would leave 32 bits"""
+    L = p1a.lib()
+    for change in (dict(n_ctx=(1 << 30) + 1), dict(Hkv=4097)):
+        assert chunk(kv=cache(**change), Hq=4097 if "Hkv" in change else 24) == SHAPE and mass(kv=cache(**change), Hq=4097 if "Hkv" in change else 24) == SHAPE, change
+    wide = dict(kv=cache(Hkv=128, pstride=1 << 24), r=rows(T=65535, n_seq=65535, max_rows=1), Hq=128)
+    assert chunk(**wide) == SHAPE and mass(**wide) == SHAPE
+    assert mass(ld=(1 << 30) + 1) == SHAPE and L.p1a_attn_mass_scratch_bytes(ctypes.byref(cache()), (1 << 30) + 1, ctypes.byref(rows()), 24) == 0
+    assert L.p1a_evict_select(4096, (1 << 30) + 1, 2, 4, None, 64, 32, 4, 8, 4096, None) == SHAPE
+    assert L.p1a_evict_select(4096, 64, 2, 4097, None, 64, 32, 4, 8, 4096, None) == SHAPE
+    assert L.p1a_kv_compact(ctypes.byref(cache()), 4096, 65535, 8, None, None, 0, None) == SHAPE
+    assert L.p1a_kv_compact(ctypes.byref(cache()), 4096, 2, 8, 4096, 4096, (1 << 30) + 1, None) == SHAPE
+
+
 def test_binding_refuses_other_types():
     torch = pytest.importorskip("torch")
     q = torch.zeros(1, 4, 64, dtype=torch.float16)

@@ -297,6 +297,24 @@ def test_mass(p1a, kv, D):
         assert np.linalg.norm(m.cpu().numpy() - want2) <= REL * np.linalg.norm(want2 - got) + 2.0 ** -24 * np.linalg.norm(want2)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("kv", list(KVS))
+def test_mass_rows_by_the_tile(p1a, kv, D):
+    """33 to 385 rows under a kv head - two to thirteen times 32, every place that rows take in turn -, several blocks of keys, positions that come to lie on
+    their ends; the tolerance is test_mass's"""
+    counts = [9, 16, 24, 25, 40, 49, 57, 64, 97]
+    lens = [9, 256, 257, 511, 513, 49, 1030, 64, 700]
+    cache = Cache(p1a, KVS[kv], 1, D, 4, lens, 25)
+    call = Call(p1a, cache, 4, counts, [n - c for n, c in zip(lens, counts)])
+    m = torch.zeros(9, 1, 1030, device="cuda")
+    p1a.attn_mass(call.q, cache.kv, dev(call.all(1).astype(np.float32)), m, call.rows, 4, call.scale)
+    want = mass_want(call, cache, np.zeros((9, 1, 1030), np.float32), 1030)
+    got = m.cpu().numpy()
+    for s in range(9):
+        assert np.linalg.norm(got[s] - want[s]) <= REL * np.linalg.norm(want[s]), s
+        assert not got[s, :, lens[s]:].any()
+
+
 @pytest.mark.parametrize("Hq, Hkv, D", SHAPES)
 def test_mass_single_tokens(p1a, Hq, Hkv, D):
     lens = [1, 2, 33, 64, 129, 500, 1500]
