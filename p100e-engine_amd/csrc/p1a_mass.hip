@@ -5,11 +5,14 @@
 // walks tiles of 32 keys, K straight into the operands of v_mfma_f32_16x16x32_f16, codes as whole numbers; a key's weights are added over the 16 lanes of its
 // columns and its entry written at once.
 // Many rows, mass_k: a wave owns 32 NU keys - their rows stay in its registers as operands of v_mfma_f32_32x32x16_f16, quantized ones in two planes
-// (p1a_tiles.hpp) - and walks the rows of q that may see them, 32 at a time; a key's sum stays with one lane until the end. The workgroup's four
-// waves (128 NU keys) share the rows: fetched, brought to two halves and put into LDS once for all; with NU = 2 a half read from LDS feeds two products
-// (one: LDS gives 128 bytes a clock and four waves would ask for 128). Where there are too few keys to fill the device, workgroups share
-// the rows of a block of keys too, leave their sums, and mass_add_k adds them in order.
-// What bounds it: the matrix pipe (2 products for f16 caches, 3 for quantized ones), 3 vector instructions a weight beside it.
+// (p1a_tiles.hpp) - and walks the rows of q that may see them, 32 at a time; a key's sum stays with one lane until the end. The workgroup's eight
+// waves (256 NU keys) share the rows: fetched, brought to two halves and put into LDS once for all; with NU = 2 a half read from LDS feeds two products
+// (one: LDS gives 128 bytes a clock and eight waves would ask for 128). Two workgroups of four waves a compute unit, which brought each row twice and had no
+// registers left to ask for it ahead, took 417 us for four prompts of 300 ... 2003 tokens (24 / 4 heads of 256, f16); this takes 285. Where there are too few
+// keys to fill the device, workgroups share the rows of a block of keys too, leave their sums, and mass_add_k adds them in order.
+// What bounds it: the matrix pipe (2 products for f16 caches, 3 for quantized ones; 144 us of the 285 at a large product's rate), the exponentials and
+// the rows' halves beside it; with few rows (64 over 30011 keys, 32 / 8 heads of 128: 57 to 62 us) 8 us of a workgroup's 30 before its first product.
+// Few rows: 32 sequences of 1000 ... 8190 keys (24 / 4 of 256, q8_0) 36 us, 4.5 TB/s of K and totals.
 #include "p1a_tiles.hpp"
 
 #include <algorithm>
@@ -180,29 +183,35 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
     // Rows of q as the operand's columns. Wave w brings rows 4 w .. 4 w + 3 of the 32: lane (row lane % 4, chunk 16 j + lane / 4; heads of 64: twice)
     auto qrow_of = [&] { return 4 * wave + (lane & 3); };
     auto qchunk_of = [&] { return (lane >> 2) & (D / 8 - 1); };
-    struct rows_raw { f4 x[NJ][2]; float lse; int pos; };
+    struct rows_raw { u4 x[NJ][2]; float lse; int pos; };
     auto fetch_rows = [&](rows_raw & r, int r0) {
         const int qrow = qrow_of(), qchunk = qchunk_of(), row = min(r0 + qrow, nrows - 1), t = token_of(P, row);
         const size_t i = (size_t) (sv.first + t) * P.Hq + (size_t) hk * P.GQA + (row - t * P.GQA);
-        auto fetch = [&](auto as_bf16) {
+        // (as they are in memory: whatever looked at them here would wait for them here)
+        const gbytes from = (gbytes) P.q + (i * D + 8 * qchunk) * (P.q_bf16 ? 2 : 4);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) r.x[j][e] = q4_at(P.q, as_bf16, i * D + (16 * j + qchunk) * 8 + 4 * e);
-        };
-        if (P.q_bf16) fetch(std::true_type{});
-        else fetch(std::false_type{});
+        for (int j = 0; j < NJ; ++j) {
+            if (P.q_bf16) r.x[j][0] = gload<u4>(from + 256 * j);
+            else {
+                r.x[j][0] = gload<u4>(from + 512 * j);
+                r.x[j][1] = gload<u4>(from + 512 * j + 16);
+            }
+        }
         r.lse = P.lse[i];
         r.pos = sv.pos0 + t;
-        if (r0 + qrow >= nrows || r.pos < 0 || r.pos >= P.R.n_ctx || r.lse == MINUS_INF) r.pos = -1;   // sees nothing
+        if (r0 + qrow >= nrows || r.pos < 0 || r.pos >= P.R.n_ctx) r.pos = -1;   // sees nothing
     };
     auto put_rows = [&](const rows_raw & r, int st) {
         const int qrow = qrow_of(), qchunk = qchunk_of();
-        float most = 0.f;
+        float most = 0.f, x[NJ][8];
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(r.x[j][e >> 2][e & 3]));
+            for (int e = 0; e < 8; ++e) {
+                const uint32_t half = r.x[j][0][e >> 1];
+                x[j][e] = __builtin_bit_cast(float, P.q_bf16 ? (e & 1 ? half & 0xffff0000u : half << 16) : r.x[j][e >> 2][e & 3]);
+                most = fmaxf(most, fabsf(x[j][e]));
+            }
         most = fmaxf(most, __shfl_xor(most, 4));
         most = fmaxf(most, __shfl_xor(most, 8));
         most = max_swap32(max_swap16(most));
@@ -212,12 +221,12 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             h8 y[2];
-            halves<2>([&](int e) { return r.x[j][e >> 2][e & 3]; }, [&](int) { return by; }, y);
+            halves<2>([&](int e) { return x[j][e]; }, [&](int) { return by; }, y);
             char * const at = to + chunk_at(qrow & 15, 16 * j + qchunk);
             *reinterpret_cast<h8 *>(at) = y[0];
             *reinterpret_cast<h8 *>(at + 2 * PL_B) = y[1];
         }
-        if (lane < 4) info[st * QR + qrow] = row_info{ldexpf(P.factor, ex), -r.lse * LOG2E, r.pos};
+        if (lane < 4) info[st * QR + qrow] = row_info{ldexpf(P.factor, ex), -r.lse * LOG2E, r.lse == MINUS_INF ? -1 : r.pos};
     };
 
         // ---- this wave's keys, AT_ONCE groups of 16 at a time through LDS ----
@@ -270,23 +279,20 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
         int r0 = (ra + split * per) * QR;
         const int r1 = min((ra + (split + 1) * per) * QR, rb * QR);
         // Step i reads the rows in place i % 4 and brings those of step i + 2, so that the waves meet after every second step only: one's
-        // products run beside another's exponentials. Rows are asked for AHEAD steps before they go to LDS: a step of short heads is over before they come
-        constexpr int AHEAD = NU * NPL * D < 512 ? 2 : 1;
-        rows_raw ring[AHEAD];
-        if (r0 < r1) fetch_rows(ring[0], r0);
-        if (AHEAD == 2 && r0 + QR < r1) fetch_rows(ring[AHEAD - 1], r0 + QR);
+        // products run beside another's exponentials (309 -> 285 us for four prompts)
+        rows_raw rr;
+        if (r0 < r1) fetch_rows(rr, r0);
         __syncthreads();                                      // (the rows go where the keys were)
-        if (r0 < r1) put_rows(ring[0], 0);
-        if (AHEAD == 1 && r0 + QR < r1) fetch_rows(ring[0], r0 + QR);
-        if (r0 + QR < r1) put_rows(ring[AHEAD - 1], 1);
-        if (AHEAD == 2 && r0 + 2 * QR < r1) fetch_rows(ring[0], r0 + 2 * QR);
+        if (r0 < r1) put_rows(rr, 0);
+        if (r0 + QR < r1) fetch_rows(rr, r0 + QR);
+        if (r0 + QR < r1) put_rows(rr, 1);
         __syncthreads();
-        auto turn = [&](int st, rows_raw & later, rows_raw & next) __attribute__((always_inline)) {
-            if (AHEAD == 1) asm volatile("" : "+v"(lane));   // (anew for each step: registers)
+        for (int st = 0; r0 < r1; r0 += QR, st = (st + 1) & 3) {
+            asm volatile("" : "+v"(lane));                    // (anew for each step: registers)
             const int c = lane & 31, g = lane >> 5;
             const k_frag qfr(lane, PL_B);
             const bool more = r0 + 2 * QR < r1;
-            if (r0 + (1 + AHEAD) * QR < r1) fetch_rows(later, r0 + (1 + AHEAD) * QR);
+            if (more) fetch_rows(rr, r0 + 2 * QR);
             const row_info my = info[st * QR + c];
             f16x s[NU];
 #pragma unroll
@@ -334,18 +340,8 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
                     for (int i = 0; i < 16; ++i) acc[u][i] += __builtin_amdgcn_exp2f(fmaf(s[u][i], my.factor, my.lse));
                 }
             }
-            if (more) put_rows(next, (st + 2) & 3);
-            r0 += QR;
+            if (more) put_rows(rr, (st + 2) & 3);
             if (st & 1) __syncthreads();
-        };
-        if constexpr (AHEAD == 1) {
-            for (int st = 0; r0 < r1; st = (st + 1) & 3) turn(st, ring[0], ring[0]);
-        } else {
-            for (int st = 0; r0 < r1; st = (st + 2) & 3) {
-                turn(st, ring[1], ring[0]);
-                if (r0 >= r1) break;
-                turn(st + 1, ring[0], ring[1]);
-            }
         }
         // ---- sums over the 32 rows' lanes; lane i of a half adds value i to its key ----
         asm volatile("" : "+v"(lane));
