@@ -8,10 +8,11 @@
 // (p1a_tiles.hpp) - and walks the rows of q that may see them, 32 at a time; a key's sum stays with one lane until the end. The workgroup's eight
 // waves (256 NU keys) share the rows: fetched, brought to two halves and put into LDS once for all; with NU = 2 a half read from LDS feeds two products
 // (one: LDS gives 128 bytes a clock and eight waves would ask for 128). Two workgroups of four waves a compute unit, which brought each row twice and had no
-// registers left to ask for it ahead, took 417 us for four prompts of 300 ... 2003 tokens (24 / 4 heads of 256, f16); this takes 285. Where there are too few
+// registers left to ask for it ahead, took 417 us for four prompts of 300 ... 2003 tokens (24 / 4 heads of 256, f16); this takes 260 to 280. Where there are too few
 // keys to fill the device, workgroups share the rows of a block of keys too, leave their sums, and mass_add_k adds them in order.
-// What bounds it: the matrix pipe (2 products for f16 caches, 3 for quantized ones; 144 us of the 285 at a large product's rate), the exponentials and
-// the rows' halves beside it; with few rows (64 over 30011 keys, 32 / 8 heads of 128: 57 to 62 us) 8 us of a workgroup's 30 before its first product.
+// What bounds it: the matrix pipe (2 products for f16 caches, 3 for quantized ones; 144 us of the 270 at a large product's rate) and, hardly beside it
+// with two waves a SIMD, the exponentials and the rows' halves; over long caches (64 rows over 30011 keys, 32 / 8 heads of 128: 57 us) 8 us of
+// a workgroup's 28 before its first product.
 // Few rows: 32 sequences of 1000 ... 8190 keys (24 / 4 of 256, q8_0) 36 us, 4.5 TB/s of K and totals.
 #include "p1a_tiles.hpp"
 
@@ -406,24 +407,28 @@ template <uint32_t KT> int launch_kt(const mass_params & P, int D, int few, dim3
 
 }   // namespace
 
-// How a call is dealt out, from its host numbers and the device: few rows as runs of steps, as many as there are places for workgroups; many rows as
-// blocks of keys, whose rows are split while there are fewer than four workgroups for every place and each has 16 times 32 rows and more.
+// How a call is dealt out, from its host numbers and the device. Up to 32 rows of a sequence under a kv head: runs of steps, as many as there are places for
+// workgroups (32 sequences of 1000 ... 8190 keys, 24 / 4 heads of 256, q8_0: 36 us; as blocks of keys 88). More: blocks of keys. Their rows are split in
+// pieces of four times 32 and more while that leaves compute units without a workgroup, of eight times while there are no more than four workgroups to each,
+// of 16 times up to eight workgroups - setting one up costs what three or four times 32 rows do, and the last of unequal ones are waited for:
+//   64 tokens over 3001 keys (32 / 8 heads of 128, f16; whole calls) 29 us unsplit, 23 in two; 256 over 3001 53 in two, 35 in four, 39 in eight;
+//   256 over 30011 177 in two, 197 in four; four prompts (24 / 4 of 256) 1240 unsplit, 475 in one or two, 335 in three, 270 in seven.
 mass_plan plan_mass(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int ld, int cus) {
     const int GQA = Hq / c.Hkv;
     const bool planes = c.type != P1A_KV_F16;
     mass_plan pl{};
     pl.few = (long long) R.max_rows * GQA <= 32 ? (R.max_rows * GQA + 15) / 16 : 0;
     const long long keys = R.window == INT32_MAX ? max_n : std::min<long long>(max_n, (long long) R.window + R.max_rows + R.n_sink + 64);
-    const long long slots = 2LL * std::max(cus, 1);
+    const long long places = std::max(cus, 1);
     pl.splits = 1;
     if (pl.few) {
-        pl.runs = (int) std::max(1LL, std::min(slots * (c.D == 256 ? 1 : 2) / c.Hkv, R.n_seq * ((keys + 127) / 128)));
+        pl.runs = (int) std::max(1LL, std::min(places * (c.D == 256 ? 2 : 4) / c.Hkv, R.n_seq * ((keys + 127) / 128)));
         return pl;
     }
     const int BK = MW * 32 * (planes && c.D == 256 ? 1 : 2);
     pl.blocks = (int) std::min<long long>((keys + BK - 1) / BK, 65536 / c.Hkv + 1);
     const long long units = (long long) pl.blocks * c.Hkv * R.n_seq, tiles = ((long long) R.max_rows * GQA + QR - 1) / QR;
-    pl.splits = (int) std::max(1LL, std::min({4 * slots / units, tiles / 16, 32LL}));
+    pl.splits = (int) std::min(32LL, std::max({1LL, std::min(places / units, tiles / 4), std::min(4 * places / units, tiles / 8), std::min(8 * places / units, tiles / 16)}));
     if (pl.splits > 1) pl.bytes = (size_t) pl.splits * R.n_seq * c.Hkv * ld * 4;
     return pl;
 }
