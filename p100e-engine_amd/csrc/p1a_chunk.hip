@@ -9,8 +9,8 @@
 // are two f16 halves (EXACT) and quantized K and V two planes (p1a_tiles.hpp): 2 products for f16 caches, 3 for quantized ones (low times low is 2^-22
 // of the result and left out). P runs up to 2^14, so its low halves end 2^-38 below the largest weight.
 // What bounds it: with a wave to a SIMD (heads of 256: O and Q fill the registers) whatever is not hidden behind that wave's own products - without the
-// loads 4096 tokens of a document through a window of 4096 (24 / 4 heads of 256, f16, bf16 out) took a fifth less. They take 534 to 560 us, 750 to 780
-// TFLOP/s (a large product of the vendor's library: 1130), 370 at that rate; eight prompts of 77 ... 2003 tokens 280 to 298.
+// loads 4096 tokens of a document through a window of 4096 (24 / 4 heads of 256, f16, bf16 out) took a fifth less. They take 508 to 600 us by card,
+// 700 to 820 TFLOP/s (a large product of the vendor's library: 1130, 370 us at that rate); eight prompts of 77 ... 2003 tokens 280 to 310.
 #include "p1a_tiles.hpp"
 
 #include <algorithm>
