@@ -9,7 +9,7 @@ namespace {
 // value a pass - until what shares the digits so far is wanted as a whole -, then one pass that lists what is above it, and of what equals it the first
 // ones, in order. A thread holds 16 consecutive values of a part of 16384; longer rows are read again for each pass (from L2). Counts go to 32 copies of
 // the histogram, one for every other lane: values of one order of magnitude share their first digit, and additions to one address wait for each other.
-// What bounds it: one compute unit's vector instructions a row, some 20 a value and pass: 1100 positions 9 us, 8190 15, 100003 78. (Eleven bits a pass,
+// What bounds it: one compute unit's vector instructions a row, some 15 a value and pass: 1100 positions 8 us, 8190 14, 100003 72. (Eleven bits a pass,
 // fewer passes, values kept in registers or LDS or asked for ahead took 92 to 145 there; several workgroups a row would need a workspace for their counts.)
 constexpr int STHR = 1024, PER = 16, PART = STHR * PER;
 
@@ -41,7 +41,7 @@ __global__ void __launch_bounds__(STHR) select_k(const float * mass, int ld, con
     const int parts = (b - a + PART - 1) / PART;
     uint32_t key[PER];
     int held = -1;
-    auto hold = [&](int part) {                               // (a key past the end stays what it is: its index tells)
+    auto hold = [&](int part) {                               // (a key past the end: 0)
         if (held == part) return;
         held = part;
         const int i0 = a + part * PART + tid * PER;
@@ -63,10 +63,16 @@ __global__ void __launch_bounds__(STHR) select_k(const float * mass, int ld, con
         __syncthreads();
         for (int part = 0; part < parts; ++part) {
             hold(part);
-            const int live = b - (a + part * PART + tid * PER);
+            // (keys past the end are 0 and count as such: the last digit looked at then seems to hold more than are there, never fewer than are wanted)
+            uint32_t * const mine = hist + (lane & 31);
+            if (shift == 24) {
 #pragma unroll
-            for (int x = 0; x < PER; ++x)
-                if (x < live && (shift == 24 || key[x] >> (shift + 8) == prefix >> (shift + 8))) atomicAdd(&hist[((key[x] >> shift) & 255) * HS + (lane & 31)], 1u);
+                for (int x = 0; x < PER; ++x) atomicAdd(&mine[(key[x] >> 24) * HS], 1u);
+            } else {
+#pragma unroll
+                for (int x = 0; x < PER; ++x)
+                    if ((key[x] ^ prefix) >> (shift + 8) == 0) atomicAdd(&mine[((key[x] >> shift) & 255) * HS], 1u);
+            }
         }
         __syncthreads();
         {
