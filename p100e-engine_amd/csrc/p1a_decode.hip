@@ -177,19 +177,20 @@ __device__ __forceinline__ u2 deq4n(uint32_t w, h2 dd) { return deq4n2(w, dd, dd
 // written as inline assembly so that the waits on them can be partial: the vector-memory counter retires in order,
 // so "at most n newer loads outstanding" (s_waitcnt vmcnt(n)) is exactly "tile x has landed" when every tile is NR
 // loads. For the same reason nothing else in the key loop may be a vector load: the page-table entry of a tile is
-// fetched with a scalar load, issued one step ahead.
+// fetched with a scalar load, issued one step ahead. (s_nop: one instruction has to stand between the write of M0 and a load that
+// goes by it, and the compiler does not look into the assembly.)
 __device__ __forceinline__ uint32_t lds_addr(const char * p) { return (uint32_t) (size_t) (const __attribute__((address_space(3))) char *) p; }
 __device__ __forceinline__ void dma16(const char * sbase, uint32_t voff, uint32_t lds) {
     // (the destination is wave-uniform by construction; say so, or a value the compiler happens to keep in a vector
     // register cannot be given to s_mov)
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(voff), "s"(sbase), "s"(__builtin_amdgcn_readfirstlane((int) lds)) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(voff), "s"(sbase), "s"(__builtin_amdgcn_readfirstlane((int) lds)) : "memory", "m0");
 }
 __device__ __forceinline__ void dma16v(const char * vaddr, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(vaddr), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" :: "v"(vaddr), "s"(lds) : "memory", "m0");
 }
 // 4 bytes per lane: lane i lands at M0 + 4 i
 __device__ __forceinline__ void dma4(const char * sbase, uint32_t voff, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" :: "v"(voff), "s"(sbase), "s"(__builtin_amdgcn_readfirstlane((int) lds)) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" :: "v"(voff), "s"(sbase), "s"(__builtin_amdgcn_readfirstlane((int) lds)) : "memory", "m0");
 }
 template <int N> __device__ __forceinline__ void wait_vm_imm() { asm volatile("s_waitcnt vmcnt(%0)" :: "n"(N) : "memory"); }
 // wait until at most `newer` tile fetches (NR loads each) issued after the wanted one are still in flight

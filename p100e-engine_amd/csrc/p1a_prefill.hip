@@ -244,8 +244,9 @@ template <class S> __device__ __forceinline__ void store_tile(const typename S::
 // GROUPED: pages hold at least 16 positions (or the cache is contiguous), so a 16-key group has one base
 __device__ __forceinline__ uint32_t lds_addr(const char * p) { return (uint32_t) (size_t) (const __attribute__((address_space(3))) char *) p; }
 // 64 lanes x 16 bytes, global (scalar base + 32-bit lane offset) -> LDS at `lds` + a constant + 16 * lane, no registers in between
+// (s_nop: one instruction has to stand between the write of M0 and a load that goes by it, and the compiler does not look in here)
 __device__ __forceinline__ void dma16_at(const char * sbase, uint32_t voff, uint32_t lds, int at) {
-    asm volatile("s_add_u32 m0, %2, %3\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(voff), "s"(sbase), "s"(lds), "i"(at) : "memory", "m0", "scc");
+    asm volatile("s_add_u32 m0, %2, %3\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" :: "v"(voff), "s"(sbase), "s"(lds), "i"(at) : "memory", "m0", "scc");
 }
 
 // D <= 128: a wave keeps all the dims of its own 32 rows (the V^T reads are few enough), so no P^T changes hands, no barrier

@@ -166,9 +166,10 @@ template <int D, int NPL> struct group<P1A_KV_F16, D, NPL> {
     static __device__ __forceinline__ int key(int lane) { return (lane & 15) ^ (4 * (lane >> 4)); }
     static constexpr int PIECES = D / 32;                     // loads of a group
     struct raw {};
-    // load j, straight to LDS: complete when vmcnt says so. (The instruction adds its offset to both addresses.)
+    // load j, straight to LDS: complete when vmcnt says so. (The instruction adds its offset to both addresses. s_nop: one
+    // instruction has to stand between the write of M0 and a load that goes by it, and the compiler does not look in here.)
     template <int j> static __device__ __forceinline__ void piece(raw &, gbytes row, char * to, int lane) {
-        asm volatile("s_add_u32 m0, %1, %2\n\tglobal_load_lds_dwordx4 %0, off offset:%3" :: "v"(row + (lane >> 4) * 16), "s"(__builtin_amdgcn_readfirstlane(lds_at(to))), "i"(960 * j), "i"(64 * j)
+        asm volatile("s_add_u32 m0, %1, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off offset:%3" :: "v"(row + (lane >> 4) * 16), "s"(__builtin_amdgcn_readfirstlane(lds_at(to))), "i"(960 * j), "i"(64 * j)
                      : "memory", "m0", "scc");
     }
     static __device__ __forceinline__ void load(gbytes row, char * to, int lane) {
