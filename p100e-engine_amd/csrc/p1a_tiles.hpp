@@ -437,7 +437,14 @@ template <uint32_t KT, int D, int NQ> __device__ __forceinline__ int q_columns(c
 // A sequence with rows has one step at least. Lane i of a wave counts for sequence s0 + i and keeps what it found out about the first 64 (all of
 // them, mostly).
 template <int TPS> struct step_runs {
-    struct of_lane { int rows, pos0, table, steps; };          // first row * 64 + rows (there are 2^21 rows at most); where its page-table row begins
+    // first row, its position, where the page-table row begins; rows (32 at most) and steps (2^30 positions: 2^23 and one) share a register - the first row may be
+    // anything up to 2^30
+    struct of_lane {
+        int first, pos0, table, work;
+        static __host__ __device__ __forceinline__ int both(int steps, int rows) { return steps << 6 | rows; }
+        __host__ __device__ __forceinline__ int steps() const { return work >> 6; }
+        __host__ __device__ __forceinline__ int rows() const { return work & 63; }
+    };
     of_lane first64;
     int first, end, per;                                      // this run's steps; steps of a run
     static __device__ __forceinline__ span span_of_rows(const rows_view & R, const seq_view & v) { return span_of<32>(R, v.pos0, v.pos0 + v.count - 1); }
@@ -446,9 +453,9 @@ template <int TPS> struct step_runs {
         if (s >= R.n_seq) return r;
         const seq_view v = seq_of(R, s);
         r.table = pg.pt && pg.rtab ? pg.rtab[s] : 0;
-        r.rows = v.first << 6 | v.count;
+        r.first = v.first;
         r.pos0 = v.pos0;
-        r.steps = v.count < 1 ? 0 : max((span_of_rows(R, v).nt + TPS - 1) / TPS, 1);
+        r.work = v.count < 1 ? 0 : r.both(max((span_of_rows(R, v).nt + TPS - 1) / TPS, 1), v.count);
         return r;
     }
     // run number `run` of `runs`; no sequence in more than `most_runs` of them. False: there is nothing for it
@@ -457,7 +464,7 @@ template <int TPS> struct step_runs {
         first64 = look(R, pg, lane);
         int n = 0, most = 0;
         for (int s0 = 0; s0 < R.n_seq; s0 += 64) {
-            const int x = s0 ? look(R, pg, s0 + lane).steps : first64.steps;
+            const int x = s0 ? look(R, pg, s0 + lane).steps() : first64.steps();
             n += __builtin_amdgcn_readlane(lanes_up_to(x), 63);
             most = max(most, x);
         }
@@ -474,15 +481,16 @@ template <int TPS> struct step_runs {
         int base = 0;
         for (int s0 = 0;; s0 += 64) {
             const of_lane x = s0 ? look(R, pg, s0 + lane) : first64;
-            const int u = base + lanes_up_to(x.steps);
+            const int u = base + lanes_up_to(x.steps());
             const unsigned long long behind = __ballot(u > at);
             if (behind) {
-                const int l = __builtin_ctzll(behind), rows = __builtin_amdgcn_readlane(x.rows, l);
+                const int l = __builtin_ctzll(behind);
+                const of_lane at_l{0, 0, 0, __builtin_amdgcn_readlane(x.work, l)};
                 f.seq = s0 + l;
-                f.steps = __builtin_amdgcn_readlane(x.steps, l);
+                f.steps = at_l.steps();
                 f.first = __builtin_amdgcn_readlane(u, l) - f.steps;
-                f.v.first = rows >> 6;
-                f.v.count = rows & 63;
+                f.v.first = __builtin_amdgcn_readlane(x.first, l);
+                f.v.count = at_l.rows();
                 f.v.pos0 = __builtin_amdgcn_readlane(x.pos0, l);
                 f.table = __builtin_amdgcn_readlane(x.table, l);
                 return f;

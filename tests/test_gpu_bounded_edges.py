@@ -1,0 +1,33 @@
+"""Calls over bounded caches at the ends of what their documentation allows, each against its formula in 64 bits. Tolerances of f32 results are those derived in
+test_gpu_bounded.py: 1e-5 in the 2-norm."""
+import numpy as np
+import pytest
+import torch
+
+import _inputs as I
+import _oracle as O
+from _bounded import Cache, rows_exact, seen
+from _gpu import dev
+
+pytestmark = pytest.mark.gpu
+
+KVS = {"f16": O.KV_F16, "q8_0": O.KV_Q8_0, "q4_0": O.KV_Q4_0}
+REL = 1e-5
+
+
+@pytest.mark.parametrize("kv", ["f16", "q8_0"])
+def test_rows_far_behind_the_first(p1a, kv):
+    """few rows of a sequence behind 2^25 rows of nobody"""
+    first, n, D = (1 << 25) + 3, 300, 64
+    T = first + 2 + 5
+    cache = Cache(p1a, KVS[kv], 1, D, 4, [n], 81)
+    q = torch.empty(T, 1, D, dtype=torch.bfloat16, device="cuda")
+    q[first:first + 2].normal_(generator=torch.Generator("cuda").manual_seed(82))
+    lse = torch.empty(T, 1, device="cuda")
+    rows = p1a.Rows(T, n_seq=1, row0=dev(np.array([first, first + 2], np.int32)), pos0=dev(np.array([n - 2], np.int32)), max_rows=2, max_n=n)
+    out, z, w, _, _ = rows_exact(q[first:first + 2].float().cpu().numpy(), cache.heads("k", 0, n), cache.heads("v", 0, n), seen(np.array([n - 2, n - 1]), n, 0, 0), 0.125)
+    lse[first:first + 2] = dev(z.astype(np.float32))
+    mass = torch.zeros(1, 1, n, device="cuda")
+    p1a.attn_mass(q, cache.kv, lse, mass, rows, 1, 0.125)
+    want = w.sum((0, 1))
+    assert np.linalg.norm(mass.cpu().numpy()[0, 0] - want) <= REL * np.linalg.norm(want)
