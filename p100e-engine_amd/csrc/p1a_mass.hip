@@ -418,7 +418,8 @@ mass_plan plan_mass(const p1a_kv & c, const rows_view & R, int Hq, int max_n, in
     const bool planes = c.type != P1A_KV_F16;
     mass_plan pl{};
     pl.few = (long long) R.max_rows * GQA <= 32 ? (R.max_rows * GQA + 15) / 16 : 0;
-    const long long keys = R.window == INT32_MAX ? max_n : std::min<long long>(max_n, (long long) R.window + R.max_rows + R.n_sink + 64);
+    // (a descriptor without positions: as if there were one)
+    const long long keys = std::max(1LL, R.window == INT32_MAX ? max_n : std::min<long long>(max_n, (long long) R.window + R.max_rows + R.n_sink + 64));
     const long long places = std::max(cus, 1);
     pl.splits = 1;
     if (pl.few) {

@@ -1,5 +1,6 @@
 """Arithmetic of the calls over bounded caches at the ends of what they take (no GPU): the kernels' own lines, compiled for the host."""
 import ctypes
+import importlib
 import os
 import shutil
 import subprocess
@@ -40,3 +41,15 @@ def test_a_sequences_rows_and_steps_fit_what_holds_them(host, first, steps, rows
     o = (ctypes.c_int * 3)()
     host.through(first, rows, steps, o)
     assert list(o) == [first, rows, steps]
+
+
+@pytest.mark.parametrize("max_rows", [1, 64])
+@pytest.mark.parametrize("kv_type", ["KV_F16", "KV_Q8_0", "KV_Q4_0"])
+def test_caches_of_no_positions_need_no_scratch(kv_type, max_rows):
+    """a descriptor with room for nothing: no row sees anything, and the work can be dealt out all the same"""
+    p1a, b = importlib.import_module("p100e-engine_amd"), importlib.import_module("p100e-engine_amd.binding")
+    kv = b.p1a_kv(getattr(p1a, kv_type), 0, 4, 256, 4096, 8192, 4096, 4096, 8, 4 * 256 * 2 << 8)
+    for window in (0, 100):
+        rows = b.p1a_rows(64, 1, max_rows, 0, 4096, 4096, 0, window, 0)
+        assert p1a.lib().p1a_attn_chunk_scratch_bytes(ctypes.byref(kv), ctypes.byref(rows), 24) == 0
+        assert p1a.lib().p1a_attn_mass_scratch_bytes(ctypes.byref(kv), 64, ctypes.byref(rows), 24) >= 0

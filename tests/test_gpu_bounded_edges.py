@@ -31,3 +31,18 @@ def test_rows_far_behind_the_first(p1a, kv):
     p1a.attn_mass(q, cache.kv, lse, mass, rows, 1, 0.125)
     want = w.sum((0, 1))
     assert np.linalg.norm(mass.cpu().numpy()[0, 0] - want) <= REL * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("counts", [[1, 1], [40, 3]])
+def test_a_cache_of_no_positions(p1a, counts):
+    """n_ctx = 0: every row sees nothing, and totals stay as they are"""
+    cache = Cache(p1a, O.KV_Q8_0, 2, 64, 4, [50, 50], 83)
+    T = sum(counts)
+    q, out, lse = torch.randn(T, 4, 64, device="cuda"), torch.full((T, 4, 64), 7.0, device="cuda"), torch.full((T, 4), 7.0, device="cuda")
+    cache.kv.n_ctx = 0
+    rows = p1a.Rows(T, n_seq=2, row0=dev(np.array([0, counts[0], T], np.int32)), pos0=dev(np.zeros(2, np.int32)), max_rows=max(counts))
+    p1a.attn_chunk(q, cache.kv, out, rows, 4, 0.125, lse=lse)
+    mass = torch.full((2, 2, 64), 3.0, device="cuda")
+    p1a.attn_mass(q, cache.kv, torch.zeros(T, 4, device="cuda"), mass, rows, 4, 0.125)
+    torch.cuda.synchronize()
+    assert (out == 0).all() and (lse == -np.inf).all() and (mass == 3).all()
