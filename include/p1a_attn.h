@@ -227,7 +227,7 @@ int p1a_warmup_prefill(int T, int p0, int Hq, int Hkv, int D, void *stream);
  * row0[n_seq] - are left as they are; a row whose position is negative or not below the descriptor's n_ctx sees nothing: its result is 0, its
  * log-sum-exp -inf. Sequence s reads the page table pt + rtab[s]; without rtab (or without pt) there is one sequence.
  * row0 and pos0 are read on the device when the kernels run; the other fields are the host's. A pair of row0 that runs backwards is an empty
- * sequence, rows past T or past max_rows of a sequence are not looked at. Page-table entries of positions that no row sees are never read, nor
+ * sequence, rows past T or past max_rows of a sequence are not looked at. Two pairs that share rows are no call's: results are then unspecified. Page-table entries of positions that no row sees are never read, nor
  * is memory behind them: a page that has left the window may be given away.
  */
 #define P1A_ROWS_F32  0

@@ -342,7 +342,7 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
         }
 }
 
-// Partials of a row -> its result: 256 / (D / 4) rows a workgroup, four dims a thread
+// Partials of a row -> its result: 256 / (D / 4) rows of one sequence a workgroup, four dims a thread
 struct chunk_merge_params {
     rows_view R;
     const float * part_o, * part_ml, * gate;
@@ -352,27 +352,14 @@ struct chunk_merge_params {
     const int * part_n;    // few rows: partials that each sequence has (1: its rows are finished), or null: nks
 };
 __global__ void __launch_bounds__(NTHR) chunk_merge_k(const chunk_merge_params P) {
-    const int tpr = P.D >> 2, sub = threadIdx.x / tpr, d = 4 * (threadIdx.x - sub * tpr);
-    const long long row = (long long) blockIdx.x * (NTHR / tpr) + sub;
-    if (row >= (long long) P.R.T * P.Hq) return;
-    const int t = (int) (row / P.Hq);
-    int a = 0, n = P.nks;
-    if (P.R.row0) {                                           // the last sequence that starts at or ahead of the row's token
-        int b = P.R.n_seq;
-        while (b - a > 1) {
-            const int m = (a + b) >> 1;
-            if (P.R.row0[m] <= t) a = m; else b = m;
-        }
-        const seq_view v = seq_of(P.R, a);
-        if (t < v.first || t >= v.first + v.count) return;    // (nobody's: left as it is)
-    } else {
-        a = t / P.R.per;
-        if (t - a * P.R.per >= P.R.max_rows) return;
-    }
-    if (P.part_n) {
-        n = min(P.part_n[a], P.nks);
-        if (n < 2) return;
-    }
+    const int tpr = P.D >> 2, per = NTHR / tpr, sub = threadIdx.x / tpr, d = 4 * (threadIdx.x - sub * tpr);
+    item_at at;                                               // (whose rows they are: as the kernels that left the partials find it, whatever row0 holds)
+    if (!find_item(P.R, blockIdx.x, P.Hq, per, threadIdx.x & 63, at)) return;
+    const int r = at.index * per + sub;                       // of the sequence
+    if (r >= (long long) at.v.count * P.Hq) return;
+    const long long row = (long long) at.v.first * P.Hq + r;
+    const int n = P.part_n ? min(P.part_n[at.seq], P.nks) : P.nks;
+    if (n < 2) return;                                        // (finished already)
     // four partials at a time, asked for together
     const float2 * ml = reinterpret_cast<const float2 *>(P.part_ml) + row * P.nks;
     const float * po = P.part_o + row * P.nks * P.D + d;
@@ -439,11 +426,13 @@ template <uint32_t KT> int launch_kt(const chunk_params & P, int D, bool exact, 
     return D == 256 ? launch_d<KT, 256>(P, exact, grid, s) : D == 128 ? launch_d<KT, 128>(P, exact, grid, s) : launch_d<KT, 64>(P, exact, grid, s);
 }
 
-// the most blocks the rows can make
-long long block_bound(const rows_view & R, int GQA) {
-    const long long each = ((long long) R.max_rows * GQA + BM - 1) / BM * R.n_seq;
-    return R.row0 ? std::min(each, (long long) R.T * GQA / BM + R.n_seq) : each;
+// the most items of `unit` that the sequences' rows times `mul` can make (as find_item counts them)
+long long item_bound(const rows_view & R, int mul, int unit) {
+    const long long each = ((long long) R.max_rows * mul + unit - 1) / unit * R.n_seq;
+    return R.row0 ? std::min(each, (long long) R.T * mul / unit + R.n_seq) : each;
 }
+// the most blocks the rows can make
+long long block_bound(const rows_view & R, int GQA) { return item_bound(R, GQA, BM); }
 
 }   // namespace
 
@@ -520,8 +509,7 @@ int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
                  : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, exact, (unsigned) grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, exact, (unsigned) grid, s);
     if (rc != P1A_OK || P.nks == 1) return rc;
     const chunk_merge_params M{a.R, P.part_o, P.part_ml, a.gate, a.out, a.lse, a.Hq, c.D, P.nks, a.out_bf16, pl.few ? P.part_n : nullptr};
-    const size_t per = NTHR / (c.D / 4);
-    chunk_merge_k<<<(unsigned) ((rows + per - 1) / per), NTHR, 0, s>>>(M);
+    chunk_merge_k<<<(unsigned) item_bound(a.R, a.Hq, NTHR / (c.D / 4)), NTHR, 0, s>>>(M);
     return launched();
 }
 

@@ -46,3 +46,31 @@ def test_a_cache_of_no_positions(p1a, counts):
     p1a.attn_mass(q, cache.kv, torch.zeros(T, 4, device="cuda"), mass, rows, 4, 0.125)
     torch.cuda.synchronize()
     assert (out == 0).all() and (lse == -np.inf).all() and (mass == 3).all()
+
+
+@pytest.mark.parametrize("times", [1, 10])                      # (up to 8 rows of four heads under a kv head: the kernel for few; ten times that: blocks)
+@pytest.mark.parametrize("row0", [[0, 8, 3, 3, 3], [8, 8, 0, 5, 5], [7, 1, 4, 4, 2], [3, 0, 3, 8, 1], [0, 8, 2, 2, 0]])
+def test_pairs_of_row0_that_run_backwards(p1a, row0, times):
+    """... are empty sequences; the others' rows come out right where the call is split and merged too, and nobody's rows are left"""
+    n, Hq, D, T = 5000, 4, 64, 9 * times
+    cache = Cache(p1a, O.KV_Q8_0, 1, D, 6, [n] * 4, 84)
+    first = np.array(row0, np.int32) * times
+    q = I.normal(I.rng(85), (T, Hq, D))
+    pos0 = np.array([n - 8 * times, n - 2000, n - 100 * times, 3000], np.int32)
+    rows = p1a.Rows(T, n_seq=4, row0=dev(first), pos0=dev(pos0), max_rows=8 * times, max_n=n)
+    assert p1a.chunk_scratch_bytes(cache.kv, rows, Hq) > 0
+    out, z = torch.full((T, Hq, D), 7.0, device="cuda"), torch.full((T, Hq), 7.0, device="cuda")
+    p1a.attn_chunk(dev(q), cache.kv, out, rows, Hq, 0.125, lse=z)
+    out, z = out.cpu().numpy(), z.cpu().numpy()
+    owned = np.zeros(T, bool)
+    for s in range(4):
+        a, b = first[s], first[s + 1]
+        if b <= a:
+            continue
+        owned[a:b] = True
+        p = pos0[s] + np.arange(b - a)
+        m = int(p[-1]) + 1
+        want, lse, _, _, qk = rows_exact(q[a:b].astype(np.float64), cache.heads("k", s, m), cache.heads("v", s, m), seen(p, m, 0, 0), 0.125)
+        assert np.linalg.norm(out[a:b] - want) <= REL * np.linalg.norm(want), s
+        assert (np.abs(z[a:b] - lse) <= REL * qk + 2.0 ** -22 * (np.abs(lse) + 16)).all(), s
+    assert (out[~owned] == 7).all() and (z[~owned] == 7).all()
