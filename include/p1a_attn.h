@@ -252,7 +252,8 @@ typedef struct p1a_rows {
  * Precision: where a result is f32 (out, or lse is asked for) q, the probabilities and quantized K / V enter the f16 products as two halves each and
  * results are within 1e-5 (relative L2) of exact ones; with bf16 results they enter rounded to f16 once. K and V values of magnitude 65504 and more
  * are beyond the products' range, as in p1a_attn_prefill. A key whose V holds an infinity or NaN reaches rows of the same sequence in the same call
- * that do not see it; keys that no row sees reach nothing.
+ * that do not see it; keys that no row sees reach nothing. A NaN or an infinity in a row of q makes that row's result NaN (its log-sum-exp and the weights
+ * it gives are then no numbers either), and no other's.
  * D = 64, 128 or 256; Hq / Hkv up to 64; T * Hq, n_ctx up to 2^30, n_seq up to 65535, Hkv up to 4096, n_seq * Hkv up to 2^22; 16-byte aligned q, out and gate; f16 caches: 16-byte aligned bases and page strides, q8_0: 4-byte aligned,
  * q4_0: 2-byte aligned; pages of any length.
  * A call of few rows is split over its keys and its partials merged by a second launch; they live in `scratch` (256-byte aligned, at least

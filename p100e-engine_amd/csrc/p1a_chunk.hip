@@ -316,8 +316,8 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
     if (!live) return;
     if (P.nks > 1) {
         float * ml = P.part_ml + (my_index * P.nks + ksp) * 2;
-        if (g == 0) { ml[0] = ref; ml[1] = l; }
-        if (ref == MINUS_INF) return;                         // (nothing seen: the merge does not look at it)
+        if (g == 0) { ml[0] = part_ref(ref, l); ml[1] = l; }
+        if (part_ref(ref, l) == MINUS_INF) return;            // (nothing seen: the merge does not look at it)
         float * po = P.part_o + (my_index * P.nks + ksp) * D;
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(NTHR, D <= 128 ? 2 : 1) chunk_k(const chunk_pa
             for (int q = 0; q < 4; ++q) *reinterpret_cast<f4 *>(po + 32 * dt + 8 * q + 4 * g) = f4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]};
         return;
     }
-    const float inv = ref == MINUS_INF ? 0.f : 1.0f / l;
-    if (P.lse && g == 0) P.lse[my_index] = ref == MINUS_INF ? MINUS_INF : (ref + log2f(l)) * LN2;
+    const float inv = my_pos < 0 ? 0.f : 1.0f / l;
+    if (P.lse && g == 0) P.lse[my_index] = (ref + log2f(l)) * LN2;
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
@@ -390,8 +390,9 @@ __global__ void __launch_bounds__(NTHR) chunk_merge_k(const chunk_merge_params P
             acc += v[k] * w;
         }
     }
-    if (P.lse && d == 0) P.lse[row] = M == MINUS_INF ? MINUS_INF : (M + log2f(l)) * LN2;
-    f4 v = acc * (M == MINUS_INF ? 0.f : 1.0f / l);
+    const int pos = at.v.pos0 + r / P.Hq;
+    if (P.lse && d == 0) P.lse[row] = (M + log2f(l)) * LN2;
+    f4 v = acc * (pos < 0 || pos >= P.R.n_ctx ? 0.f : 1.0f / l);
     const size_t e = (size_t) row * P.D + d;
     if (P.gate) {
         const f4 gt = *reinterpret_cast<const f4 *>(P.gate + e);

@@ -336,14 +336,15 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
                 if (pieces > 1) {
                     if (d == 0) {
                         float * pm = P.part_ml + (row * P.nks + piece) * 2;
-                        pm[0] = M;
+                        pm[0] = part_ref(M, lt);
                         pm[1] = lt;
                     }
-                    if (M != MINUS_INF) *reinterpret_cast<f4 *>(P.part_o + (row * P.nks + piece) * D + d) = acc;
+                    if (part_ref(M, lt) != MINUS_INF) *reinterpret_cast<f4 *>(P.part_o + (row * P.nks + piece) * D + d) = acc;
                     continue;
                 }
-                if (P.lse && d == 0) P.lse[row] = M == MINUS_INF ? MINUS_INF : (M + log2f(lt)) * LN2;
-                f4 v = acc * (M == MINUS_INF ? 0.f : 1.0f / lt);
+                if (P.lse && d == 0) P.lse[row] = (M + log2f(lt)) * LN2;
+                const int at = sv.pos0 + tok_of(col);
+                f4 v = acc * (at < 0 || at >= P.R.n_ctx ? 0.f : 1.0f / lt);
                 if (P.gate) {
                     const f4 gt = *reinterpret_cast<const f4 *>(P.gate + row * D + d);
 #pragma unroll

@@ -547,6 +547,10 @@ struct chunk_params {
     float * part_o;        // [T * Hq][nks][D], relative to r
     float * part_ml;       // [T * Hq][nks][2]: r, l
 };
+// A row that sees something has itself to see: whether it sees nothing (result 0, log-sum-exp -inf) is a matter of its position. Where q holds a NaN or an infinity
+// all its scores may be NaN: no maximum, so r = -inf as if nothing had been seen, but l is NaN, and result and log-sum-exp become that. As a partial such a row
+// says so with a reference of 0.
+__device__ __forceinline__ float part_ref(float r, float l) { return r == MINUS_INF && !(l == 0.f) ? 0.f : r; }
 __device__ __forceinline__ float gate_of(float g) { return 1.0f / (1.0f + expf(-g)); }
 // four results of a row, at element i of out
 __device__ __forceinline__ void put4(void * out, bool bf16, size_t i, f4 v) {

@@ -74,3 +74,36 @@ def test_pairs_of_row0_that_run_backwards(p1a, row0, times):
         assert np.linalg.norm(out[a:b] - want) <= REL * np.linalg.norm(want), s
         assert (np.abs(z[a:b] - lse) <= REL * qk + 2.0 ** -22 * (np.abs(lse) + 16)).all(), s
     assert (out[~owned] == 7).all() and (z[~owned] == 7).all()
+
+
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("n", [40, 6000])                       # (unsplit, and split and merged)
+@pytest.mark.parametrize("T", [1, 3, 40])
+@pytest.mark.parametrize("kv", list(KVS))
+def test_rows_of_nan_stay_nan(p1a, kv, T, n, D):
+    """a row of q with a NaN or an infinity gives NaN under each head it is in, its log-sum-exp too, whatever the plan; its neighbours give what they do without it;
+    its weights are NaN wherever it sees, under its kv head alone"""
+    Hq, Hkv = 8, 2
+    cache = Cache(p1a, KVS[kv], Hkv, D, 6, [n], 86)
+    q = dev(I.normal(I.rng(87), (T, Hq, D)))
+    bad = q.clone()
+    bad[T // 2, 1, 5] = float("nan")
+    bad[T - 1, 3, 0] = float("inf")
+    hit = torch.zeros(T, Hq, dtype=torch.bool, device="cuda")
+    hit[T // 2, 1] = hit[T - 1, 3] = True
+    rows = p1a.Rows(T, p0=n - T)
+    for out_bf16 in (False, True):
+        got = []
+        for x in (q, bad):
+            out = torch.full((T, Hq, D), 7.0, dtype=torch.bfloat16 if out_bf16 else torch.float32, device="cuda")
+            z = None if out_bf16 else torch.full((T, Hq), 7.0, device="cuda")
+            p1a.attn_chunk(x, cache.kv, out, rows, Hq, D ** -0.5, lse=z)
+            got.append((out, z))
+        (clean, z0), (out, z) = got
+        assert out[hit].isnan().all() and torch.equal(out[~hit], clean[~hit])
+        if z is not None:
+            assert z[T // 2, 1].isnan() and not z[T - 1, 3].isfinite() and z[T - 1, 3] != -np.inf and torch.equal(z[~hit], z0[~hit])
+            masses = [torch.zeros(1, Hkv, n, device="cuda") for _ in range(2)]
+            for m, x, zz in zip(masses, (q, bad), (z0, z)):
+                p1a.attn_mass(x, cache.kv, zz, m, rows, Hq, D ** -0.5)
+            assert masses[1][0, 0].isnan().all() and torch.equal(masses[1][0, 1], masses[0][0, 1])
