@@ -272,8 +272,9 @@ size_t p1a_attn_chunk_scratch_bytes(const p1a_kv *c, const p1a_rows *rows, int H
  *     mass[s][h][j] += sum over the rows t of sequence s and the q heads i of kv head h of exp(scale * q[t][i] . K[j][h] - lse[t][i])
  * over the positions j < ld that row t sees; lse [T][Hq] as p1a_attn_chunk leaves it (a row with lse = -inf adds nothing). Entries that no row
  * sees are left as they are. f32 accuracy whatever the cache; every entry is summed in a fixed order: the same bits every time. Shapes and
- * alignment as for p1a_attn_chunk, ld up to 2^30. Calls of many rows over few keys add up partial sums of the size of `mass`, in `scratch` (256-byte aligned, at
- * least p1a_attn_mass_scratch_bytes) or, with NULL or less, the library's buffers, as p1a_attn_chunk's partials.
+ * alignment as for p1a_attn_chunk, ld up to 2^30. Calls of many rows over few keys add up partial sums of the positions that a window and n_ctx
+ * let them see, 256 MB at most, in `scratch` (256-byte aligned, at least p1a_attn_mass_scratch_bytes) or, with NULL or less, the library's
+ * buffers, as p1a_attn_chunk's partials.
  */
 int p1a_attn_mass(const void *q, int q_type, const p1a_kv *c, const float *lse, float *mass, int ld, const p1a_rows *rows, int Hq, float scale,
                   void *scratch, size_t scratch_bytes, void *stream);

@@ -28,11 +28,11 @@ struct mass_params {
     const void * q;
     const float * lse;
     float * mass;
-    float * part;          // [splits][n_seq][Hkv][ld]
+    float * part;          // [splits][n_seq][Hkv][pld]: sums of the positions of the list of tiles, in its order
     const char * kc;
     kv_view pg;
     rows_view R;
-    int Hq, Hkv, GQA, ld, q_bf16;
+    int Hq, Hkv, GQA, ld, pld, q_bf16;
     uint32_t gqa_magic;
     float factor, sign;
     int runs;              // few rows: workgroups of a kv head
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
     const size_t head_off = (size_t) hk * head_bytes(KT, D);
     const int nrows = sv.count * P.GQA;
     const size_t entries = (size_t) seq * P.Hkv + hk;
-    float * const mass = P.splits > 1 ? P.part + ((size_t) split * P.R.n_seq * P.Hkv + entries) * P.ld : P.mass + entries * P.ld;
+    float * const mass = P.splits > 1 ? P.part + ((size_t) split * P.R.n_seq * P.Hkv + entries) * P.pld : P.mass + entries * P.ld;
 
     for (int b = bx * TB; b < sp.nt; b += P.blocks * TB) {
     // (the lane's number anew for each block, and once more for the sums: what follows from it would be worked out ahead of the loop and kept)
@@ -357,9 +357,12 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
                 x += __shfl_xor(x, 16);
                 if (c == i) mine = x;
             }
-            const int j = tile[u] * 32 + mfma_row(c & 15, g);
+            const int i = b + wave * NU + u, at = mfma_row(c & 15, g), j = tile[u] * 32 + at;
             const bool seen = j <= sp.pmax && (j >= sp.lo || j < sp.ns) && j < P.ld;
-            if (c < 16 && b + wave * NU + u < sp.nt && seen) mass[j] = P.splits > 1 ? mine : mass[j] + mine;
+            if (c < 16 && i < sp.nt && seen) {
+                if (P.splits > 1) mass[i * 32 + at] = mine;   // (i is at most the tile's number)
+                else mass[j] += mine;
+            }
         }
         }
         __syncthreads();                                      // (the next keys go where the rows were)
@@ -368,15 +371,17 @@ __global__ void __launch_bounds__(MTHR, 2) mass_k(const mass_params P) {
 
 // the splits' sums, in order, onto the totals of the positions that some row sees
 __global__ void __launch_bounds__(256) mass_add_k(const mass_params P) {
-    const int j = blockIdx.x * 256 + threadIdx.x, hk = blockIdx.y, seq = blockIdx.z;
+    const int x = blockIdx.x * 256 + threadIdx.x, hk = blockIdx.y, seq = blockIdx.z;
     const seq_view sv = seq_of<true>(P.R, seq);
-    if (sv.count < 1 || j >= P.ld) return;
+    if (sv.count < 1 || x >= P.pld) return;
     const span sp = span_of<32>(P.R, sv.pos0, sv.pos0 + sv.count - 1);
-    if (sp.nt == 0 || j > sp.pmax || !(j >= sp.lo || j < sp.ns)) return;
-    const size_t i = ((size_t) seq * P.Hkv + hk) * P.ld + j, step = (size_t) P.R.n_seq * P.Hkv * P.ld;
-    float x = 0.f;
-    for (int k = 0; k < P.splits; ++k) x += P.part[k * step + i];
-    P.mass[i] += x;
+    const int j = sp.tile(x >> 5) * 32 + (x & 31);
+    if (x >> 5 >= sp.nt || j > sp.pmax || !(j >= sp.lo || j < sp.ns) || j >= P.ld) return;
+    const size_t entries = (size_t) seq * P.Hkv + hk, step = (size_t) P.R.n_seq * P.Hkv * P.pld;
+    const float * const part = P.part + entries * P.pld + x;
+    float sum = 0.f;
+    for (int k = 0; k < P.splits; ++k) sum += part[k * step];
+    P.mass[entries * P.ld + j] += sum;
 }
 
 template <class F> int launch_big(F kernel, std::atomic<uint32_t> & attr_set, int lds, const mass_params & P, dim3 grid, hipStream_t s) {
@@ -413,6 +418,7 @@ template <uint32_t KT> int launch_kt(const mass_params & P, int D, int few, dim3
 // of 16 times up to eight workgroups - setting one up costs what three or four times 32 rows do, and the last of unequal ones are waited for:
 //   64 tokens over 3001 keys (32 / 8 heads of 128, f16; whole calls) 29 us unsplit, 23 in two; 256 over 3001 53 in two, 35 in four, 39 in eight;
 //   256 over 30011 177 in two, 197 in four; four prompts (24 / 4 of 256) 1240 unsplit, 475 in one or two, 335 in three, 270 in seven.
+// Partial sums take 256 MB at most: as many splits as fit.
 mass_plan plan_mass(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int ld, int cus) {
     const int GQA = Hq / c.Hkv;
     const bool planes = c.type != P1A_KV_F16;
@@ -430,7 +436,11 @@ mass_plan plan_mass(const p1a_kv & c, const rows_view & R, int Hq, int max_n, in
     pl.blocks = (int) std::min<long long>((keys + BK - 1) / BK, 65536 / c.Hkv + 1);
     const long long units = (long long) pl.blocks * c.Hkv * R.n_seq, tiles = ((long long) R.max_rows * GQA + QR - 1) / QR;
     pl.splits = (int) std::min(32LL, std::max({1LL, std::min(places / units, tiles / 4), std::min(4 * places / units, tiles / 8), std::min(8 * places / units, tiles / 16)}));
-    if (pl.splits > 1) pl.bytes = (size_t) pl.splits * R.n_seq * c.Hkv * ld * 4;
+    // (positions of a sequence's tiles: what n_ctx allows, as max_n may be less than what there is)
+    pl.pld = (int) std::min<long long>(ld, R.window == INT32_MAX ? R.n_ctx : std::min<long long>(R.n_ctx, (long long) R.window + R.max_rows + R.n_sink) + 96);
+    const size_t each = (size_t) R.n_seq * c.Hkv * pl.pld * 4;
+    pl.splits = (int) std::max(1LL, std::min<long long>(pl.splits, (256LL << 20) / (long long) std::max<size_t>(each, 1)));
+    if (pl.splits > 1) pl.bytes = pl.splits * each;
     return pl;
 }
 
@@ -442,7 +452,7 @@ int launch_mass(const p1a_kv & c, const mass_args & a, hipStream_t s) {
     P.factor = a.scale == 0.f ? 1.f : (a.scale < 0 ? -a.scale : a.scale) * LOG2E;
     P.sign = a.scale == 0.f ? 0.f : a.scale < 0 ? -1.f : 1.f;
     const mass_plan pl = plan_mass(c, a.R, a.Hq, a.max_n, a.ld, cu_count());
-    P.runs = pl.runs; P.blocks = pl.blocks; P.splits = pl.splits; P.part = nullptr;
+    P.runs = pl.runs; P.blocks = pl.blocks; P.splits = pl.splits; P.pld = pl.pld; P.part = nullptr;
     if (pl.splits > 1) {
         if (a.scratch && !((uintptr_t) a.scratch & 255) && a.scratch_bytes >= pl.bytes) P.part = (float *) a.scratch;
         else {
@@ -454,7 +464,7 @@ int launch_mass(const p1a_kv & c, const mass_args & a, hipStream_t s) {
     const int rc = c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, pl.few, grid, s)
                  : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, pl.few, grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, pl.few, grid, s);
     if (rc != P1A_OK || pl.splits == 1) return rc;
-    mass_add_k<<<dim3((a.ld + 255) / 256, c.Hkv, a.R.n_seq), 256, 0, s>>>(P);
+    mass_add_k<<<dim3((pl.pld + 255) / 256, c.Hkv, a.R.n_seq), 256, 0, s>>>(P);
     return launched();
 }
 

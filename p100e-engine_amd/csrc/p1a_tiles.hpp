@@ -584,7 +584,7 @@ struct mass_args {
     float scale;
     void * scratch; size_t scratch_bytes;
 };
-struct mass_plan { int few, runs, blocks, splits; size_t bytes; };   // (few as in chunk_plan; bytes of scratch)
+struct mass_plan { int few, runs, blocks, splits, pld; size_t bytes; };   // (few as in chunk_plan; pld: positions of a partial row; bytes of scratch)
 mass_plan plan_mass(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int ld, int cus);
 int launch_mass(const p1a_kv & c, const mass_args & a, hipStream_t s);
 int launch_evict_select(const float * mass, int ld, int n_seq, int Hkv, const int32_t * n_dev, int n, int budget, int n_sink, int n_recent, int32_t * keep, hipStream_t s);

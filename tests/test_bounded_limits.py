@@ -53,3 +53,16 @@ def test_caches_of_no_positions_need_no_scratch(kv_type, max_rows):
         rows = b.p1a_rows(64, 1, max_rows, 0, 4096, 4096, 0, window, 0)
         assert p1a.lib().p1a_attn_chunk_scratch_bytes(ctypes.byref(kv), ctypes.byref(rows), 24) == 0
         assert p1a.lib().p1a_attn_mass_scratch_bytes(ctypes.byref(kv), 64, ctypes.byref(rows), 24) >= 0
+
+
+def test_partial_sums_of_weights_go_by_what_rows_see():
+    """... and not by the length of the totals' rows, nor without bound"""
+    p1a, b = importlib.import_module("p100e-engine_amd"), importlib.import_module("p100e-engine_amd.binding")
+    kv = b.p1a_kv(p1a.KV_F16, 1 << 20, 4, 256, 4096, 8192, 4096, 4096, 8, 4 * 256 * 2 << 8)
+    for n_seq in (1, 4):
+        rows = b.p1a_rows(4096, n_seq, 4096, 0, 4096, 4096, 0, 512, 4)
+        need = p1a.lib().p1a_attn_mass_scratch_bytes(ctypes.byref(kv), 1 << 20, ctypes.byref(rows), 24)
+        assert 0 < need <= 32 * n_seq * 4 * 4 * (512 + 4096 + 4 + 96)              # (32 splits at most)
+    for max_n in (0, 3000):                                    # (understated, maybe: totals have to fit all the same)
+        rows = b.p1a_rows(4096, 1, 4096, max_n, 4096, 4096, 0, 0, 0)
+        assert p1a.lib().p1a_attn_mass_scratch_bytes(ctypes.byref(kv), 1 << 20, ctypes.byref(rows), 24) <= 256 << 20

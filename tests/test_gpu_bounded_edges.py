@@ -107,3 +107,34 @@ def test_rows_of_nan_stay_nan(p1a, kv, T, n, D):
             for m, x, zz in zip(masses, (q, bad), (z0, z)):
                 p1a.attn_mass(x, cache.kv, zz, m, rows, Hq, D ** -0.5)
             assert masses[1][0, 0].isnan().all() and torch.equal(masses[1][0, 1], masses[0][0, 1])
+
+
+@pytest.mark.parametrize("window, n_sink, ld, max_n", [(300, 70, 20000, 0), (1000, 0, 4500, 0), (64, 3, 2900, 100), (0, 0, 20000, 700), (5, 33, 20000, 0), (100, 4000, 20000, 0)])
+@pytest.mark.parametrize("kv", ["f16", "q8_0"])
+def test_partial_sums_of_weights(p1a, kv, window, n_sink, ld, max_n):
+    """many rows shared among workgroups: rows of totals far longer than what is seen, shorter too, max_n understated; entries that no row sees are left"""
+    lens, counts, Hq, D = [5000, 4000, 3001], [600, 41, 333], 4, 64
+    cache = Cache(p1a, KVS[kv], 1, D, 5, lens, 88)
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    pos0 = np.array([n - c for n, c in zip(lens, counts)], np.int32)
+    q = I.normal(I.rng(89), (first[-1], Hq, D))
+    rows = p1a.Rows(int(first[-1]), n_seq=3, row0=dev(first), pos0=dev(pos0), max_rows=600, max_n=max_n, window=window, n_sink=n_sink)
+    need = p1a.mass_scratch_bytes(cache.kv, ld, rows, Hq)
+    assert need > 0
+    exact = []
+    for s, n in enumerate(lens):
+        p = pos0[s] + np.arange(counts[s])
+        see = seen(p, n, window, n_sink)
+        exact.append(rows_exact(q[first[s]:first[s + 1]].astype(np.float64), cache.heads("k", s, n), cache.heads("v", s, n), see, 0.125) + (see,))
+    lse = dev(np.concatenate([e[1] for e in exact]).astype(np.float32))
+    for scratch in (None, torch.full((need,), 255, dtype=torch.uint8, device="cuda")):
+        mass = torch.full((3, 1, ld), 0.5, device="cuda")
+        p1a.attn_mass(dev(q), cache.kv, lse, mass, rows, Hq, 0.125, scratch=scratch)
+        got = mass.cpu().numpy().astype(np.float64)[:, 0]
+        for s, e in enumerate(exact):
+            n = min(lens[s], ld)
+            want = e[2].sum((0, 1))[:n]
+            assert np.linalg.norm(got[s, :n] - 0.5 - want) <= REL * np.linalg.norm(want) + 2.0 ** -24 * np.linalg.norm(want + 0.5), s
+            untouched = np.ones(ld, bool)
+            untouched[:n] = ~e[5].any(0)[:n]
+            assert (got[s][untouched] == 0.5).all()
