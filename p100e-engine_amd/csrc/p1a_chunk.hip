@@ -443,8 +443,9 @@ long long block_bound(const rows_view & R, int GQA) { return item_bound(R, GQA, 
 //     results), and 3 for a merge (four turns of 17 ... 150 tokens through a window of 2048, 32 / 8 of 128, q4_0: 52 + 8 us, unsplit 110; 24 sequences of
 //     1 ... 500 tokens over 500 ... 7000 keys, f16: 147 + 22, unsplit 225).
 //   few rows: as many runs of 128-key steps as there are places for workgroups, unless one for each sequence takes no longer than a run, its
-//     set-up (3), a second sequence's (2) and the merge (3) (the 32 tokens: 52 + 5 us, a workgroup for each sequence 109). Partials stay within 64 MB: fewer
-//     runs to a sequence where there are many rows.
+//     set-up (3), a second sequence's (2) and the merge (3) (the 32 tokens: 52 + 5 us, a workgroup for each sequence 109).
+// Partials take 64 MB (few rows) and 256 MB (blocks) at most: fewer to a row where there are many rows, none where two would be more. They go by T, rows of no
+// sequence among them.
 chunk_plan plan_chunk(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int cus) {
     const int GQA = Hq / c.Hkv;
     chunk_plan pl{};
@@ -459,7 +460,7 @@ chunk_plan plan_chunk(const p1a_kv & c, const rows_view & R, int Hq, int max_n, 
     if (pl.few) {
         pl.nks = 1;
         const long long runs = std::min(std::max(slots / c.Hkv, 1LL), R.n_seq * nt), per = (R.n_seq * nt + runs - 1) / runs;
-        const long long most = std::min({64LL, runs, nt + 1, std::max(2LL, (64LL << 20) / (long long) (rows * row_bytes))});
+        const long long most = std::min({64LL, runs, nt + 1, (64LL << 20) / (long long) (rows * row_bytes)});
         if (most > 1 && (units + slots - 1) / slots * (nt + 3) > std::max(per, (nt + most - 2) / (most - 1)) + 8) {
             pl.runs = (int) runs;
             pl.nks = (int) most;
@@ -467,7 +468,7 @@ chunk_plan plan_chunk(const p1a_kv & c, const rows_view & R, int Hq, int max_n, 
     } else {
         auto cost = [&](long long k) { return (units * k + slots - 1) / slots * ((nt + k - 1) / k + 3) + (k > 1 ? 3 : 0); };
         long long best = 1;
-        for (long long k = 2; k <= 64 && k <= nt; ++k) if (cost(k) < cost(best)) best = k;
+        for (long long k = 2; k <= std::min({64LL, nt, (256LL << 20) / (long long) (rows * row_bytes)}); ++k) if (cost(k) < cost(best)) best = k;
         pl.nks = (int) best;
     }
     if (pl.nks > 1) {

@@ -66,3 +66,23 @@ def test_partial_sums_of_weights_go_by_what_rows_see():
     for max_n in (0, 3000):                                    # (understated, maybe: totals have to fit all the same)
         rows = b.p1a_rows(4096, 1, 4096, max_n, 4096, 4096, 0, 0, 0)
         assert p1a.lib().p1a_attn_mass_scratch_bytes(ctypes.byref(kv), 1 << 20, ctypes.byref(rows), 24) <= 256 << 20
+
+
+def chunk_bytes(T, n_seq, max_rows, n_ctx, Hq, Hkv, D):
+    p1a, b = importlib.import_module("p100e-engine_amd"), importlib.import_module("p100e-engine_amd.binding")
+    kv = b.p1a_kv(p1a.KV_F16, n_ctx, Hkv, D, 4096, 8192, 4096, 4096, 8, Hkv * D * 2 << 8)
+    rows = b.p1a_rows(T, n_seq, max_rows, 0, 4096, 4096, 0, 0, 0)
+    return p1a.lib().p1a_attn_chunk_scratch_bytes(ctypes.byref(kv), ctypes.byref(rows), Hq)
+
+
+@pytest.mark.parametrize("n_seq", [1, 64, 256, 1024, 4096, 16384, 65535])
+def test_partials_of_few_rows_are_bounded(n_seq):
+    """single tokens: partials of at most 64 MB and the words beside them, whatever the number of sequences"""
+    assert chunk_bytes(n_seq, n_seq, 1, 32768, 32, 8, 128) <= (64 << 20) + 4 * n_seq + 1024
+    assert chunk_bytes(1 << 25, n_seq, 1, 32768, 32, 8, 128) == 0                  # (many rows of no sequence)
+
+
+@pytest.mark.parametrize("T, n_seq, max_rows, n_ctx, Hq, Hkv, D", [(91206, 64, 2145, 973763, 128, 8, 128), (2110, 1, 512, 1 << 18, 24, 4, 256), (1 << 20, 24, 100, 8192, 32, 8, 128),
+                                                                   (45012, 16, 4802, 6588, 16, 1, 128)])
+def test_partials_of_blocks_are_bounded(T, n_seq, max_rows, n_ctx, Hq, Hkv, D):
+    assert chunk_bytes(T, n_seq, max_rows, n_ctx, Hq, Hkv, D) <= (256 << 20) + 1024
