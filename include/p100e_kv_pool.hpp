@@ -52,6 +52,8 @@ public:
     void seq_restore(int id) { ck(p1a_seq_restore(need(), id)); }
     void seq_restore_prefix(int id, int n) { ck(p1a_seq_restore_prefix(need(), id, n)); }
     void seq_truncate(int id, int n) { ck(p1a_seq_truncate(need(), id, n)); }
+    // (no counterpart: behind p1a_kv_compact on every layer, the first n_keep slots stay)
+    void seq_evict(int id, int n_keep) { ck(p1a_seq_evict(need(), id, n_keep)); }
     int seq_fork(int src, int n) { return ck(p1a_seq_fork(need(), src, n)); }
     void pages_out(int id, int p0, int n, char * dst) { ck(p1a_seq_pages_out(need(), id, p0, n, dst)); }
     // what a forward step / tp_model::rollback (tp_model.cu:3159-3170) do to a sequence's bookkeeping
