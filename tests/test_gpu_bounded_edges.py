@@ -138,3 +138,81 @@ def test_partial_sums_of_weights(p1a, kv, window, n_sink, ld, max_n):
             untouched = np.ones(ld, bool)
             untouched[:n] = ~e[5].any(0)[:n]
             assert (got[s][untouched] == 0.5).all()
+
+
+def test_sequences_of_two_layers_are_evicted_in_turn(p1a):
+    """totals of each layer's own, one sequence shorter than the budget, and twice, over what was held each time: every layer keeps what its own totals say, the
+    short sequence stays whole, pages come back from the long ones alone"""
+    L, Hq, Hkv, D, psh, n_ctx, budget, n_sink, n_recent = 2, 8, 2, 64, 4, 512, 64, 4, 16
+    hb = O.row_bytes(O.KV_Q8_0, 1, D)
+    pool = p1a.Pool(p1a.KV_Q8_0, L, Hkv, D, psh, n_ctx, 4, 2048)
+    held = [300, 40, 129]
+    seqs = [pool.seq_create() for _ in held]
+    g = I.rng(90)
+
+    def raw(s):
+        """[layer][K | V][position][Hkv][head bytes] of what sequence s holds"""
+        torch.cuda.synchronize()
+        n = pool.seq_pages(seqs[s])
+        buf = torch.empty(n * 2 * L * (1 << psh) * Hkv * hb, dtype=torch.uint8, pin_memory=True)
+        pool.pages_out(seqs[s], 0, n, buf.data_ptr())
+        torch.cuda.synchronize()
+        x = buf.numpy().reshape(n, 2, L, 1 << psh, Hkv, hb).transpose(2, 1, 0, 3, 4, 5)
+        return np.ascontiguousarray(x).reshape(L, 2, n << psh, Hkv, hb)[:, :, :held[s]].copy()
+
+    def add(counts):
+        for s, c in enumerate(counts):
+            pool.seq_advance(seqs[s], None, c)
+            for layer in range(L):
+                k, v = (dev(I.normal(g, (c, Hkv, D))) for _ in range(2))
+                p1a.kv_append(pool.cache_seq(layer, seqs[s]), k, v, held[s], c)
+            held[s] += c
+        pool.set_rows(seqs)
+
+    counts, held = held, [0, 0, 0]
+    add(counts)
+    layers = [pool.cache_rows(i) for i in range(L)]
+    mass = [torch.zeros(3, Hkv, n_ctx, device="cuda") for _ in range(L)]
+    keep = torch.empty(3, Hkv, budget, dtype=torch.int32, device="cuda")
+    for turn in range(2):
+        first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+        T = int(first[-1])
+        q = dev(I.normal(g, (T, Hq, D)))
+        rows = p1a.Rows(T, n_seq=3, row0=dev(first), pos0=dev(np.array([h - c for h, c in zip(held, counts)], np.int32)), max_rows=max(counts), max_n=max(held))
+        out, lse = torch.empty(T, Hq, D, device="cuda"), torch.empty(T, Hq, device="cuda")
+        for i, (kv, m) in enumerate(zip(layers, mass)):
+            p1a.attn_chunk(q * (1 + i), kv, out, rows, Hq, 0.125, lse=lse)
+            p1a.attn_mass(q * (1 + i), kv, lse, m, rows, Hq, 0.125)
+        before, totals = [raw(s) for s in range(3)], [m.cpu().numpy() for m in mass]
+        n = dev(np.array(held, np.int32))
+        lists = []
+        for kv, m in zip(layers, mass):
+            p1a.evict_select(m, n, keep, n_sink=n_sink, n_recent=n_recent)
+            p1a.kv_compact(kv, keep, mass=m, mass_out=m)
+            lists.append(keep.cpu().numpy())
+        assert turn or not np.array_equal(lists[0][0], lists[1][0])      # (later on the old totals outweigh the new ones in both)
+        free, was = pool.free_pages, list(held)
+        for s, seq in enumerate(seqs):
+            if held[s] > budget:
+                pool.seq_evict(seq, budget)
+            held[s] = min(held[s], budget)
+            assert pool.seq_len(seq) == held[s]
+        assert pool.free_pages - free == sum(-(-w // 16) - -(-h // 16) for w, h in zip(was, held))
+        for s in range(3):
+            now = raw(s)
+            for i in range(L):
+                kept = lists[i][s, :, :held[s]]
+                t = totals[i][s]
+                for h in range(Hkv):
+                    if was[s] <= budget:
+                        assert np.array_equal(kept[h], np.arange(was[s]))
+                    else:
+                        mid = np.arange(n_sink, was[s] - n_recent)
+                        best = mid[np.lexsort((mid, -t[h][mid]))][:budget - n_sink - n_recent]
+                        assert np.array_equal(kept[h], np.sort(np.concatenate([np.arange(n_sink), best, np.arange(was[s] - n_recent, was[s])])))
+                    assert np.array_equal(now[i][:, :, h], before[s][i][:, kept[h], h])
+                    assert np.array_equal(mass[i][s, h, :held[s]].cpu().numpy(), t[h][kept[h]]) and not mass[i][s, h, held[s]:].any()
+        counts = [20, 3, 9]
+        if turn == 0:
+            add(counts)
+    pool.close()
