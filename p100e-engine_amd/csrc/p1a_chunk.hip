@@ -499,7 +499,7 @@ int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
             P.part_o = (float *) ((char *) a.scratch + pl.bytes_n + pl.bytes_ml);
         } else {
             float * first;
-            if (!split_scratch(s, pl.bytes_o, pl.bytes_n + pl.bytes_ml, P.part_o, first)) return P1A_E_SCRATCH;
+            if (!split_scratch(s, kept_bytes(pl.bytes_o), kept_bytes(pl.bytes_n + pl.bytes_ml), P.part_o, first)) return P1A_E_SCRATCH;
             P.part_n = (int *) first;
             P.part_ml = (float *) ((char *) first + pl.bytes_n);
         }

@@ -457,7 +457,7 @@ int launch_mass(const p1a_kv & c, const mass_args & a, hipStream_t s) {
         if (a.scratch && !((uintptr_t) a.scratch & 255) && a.scratch_bytes >= pl.bytes) P.part = (float *) a.scratch;
         else {
             float * unused;
-            if (!split_scratch(s, pl.bytes, 256, P.part, unused)) return P1A_E_SCRATCH;
+            if (!split_scratch(s, kept_bytes(pl.bytes), kept_bytes(1), P.part, unused)) return P1A_E_SCRATCH;
         }
     }
     const dim3 grid = pl.few ? dim3((unsigned) ((pl.runs + 7) / 8 * 8 * c.Hkv)) : dim3((unsigned) (pl.blocks * c.Hkv * pl.splits), a.R.n_seq);

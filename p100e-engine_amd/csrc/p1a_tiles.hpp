@@ -560,6 +560,13 @@ __device__ __forceinline__ void put4(void * out, bool bf16, size_t i, f4 v) {
 }
 
 // host side (p1a_api.hip)
+// What the library's own buffers are asked for where a call has these bytes: the next power of two. A buffer that is replaced stays allocated (a recorded graph may
+// hold it), and there is room for so many only: calls that grow row by row replace it a dozen times, not each time.
+inline size_t kept_bytes(size_t bytes) {
+    size_t n = 64 << 10;
+    while (n < bytes) n *= 2;
+    return n;
+}
 struct chunk_args {
     const void * q; void * out; const float * gate; float * lse;
     bool q_bf16, out_bf16;

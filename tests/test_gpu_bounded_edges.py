@@ -216,3 +216,23 @@ def test_sequences_of_two_layers_are_evicted_in_turn(p1a):
         if turn == 0:
             add(counts)
     pool.close()
+
+
+def test_partials_of_growing_calls(p1a):
+    """calls that grow row by row, without scratch of their own, on a stream of theirs: none is refused, and what the library keeps for them stays within twice the
+    largest one's (and as much again in buffers it replaced)"""
+    n, D, most = 6000, 64, 700
+    cache = Cache(p1a, O.KV_F16, 1, D, 6, [n], 91)
+    q, out = torch.randn(most, 1, D, device="cuda"), torch.empty(most, 1, D, device="cuda")
+    lse, mass = torch.empty(most, 1, device="cuda"), torch.zeros(1, 1, n, device="cuda")
+    need = 0
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    with torch.cuda.stream(torch.cuda.Stream()):
+        for T in range(33, most):
+            rows = p1a.Rows(T, p0=n - T)
+            need = max(need, p1a.chunk_scratch_bytes(cache.kv, rows, 1), p1a.mass_scratch_bytes(cache.kv, n, rows, 1))
+            p1a.attn_chunk(q, cache.kv, out, rows, 1, 0.125, lse=lse)
+            p1a.attn_mass(q, cache.kv, lse, mass, rows, 1, 0.125)
+        torch.cuda.synchronize()
+    assert free - torch.cuda.mem_get_info()[0] <= 4 * need + (64 << 20)             # (64 MB: what the runtime takes for a stream)
