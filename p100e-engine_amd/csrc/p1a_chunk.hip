@@ -468,7 +468,7 @@ chunk_plan plan_chunk(const p1a_kv & c, const rows_view & R, int Hq, int max_n, 
     } else {
         auto cost = [&](long long k) { return (units * k + slots - 1) / slots * ((nt + k - 1) / k + 3) + (k > 1 ? 3 : 0); };
         long long best = 1;
-        for (long long k = 2; k <= std::min({64LL, nt, (256LL << 20) / (long long) (rows * row_bytes)}); ++k) if (cost(k) < cost(best)) best = k;
+        for (long long k = 2; k <= std::min({64LL, nt, (256LL << 20) / (long long) (rows * row_bytes), 0xffffffLL / units}); ++k) if (cost(k) < cost(best)) best = k;
         pl.nks = (int) best;
     }
     if (pl.nks > 1) {
@@ -504,8 +504,7 @@ int launch_chunk(const p1a_kv & c, const chunk_args & a, hipStream_t s) {
             P.part_ml = (float *) ((char *) first + pl.bytes_n);
         }
     }
-    const long long grid = block_bound(a.R, P.GQA) * P.nks * c.Hkv;
-    if (grid > 0xffffff) { set_error("p1a_attn_chunk: too many rows for one call"); return P1A_E_SHAPE; }
+    const long long grid = pl.few ? 0 : block_bound(a.R, P.GQA) * P.nks * c.Hkv;   // (up to 2^23 blocks of rows and one more for each of 2^22 pairs: below 2^24)
     const bool exact = !a.out_bf16 || a.lse;
     const int rc = pl.few ? launch_step(c, P, pl.few, exact, s) : c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, exact, (unsigned) grid, s)
                  : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, exact, (unsigned) grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, exact, (unsigned) grid, s);

@@ -236,3 +236,27 @@ def test_partials_of_growing_calls(p1a):
             p1a.attn_mass(q, cache.kv, lse, mass, rows, 1, 0.125)
         torch.cuda.synchronize()
     assert free - torch.cuda.mem_get_info()[0] <= 4 * need + (64 << 20)             # (64 MB: what the runtime takes for a stream)
+
+
+def test_sequences_by_the_ten_thousand(p1a):
+    """40000 sequences, three of which have rows: nothing is refused, and they come out right"""
+    n_seq, n, Hkv, D = 40000, 8192, 8, 64
+    cache = Cache(p1a, O.KV_Q4_0, Hkv, D, 12, [n, n, n], 92)
+    at, counts = {5: 0, 20000: 1, 39999: 2}, np.zeros(n_seq, np.int64)
+    counts[list(at)] = [1, 3, 2]
+    first = np.concatenate([[0], np.cumsum(counts)]).astype(np.int32)
+    pos0 = np.full(n_seq, n - 3, np.int32)
+    table = np.zeros(n_seq, np.int32)
+    for s, i in at.items():
+        table[s] = i * cache.max_pages
+    cache.kv.rtab = dev(table)
+    q = I.normal(I.rng(93), (6, Hkv, D))
+    rows = p1a.Rows(6, n_seq=n_seq, row0=dev(first), pos0=dev(pos0), max_rows=3, max_n=n)
+    out, lse = torch.full((6, Hkv, D), 7.0, device="cuda"), torch.full((6, Hkv), 7.0, device="cuda")
+    p1a.attn_chunk(dev(q), cache.kv, out, rows, Hkv, 0.125, lse=lse)
+    for s, i in at.items():
+        a, b = first[s], first[s + 1]
+        p = n - 3 + np.arange(b - a)
+        want, z, _, _, qk = rows_exact(q[a:b].astype(np.float64), cache.heads("k", i, n), cache.heads("v", i, n), seen(p, n, 0, 0), 0.125)
+        assert np.linalg.norm(out[a:b].cpu().numpy() - want) <= REL * np.linalg.norm(want)
+        assert (np.abs(lse[a:b].cpu().numpy() - z) <= REL * qk + 2.0 ** -22 * (np.abs(z) + 16)).all()
