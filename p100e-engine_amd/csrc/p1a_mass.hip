@@ -62,7 +62,8 @@ __global__ void __launch_bounds__(NTHR, D == 256 && NT == 2 ? 1 : 2) mass_step_k
     const size_t head_off = (size_t) hk * head_bytes(KT, D);
 
     for (int at_step = steps.first; at_step < steps.end;) {
-        const auto f = steps.find(P.R, P.pg, at_step, lane);
+        typename step_runs<NW>::found f;
+        if (!steps.find(P.R, P.pg, at_step, lane, f)) return;
         const seq_view & sv = f.v;
         const int R = min(sv.count * P.GQA, 16 * NT);
         const span sp = step_runs<NW>::span_of_rows(P.R, sv);

@@ -69,8 +69,9 @@ __global__ void __launch_bounds__(NTHR, D == 256 && (KT == P1A_KV_F16 || NT == 2
     const int lane = tid & 63, c = lane & 15, g = lane >> 4;
     // whose step that is, and the sequence's runs, which of them this is
     typename step_runs<NW>::found f;
-    if (P.nks > 1) f = steps.find(P.R, P.pg, at_step, lane);
-    else {                                                    // a sequence each
+    if (P.nks > 1) {
+        if (!steps.find(P.R, P.pg, at_step, lane, f)) return;
+    } else {                                                    // a sequence each
         f.seq = run; f.first = 0; f.steps = 1 << 24;
         f.v = seq_of<true>(P.R, run);
         f.table = P.pg.pt && P.pg.rtab ? sload_i32(P.pg.rtab + run) : 0;

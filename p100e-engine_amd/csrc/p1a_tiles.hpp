@@ -474,12 +474,12 @@ template <int TPS> struct step_runs {
         end = min(first + per, n);
         return first < end;
     }
-    // the sequence that holds step `at` (of begin()'s run), where its steps begin and how many it has
+    // the sequence that holds step `at` (of begin()'s run), where its steps begin and how many it has. False: none does - row0 or pos0 have been
+    // written since begin() read them
     struct found { int seq, first, steps, table; seq_view v; };
-    __device__ __forceinline__ found find(const rows_view & R, const kv_view & pg, int at, int lane) const {
-        found f;
+    __device__ __forceinline__ bool find(const rows_view & R, const kv_view & pg, int at, int lane, found & f) const {
         int base = 0;
-        for (int s0 = 0;; s0 += 64) {
+        for (int s0 = 0; s0 < R.n_seq; s0 += 64) {
             const of_lane x = s0 ? look(R, pg, s0 + lane) : first64;
             const int u = base + lanes_up_to(x.steps());
             const unsigned long long behind = __ballot(u > at);
@@ -493,10 +493,11 @@ template <int TPS> struct step_runs {
                 f.v.count = at_l.rows();
                 f.v.pos0 = __builtin_amdgcn_readlane(x.pos0, l);
                 f.table = __builtin_amdgcn_readlane(x.table, l);
-                return f;
+                return true;
             }
             base = __builtin_amdgcn_readlane(u, 63);
         }
+        return false;
     }
 };
 // The rows of a lane's keys: key c of each half of a tile of 32
