@@ -376,6 +376,16 @@ def attn_prefill(q, c, out, T, p0, Hq, scale, gate=None, scratch=None):
     _check((_call or _calls()).prefill(q, c, out, gate, T, p0, Hq, scale, scratch, nbytes), "attn_prefill")
 
 
+def _of(t, f32, least, what):
+    """the address of a tensor of at least `least` numbers on end, float32 or int32; None: none"""
+    if t is None:
+        return None
+    d = t.dtype
+    if d.itemsize != 4 or d.is_floating_point != f32 or t.numel() < least or not t.is_contiguous():
+        raise P1AError(f"{what}: {least} numbers of type {'float32' if f32 else 'int32'} on end, not {tuple(t.shape)} of {d}")
+    return t.data_ptr()
+
+
 class Rows:
     """Which rows a call over bounded caches has, whose they are and what they see (include/p1a_attn.h, p1a_rows): T rows of n_seq sequences, sequence s
     having row0[s] .. row0[s + 1] - 1 (int32 on the device; None: T / n_seq each), the first of them at position pos0[s] (int32 on the device; None: p0).
@@ -383,7 +393,7 @@ class Rows:
 
     def __init__(self, T, n_seq=1, row0=None, pos0=None, p0=0, max_rows=0, max_n=0, window=0, n_sink=0):
         self._keep = (row0, pos0)
-        self._st = p1a_rows(T, n_seq, max_rows, max_n, _ptr(row0), _ptr(pos0), p0, window, n_sink)
+        self._st = p1a_rows(T, n_seq, max_rows, max_n, _of(row0, False, n_seq + 1, "row0"), _of(pos0, False, n_seq, "pos0"), p0, window, n_sink)
         self._ref = ctypes.byref(self._st)
 
 
@@ -406,8 +416,8 @@ def attn_chunk(q, c, out, rows, Hq, scale, gate=None, lse=None, scratch=None):
     """Attention of the new tokens of several sequences, windows and sinks among what `rows` says: q, out [T][Hq][D] float32 or bfloat16, gate [T][Hq*D] and
     lse [T][Hq] float32 or None."""
     nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    _check(lib().p1a_attn_chunk(_ptr(q), _row_type(q), ctypes.byref(c.struct()), _ptr(out), _row_type(out), _ptr(gate), _ptr(lse), rows._ref, Hq, scale,
-                                _ptr(scratch), nbytes, _stream()), "attn_chunk")
+    _check(lib().p1a_attn_chunk(_ptr(q), _row_type(q), ctypes.byref(c.struct()), _ptr(out), _row_type(out), _of(gate, True, 0, "gate"),
+                                _of(lse, True, rows._st.T * Hq, "lse"), rows._ref, Hq, scale, _ptr(scratch), nbytes, _stream()), "attn_chunk")
 
 
 def chunk_scratch_bytes(c, rows, Hq):
@@ -417,8 +427,9 @@ def chunk_scratch_bytes(c, rows, Hq):
 def attn_mass(q, c, lse, mass, rows, Hq, scale, scratch=None):
     """Adds the attention weight that the rows give to every cache position to mass [n_seq][Hkv][ld] float32; lse as attn_chunk leaves it."""
     nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    _check(lib().p1a_attn_mass(_ptr(q), _row_type(q), ctypes.byref(c.struct()), _ptr(lse), _ptr(mass), mass.shape[-1], rows._ref, Hq, scale, _ptr(scratch), nbytes,
-                               _stream()), "attn_mass")
+    kv, st, ld = c.struct(), rows._st, mass.shape[-1]
+    _check(lib().p1a_attn_mass(_ptr(q), _row_type(q), ctypes.byref(kv), _of(lse, True, st.T * Hq, "lse"), _of(mass, True, st.n_seq * kv.Hkv * ld, "mass"), ld, rows._ref, Hq, scale,
+                               _ptr(scratch), nbytes, _stream()), "attn_mass")
 
 
 def mass_scratch_bytes(c, ld, rows, Hq):
@@ -428,16 +439,23 @@ def mass_scratch_bytes(c, ld, rows, Hq):
 def evict_select(mass, n, keep, n_sink=0, n_recent=0):
     """The positions that stay, ascending: keep [n_seq][Hkv][budget] int32 of mass [n_seq][Hkv][ld] float32; n: positions held, a number or int32 [n_seq] on
     the device."""
-    n_dev, n_host = (None, n) if isinstance(n, int) else (_ptr(n), 0)
-    _check(lib().p1a_evict_select(_ptr(mass), mass.shape[-1], mass.shape[0], mass.shape[1], n_dev, n_host, keep.shape[-1], n_sink, n_recent, _ptr(keep), _stream()),
-           "evict_select")
+    n_seq, Hkv, ld = mass.shape
+    budget = keep.shape[-1]
+    n_dev, n_host = (None, n) if isinstance(n, int) else (_of(n, False, n_seq, "n"), 0)
+    _check(lib().p1a_evict_select(_of(mass, True, 0, "mass"), ld, n_seq, Hkv, n_dev, n_host, budget, n_sink, n_recent,
+                                  _of(keep, False, n_seq * Hkv * budget, "keep"), _stream()), "evict_select")
 
 
 def kv_compact(c, keep, mass=None, mass_out=None):
     """Moves the rows that keep [n_seq][Hkv][budget] lists to the front of the sequences' pages, in place, and the totals with them (mass_out: mass itself, or
     another tensor of its shape)."""
-    _check(lib().p1a_kv_compact(ctypes.byref(c.struct()), _ptr(keep), keep.shape[0], keep.shape[-1], _ptr(mass), _ptr(mass_out), 0 if mass is None else mass.shape[-1],
-                                _stream()), "kv_compact")
+    n_seq, Hkv, budget = keep.shape
+    ld = 0 if mass is None else mass.shape[-1]
+    kv = c.struct()
+    if Hkv != kv.Hkv:
+        raise P1AError(f"keep: lists of {Hkv} kv heads for a cache of {kv.Hkv}")
+    _check(lib().p1a_kv_compact(ctypes.byref(kv), _of(keep, False, 0, "keep"), n_seq, budget, _of(mass, True, n_seq * Hkv * ld, "mass"),
+                                _of(mass_out, True, n_seq * Hkv * ld, "mass_out"), ld, _stream()), "kv_compact")
 
 
 def sigmoid_mul(x, g):

@@ -86,3 +86,32 @@ def test_partials_of_few_rows_are_bounded(n_seq):
                                                                    (45012, 16, 4802, 6588, 16, 1, 128)])
 def test_partials_of_blocks_are_bounded(T, n_seq, max_rows, n_ctx, Hq, Hkv, D):
     assert chunk_bytes(T, n_seq, max_rows, n_ctx, Hq, Hkv, D) <= (256 << 20) + 1024
+
+
+def test_the_binding_refuses_tensors_that_would_be_misread():
+    """numbers of another size, too few of them, or not on end: a position in 64 bits would be read as two"""
+    torch = pytest.importorskip("torch")
+    p1a = importlib.import_module("p100e-engine_amd")
+    i32 = dict(dtype=torch.int32)
+    for bad in (dict(row0=torch.zeros(4, dtype=torch.int64)), dict(pos0=torch.zeros(3, dtype=torch.int64)), dict(pos0=torch.zeros(3)), dict(row0=torch.zeros(3, **i32)),
+                dict(pos0=torch.zeros(2, **i32)), dict(pos0=torch.zeros(6, **i32)[::2])):
+        with pytest.raises(p1a.P1AError, match=next(iter(bad))):
+            p1a.Rows(9, n_seq=3, **bad)
+    rows = p1a.Rows(9, n_seq=3, row0=torch.zeros(4, **i32), pos0=torch.zeros(3, **i32))
+    cache = p1a.KVCache(p1a.KV_F16, 64, 1, 64, 4096, 8192)
+    q, lse, mass, keep = torch.zeros(9, 2, 64), torch.zeros(9, 2), torch.zeros(3, 1, 64), torch.zeros(3, 1, 8, **i32)
+    for x in (lse.bfloat16(), lse[:8], torch.zeros(2, 9).t()):
+        with pytest.raises(p1a.P1AError, match="lse"):
+            p1a.attn_chunk(q, cache, q, rows, 2, 0.1, lse=x)
+        with pytest.raises(p1a.P1AError, match="lse"):
+            p1a.attn_mass(q, cache, x, mass, rows, 2, 0.1)
+    with pytest.raises(p1a.P1AError, match="gate"):
+        p1a.attn_chunk(q, cache, q, rows, 2, 0.1, gate=torch.zeros(9, 128, dtype=torch.bfloat16))
+    for x in (mass.double(), mass[:2], torch.zeros(3, 1, 128)[..., ::2]):
+        with pytest.raises(p1a.P1AError, match="mass"):
+            p1a.attn_mass(q, cache, lse, x, rows, 2, 0.1)
+    for call, what in ((lambda: p1a.evict_select(mass.double(), 9, keep), "mass"), (lambda: p1a.evict_select(mass, torch.zeros(3, dtype=torch.int64), keep), "n"),
+                       (lambda: p1a.evict_select(mass, 9, keep.long()), "keep"), (lambda: p1a.evict_select(mass, 9, keep[:2]), "keep"), (lambda: p1a.kv_compact(cache, keep.long()), "keep"),
+                       (lambda: p1a.kv_compact(cache, torch.zeros(3, 2, 8, **i32)), "keep"), (lambda: p1a.kv_compact(cache, keep, mass=mass, mass_out=mass[:2]), "mass_out")):
+        with pytest.raises(p1a.P1AError, match=what):
+            call()
