@@ -376,13 +376,19 @@ def attn_prefill(q, c, out, T, p0, Hq, scale, gate=None, scratch=None):
     _check((_call or _calls()).prefill(q, c, out, gate, T, p0, Hq, scale, scratch, nbytes), "attn_prefill")
 
 
+_F32 = _I32 = None      # torch.float32 and torch.int32, once torch is there
+
+
 def _of(t, f32, least, what):
     """the address of a tensor of at least `least` numbers on end, float32 or int32; None: none"""
+    global _F32, _I32
     if t is None:
         return None
-    d = t.dtype
-    if d.itemsize != 4 or d.is_floating_point != f32 or t.numel() < least or not t.is_contiguous():
-        raise P1AError(f"{what}: {least} numbers of type {'float32' if f32 else 'int32'} on end, not {tuple(t.shape)} of {d}")
+    if _F32 is None:
+        import torch
+        _F32, _I32 = torch.float32, torch.int32
+    if t.dtype is not (_F32 if f32 else _I32) or t.numel() < least or not t.is_contiguous():
+        raise P1AError(f"{what}: {least} numbers of type {'float32' if f32 else 'int32'} on end, not {tuple(t.shape)} of {t.dtype}")
     return t.data_ptr()
 
 
@@ -392,7 +398,7 @@ class Rows:
     max_rows, max_n: the most rows and positions of a sequence, where the host knows them. One object serves every layer of a step."""
 
     def __init__(self, T, n_seq=1, row0=None, pos0=None, p0=0, max_rows=0, max_n=0, window=0, n_sink=0):
-        self._keep = (row0, pos0)
+        self._keep, self.T, self.n_seq = (row0, pos0), T, n_seq
         self._st = p1a_rows(T, n_seq, max_rows, max_n, _of(row0, False, n_seq + 1, "row0"), _of(pos0, False, n_seq, "pos0"), p0, window, n_sink)
         self._ref = ctypes.byref(self._st)
 
@@ -415,9 +421,20 @@ def _row_type(t):
 def attn_chunk(q, c, out, rows, Hq, scale, gate=None, lse=None, scratch=None):
     """Attention of the new tokens of several sequences, windows and sinks among what `rows` says: q, out [T][Hq][D] float32 or bfloat16, gate [T][Hq*D] and
     lse [T][Hq] float32 or None."""
-    nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    _check(lib().p1a_attn_chunk(_ptr(q), _row_type(q), ctypes.byref(c.struct()), _ptr(out), _row_type(out), _of(gate, True, 0, "gate"),
-                                _of(lse, True, rows._st.T * Hq, "lse"), rows._ref, Hq, scale, _ptr(scratch), nbytes, _stream()), "attn_chunk")
+    qt, ot = _row_types.get(q.dtype), _row_types.get(out.dtype)
+    if qt is None or ot is None:
+        qt, ot = _row_type(q), _row_type(out)
+    # (a call of few rows is bound by the host: what is None costs nothing, and a type known already a look-up)
+    if gate is not None:
+        gate = _of(gate, True, 0, "gate")
+    if lse is not None:
+        if lse.dtype is not _F32 or lse.numel() < rows.T * Hq or not lse.is_contiguous():
+            _of(lse, True, rows.T * Hq, "lse")
+        lse = lse.data_ptr()
+    to, nbytes = (None, 0) if scratch is None else (scratch.data_ptr(), scratch.nbytes)
+    rc = (_lib or lib()).p1a_attn_chunk(q.data_ptr(), qt, ctypes.byref(c.struct()), out.data_ptr(), ot, gate, lse, rows._ref, Hq, scale, to, nbytes, _stream())
+    if rc:
+        _check(rc, "attn_chunk")
 
 
 def chunk_scratch_bytes(c, rows, Hq):
@@ -426,10 +443,15 @@ def chunk_scratch_bytes(c, rows, Hq):
 
 def attn_mass(q, c, lse, mass, rows, Hq, scale, scratch=None):
     """Adds the attention weight that the rows give to every cache position to mass [n_seq][Hkv][ld] float32; lse as attn_chunk leaves it."""
-    nbytes = 0 if scratch is None else scratch.numel() * scratch.element_size()
-    kv, st, ld = c.struct(), rows._st, mass.shape[-1]
-    _check(lib().p1a_attn_mass(_ptr(q), _row_type(q), ctypes.byref(kv), _of(lse, True, st.T * Hq, "lse"), _of(mass, True, st.n_seq * kv.Hkv * ld, "mass"), ld, rows._ref, Hq, scale,
-                               _ptr(scratch), nbytes, _stream()), "attn_mass")
+    kv, ld = c.struct(), mass.shape[-1]
+    n, entries = rows.T * Hq, rows.n_seq * kv.Hkv * ld
+    if lse.dtype is not _F32 or mass.dtype is not _F32 or lse.numel() < n or mass.numel() < entries or not lse.is_contiguous() or not mass.is_contiguous():
+        _of(lse, True, n, "lse")
+        _of(mass, True, entries, "mass")
+    to, nbytes = (None, 0) if scratch is None else (scratch.data_ptr(), scratch.nbytes)
+    rc = (_lib or lib()).p1a_attn_mass(q.data_ptr(), _row_type(q), ctypes.byref(kv), lse.data_ptr(), mass.data_ptr(), ld, rows._ref, Hq, scale, to, nbytes, _stream())
+    if rc:
+        _check(rc, "attn_mass")
 
 
 def mass_scratch_bytes(c, ld, rows, Hq):
@@ -441,21 +463,32 @@ def evict_select(mass, n, keep, n_sink=0, n_recent=0):
     the device."""
     n_seq, Hkv, ld = mass.shape
     budget = keep.shape[-1]
+    if mass.dtype is not _F32 or keep.dtype is not _I32 or keep.numel() < n_seq * Hkv * budget or not mass.is_contiguous() or not keep.is_contiguous():
+        _of(mass, True, 0, "mass")
+        _of(keep, False, n_seq * Hkv * budget, "keep")
     n_dev, n_host = (None, n) if isinstance(n, int) else (_of(n, False, n_seq, "n"), 0)
-    _check(lib().p1a_evict_select(_of(mass, True, 0, "mass"), ld, n_seq, Hkv, n_dev, n_host, budget, n_sink, n_recent,
-                                  _of(keep, False, n_seq * Hkv * budget, "keep"), _stream()), "evict_select")
+    rc = (_lib or lib()).p1a_evict_select(mass.data_ptr(), ld, n_seq, Hkv, n_dev, n_host, budget, n_sink, n_recent, keep.data_ptr(), _stream())
+    if rc:
+        _check(rc, "evict_select")
 
 
 def kv_compact(c, keep, mass=None, mass_out=None):
     """Moves the rows that keep [n_seq][Hkv][budget] lists to the front of the sequences' pages, in place, and the totals with them (mass_out: mass itself, or
     another tensor of its shape)."""
     n_seq, Hkv, budget = keep.shape
-    ld = 0 if mass is None else mass.shape[-1]
-    kv = c.struct()
+    kv, ld, m, to = c.struct(), 0, None, None
     if Hkv != kv.Hkv:
         raise P1AError(f"keep: lists of {Hkv} kv heads for a cache of {kv.Hkv}")
-    _check(lib().p1a_kv_compact(ctypes.byref(kv), _of(keep, False, 0, "keep"), n_seq, budget, _of(mass, True, n_seq * Hkv * ld, "mass"),
-                                _of(mass_out, True, n_seq * Hkv * ld, "mass_out"), ld, _stream()), "kv_compact")
+    if keep.dtype is not _I32 or not keep.is_contiguous():
+        _of(keep, False, 0, "keep")
+    if mass is not None:
+        ld = mass.shape[-1]
+        m = to = _of(mass, True, n_seq * Hkv * ld, "mass")
+    if mass_out is not mass:
+        to = _of(mass_out, True, n_seq * Hkv * ld, "mass_out")
+    rc = (_lib or lib()).p1a_kv_compact(ctypes.byref(kv), keep.data_ptr(), n_seq, budget, m, to, ld, _stream())
+    if rc:
+        _check(rc, "kv_compact")
 
 
 def sigmoid_mul(x, g):
