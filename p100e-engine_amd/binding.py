@@ -399,7 +399,11 @@ class Rows:
 
     def __init__(self, T, n_seq=1, row0=None, pos0=None, p0=0, max_rows=0, max_n=0, window=0, n_sink=0):
         self._keep, self.T, self.n_seq = (row0, pos0), T, n_seq
-        self._st = p1a_rows(T, n_seq, max_rows, max_n, _of(row0, False, n_seq + 1, "row0"), _of(pos0, False, n_seq, "pos0"), p0, window, n_sink)
+        if row0 is not None:
+            row0 = row0.data_ptr() if row0.dtype is _I32 and row0.numel() > n_seq and row0.is_contiguous() else _of(row0, False, n_seq + 1, "row0")
+        if pos0 is not None:
+            pos0 = pos0.data_ptr() if pos0.dtype is _I32 and pos0.numel() >= n_seq and pos0.is_contiguous() else _of(pos0, False, n_seq, "pos0")
+        self._st = p1a_rows(T, n_seq, max_rows, max_n, row0, pos0, p0, window, n_sink)
         self._ref = ctypes.byref(self._st)
 
 
@@ -466,7 +470,10 @@ def evict_select(mass, n, keep, n_sink=0, n_recent=0):
     if mass.dtype is not _F32 or keep.dtype is not _I32 or keep.numel() < n_seq * Hkv * budget or not mass.is_contiguous() or not keep.is_contiguous():
         _of(mass, True, 0, "mass")
         _of(keep, False, n_seq * Hkv * budget, "keep")
-    n_dev, n_host = (None, n) if isinstance(n, int) else (_of(n, False, n_seq, "n"), 0)
+    if isinstance(n, int):
+        n_dev, n_host = None, n
+    else:
+        n_dev, n_host = n.data_ptr() if n.dtype is _I32 and n.numel() >= n_seq and n.is_contiguous() else _of(n, False, n_seq, "n"), 0
     rc = (_lib or lib()).p1a_evict_select(mass.data_ptr(), ld, n_seq, Hkv, n_dev, n_host, budget, n_sink, n_recent, keep.data_ptr(), _stream())
     if rc:
         _check(rc, "evict_select")
@@ -483,9 +490,11 @@ def kv_compact(c, keep, mass=None, mass_out=None):
         _of(keep, False, 0, "keep")
     if mass is not None:
         ld = mass.shape[-1]
-        m = to = _of(mass, True, n_seq * Hkv * ld, "mass")
+        least = n_seq * Hkv * ld
+        m = to = mass.data_ptr() if mass.dtype is _F32 and mass.numel() >= least and mass.is_contiguous() else _of(mass, True, least, "mass")
     if mass_out is not mass:
-        to = _of(mass_out, True, n_seq * Hkv * ld, "mass_out")
+        least = n_seq * Hkv * ld
+        to = mass_out.data_ptr() if mass_out is not None and mass_out.dtype is _F32 and mass_out.numel() >= least and mass_out.is_contiguous() else _of(mass_out, True, least, "mass_out")
     rc = (_lib or lib()).p1a_kv_compact(ctypes.byref(kv), keep.data_ptr(), n_seq, budget, m, to, ld, _stream())
     if rc:
         _check(rc, "kv_compact")
