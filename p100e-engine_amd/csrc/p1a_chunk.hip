@@ -8,9 +8,11 @@
 // P = exp2(scale log2 e S - r), O and l are sums over P and rescaled when the row's maximum comes out of [r + 8 - inf, r + 14]. Where results are f32, q and P
 // are two f16 halves (EXACT) and quantized K and V two planes (p1a_tiles.hpp): 2 products for f16 caches, 3 for quantized ones (low times low is 2^-22
 // of the result and left out). P runs up to 2^14, so its low halves end 2^-38 below the largest weight.
-// What bounds it: with a wave to a SIMD (heads of 256: O and Q fill the registers) whatever is not hidden behind that wave's own products - without the
-// loads 4096 tokens of a document through a window of 4096 (24 / 4 heads of 256, f16, bf16 out) took a fifth less. They take 508 to 600 us by card,
-// 700 to 820 TFLOP/s (a large product of the vendor's library: 1130, 370 us at that rate); eight prompts of 77 ... 2003 tokens 280 to 310.
+// What bounds it, heads of 256 and f16: a tile of 64 keys asks LDS for as many clocks as the matrix pipe - 256 KB, as every wave reads all of K and V, and 64 products
+// of a wave: 2048 each -, and with a wave to a SIMD (O and Q fill the registers) whatever is not hidden behind that wave's own products waits: 4096 tokens of a
+// document through a window of 4096 (24 / 4 heads, bf16 out) keep the pipe busy for 36 % of the time, the waves wait for 39 %; without the loads they took a fifth
+// less. They take 508 to 600 us by card, 700 to 820 TFLOP/s (a large product of the vendor's library: 1130, 370 us at that rate); eight prompts of 77 ... 2003
+// tokens 280 to 310. (p1a_prefill.hip, a wave to a SIMD too, shares V between two waves, 1536 clocks of LDS, and reaches 1.1 PFLOP/s.)
 #include "p1a_tiles.hpp"
 
 #include <algorithm>
@@ -441,7 +443,7 @@ long long block_bound(const rows_view & R, int GQA) { return item_bound(R, GQA, 
 // 260 keys, 4 / 1 heads of 64: 7 us, as a block 9 and 2 of merging; 32 tokens through 4096 keys, 24 / 4 of 256, q8_0: 52 + 5, as blocks 164 + 5).
 //   blocks of rows: the number of workgroups that share a block's keys minimises rounds of workgroups x (64-key tiles of a workgroup + 3 for its set-up and
 //     results), and 3 for a merge (four turns of 17 ... 150 tokens through a window of 2048, 32 / 8 of 128, q4_0: 52 + 8 us, unsplit 110; 24 sequences of
-//     1 ... 500 tokens over 500 ... 7000 keys, f16: 147 + 22, unsplit 225).
+//     1 ... 500 tokens over 500 ... 7000 keys, f16: 147 + 19, unsplit 225).
 //   few rows: as many runs of 128-key steps as there are places for workgroups, unless one for each sequence takes no longer than a run, its
 //     set-up (3), a second sequence's (2) and the merge (3) (the 32 tokens: 52 + 5 us, a workgroup for each sequence 109).
 // Partials take 64 MB (few rows) and 256 MB (blocks) at most: fewer to a row where there are many rows, none where two would be more. They go by T, rows of no

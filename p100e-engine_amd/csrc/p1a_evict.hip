@@ -10,7 +10,8 @@ namespace {
 // ones, in order. A thread holds 16 consecutive values of a part of 16384; longer rows are read again for each pass (from L2). Counts go to 32 copies of
 // the histogram, one for every other lane: values of one order of magnitude share their first digit, and additions to one address wait for each other.
 // What bounds it: one compute unit's vector instructions a row, some 15 a value and pass: 1100 positions 8 us, 8190 14, 100003 72. (Eleven bits a pass,
-// fewer passes, values kept in registers or LDS or asked for ahead took 92 to 145 there; several workgroups a row would need a workspace for their counts.)
+// fewer passes, values kept in registers or LDS or asked for ahead took 92 to 145 there; several workgroups a row, their counts in scratch, have not
+// been built: eight rows leave 248 compute units idle.)
 constexpr int STHR = 1024, PER = 16, PART = STHR * PER;
 
 // larger values have larger keys; -0 is 0, a NaN is below everything
