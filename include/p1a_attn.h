@@ -227,8 +227,8 @@ int p1a_warmup_prefill(int T, int p0, int Hq, int Hkv, int D, void *stream);
  * row0[n_seq] - are left as they are; a row whose position is negative or not below the descriptor's n_ctx sees nothing: its result is 0, its
  * log-sum-exp -inf. Sequence s reads the page table pt + rtab[s]; without rtab (or without pt) there is one sequence.
  * row0 and pos0 are read on the device when the kernels run; the other fields are the host's. A pair of row0 that runs backwards is an empty
- * sequence, rows past T or past max_rows of a sequence are not looked at. Two pairs that share rows are no call's: results are then unspecified. Page-table entries of positions that no row sees are never read, nor
- * is memory behind them: a page that has left the window may be given away.
+ * sequence, rows past T or past max_rows of a sequence are not looked at. Two pairs that share rows are no call's: results are then unspecified.
+ * Page-table entries of positions that no row sees are never read, nor is memory behind them: a page that has left the window may be given away.
  */
 #define P1A_ROWS_F32  0
 #define P1A_ROWS_BF16 1
@@ -256,7 +256,7 @@ typedef struct p1a_rows {
  * it gives are then no numbers either), and no other's.
  * D = 64, 128 or 256; Hq / Hkv up to 64; T * Hq, n_ctx up to 2^30, n_seq up to 65535, Hkv up to 4096, n_seq * Hkv up to 2^22; 16-byte aligned q, out and gate; f16 caches: 16-byte aligned bases and page strides, q8_0: 4-byte aligned,
  * q4_0: 2-byte aligned; pages of any length.
- * A call of few rows is split over its keys and its partials merged by a second launch; they live in `scratch` (256-byte aligned, at least
+ * A call of few rows is split over its keys and its partials - 256 MB at most, counted by T - merged by a second launch; they live in `scratch` (256-byte aligned, at least
  * p1a_attn_chunk_scratch_bytes) or, with NULL or less, in the library's buffers of (device, stream), under the rules of p1a_attn_prefill's: nothing is
  * allocated during stream capture (P1A_E_SCRATCH: make one eager call first, or bring scratch), graphs captured on one stream share them - replay
  * such graphs one behind the other, or bring scratch for each. Result bits depend on the call's numbers - the
