@@ -302,6 +302,71 @@ int p1a_evict_select(const float *mass, int ld, int n_seq, int Hkv, const int32_
  */
 int p1a_kv_compact(const p1a_kv *c, const int32_t *keep, int n_seq, int budget, const float *mass, float *mass_out, int ld, void *stream);
 
+/*
+ * ---- Trees of drafted tokens (no counterparts in the reference, whose drafts are chains) ----
+ *
+ * Per sequence a step has nodes: node 0 is the last token that is certain, node i > 0 a drafted token with a parent among nodes 0 .. i - 1; a chain is the tree
+ * where i's parent is i - 1. Node i of sequence s is row row0[s] + i of p1a_rows and stands in cache slot pos0[s] + i, its rotary position is pos0[s] + its depth. A
+ * step: p1a_tree_rows; per layer p1a_attn_prep_mrope (sect = s0 = 1: cache rows from `slot`, rotary positions from `pos`) and p1a_attn_tree; p1a_tree_verify on the rows'
+ * logits; p1a_tree_commit, after which the sequence holds pos0[s] + 1 + n_accept[s] positions. A sequence has at most P1A_TREE_NODES nodes (rows->max_rows says how
+ * many it may have here); rows of no sequence are left as they are.
+ */
+#define P1A_TREE_NODES 1024
+
+/*
+ * From the parents (parent [T] int32, a node's number in its own tree; what is not in 0 .. i - 1 makes i a node without parent): mask [T][words], bit b of word w set where
+ * the row sees node 32 w + b of its tree - itself and the nodes above it -, 32 words >= rows->max_rows; pos [T] = pos0 + the nodes above it; slot [T] = pos0 + i. pos and slot
+ * may be NULL. rows->window, n_sink, max_n are not looked at.
+ */
+int p1a_tree_rows(const int32_t *parent, const p1a_rows *rows, uint32_t *mask, int words, int32_t *pos, int32_t *slot, void *stream);
+
+/*
+ * Attention of the nodes' rows over the cache, which holds their own K and V in their slots: as p1a_attn_chunk, but row i of sequence s sees the positions j < pos0[s] - with
+ * a window those with j > p - window or j < n_sink, p = pos0[s] + the nodes of its mask - 1 (pos0[s] for an empty one) - and of its tree the slots pos0[s] + b whose bit b is set
+ * in mask [T][words], whatever the window. Any mask may be given; bits of nodes that the sequence does not have are not looked at, 32 words >= rows->max_rows. A row
+ * that sees nothing, or whose slot is negative or not below n_ctx, has the result 0 and the log-sum-exp -inf.
+ * Types, precision, alignment, limits, scratch and capture as for p1a_attn_chunk (partials: 128 MB at most); from one node to P1A_TREE_NODES.
+ */
+int p1a_attn_tree(const void *q, int q_type, const p1a_kv *c, void *out, int out_type, const float *gate, float *lse, const p1a_rows *rows,
+                  const uint32_t *mask, int words, int Hq, float scale, void *scratch, size_t scratch_bytes, void *stream);
+/* bytes of partials such a call has (0: none); f32: whether it has f32 results (out or lse) */
+size_t p1a_attn_tree_scratch_bytes(const p1a_kv *c, const p1a_rows *rows, int Hq, int f32);
+
+/*
+ * Which drafted tokens stand, by sampling that leaves the target's distribution as it is. The walk starts at node 0. At node r with the target's distribution p and the draft's q
+ * (both of row r: of the token behind it) and the children c in ascending order, each with its token x:
+ *     left = p, mass = 1, gone = 0;  c is accepted, and the walk goes on there, if u[c] * share * mass < left[x], share = q[x] / (1 - gone);  otherwise
+ *     left = max(left - mass / (1 - gone) * q, 0), mass = sum(left), and for children drawn without replacement (P1A_VERIFY_DISTINCT) gone += q[x].
+ * Without a draft (draft NULL: tokens proposed without probabilities) share = 1, and a rejection takes x out: mass -= left[x], left[x] = 0.
+ * Where no child is accepted the walk ends: next[s] is drawn from `left` - the lowest j whose running sum passes u_next[s] * sum(left) -, or from p where nothing is left.
+ * Sums and comparisons are made in 64 bits. u, u_next: f32 in [0, 1).
+ *   target [T] rows of V values, ld_target apart (0: V), type P1A_ROWS_F32 or _BF16: logits - p = softmax(logits / temp[s]), temp [n_seq] f32 or NULL: 1; temp <= 0 (or NaN): the token of
+ *     the largest logit, the lowest of equals, with certainty - or, with P1A_VERIFY_PROBS, probabilities as they are (temp is not looked at). A NaN counts as no weight (a negative
+ *     probability too); infinite logits share everything.
+ *   draft [T] rows of V probabilities, ld_draft apart (0: V), of draft_type; rows of nodes without children are not read.
+ *   token [T] int32; a node whose token is not in 0 .. V - 1 is passed over. parent [T] as above, or NULL: chains.
+ *   max_children: the most children of a node that are looked at with a draft (>= 1; parent == NULL: 1 whatever it is); further ones are passed over. It costs a launch each.
+ *   n_accept [n_seq]: accepted tokens; path [n_seq][ld_path]: their nodes in order, -1 behind them (ld_path >= 1; what does not fit is left out, n_accept counts it); next [n_seq]: the token behind
+ *     them, -1 where its row has no weight at all or the sequence no rows.
+ * row0 as ever; pos0 and the rest of p1a_rows are not looked at. V up to 2^20, rows 16-byte aligned when ld and V allow it and aligned to their type otherwise, T up to 2^20.
+ * Scratch (sums of stretches of rows, p1a_tree_verify_scratch_bytes) under the rules of p1a_attn_chunk. The same bits every time.
+ */
+#define P1A_VERIFY_PROBS    1
+#define P1A_VERIFY_DISTINCT 2
+int p1a_tree_verify(const void *target, int target_type, size_t ld_target, const void *draft, int draft_type, size_t ld_draft, int V, const int32_t *token,
+                    const int32_t *parent, const float *temp, const float *u, const float *u_next, int32_t *n_accept, int32_t *path, int ld_path, int32_t *next,
+                    const p1a_rows *rows, int max_children, int flags, void *scratch, size_t scratch_bytes, void *stream);
+size_t p1a_tree_verify_scratch_bytes(const p1a_rows *rows, int V, int flags);
+
+/*
+ * Moves the accepted nodes' rows of K and V behind node 0's, in place, in `n_layers` layers at once: slot pos0[s] + 1 + k becomes what slot pos0[s] + path[s][k] was, for k
+ * < n_accept[s] (cut to 0 .. ld_path). path is ascending, as p1a_tree_verify leaves it: entries not above their own index, not below the sequence's nodes, or whose slots are
+ * negative or not below n_ctx move nothing. `layers`: descriptors in host memory, alike in everything but k and v; n_layers up to P1A_TREE_LAYERS. Pages that a page table names twice, for
+ * slots of two sequences, are no call's. Alignment: 2 bytes for every cache type.
+ */
+#define P1A_TREE_LAYERS 128
+int p1a_tree_commit(const p1a_kv *layers, int n_layers, const p1a_rows *rows, const int32_t *n_accept, const int32_t *path, int ld_path, void *stream);
+
 /* Standalone sigmoid gate x[i] *= 1 / (1 + exp(-g[i])). Replaces k::sigmoid_mul, src/kernels.cu:85-93. */
 int p1a_sigmoid_mul(float *x, const float *g, size_t n, void *stream);
 

@@ -11,4 +11,5 @@ from .binding import (  # noqa: F401
     get_nsplit, kv_append, kv_append_dev, kv_append_rows, kv_fill_random, kv_row_bytes, lib, lib_path, prefill_scratch_bytes, prefill_key_splits,
     set_nsplit, sigmoid_mul, warmup, reload_env, decode_scratch_bytes, decode_footprint_bytes, numerics_id, warmup_prefill, set_prefill_staging_limit, bench_decode_split_only, bench_stream_read, EXPORTS, Pool, verify_accept, p1a_kv,
     Rows, attn_chunk, chunk_scratch_bytes, attn_mass, mass_scratch_bytes, evict_select, kv_compact,
+    Layers, attn_tree, tree_commit, tree_rows, tree_scratch_bytes, tree_verify, verify_scratch_bytes,
 )

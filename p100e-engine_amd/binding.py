@@ -13,6 +13,7 @@ EXPORTS = [
     "p1a_kv_row_bytes", "p1a_kv_append", "p1a_kv_fill_random", "p1a_attn_prep", "p1a_attn_prep_mrope", "p1a_attn_decode", "p1a_attn_decode_a16", "p1a_attn_decode_noalloc", "p1a_a16_bytes", "p1a_ew_quant", "p1a_attn_prefill", "p1a_attn_prefill_scratch_bytes", "p1a_attn_prefill_key_splits", "p1a_attn_prefill_call_splits",
     "p1a_sigmoid_mul", "p1a_warmup", "p1a_get_nsplit", "p1a_set_nsplit", "p1a_reload_env", "p1a_warmup_prefill", "p1a_set_prefill_staging_limit", "p1a_bench_decode_split_only", "p1a_bench_stream_read", "p1a_release", "p1a_last_error",
     "p1a_attn_chunk", "p1a_attn_chunk_scratch_bytes", "p1a_attn_mass", "p1a_attn_mass_scratch_bytes", "p1a_evict_select", "p1a_kv_compact", "p1a_seq_evict",
+    "p1a_tree_rows", "p1a_attn_tree", "p1a_attn_tree_scratch_bytes", "p1a_tree_verify", "p1a_tree_verify_scratch_bytes", "p1a_tree_commit",
     "p1a_version", "p1a_decode_scratch_bytes", "p1a_decode_footprint_bytes", "p1a_numerics_id",
     # include/p1a_pool.h
     "p1a_pool_create", "p1a_pool_destroy", "p1a_pool_n_pages", "p1a_pool_free_pages", "p1a_pool_max_pages", "p1a_pool_page_bytes",
@@ -128,6 +129,18 @@ def lib():
     L.p1a_evict_select.argtypes = [vp, i32, i32, i32, vp, i32, i32, i32, i32, vp, vp]
     L.p1a_kv_compact.restype = i32
     L.p1a_kv_compact.argtypes = [kvp, vp, i32, i32, vp, vp, i32, vp]
+    L.p1a_tree_rows.restype = i32
+    L.p1a_tree_rows.argtypes = [vp, rp, vp, i32, vp, vp, vp]
+    L.p1a_attn_tree.restype = i32
+    L.p1a_attn_tree.argtypes = [vp, i32, kvp, vp, i32, vp, vp, rp, vp, i32, i32, f32, vp, sz, vp]
+    L.p1a_attn_tree_scratch_bytes.restype = sz
+    L.p1a_attn_tree_scratch_bytes.argtypes = [kvp, rp, i32, i32]
+    L.p1a_tree_verify.restype = i32
+    L.p1a_tree_verify.argtypes = [vp, i32, sz, vp, i32, sz, i32, vp, vp, vp, vp, vp, vp, vp, i32, vp, rp, i32, i32, vp, sz, vp]
+    L.p1a_tree_verify_scratch_bytes.restype = sz
+    L.p1a_tree_verify_scratch_bytes.argtypes = [rp, i32, i32]
+    L.p1a_tree_commit.restype = i32
+    L.p1a_tree_commit.argtypes = [vp, i32, rp, vp, vp, i32, vp]
     L.p1a_kv_fill_random.restype = i32
     L.p1a_kv_fill_random.argtypes = [kvp, i32, i32, ctypes.c_uint32, vp]
     L.p1a_attn_prefill_key_splits.restype = i32
@@ -498,6 +511,95 @@ def kv_compact(c, keep, mass=None, mass_out=None):
     rc = (_lib or lib()).p1a_kv_compact(ctypes.byref(kv), keep.data_ptr(), n_seq, budget, m, to, ld, _stream())
     if rc:
         _check(rc, "kv_compact")
+
+
+def tree_rows(parent, rows, mask, pos=None, slot=None):
+    """From the parents of drafted trees' nodes (parent int32 [T]): which nodes a row sees, mask int32 [T][words] (a bit each), its rotary position and its cache
+    slot, int32 [T] each or None."""
+    T, words = rows.T, mask.shape[-1]
+    if pos is not None:
+        pos = _of(pos, False, T, "pos")
+    if slot is not None:
+        slot = _of(slot, False, T, "slot")
+    rc = (_lib or lib()).p1a_tree_rows(_of(parent, False, T, "parent"), rows._ref, _of(mask, False, T * words, "mask"), words, pos, slot, _stream())
+    if rc:
+        _check(rc, "tree_rows")
+
+
+def attn_tree(q, c, out, rows, mask, Hq, scale, gate=None, lse=None, scratch=None):
+    """Attention of drafted trees' rows: what is in front of the tree (through `rows`' window) and, of the tree, what mask int32 [T][words] says. q, out
+    [T][Hq][D] float32 or bfloat16, gate [T][Hq*D] and lse [T][Hq] float32 or None."""
+    qt, ot, T = _row_types.get(q.dtype), _row_types.get(out.dtype), rows.T
+    if qt is None or ot is None:
+        qt, ot = _row_type(q), _row_type(out)
+    kv, words = c.struct(), mask.shape[-1]
+    n = T * Hq * kv.D
+    if q.numel() < n or out.numel() < n or not q.is_contiguous() or not out.is_contiguous():
+        raise P1AError(f"q and out: {n} numbers on end, not {tuple(q.shape)} and {tuple(out.shape)}")
+    if gate is not None:
+        gate = _of(gate, True, n, "gate")
+    if lse is not None:
+        lse = _of(lse, True, T * Hq, "lse")
+    to, nbytes = (None, 0) if scratch is None else (scratch.data_ptr(), scratch.nbytes)
+    rc = (_lib or lib()).p1a_attn_tree(q.data_ptr(), qt, ctypes.byref(kv), out.data_ptr(), ot, gate, lse, rows._ref, _of(mask, False, T * words, "mask"), words, Hq, scale,
+                                       to, nbytes, _stream())
+    if rc:
+        _check(rc, "attn_tree")
+
+
+def tree_scratch_bytes(c, rows, Hq, f32=True):
+    """bytes of partials of an attn_tree call; f32: out is float32, or lse is asked for"""
+    return int(lib().p1a_attn_tree_scratch_bytes(ctypes.byref(c.struct()), rows._ref, Hq, 1 if f32 else 0))
+
+
+def _weights(t, T, what):
+    """address, type and distance of T rows of numbers [T][V], float32 or bfloat16"""
+    if t.dim() != 2 or t.shape[0] < T or (t.shape[1] > 1 and t.stride(1) != 1) or t.stride(0) < t.shape[1]:
+        raise P1AError(f"{what}: {T} rows of numbers on end, not {tuple(t.shape)} with strides {t.stride()}")
+    return t.data_ptr(), _row_type(t), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def tree_verify(target, token, rows, u, u_next, n_accept, path, next, parent=None, draft=None, temp=None, logits=True, max_children=1, distinct=False, scratch=None):
+    """Which drafted tokens stand, and the token behind them: target [T][V] logits (of temperatures temp [n_seq]; 0: the largest one) or, with logits=False,
+    probabilities, draft [T][V] probabilities or None, float32 or bfloat16; token, parent int32 [T] (parent None: chains), u float32 [T] and u_next [n_seq] in
+    [0, 1). Writes n_accept [n_seq], path [n_seq][..] and next [n_seq], int32. max_children: children of a node that are looked at with a draft; distinct:
+    siblings were drawn without replacement."""
+    T, S = rows.T, rows.n_seq
+    tp, tt, tld = _weights(target, T, "target")
+    V, width = target.shape[1], path.shape[-1]
+    dp, dt, dld = (None, 0, 0) if draft is None else _weights(draft, T, "draft")
+    if draft is not None and draft.shape[1] != V:
+        raise P1AError(f"draft: rows of {draft.shape[1]} numbers beside {V}")
+    to, nbytes = (None, 0) if scratch is None else (scratch.data_ptr(), scratch.nbytes)
+    rc = (_lib or lib()).p1a_tree_verify(tp, tt, tld, dp, dt, dld, V, _of(token, False, T, "token"), _of(parent, False, T, "parent"), _of(temp, True, S, "temp"), _of(u, True, T, "u"),
+                                         _of(u_next, True, S, "u_next"), _of(n_accept, False, S, "n_accept"), _of(path, False, S * width, "path"), width, _of(next, False, S, "next"),
+                                         rows._ref, max_children, (0 if logits else 1) | (2 if distinct else 0), to, nbytes, _stream())
+    if rc:
+        _check(rc, "tree_verify")
+
+
+def verify_scratch_bytes(rows, V, logits=True):
+    return int(lib().p1a_tree_verify_scratch_bytes(rows._ref, V, 0 if logits else 1))
+
+
+class Layers:
+    """The caches of several layers, alike in everything but their memory, as tree_commit takes them; one object serves every step."""
+
+    def __init__(self, caches):
+        caches = list(caches)
+        self._keep, self.n = caches, len(caches)
+        self._st = (p1a_kv * max(self.n, 1))(*[c.struct() for c in caches])
+        self._at = ctypes.addressof(self._st)
+
+
+def tree_commit(layers, rows, n_accept, path):
+    """Moves the accepted nodes' rows of K and V behind node 0's, in every layer: n_accept int32 [n_seq], path int32 [n_seq][..] as tree_verify leaves them."""
+    if not isinstance(layers, Layers):
+        layers = Layers(layers)
+    width = path.shape[-1]
+    rc = (_lib or lib()).p1a_tree_commit(layers._at, layers.n, rows._ref, _of(n_accept, False, rows.n_seq, "n_accept"), _of(path, False, rows.n_seq * width, "path"), width, _stream())
+    if rc:
+        _check(rc, "tree_commit")
 
 
 def sigmoid_mul(x, g):

@@ -244,6 +244,22 @@ int rows_ok(const p1a_kv * c, const p1a_rows * r, int Hq, const char * who, rows
     if (!r->pos0) max_n = (int) std::max(1LL, std::min<long long>(max_n, (long long) r->p0 + r->T));
     return P1A_OK;
 }
+// the rows of a call on drafted trees that has no cache
+int tree_rows_ok(const p1a_rows * r, const char * who, bool with_pos, rows_view & R) {
+    if (!r || r->T < 0 || r->n_seq < 0 || r->max_rows < 0) { set_error("%s: no rows, or a negative count among them", who); return P1A_E_ARG; }
+    if (with_pos && !r->pos0 && r->n_seq > 1) { set_error("%s: %d sequences need positions in device memory", who, r->n_seq); return P1A_E_ARG; }
+    if (!r->row0 && r->n_seq > 0 && r->T % r->n_seq) { set_error("%s: %d rows do not divide among %d sequences", who, r->T, r->n_seq); return P1A_E_ARG; }
+    R.row0 = r->row0; R.pos0 = r->pos0; R.T = r->T; R.n_seq = r->n_seq; R.p0 = r->p0;
+    R.per = r->row0 || !r->n_seq ? 0 : r->T / r->n_seq;
+    R.max_rows = r->max_rows && r->max_rows < r->T ? r->max_rows : r->T;
+    if (!r->row0 && R.per < R.max_rows) R.max_rows = R.per;
+    R.window = INT32_MAX; R.n_sink = 0; R.n_ctx = 1 << 30;
+    if (r->T > 1 << 20 || r->n_seq > 65535 || R.max_rows > P1A_TREE_NODES) {
+        set_error("%s: unsupported shape (T=%d n_seq=%d, %d nodes of a sequence): up to 2^20, 65535, %d", who, r->T, r->n_seq, R.max_rows, P1A_TREE_NODES);
+        return P1A_E_SHAPE;
+    }
+    return P1A_OK;
+}
 bool rows_type_ok(int type, const char * who) {
     if (type == P1A_ROWS_F32 || type == P1A_ROWS_BF16) return true;
     set_error("%s: unknown type of rows %d", who, type);
@@ -506,6 +522,97 @@ int p1a_kv_compact(const p1a_kv * c, const int32_t * keep, int n_seq, int budget
     if (mass && mass != mass_out && mass < mass_out + (size_t) n_seq * c->Hkv * ld && mass_out < mass + (size_t) n_seq * c->Hkv * ld) { set_error("%s: mass and mass_out overlap in part", who); return P1A_E_ARG; }
     if (!n_seq || (!budget && !mass)) return P1A_OK;
     return launch_kv_compact(*c, keep, n_seq, budget, mass, mass_out, ld, (hipStream_t) stream);
+}
+
+int p1a_tree_rows(const int32_t * parent, const p1a_rows * rows, uint32_t * mask, int words, int32_t * pos, int32_t * slot, void * stream) {
+    static const char * const who = "p1a_tree_rows";
+    rows_view R;
+    const int rc = tree_rows_ok(rows, who, true, R);
+    if (rc != P1A_OK) return rc;
+    if (!parent || !mask || words < 0) { set_error("%s: null parent / mask or negative words", who); return P1A_E_ARG; }
+    if ((long long) words * 32 < R.max_rows || words > P1A_TREE_NODES / 32) { set_error("%s: %d words for trees of %d nodes", who, words, R.max_rows); return P1A_E_SHAPE; }
+    if (((uintptr_t) parent | (uintptr_t) mask | (uintptr_t) pos | (uintptr_t) slot) & 3) { set_error("%s: pointers must be 4-byte aligned", who); return P1A_E_SHAPE; }
+    if (!rows->T || !rows->n_seq) return P1A_OK;
+    return launch_tree_rows(parent, R, mask, words, pos, slot, (hipStream_t) stream);
+}
+
+int p1a_attn_tree(const void * q, int q_type, const p1a_kv * c, void * out, int out_type, const float * gate, float * lse, const p1a_rows * rows,
+                  const uint32_t * mask, int words, int Hq, float scale, void * scratch, size_t scratch_bytes, void * stream) {
+    static const char * const who = "p1a_attn_tree";
+    chunk_args a;
+    const int rc = rows_ok(c, rows, Hq, who, a.R, a.max_n);
+    if (rc != P1A_OK) return rc;
+    if (!q || !out || !mask || words < 0) { set_error("%s: null q / out / mask or negative words", who); return P1A_E_ARG; }
+    if (!rows_type_ok(q_type, who) || !rows_type_ok(out_type, who)) return P1A_E_ARG;
+    if (((uintptr_t) q | (uintptr_t) out | (uintptr_t) gate) & 15 || ((uintptr_t) lse | (uintptr_t) mask) & 3) { set_error("%s: q/out/gate must be 16-byte aligned, lse and mask 4-byte", who); return P1A_E_SHAPE; }
+    if (a.R.max_rows > P1A_TREE_NODES || (long long) words * 32 < a.R.max_rows || words > P1A_TREE_NODES / 32) { set_error("%s: %d words for trees of %d nodes (up to %d)", who, words, a.R.max_rows, P1A_TREE_NODES); return P1A_E_SHAPE; }
+    if (!rows->T || !rows->n_seq) return P1A_OK;
+    a.q = q; a.out = out; a.gate = gate; a.lse = lse; a.q_bf16 = q_type == P1A_ROWS_BF16; a.out_bf16 = out_type == P1A_ROWS_BF16;
+    a.Hq = Hq; a.scale = scale; a.scratch = scratch; a.scratch_bytes = scratch_bytes;
+    return launch_tree(*c, a, mask, words, (hipStream_t) stream);
+}
+
+size_t p1a_attn_tree_scratch_bytes(const p1a_kv * c, const p1a_rows * rows, int Hq, int f32) {
+    static const char * const who = "p1a_attn_tree_scratch_bytes";
+    rows_view R;
+    int max_n;
+    if (rows_ok(c, rows, Hq, who, R, max_n) != P1A_OK || !rows->T || !rows->n_seq || R.max_rows > P1A_TREE_NODES) return 0;
+    const tree_plan pl = plan_tree(*c, R, Hq, max_n, f32 != 0, cu_count());
+    return pl.bytes_n + pl.bytes_ml + pl.bytes_o;
+}
+
+int p1a_tree_verify(const void * target, int target_type, size_t ld_target, const void * draft, int draft_type, size_t ld_draft, int V, const int32_t * token,
+                    const int32_t * parent, const float * temp, const float * u, const float * u_next, int32_t * n_accept, int32_t * path, int ld_path, int32_t * next,
+                    const p1a_rows * rows, int max_children, int flags, void * scratch, size_t scratch_bytes, void * stream) {
+    static const char * const who = "p1a_tree_verify";
+    verify_args a;
+    const int rc = tree_rows_ok(rows, who, false, a.R);
+    if (rc != P1A_OK) return rc;
+    if (!target || !token || !u || !u_next || !n_accept || !path || !next || ld_path < 1 || V < 1 || flags & ~(P1A_VERIFY_PROBS | P1A_VERIFY_DISTINCT) || (draft && parent && max_children < 1)) {
+        set_error("%s: null argument, unknown flag, or a count below 1 (ld_path=%d V=%d max_children=%d)", who, ld_path, V, max_children);
+        return P1A_E_ARG;
+    }
+    if (!rows_type_ok(target_type, who) || (draft && !rows_type_ok(draft_type, who))) return P1A_E_ARG;
+    if (!ld_target) ld_target = V;
+    if (!ld_draft) ld_draft = V;
+    if (V > 1 << 20 || ld_target < (size_t) V || ld_draft < (size_t) V || ld_target > (size_t) 1 << 40 || ld_draft > (size_t) 1 << 40) { set_error("%s: unsupported shape (V=%d, rows %zu and %zu apart)", who, V, ld_target, ld_draft); return P1A_E_SHAPE; }
+    const uintptr_t words = (uintptr_t) token | (uintptr_t) parent | (uintptr_t) temp | (uintptr_t) u | (uintptr_t) u_next | (uintptr_t) n_accept | (uintptr_t) path | (uintptr_t) next;
+    if (words & 3 || (uintptr_t) target & (target_type == P1A_ROWS_BF16 ? 1 : 3) || (draft && (uintptr_t) draft & (draft_type == P1A_ROWS_BF16 ? 1 : 3))) { set_error("%s: tensors must be aligned to their types", who); return P1A_E_SHAPE; }
+    if (!rows->n_seq) return P1A_OK;
+    a.target = target; a.draft = draft; a.ld_target = ld_target; a.ld_draft = ld_draft; a.token = token; a.parent = parent; a.temp = temp; a.u = u; a.u_next = u_next;
+    a.n_accept = n_accept; a.path = path; a.next = next; a.V = V; a.ld_path = ld_path; a.max_children = max_children;
+    a.target_bf16 = target_type == P1A_ROWS_BF16; a.draft_bf16 = draft && draft_type == P1A_ROWS_BF16; a.logits = !(flags & P1A_VERIFY_PROBS); a.distinct = flags & P1A_VERIFY_DISTINCT;
+    a.scratch = scratch; a.scratch_bytes = scratch_bytes;
+    return launch_verify(a, (hipStream_t) stream);
+}
+
+size_t p1a_tree_verify_scratch_bytes(const p1a_rows * rows, int V, int flags) {
+    rows_view R;
+    if (tree_rows_ok(rows, "p1a_tree_verify_scratch_bytes", false, R) != P1A_OK || !rows->n_seq || V < 1 || V > 1 << 20) return 0;
+    return plan_verify(R, V, !(flags & P1A_VERIFY_PROBS)).bytes;
+}
+
+int p1a_tree_commit(const p1a_kv * layers, int n_layers, const p1a_rows * rows, const int32_t * n_accept, const int32_t * path, int ld_path, void * stream) {
+    static const char * const who = "p1a_tree_commit";
+    rows_view R;
+    const int rc = tree_rows_ok(rows, who, true, R);
+    if (rc != P1A_OK) return rc;
+    if (!layers || n_layers < 0 || !n_accept || !path || ld_path < 1) { set_error("%s: null argument or a bad count (n_layers=%d ld_path=%d)", who, n_layers, ld_path); return P1A_E_ARG; }
+    if (n_layers > P1A_TREE_LAYERS) { set_error("%s: %d layers, up to %d a call", who, n_layers, P1A_TREE_LAYERS); return P1A_E_SHAPE; }
+    for (int i = 0; i < n_layers; ++i) {
+        const p1a_kv & c = layers[i], & f = layers[0];
+        if (!kv_ok(&c, who)) return P1A_E_ARG;
+        if (c.type != f.type || c.n_ctx != f.n_ctx || c.Hkv != f.Hkv || c.D != f.D || c.pt != f.pt || c.rtab != f.rtab || c.psh != f.psh || c.pstride != f.pstride || c.n_ctx < 0) {
+            set_error("%s: layer %d has another shape or page table than the first, or a negative n_ctx", who, i);
+            return P1A_E_ARG;
+        }
+        if (R.n_seq > 1 && (!c.pt || !c.rtab)) { set_error("%s: %d sequences need a page table and a row table", who, R.n_seq); return P1A_E_ARG; }
+        if ((((uintptr_t) c.k | (uintptr_t) c.v) & 1) || (c.pt && (c.pstride & 1))) { set_error("%s: cache base and page stride must be 2-byte aligned", who); return P1A_E_SHAPE; }
+    }
+    if (((uintptr_t) n_accept | (uintptr_t) path) & 3) { set_error("%s: n_accept and path must be 4-byte aligned", who); return P1A_E_SHAPE; }
+    if (!rows->T || !rows->n_seq || !n_layers) return P1A_OK;
+    R.n_ctx = layers[0].n_ctx;
+    return launch_tree_commit(layers, n_layers, R, n_accept, path, ld_path, (hipStream_t) stream);
 }
 
 int p1a_sigmoid_mul(float * x, const float * g, size_t n, void * stream) {

@@ -595,6 +595,29 @@ struct mass_args {
 struct mass_plan { int few, runs, blocks, splits, pld; size_t bytes; };   // (few as in chunk_plan; pld: positions of a partial row; bytes of scratch)
 mass_plan plan_mass(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int ld, int cus);
 int launch_mass(const p1a_kv & c, const mass_args & a, hipStream_t s);
+struct tree_plan {
+    int NT, max_groups;                // tiles of 16 columns of a wave; groups of waves' columns that a sequence may have
+    int nks, runs;                     // as in chunk_params
+    size_t bytes_n, bytes_ml, bytes_o; // scratch (0: no partials), in this order
+};
+tree_plan plan_tree(const p1a_kv & c, const rows_view & R, int Hq, int max_n, bool exact, int cus);
+int launch_tree(const p1a_kv & c, const chunk_args & a, const uint32_t * mask, int words, hipStream_t s);
+int launch_tree_rows(const int32_t * parent, const rows_view & R, uint32_t * mask, int words, int32_t * pos, int32_t * slot, hipStream_t s);
+int launch_tree_commit(const p1a_kv * layers, int n_layers, const rows_view & R, const int32_t * n_accept, const int32_t * path, int ld_path, hipStream_t s);
+struct verify_args {
+    const void * target, * draft;
+    size_t ld_target, ld_draft;
+    const int32_t * token, * parent;
+    const float * temp, * u, * u_next;
+    int32_t * n_accept, * path, * next;
+    rows_view R;
+    int V, ld_path, max_children;
+    bool target_bf16, draft_bf16, logits, distinct;
+    void * scratch; size_t scratch_bytes;
+};
+struct verify_plan { int stretches; size_t at[15], bytes; };   // stretches of a row; where the parts of the scratch begin (p1a_verify.hip), and all of it
+verify_plan plan_verify(const rows_view & R, int V, bool logits);
+int launch_verify(const verify_args & a, hipStream_t s);
 int launch_evict_select(const float * mass, int ld, int n_seq, int Hkv, const int32_t * n_dev, int n, int budget, int n_sink, int n_recent, int32_t * keep, hipStream_t s);
 int launch_kv_compact(const p1a_kv & c, const int32_t * keep, int n_seq, int budget, const float * mass, float * mass_out, int ld, hipStream_t s);
 
