@@ -1,14 +1,13 @@
 // Attention of the rows of drafted trees - per sequence a few to a thousand nodes, each of which sees what is in front of the tree and its own path - over
 // paged caches: p1a_attn_tree.
 //
-// Work: a column is one q head of a node's row. A sequence's columns under a kv head are cut into blocks of 16 NT, its blocks into groups of at most four; the
-// four waves of a workgroup take a block each and walk the same tiles of 32 keys (four blocks), or share the keys among the waves of a block (one block or two).
-// Waves share nothing but what the L1 cache holds for them: each reads its own keys, converts them and keeps its own sums. Steps - a tile for every stream of
-// keys - are counted through over all groups of all sequences, and a workgroup takes a run of them as long as every other's, whatever the lengths; a group
-// that lies in one run is finished there, the others' partials are merged by tree_merge_k.
-// Arithmetic: S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16, one pass with a running reference of every column. With bf16 results q, P, K and V
-// enter as one f16 each, a quantized value times its scale; where results are f32 (EXACT) q and P are two halves, codes stay whole numbers and their
-// scales multiply fp32 results (K) or P (V), as in p1a_step.hip.
+// Work: a column is one q head of a node's row. Where sequences have up to 32 columns under a kv head (few_k) the four waves of a workgroup share the keys, each with
+// tiles of 32 of its own; where they have more (team_k) the waves share tiles in LDS and take 32 columns each, up to 128 a group. Steps - 128 keys, or a tile - are
+// counted through over all groups of all sequences, and a workgroup takes a run of them as long as every other's, whatever the lengths; a group that lies in one run
+// is finished there, the others' partials are merged by tree_merge_k.
+// Arithmetic: S^T = K Q^T and O^T = V^T P^T on f16 matrix instructions, one pass with a running reference of every column. With bf16 results q, P, K and V enter as one f16
+// each, a quantized value times its scale; where results are f32 (EXACT) q and P are two halves and quantized K and V two planes (team_k) or whole numbers whose
+// scales multiply fp32 results (K) or P (V; few_k), as in p1a_chunk.hip and p1a_step.hip.
 // Only the last tiles hold nodes of the tree: there a column's 32 bits of its mask are shifted out of two words.
 #include "p1a_tiles.hpp"
 
@@ -18,21 +17,16 @@
 namespace p1a {
 namespace {
 
-constexpr int NW = 4, NTHR = NW * 64, PC = 8;                 // waves; columns of a wave folded at a time
+constexpr int NW = 4, NTHR = NW * 64, PC = 8;                 // waves; columns folded at a time
+constexpr int COLS = 32 * NW;                                 // columns of a group of team_k
 
-// ---- what a sequence's rows make ----
-struct shape {
-    int cols, blocks, groups, bpg, cb, ks;                    // columns; blocks of columns; groups; blocks of a group; waves side by side; streams of keys
-};
-__host__ __device__ __forceinline__ shape shape_of(int rows, int GQA, int BC) {
-    shape s;
+struct group_of { int cols, blocks, groups, bpg; };           // a sequence's columns under a kv head, blocks of BC of them, groups of at most `waves` blocks, a group's blocks
+__host__ __device__ __forceinline__ group_of groups_of(int rows, int GQA, int BC, int waves) {
+    group_of s;
     s.cols = rows * GQA;
     s.blocks = (s.cols + BC - 1) / BC;
-    s.groups = (s.blocks + NW - 1) / NW;
+    s.groups = (s.blocks + waves - 1) / waves;
     s.bpg = s.groups ? (s.blocks + s.groups - 1) / s.groups : 1;
-    s.cb = s.bpg < 3 ? s.bpg : 4;
-    if (s.cb < 1) s.cb = 1;
-    s.ks = NW / s.cb;
     return s;
 }
 
@@ -42,11 +36,12 @@ struct tree_params : chunk_params {
 };
 
 // ---- runs of steps of equal length over the groups of all sequences (lane i of a wave counts for sequence s0 + i) ----
-template <int BC> struct tree_runs {
+// BN: keys of a tile; TPS: tiles of a step; BC: columns of a block; WAVES: blocks of a group
+template <int BN, int TPS, int BC, int WAVES> struct tree_runs {
     struct of_lane { int first, pos0, table, rows, per_group, steps; };
     of_lane first64;
     int first, end, per;
-    static __device__ __forceinline__ span span_of_rows(const rows_view & R, const seq_view & v) { return span_of<32>(R, v.pos0, v.pos0 + v.count - 1); }
+    static __device__ __forceinline__ span span_of_rows(const rows_view & R, const seq_view & v) { return span_of<BN>(R, v.pos0, v.pos0 + v.count - 1); }
     static __device__ __forceinline__ of_lane look(const rows_view & R, const kv_view & pg, int GQA, int s) {
         of_lane r{0, 0, 0, 0, 0, 0};
         if (s >= R.n_seq) return r;
@@ -56,9 +51,8 @@ template <int BC> struct tree_runs {
         r.pos0 = v.pos0;
         r.rows = v.count;
         if (v.count > 0) {
-            const shape h = shape_of(v.count, GQA, BC);
-            r.per_group = max((span_of_rows(R, v).nt + h.ks - 1) / h.ks, 1);
-            r.steps = r.per_group * h.groups;
+            r.per_group = max((span_of_rows(R, v).nt + TPS - 1) / TPS, 1);
+            r.steps = r.per_group * groups_of(v.count, GQA, BC, WAVES).groups;
         }
         return r;
     }
@@ -155,18 +149,19 @@ template <uint32_t KT, int D> struct keysd {
     }
 };
 
-template <uint32_t KT, int D, int NT, bool EXACT> struct tree_cfg {
+template <uint32_t KT, int D, int NT, bool EXACT> struct few_cfg {
     static constexpr bool F16 = KT == P1A_KV_F16, CODES = EXACT && !F16;      // codes as whole numbers, scales outside of the products
     static constexpr int VT_B = 2 * plane_bytes(D);           // 32 keys of V
     static constexpr int V_B = (F16 ? 2 : 1) * VT_B;
     static constexpr int TAB = CODES ? keys16<KT, D>::TAB : 0;
     static constexpr int WAVE_B = V_B + 4 * TAB * 4;          // and the scales of 2 x 16 keys of K and V
-    // (the low halves of q, where registers do not hold them: a block's, its streams write the same. One tile of columns: calls of one block)
-    static constexpr bool QL = CODES && NT * D >= 256;
+    // (the low halves of q, where registers do not hold them: the same for every wave, each writes all of them)
+    static constexpr bool QL = EXACT && (CODES || D == 128) && NT * D >= 256;
     static constexpr int QL_B = QL ? NT * D * 32 : 0, ML_B = NW * 2 * 16 * NT * 4;
     static constexpr bool ML_OVER = 4 * TAB * 4 >= ML_B;      // references and sums go where the first wave's scales were
-    static constexpr int ML_AT = ML_OVER ? V_B : NW * WAVE_B + (NT == 1 ? 1 : NW) * QL_B, LDS = NW * WAVE_B + (NT == 1 ? 1 : NW) * QL_B + (ML_OVER ? 0 : ML_B);
-    static constexpr int WGS = LDS <= 80 * 1024 && !(D == 256 && NT == 2) ? 2 : 1;   // workgroups of a compute unit
+    static_assert(D == 256 || 2 * NW * (WAVE_B + QL_B / NW + ML_B / NW) <= 160 * 1024, "two workgroups' LDS");
+    static constexpr int ML_AT = ML_OVER ? V_B : NW * WAVE_B + QL_B, LDS = NW * WAVE_B + QL_B + (ML_OVER ? 0 : ML_B);
+    static constexpr int WGS = D == 256 ? 1 : 2;              // workgroups of a compute unit
     static_assert(PC * (D + 4) * 4 <= V_B, "folded columns fit where V was");
 };
 
@@ -177,58 +172,103 @@ __device__ __forceinline__ uint32_t mask_bits(const uint32_t * row, int words, i
     return __builtin_amdgcn_alignbit(hi, lo, at & 31);
 }
 
+// The kernel's arguments, read again from here on: kept in registers from the kernel's start to its end they and what follows from them are too many, and
+// would be spilled to lanes of vector registers
+typedef const __attribute__((address_space(4))) tree_params * args;
+__device__ __forceinline__ const tree_params & read_again() {
+    args p = (args) __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const tree_params *) p;
+}
+
+// What the row of a sequence's node `tok` sees of the 32 keys from k0 on: key j where (j <= hi && (j > lo || j < sk)) or bit j
+struct sight { int hi, lo, sk; uint32_t bits; };
+__device__ __forceinline__ sight sight_of(const tree_params & P, const seq_view & sv, int tok, int k0) {
+    const int slot = sv.pos0 + tok, at = k0 - sv.pos0;
+    const bool live = slot >= 0 && slot < P.R.n_ctx;
+    const uint32_t * const row = P.mask + (size_t) (sv.first + tok) * P.words;
+    sight v{live ? sv.pos0 - 1 - k0 : INT32_MIN / 2, -1 - k0, 0, 0};
+    if (P.R.window != INT32_MAX) {                            // (its place: as many nodes behind the first as its path has)
+        int nodes = 0;
+        for (int w = 0; 32 * w < sv.count; ++w) nodes += __popc(sv.count - 32 * w >= 32 ? row[w] : row[w] & ((1u << (sv.count - 32 * w)) - 1));
+        v.lo = sv.pos0 + max(nodes - 1, 0) - P.R.window - k0;
+        v.sk = P.R.n_sink - k0;
+    }
+    if (live && at > -32) {
+        const int left = sv.count - at;                       // nodes that are there
+        v.bits = mask_bits(row, P.words, at);
+        v.bits = left >= 32 ? v.bits : left > 0 ? v.bits & ((1u << left) - 1) : 0;
+    }
+    return v;
+}
+
+// Four results of a row from its sums relative to M: a partial (piece >= 0) or what the call is to give
+__device__ __forceinline__ void finish(const tree_params & P, size_t row, int d, int D, int piece, f4 acc, float M, float l) {
+    if (piece >= 0) {
+        if (d == 0) *reinterpret_cast<float2 *>(P.part_ml + (row * P.nks + piece) * 2) = float2{part_ref(M, l), l};
+        if (part_ref(M, l) != MINUS_INF) *reinterpret_cast<f4 *>(P.part_o + (row * P.nks + piece) * D + d) = acc;
+        return;
+    }
+    if (P.lse && d == 0) P.lse[row] = (M + log2f(l)) * LN2;
+    f4 v = acc * (l == 0.f ? 0.f : 1.0f / l);                 // (nothing seen: 0)
+    if (P.gate) {
+        const f4 gt = *reinterpret_cast<const f4 *>(P.gate + row * D + d);
+#pragma unroll
+        for (int y = 0; y < 4; ++y) v[y] *= gate_of(gt[y]);
+    }
+    put4(P.out, P.out_bf16, row * D + d, v);
+}
+
 template <uint32_t KT, int D, int NT, bool EXACT>
-__global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_k(const tree_params P) {
-    using C = tree_cfg<KT, D, NT, EXACT>;
+__global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(const tree_params) {
+    const tree_params & P0 = read_again();
+    const int Hkv = P0.Hkv, runs = P0.runs;
+    using C = few_cfg<KT, D, NT, EXACT>;
     constexpr bool F16 = C::F16, CODES = C::CODES;
     using K = typename std::conditional<F16 || CODES, keys16<KT, D>, keysd<KT, D>>::type;
     using G = group<KT, D, CODES ? 0 : 1>;
-    constexpr int NB = D / 32, NDT = D / 16, NQ = EXACT ? 2 : 1, PL_B = plane_bytes(D), BC = 16 * NT;
+    constexpr int NB = D / 32, NDT = D / 16, NQ = EXACT ? 2 : 1, PL_B = plane_bytes(D);
+    using runs_t = tree_runs<32, NW, 16 * NT, 1>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // the kv heads of a run of steps, whose rows have cache lines in common, on one XCD
-    const int xcd = blockIdx.x & 7, jx = blockIdx.x >> 3, hk = jx % P.Hkv, run = jx / P.Hkv * 8 + xcd;
-    if (run >= P.runs) return;
-    auto tok_of = [&](int r) {
-        const int t = (int) __umulhi((uint32_t) r, P.gqa_magic);
-        return r - t * P.GQA >= P.GQA ? t + 1 : t;
-    };
-    tree_runs<BC> steps;
+    const int xcd = blockIdx.x & 7, jx = blockIdx.x >> 3, hk = jx % Hkv, run = jx / Hkv * 8 + xcd;
+    if (run >= runs) return;
+    runs_t steps;
     steps.first = 0;
     steps.end = 1;
     steps.per = 1 << 30;
-    if (P.nks > 1 && !steps.begin(P.R, P.pg, P.GQA, run, P.runs, P.nks)) return;
+    if (P0.nks > 1 && !steps.begin(P0.R, P0.pg, P0.GQA, run, runs, P0.nks)) return;
     char * const mine = lds + wave * C::WAVE_B;
     float * const tk = reinterpret_cast<float *>(mine + C::V_B), * const tv = tk + 2 * C::TAB;
     const size_t head_off = (size_t) hk * head_bytes(KT, D);
 
   for (int at_step = steps.first; at_step < steps.end;) {
+    const tree_params & P = read_again();
+    auto tok_of = [&](int r) {
+        const int t = (int) __umulhi((uint32_t) r, P.gqa_magic);
+        return r - t * P.GQA >= P.GQA ? t + 1 : t;
+    };
     // (the lane's number anew for each group: what follows from it would be worked out ahead of the loop and kept)
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));
     const int lane = tid & 63, c = lane & 15, g = lane >> 4;
-    typename tree_runs<BC>::found f;
+    typename runs_t::found f;
     if (P.nks > 1) {
         if (!steps.find(P.R, P.pg, P.GQA, at_step, lane, f)) return;
-    } else {                                                  // a group each
-        f.seq = run / P.max_groups; f.group = run - f.seq * P.max_groups; f.first = 0; f.steps = 1 << 26;
+    } else {                                                  // a sequence each
+        f.seq = run; f.group = 0; f.first = 0; f.steps = 1 << 26;
         f.v = seq_of<true>(P.R, f.seq);
         f.table = P.pg.pt && P.pg.rtab ? sload_i32(P.pg.rtab + f.seq) : 0;
         if (f.v.count < 1) return;
     }
     const seq_view & sv = f.v;
-    const shape sh = shape_of(sv.count, P.GQA, BC);
-    if (P.nks == 1 && f.group >= sh.groups) return;
     const int run0 = f.first / steps.per, pieces = P.nks > 1 ? (f.first + f.steps - 1) / steps.per - run0 + 1 : 1, piece = P.nks > 1 ? run - run0 : 0;
-    const int beside = wave & (sh.cb - 1), stream = wave / sh.cb;   // (cb: 1, 2 or 4)
-    const int block = f.group * sh.bpg + beside, col0 = block * BC;
-    const bool busy = beside < sh.bpg && col0 < sh.cols;
-    const int R = busy ? min(sh.cols - col0, BC) : 1;         // (a wave without a block looks at column 0 and writes nothing)
-    const int first_col = busy ? col0 : 0;
+    const int R = min(sv.count * P.GQA, 16 * NT);
     auto row_index = [&](int r) { const int t = tok_of(r); return (size_t) (sv.first + t) * P.Hq + (size_t) hk * P.GQA + (r - t * P.GQA); };
-    const span sp = tree_runs<BC>::span_of_rows(P.R, sv);
-    const int ta = (at_step - f.first) * sh.ks, tb = P.nks > 1 ? min((min(steps.end, f.first + f.steps) - f.first) * sh.ks, sp.nt) : sp.nt;
+    const span sp = runs_t::span_of_rows(P.R, sv);
+    const int ta = (at_step - f.first) * NW, tb = P.nks > 1 ? min((min(steps.end, f.first + f.steps) - f.first) * NW, sp.nt) : sp.nt;
     at_step = f.first + f.steps;
     // positions that all rows see
     const bool odd = sv.pos0 < 0 || sv.pos0 + sv.count > P.R.n_ctx;
@@ -246,12 +286,12 @@ __global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_
         return __builtin_bit_cast(h4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4 __attribute__((address_space(3))) *) (grp + vbase[dt & 1] + (dt >> 1) * 1024)));
     };
     struct none {};
-    typename K::raw kr[2];
+    typename K::raw kr[2], kn[2];                             // K of the tile in hand, and of the next one
     typename std::conditional<F16, none, typename group<F16 ? P1A_KV_Q8_0 : KT, D, CODES ? 0 : 1>::raw>::type vr[2];
     typename keys16<KT, D>::scales vs[2];
     auto ask_k = [&](const where & w) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) K::load(kr[x], (gbytes) P.kc + w.off[x], g);
+        for (int x = 0; x < 2; ++x) K::load(kn[x], (gbytes) P.kc + w.off[x], g);
     };
     auto ask_v = [&](const where & w, int st) {
 #pragma unroll
@@ -266,9 +306,14 @@ __global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_
         }
     };
 
-    int i = busy ? ta + stream : tb;
+    // page-table entries are asked for a tile ahead of the rows, which come a tile ahead of their products
+    int i = ta + wave;
+    auto tile_of = [&](int i) { return sp.tile(min(i, tb - 1)); };   // (past the last: that one once more, unused)
+    key_rows::pages pg;
     if (i < tb) {
-        const where at = keys.at(sp.tile(i), keys.pages_of(sp.tile(i)));
+        const key_rows::pages now = keys.pages_of(tile_of(i));
+        pg = keys.pages_of(tile_of(i + NW));
+        const where at = keys.at(tile_of(i), now);
         ask_v(at, 0);
         ask_k(at);
     }
@@ -276,12 +321,12 @@ __global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_
     // ---- Q^T: columns 16 n + c ----
     constexpr int NQR = C::QL ? 1 : NQ;                       // halves in registers
     h8 qf[NT][NQR][NB];
-    char * const ql = lds + NW * C::WAVE_B + beside * C::QL_B + lane * 16;
+    char * const ql = lds + NW * C::WAVE_B + lane * 16;
     auto q_at = [&](int n, int k, int b) { return k < NQR ? qf[n][k < NQR ? k : 0][b] : *reinterpret_cast<const h8 *>(ql + (n * NB + b) * 1024); };
     float factor[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const size_t row = row_index(first_col + min(16 * n + c, R - 1));
+        const size_t row = row_index(min(16 * n + c, R - 1));
         h8 qq[NQ][NB];
         if constexpr (F16 || CODES) factor[n] = ldexpf(P.factor, q_columns<KT, D, NQ>(P.q, P.q_bf16, row, P.sign, g, qq));
         else {
@@ -328,11 +373,19 @@ __global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt) o[n][dt] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    for (int st = 0; i < tb; i += sh.ks, st ^= 1) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) kr[x] = kn[x];
+    for (int st = 0; i < tb; i += NW, st ^= 1) {
         const int k0 = sp.tile(i) * 32;
-        const bool more = i + sh.ks < tb;
-        key_rows::pages pg;
-        if (more) pg = keys.pages_of(sp.tile(i + sh.ks));
+        const bool more = i + NW < tb;                     // (no load is left behind: V's go to LDS, where results are folded)
+        // what was asked for a tile ago is there; now the next tile
+        if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const where at = keys.at(tile_of(i + NW), pg);
+        pg = keys.pages_of(tile_of(i + 2 * NW));
+        if (more) {
+            if constexpr (F16) ask_v(at, st ^ 1);
+            ask_k(at);
+        }
         // ---- V's values (or codes, and all scales) into LDS ----
         if constexpr (CODES) {
             float dm = 0.f;
@@ -357,10 +410,12 @@ __global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_
                 keys16<KT, D>::put(tv + x * C::TAB, vs[x], c, g, -E);
                 G::store(vr[x], mine + x * PL_B, lane);
             }
+            if (more) ask_v(at, 0);
             __builtin_amdgcn_wave_barrier();
         } else if constexpr (!F16) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) G::store(vr[x], mine + x * PL_B, lane);
+            if (more) ask_v(at, 0);
             __builtin_amdgcn_wave_barrier();
         }
         // ---- S^T ----
@@ -381,36 +436,13 @@ __global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_
                 }
             }
         }
-        // (V of this tile was asked for ahead of its K)
-        if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if (more) {
-            const where at = keys.at(sp.tile(i + sh.ks), pg);
-            ask_v(at, st ^ 1);
-            ask_k(at);
-        }
         // ---- what a column does not see: in front of the tree by its window, in the tree by its mask ----
         if (!(k0 + 31 <= all_hi && k0 >= all_lo)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const int tok = tok_of(first_col + min(16 * n + c, R - 1)), slot = sv.pos0 + tok, from = k0 + 4 * g;
-                const bool live = slot >= 0 && slot < P.R.n_ctx;
-                const uint32_t * const row = P.mask + (size_t) (sv.first + tok) * P.words;
-                int lo = -1, sk = 0;
-                if (P.R.window != INT32_MAX) {                // (its place: as many nodes behind the first as its path has)
-                    int nodes = 0;
-                    for (int w = 0; 32 * w < sv.count; ++w) nodes += __popc(sv.count - 32 * w >= 32 ? row[w] : row[w] & ((1u << (sv.count - 32 * w)) - 1));
-                    lo = sv.pos0 + max(nodes - 1, 0) - P.R.window - from;
-                    sk = P.R.n_sink - from;
-                } else lo = -1 - from;
-                const int hi = live ? sv.pos0 - 1 - from : INT32_MIN;
-                uint32_t bits = 0;
-                const int at = k0 - sv.pos0;
-                if (live && at > -32) {
-                    bits = mask_bits(row, P.words, at);
-                    const int left = sv.count - at;           // nodes that are there
-                    bits = left >= 32 ? bits : left > 0 ? bits & ((1u << left) - 1) : 0;
-                }
-                bits >>= 4 * g;
+                const sight v = sight_of(P, sv, tok_of(min(16 * n + c, R - 1)), k0);
+                const int hi = v.hi - 4 * g, lo = v.lo - 4 * g, sk = v.sk - 4 * g;
+                const uint32_t bits = v.bits >> (4 * g);
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -480,19 +512,25 @@ __global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_
                     }
             __builtin_amdgcn_sched_barrier(0);
         }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) kr[x] = kn[x];
     }
 
-    // ---- fold the streams of each block, in their order ----
+    // ---- results: lane (column c, group g) holds dims 16 dt + 4 g .. ----
     {
     asm volatile("" : "+v"(tid));
     const int c = tid & 15, g = (tid >> 4) & 3;
-    auto ml = [&](int w, int which, int col) -> float & { return reinterpret_cast<float *>(lds + C::ML_AT)[(w * 2 + which) * 16 * NT + col]; };
-    if constexpr (C::ML_OVER) __syncthreads();                // (until the first wave has done with its scales)
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         l[n] += __shfl_xor(l[n], 16);
         l[n] += __shfl_xor(l[n], 32);
-        if (g == 0) { ml(wave, 0, 16 * n + c) = ref[n]; ml(wave, 1, 16 * n + c) = l[n]; }
+    }
+    // ---- fold the waves, in their order, eight columns at a time ----
+    auto ml = [&](int w, int which, int col) -> float & { return reinterpret_cast<float *>(lds + C::ML_AT)[(w * 2 + which) * 16 * NT + col]; };
+    if constexpr (C::ML_OVER) __syncthreads();                // (until the first wave has done with its scales)
+    if (g == 0) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) { ml(wave, 0, 16 * n + c) = ref[n]; ml(wave, 1, 16 * n + c) = l[n]; }
     }
     float * const parked = reinterpret_cast<float *>(mine);
     constexpr int OS = D + 4, D4 = D / 4;
@@ -500,8 +538,9 @@ __global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_
     for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int half = 0; half < 16; half += PC) {
-            const int h0 = 16 * n + half;                     // columns h0 .. of every block
-            if (n || half) __syncthreads();
+            const int h0 = 16 * n + half;
+            if (h0 >= R) break;
+            if (h0) __syncthreads();
             if (c >= half && c < half + PC) {
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt) {
@@ -514,42 +553,417 @@ __global__ void __launch_bounds__(NTHR, (tree_cfg<KT, D, NT, EXACT>::WGS)) tree_
                 }
             }
             __syncthreads();
-            for (int t = tid; t < sh.bpg * PC * D4; t += NTHR) {
-                const int u = t / D4, d = 4 * (t - u * D4), b = u / PC, cc = u - b * PC, col = h0 + cc;
-                const int at = (f.group * sh.bpg + b) * BC + col;             // of the sequence's columns
-                if (at >= sh.cols) continue;
-                float M = MINUS_INF, lt = 0.f;
-                f4 acc = {0.f, 0.f, 0.f, 0.f};
-                for (int k = 0; k < sh.ks; ++k) M = fmaxf(M, ml(k * sh.cb + b, 0, col));
-                for (int k = 0; k < sh.ks; ++k) {
-                    const int w = k * sh.cb + b;
-                    const float m = ml(w, 0, col), fw = m == MINUS_INF ? 0.f : __builtin_amdgcn_exp2f(m - M), lw = ml(w, 1, col);
-                    lt += m == MINUS_INF ? lw : lw * fw;      // (no maximum: 0, or NaN where scores were)
-                    if (m != MINUS_INF) acc += *reinterpret_cast<const f4 *>(reinterpret_cast<const float *>(lds + w * C::WAVE_B) + cc * OS + d) * fw;
-                }
-                const size_t row = row_index(at);
-                if (pieces > 1) {
-                    if (d == 0) {
-                        float * pm = P.part_ml + (row * P.nks + piece) * 2;
-                        pm[0] = part_ref(M, lt);
-                        pm[1] = lt;
-                    }
-                    if (part_ref(M, lt) != MINUS_INF) *reinterpret_cast<f4 *>(P.part_o + (row * P.nks + piece) * D + d) = acc;
-                    continue;
-                }
-                if (P.lse && d == 0) P.lse[row] = (M + log2f(lt)) * LN2;
-                f4 v = acc * (lt == 0.f ? 0.f : 1.0f / lt);   // (nothing seen: 0)
-                if (P.gate) {
-                    const f4 gt = *reinterpret_cast<const f4 *>(P.gate + row * D + d);
+            for (int t = tid; t < (min(h0 + PC, R) - h0) * D4; t += NTHR) {
+                const int cc = t / D4, d = 4 * (t - cc * D4), col = h0 + cc;
+                float m[NW], lw[NW], M = MINUS_INF, lt = 0.f;
+                f4 x[NW], acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) v[y] *= gate_of(gt[y]);
+                for (int w = 0; w < NW; ++w) {
+                    m[w] = ml(w, 0, col);
+                    lw[w] = ml(w, 1, col);
+                    x[w] = *reinterpret_cast<const f4 *>(reinterpret_cast<const float *>(lds + w * C::WAVE_B) + cc * OS + d);
+                    M = fmaxf(M, m[w]);
                 }
-                put4(P.out, P.out_bf16, row * D + d, v);
+#pragma unroll
+                for (int w = 0; w < NW; ++w) {
+                    const float fw = m[w] == MINUS_INF ? 0.f : __builtin_amdgcn_exp2f(m[w] - M);
+                    lt += m[w] == MINUS_INF ? lw[w] : lw[w] * fw;     // (no maximum: 0, or NaN where scores were)
+                    acc += x[w] * fw;
+                }
+                finish(P, row_index(col), d, D, pieces > 1 ? piece : -1, acc, M, lt);
             }
         }
     }
     if (P.nks > 1 && piece == 0 && hk == 0 && tid == 0) P.part_n[f.seq * P.max_groups + f.group] = pieces;
     __syncthreads();                                          // (what was folded is read; the next group's V goes there)
+  }
+}
+
+// ---- more columns: waves that share tiles ----
+template <uint32_t KT, int D, bool EXACT> struct team_cfg {
+    static constexpr bool F16 = KT == P1A_KV_F16;
+    static constexpr int NPL = group_planes(KT, EXACT), BN = 32, NG = BN / 16, G_B = NPL * plane_bytes(D), T_B = NG * G_B;   // T_B: K or V of a tile
+    // Tiles are asked for four steps ahead. f16 goes to LDS by itself: places for four; the others wait in registers, two deep, and LDS holds two
+    static constexpr int PLACES = F16 ? 4 : 2;
+    static constexpr int LDS = 2 * PLACES * T_B;
+    static constexpr int WGS = D <= 128 ? 2 : 1;
+};
+
+// a quantized group's way into LDS in parts, to stand between products
+template <uint32_t KT, int D, int NPL> struct parts;
+template <int D, int NPL> struct parts<P1A_KV_Q8_0, D, NPL> {
+    using G = group<P1A_KV_Q8_0, D, NPL>;
+    static constexpr int N = 2 * G::NJ;
+    template <int i> static __device__ __forceinline__ void store(const typename G::raw & r, char * to, int lane) {
+        constexpr int j = i / 2, x = i % 2;
+        const int q = lane >> 4, k = lane & 15;
+        const uint32_t s = q & 2 ? r.d[j] >> 16 : r.d[j] & 0xffff;
+        const h2 d = __builtin_bit_cast(h2, s | (s << 16));
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) times4<NPL>(r.w[j][2 * x + e] ^ 0x80808080u, 1152.f, d, h + 2 * e, l + 2 * e);
+        char * const at = to + chunk_at(k, 8 * j + 2 * q + x);
+        *reinterpret_cast<u4 *>(at) = u4{h[0], h[1], h[2], h[3]};
+        if constexpr (NPL == 2) *reinterpret_cast<u4 *>(at + plane_bytes(D)) = u4{l[0], l[1], l[2], l[3]};
+    }
+};
+template <int D, int NPL> struct parts<P1A_KV_Q4_0, D, NPL> {
+    using G = group<P1A_KV_Q4_0, D, NPL>;
+    static constexpr int N = 4 * G::NJ;
+    template <int i> static __device__ __forceinline__ void store(const typename G::raw & r, char * to, int lane) {
+        constexpr int j = i / 4, x = i % 4;
+        const int k = lane & 15, b = 4 * j + (lane >> 4);
+        if (G::NB % 4 && b >= G::NB) return;
+        const h2 d = __builtin_bit_cast(h2, r.d[j] | (r.d[j] << 16));
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t w = r.w[j][2 * (x & 1) + e];
+            times4<NPL>((x & 2 ? w >> 4 : w) & 0x0f0f0f0fu, 1032.f, d, h + 2 * e, l + 2 * e);
+        }
+        char * const at = to + chunk_at(k, 4 * b + x);
+        *reinterpret_cast<u4 *>(at) = u4{h[0], h[1], h[2], h[3]};
+        if constexpr (NPL == 2) *reinterpret_cast<u4 *>(at + plane_bytes(D)) = u4{l[0], l[1], l[2], l[3]};
+    }
+};
+template <int D, int NPL> struct parts<P1A_KV_F16, D, NPL> {
+    static constexpr int N = 0;
+};
+
+// Position that the row of key j is fetched from, one that some row sees: j itself, or the nearest of its 16 keys that is, or (none of them) of the tile - so that the 16 rows
+// lie in one page wherever pages have 16 positions and more
+template <int BN> __device__ __forceinline__ int seen_in_group(const span & s, int k0, int kb, int j) {
+    if (j > s.pmax) return s.pmax;
+    if (j >= s.lo || j < s.ns) return j;
+    return s.lo < kb + 16 ? s.lo : s.ns > kb ? s.ns - 1 : k0 + BN > s.lo ? s.lo : s.ns - 1;
+}
+
+template <uint32_t KT, int D, bool EXACT>
+__global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(const tree_params) {
+    const tree_params & P0 = read_again();
+    const int Hkv = P0.Hkv, runs = P0.runs;
+    using C = team_cfg<KT, D, EXACT>;
+    using G = group<KT, D, C::NPL>;
+    using PT = parts<KT, D, C::NPL>;
+    constexpr bool F16 = C::F16;
+    constexpr int BN = C::BN, G_B = C::G_B, T_B = C::T_B, PL_B = plane_bytes(D), NPL = C::NPL;
+    constexpr int NKS = D / 16, NDT = D / 32, NQ = EXACT ? 2 : 1, PF_K = NPL == 2 ? 1 : EXACT ? 2 : 4, PF_V = NPL == 2 ? 1 : EXACT ? 2 : 3;
+    using runs_t = tree_runs<BN, 1, 32, NW>;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int xcd = blockIdx.x & 7, jx = blockIdx.x >> 3, hk = jx % Hkv, run = jx / Hkv * 8 + xcd;
+    if (run >= runs) return;
+    runs_t steps;
+    steps.first = 0;
+    steps.end = 1;
+    steps.per = 1 << 30;
+    if (P0.nks > 1 && !steps.begin(P0.R, P0.pg, P0.GQA, run, runs, P0.nks)) return;
+    const size_t head_off = (size_t) hk * head_bytes(KT, D);
+    // wave w brings group w % 2 of every tile's K (waves 0 and 1) or V
+    const int grp = wave & 1;
+    const bool my_v = wave >= 2;
+    char * const k_place = lds, * const v_place = lds + C::PLACES * T_B;
+
+  for (int at_step = steps.first; at_step < steps.end;) {
+    const tree_params & P = read_again();
+    auto tok_of = [&](int r) {
+        const int t = (int) __umulhi((uint32_t) r, P.gqa_magic);
+        return r - t * P.GQA >= P.GQA ? t + 1 : t;
+    };
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    const int lane = tid & 63, c = lane & 31, g = lane >> 5;
+    typename runs_t::found f;
+    if (P.nks > 1) {
+        if (!steps.find(P.R, P.pg, P.GQA, at_step, lane, f)) return;
+    } else {                                                  // a group each
+        f.seq = run / P.max_groups; f.group = run - f.seq * P.max_groups; f.first = 0; f.steps = 1 << 26;
+        f.v = seq_of<true>(P.R, f.seq);
+        f.table = P.pg.pt && P.pg.rtab ? sload_i32(P.pg.rtab + f.seq) : 0;
+        if (f.v.count < 1) return;
+    }
+    const seq_view & sv = f.v;
+    const group_of sh = groups_of(sv.count, P.GQA, 32, NW);
+    if (P.nks == 1 && f.group >= sh.groups) return;
+    const int run0 = f.first / steps.per, pieces = P.nks > 1 ? (f.first + f.steps - 1) / steps.per - run0 + 1 : 1, piece = P.nks > 1 ? run - run0 : 0;
+    const int col0 = (f.group * sh.bpg + wave) * 32, ncols = wave < sh.bpg ? min(sh.cols - col0, 32) : 0;   // this wave's columns (none: it brings keys only)
+    const int my_col = ncols > 0 ? col0 + min(c, ncols - 1) : 0, my_tok = tok_of(my_col);
+    const size_t my_row = (size_t) (sv.first + my_tok) * P.Hq + (size_t) hk * P.GQA + (my_col - my_tok * P.GQA);
+    const span sp = runs_t::span_of_rows(P.R, sv);
+    const int ta = at_step - f.first, tb = P.nks > 1 ? min(min(steps.end, f.first + f.steps) - f.first, sp.nt) : sp.nt;
+    at_step = f.first + f.steps;
+    // positions that all rows see
+    const bool odd = sv.pos0 < 0 || sv.pos0 + sv.count > P.R.n_ctx;
+    const int all_hi = odd ? -1 : sv.pos0 - 1, all_lo = P.R.window == INT32_MAX ? 0 : sp.pmax - P.R.window + 1;
+
+    // ---- where rows of the cache are ----
+    const gbytes from = (gbytes) (my_v ? P.vc : P.kc);
+    const int32_t * const ptab = P.pg.pt ? P.pg.pt + f.table : nullptr;
+    const bool paged16 = P.pg.psh >= 4;
+    auto tile_of = [&](int i) { return sp.tile(min(i, tb - 1)); };   // (past the last: that one once more, unused)
+    auto pos_of = [&](int tile) { return seen_in_group<BN>(sp, tile * BN, tile * BN + 16 * grp, tile * BN + 16 * grp + G::key(lane)); };
+    // (one page for the wave's 16 keys: through the scalar cache, beside the counter that tiles are waited for by)
+    auto page_of = [&](int tile) {
+        int page = 0;
+        if (ptab) {
+            if (paged16) page = sload_i32(ptab + (__builtin_amdgcn_readfirstlane(pos_of(tile)) >> P.pg.psh));
+            else {
+                page = ptab[pos_of(tile) >> P.pg.psh];
+                asm volatile("" : "+v"(page));
+            }
+        }
+        return page;
+    };
+    auto row_of = [&](int tile, int page) {
+        const int j = pos_of(tile);
+        return head_off + (ptab ? (size_t) page * P.pg.pstride + (size_t) (j & ((1 << P.pg.psh) - 1)) * P.pg.rowb : (size_t) j * P.pg.rowb);
+    };
+
+    // ---- Q^T operands: lane (column c, half g) holds dims 16 ks + 8 g .. + 7 ----
+    h8 qf[NQ][NKS];
+    float factor = P.factor;
+    auto load_q = [&] {
+        f4 x[NKS][2];
+        float most = 0.f;
+        auto fetch = [&](auto as_bf16) {
+#pragma unroll
+            for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) x[ks][e] = q4_at(P.q, as_bf16, my_row * D + 16 * ks + 8 * g + 4 * e);
+        };
+        if (P.q_bf16) fetch(std::true_type{});
+        else fetch(std::false_type{});
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[ks][e >> 2][e & 3]));
+        const int ex = row_exponent(max_swap32(most));
+        factor = ldexpf(factor, ex);
+        const float by = ldexpf(P.sign, -ex);
+#pragma unroll
+        for (int ks = 0; ks < NKS; ++ks) {
+            h8 r[NQ];
+            halves<NQ>([&](int e) { return x[ks][e >> 2][e & 3]; }, [&](int) { return by; }, r);
+#pragma unroll
+            for (int k = 0; k < NQ; ++k) {
+                qf[k][ks] = r[k];
+                // (in accumulation registers, where the products read it as it is: what vector instructions work on has the others)
+                if constexpr (D == 256) asm volatile("" : "+a"(qf[k][ks]));
+            }
+        }
+    };
+
+    f16x o[NDT];
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    float ref = MINUS_INF, l = 0.f, mx = MINUS_INF;           // mx: the column's largest score of the tile in hand
+
+    const k_frag kf(lane, G_B);
+    const v_frag vf(lane);
+    // (a place in LDS as a number the compiler does not see through - offsets from it fit the instructions, those from the start do not)
+    auto hidden = [&](int at) {
+        asm volatile("" : "+s"(at));
+        return (const char *) lds + at;
+    };
+    auto s_product = [&](f16x & s, int ks, const h8 (&a)[NPL]) {
+        if (ks == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s[i] = 0.f;
+        }
+        s = mfma32(a[0], qf[0][ks], s);
+        if constexpr (EXACT) s = mfma32(a[0], qf[NQ - 1][ks], s);
+        if constexpr (NPL == 2) s = mfma32(a[NPL - 1], qf[0][ks], s);
+    };
+    auto mask = [&](f16x & s, int k0) {
+        const sight v = sight_of(P, sv, my_tok, k0);
+        const int hi = v.hi - 4 * g, lo = v.lo - 4 * g, sk = v.sk - 4 * g;
+        const uint32_t bits = v.bits >> (4 * g);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int j = mfma_row(i, 0);                     // (and 4 g)
+            s[i] = (j <= hi && (j > lo || j < sk)) || (bits >> j & 1) ? s[i] : MINUS_INF;
+        }
+    };
+    float top = -MINUS_INF;
+    asm volatile("" : "+s"(top));
+    auto most_of = [&](const f16x & s) {
+        float m = MINUS_INF;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = larger(m, s[i], top);
+        return m;
+    };
+    auto whole = [&](int k0) { return k0 + BN - 1 <= all_hi && k0 >= all_lo; };
+
+    // ---- what a wave brings: of item e K of tile e or V of tile e - 1. Item e is asked for at step e - 4 and in LDS at the end of step e - 2 ----
+    typename G::raw raw[2];
+    auto to_of = [&](int e) { return (my_v ? v_place + (e + C::PLACES - 1) % C::PLACES * T_B : k_place + e % C::PLACES * T_B) + grp * G_B; };
+    int page = 0;                                             // of the item that is asked for next
+    size_t row = 0;
+    auto tile_of_item = [&](int e) { return tile_of(ta + max(e - (my_v ? 1 : 0), 0)); };
+    auto next_row = [&](int e) {                              // item e's row; the page of the one behind it
+        row = row_of(tile_of_item(e), page);
+        page = page_of(tile_of_item(e + 1));
+    };
+    auto load = [&](auto y, int e, typename G::raw & r) __attribute__((always_inline)) { G::template piece<y>(r, from + row, to_of(e), lane); };
+    auto part = [&](auto y, int e, const typename G::raw & r) __attribute__((always_inline)) { if constexpr (!F16) PT::template store<y>(r, to_of(e), lane); };
+    // ---- a step: P of this tile beside the products S^T of the next one, then O^T beside the next one's maximum; item i + 4 is asked for, item i + 2 put down ----
+    auto step = [&](int i, int next, f16x & s, f16x & sn, typename G::raw & r) __attribute__((always_inline)) {
+        const char * const kp = hidden((i + 1) % C::PLACES * T_B), * const vp = hidden((C::PLACES + i % C::PLACES) * T_B);
+        const bool fresh = ref == MINUS_INF, move = mx > (fresh ? MINUS_INF : ref + (HEAD + STEP));
+        if (__builtin_expect(__any(move), 0)) {
+            const float to = move ? mx - HEAD : ref, alpha = fresh ? 1.f : __builtin_amdgcn_exp2f(ref - to);   // (fresh: nothing accumulated)
+            ref = to;
+            l *= alpha;
+#pragma unroll
+            for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) o[dt][k] *= alpha;
+        }
+        const float nr = ref == MINUS_INF ? 0.f : -ref;       // (a column that has seen nothing: exp2(-inf))
+        constexpr int NF = 2 * NDT;
+        h8 pb[NQ][2];
+        float ls[2] = {0.f, 0.f};
+        auto k_read = [&](int ks, int pl) { return kf.read(kp + pl * PL_B, ks); };
+        auto v_read = [&](int f, int pl) { return vf.read(vp + (f / NDT) * G_B + pl * PL_B, f % NDT); };
+        // (operands from LDS are asked for a few products ahead, and no further: registers)
+        h8 fr[PF_K][NPL];
+#pragma unroll
+        for (int k = 0; k < PF_K; ++k)
+#pragma unroll
+            for (int pl = 0; pl < NPL; ++pl) fr[k][pl] = k_read(k, pl);
+        each<NKS>([&](auto k) __attribute__((always_inline)) {
+            h8 a[NPL];
+#pragma unroll
+            for (int pl = 0; pl < NPL; ++pl) {
+                a[pl] = fr[k % PF_K][pl];
+                if (k + PF_K < NKS) fr[k % PF_K][pl] = k_read(k + PF_K, pl);
+            }
+            s_product(sn, k, a);
+#pragma unroll
+            for (int v = k * 16 / NKS / 2 * 2; v < (k + 1) * 16 / NKS / 2 * 2; v += 2) {   // pairs of values of P
+                const float p0 = __builtin_amdgcn_exp2f(fmaf(s[v], factor, nr)), p1 = __builtin_amdgcn_exp2f(fmaf(s[v + 1], factor, nr));
+                ls[0] += p0;
+                ls[1] += p1;
+                asm volatile("" : "+v"(ls[0]), "+v"(ls[1]));  // (here: put off, all of P would stay in registers)
+                h2 h = __builtin_convertvector(f2w{p0, p1}, h2);
+                asm("" : "+v"(h));
+                pb[0][v >> 3][v & 7] = h[0];
+                pb[0][v >> 3][(v & 7) + 1] = h[1];
+                if constexpr (EXACT) {
+                    pb[NQ - 1][v >> 3][v & 7] = (half_t) (p0 - (float) h[0]);
+                    pb[NQ - 1][v >> 3][(v & 7) + 1] = (half_t) (p1 - (float) h[1]);
+                }
+            }
+            // (a part of what is put down every few products: one behind the other they would hold the wave)
+            each<PT::N>([&](auto y) __attribute__((always_inline)) { if constexpr (y * 2 < PT::N && (y * 2 + 1) * NKS / (PT::N + 1) == k) part(y, i + 2, r); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        l += ls[0] + ls[1];
+        h8 fv[PF_V][NPL];
+#pragma unroll
+        for (int f = 0; f < PF_V; ++f)
+#pragma unroll
+            for (int pl = 0; pl < NPL; ++pl) fv[f][pl] = v_read(f, pl);
+        mx = MINUS_INF;
+        each<NF>([&](auto f) __attribute__((always_inline)) {
+            constexpr int ps = f / NDT, dt = f % NDT;
+            h8 a[NPL];
+#pragma unroll
+            for (int pl = 0; pl < NPL; ++pl) {
+                a[pl] = fv[f % PF_V][pl];
+                if (f + PF_V < NF) fv[f % PF_V][pl] = v_read(f + PF_V, pl);
+            }
+            o[dt] = mfma32(a[0], pb[0][ps], o[dt]);
+            if constexpr (EXACT) o[dt] = mfma32(a[0], pb[NQ - 1][ps], o[dt]);
+            if constexpr (NPL == 2) o[dt] = mfma32(a[NPL - 1], pb[0][ps], o[dt]);
+#pragma unroll
+            for (int v = f * 16 / NF; v < (f + 1) * 16 / NF; ++v) mx = larger(mx, sn[v], top);
+            asm volatile("" : "+v"(mx));
+            each<PT::N>([&](auto y) __attribute__((always_inline)) { if constexpr (y * 2 >= PT::N && (y * 2 - PT::N) * NF / PT::N == f) part(y, i + 2, r); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        if (__builtin_expect(!whole(next * BN), 0)) {
+            mask(sn, next * BN);
+            mx = most_of(sn);
+        }
+        mx = max_swap32(mx) * factor;
+    };
+
+    // what was asked for `left` items ago and earlier is there, and put down; every wave
+    auto arrived = [&](auto left) __attribute__((always_inline)) {
+        if constexpr (F16) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "i"(left * G::PIECES) : "memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto ask = [&](int e, typename G::raw & r) __attribute__((always_inline)) {
+        next_row(e);
+        each<G::PIECES>([&](auto y) __attribute__((always_inline)) { load(y, e, r); });
+    };
+    auto put = [&](int e, const typename G::raw & r) __attribute__((always_inline)) { each<PT::N>([&](auto y) __attribute__((always_inline)) { part(y, e, r); }); };
+    if (ta < tb) {
+        page = page_of(tile_of_item(0));
+        ask(0, raw[0]);
+        ask(1, raw[1]);
+        if constexpr (F16) {
+            ask(2, raw[0]);
+            ask(3, raw[1]);
+        }
+        load_q();
+        if constexpr (!F16) {
+            put(0, raw[0]);
+            ask(2, raw[0]);
+        }
+        arrived(std::integral_constant<int, 3>{});
+        f16x sa, sb;
+        if (ncols > 0) {
+            const char * const kp = hidden(0);
+#pragma unroll
+            for (int k = 0; k < NKS; ++k) {
+                h8 a[NPL];
+#pragma unroll
+                for (int pl = 0; pl < NPL; ++pl) a[pl] = kf.read(kp + pl * PL_B, k);
+                s_product(sa, k, a);
+            }
+            if (!whole(tile_of(ta) * BN)) mask(sa, tile_of(ta) * BN);
+            mx = max_swap32(most_of(sa)) * factor;
+        }
+        if constexpr (!F16) {
+            put(1, raw[1]);
+            ask(3, raw[1]);
+        }
+        arrived(std::integral_constant<int, 2>{});
+        // tile i (counted from ta): K(i + 1) and V(i) are there
+        auto turn = [&](int i, f16x & s, f16x & sn, typename G::raw & r) __attribute__((always_inline)) {
+            if constexpr (F16) ask(i + 4, r);
+            if (ncols > 0) step(i, tile_of(ta + i + 1), s, sn, r);
+            else put(i + 2, r);
+            if constexpr (!F16) ask(i + 4, r);
+            arrived(std::integral_constant<int, 2>{});
+        };
+        for (int i = 0;;) {
+            turn(i, sa, sb, raw[0]);
+            if (++i + ta == tb) break;
+            turn(i, sb, sa, raw[1]);
+            if (++i + ta == tb) break;
+        }
+        if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");   // (nothing is on its way to LDS when the next group begins)
+    }
+
+    // ---- results: lane (column c, half g) holds dims 32 dt + 8 (i / 4) + 4 g + i % 4 ----
+    {
+    const tree_params & P = read_again();
+    l += __shfl_xor(l, 32);
+    if (c < ncols) {
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                finish(P, my_row, 32 * dt + 8 * q + 4 * g, D, pieces > 1 ? piece : -1, f4{o[dt][4 * q], o[dt][4 * q + 1], o[dt][4 * q + 2], o[dt][4 * q + 3]}, ref, l);
+    }
+    if (P.nks > 1 && piece == 0 && hk == 0 && threadIdx.x == 0) P.part_n[f.seq * P.max_groups + f.group] = pieces;
+    }
   }
 }
 
@@ -559,7 +973,7 @@ struct tree_merge_params {
     const float * part_o, * part_ml, * gate;
     void * out;
     float * lse;
-    int Hq, GQA, D, nks, out_bf16, BC, max_groups;
+    int Hq, GQA, D, nks, out_bf16, BC, waves, max_groups;
     const int * part_n;    // [n_seq][max_groups] partials of a group's rows (1: they are finished)
 };
 __global__ void __launch_bounds__(NTHR) tree_merge_k(const tree_merge_params P) {
@@ -569,7 +983,7 @@ __global__ void __launch_bounds__(NTHR) tree_merge_k(const tree_merge_params P) 
     const int r = at.index * per + sub;                       // of the sequence
     if (r >= (long long) at.v.count * P.Hq) return;
     const int t = r / P.Hq, h = r - t * P.Hq;
-    const shape sh = shape_of(at.v.count, P.GQA, P.BC);
+    const group_of sh = groups_of(at.v.count, P.GQA, P.BC, P.waves);
     const int n = min(P.part_n[at.seq * P.max_groups + (t * P.GQA + h % P.GQA) / (sh.bpg * P.BC)], P.nks);
     if (n < 2) return;                                        // (finished already)
     const long long row = (long long) at.v.first * P.Hq + r;
@@ -614,35 +1028,32 @@ __global__ void __launch_bounds__(NTHR) tree_merge_k(const tree_merge_params P) 
     put4(P.out, P.out_bf16, e, v);
 }
 
+// (NT = 0: team_k)
 template <uint32_t KT, int D, int NT, bool EXACT> int launch_cfg(const tree_params & P, unsigned grid, hipStream_t s) {
-    constexpr int lds = tree_cfg<KT, D, NT, EXACT>::LDS;
+    constexpr int lds = [] { if constexpr (NT) return few_cfg<KT, D, NT, EXACT>::LDS; else return team_cfg<KT, D, EXACT>::LDS; }();
+    auto * const k = [] { if constexpr (NT) return few_k<KT, D, NT, EXACT>; else return team_k<KT, D, EXACT>; }();
     // (the attribute belongs to the function on ONE device: remembered per device, set again on another)
     static std::atomic<uint32_t> attr_set{0};
     int dev = 0;
     (void) hipGetDevice(&dev);
     const uint32_t bit = 1u << (dev & 31);
     if (!(attr_set.load(std::memory_order_acquire) & bit)) {
-        if (hipFuncSetAttribute((const void *) tree_k<KT, D, NT, EXACT>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
+        if (hipFuncSetAttribute((const void *) k, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess) {
             (void) hipGetLastError();
             set_error("p1a_attn_tree: cannot reserve %d bytes of LDS", lds);
             return P1A_E_LAUNCH;
         }
         attr_set.fetch_or(bit, std::memory_order_release);
     }
-    tree_k<KT, D, NT, EXACT><<<grid, NTHR, lds, s>>>(P);
+    k<<<grid, NTHR, lds, s>>>(P);
     return launched();
 }
-template <uint32_t KT, int D> int launch_d(const tree_params & P, int NT, bool exact, unsigned grid, hipStream_t s) {
-    if (NT == 1) return exact ? launch_cfg<KT, D, 1, true>(P, grid, s) : launch_cfg<KT, D, 1, false>(P, grid, s);
-    return exact ? launch_cfg<KT, D, 2, true>(P, grid, s) : launch_cfg<KT, D, 2, false>(P, grid, s);
-}
-template <uint32_t KT> int launch_kt(const tree_params & P, int D, int NT, bool exact, unsigned grid, hipStream_t s) {
-    return D == 256 ? launch_d<KT, 256>(P, NT, exact, grid, s) : D == 128 ? launch_d<KT, 128>(P, NT, exact, grid, s) : launch_d<KT, 64>(P, NT, exact, grid, s);
-}
-// workgroups of a compute unit: as tree_cfg has it
-template <uint32_t KT> int wgs_kt(int D, int NT, bool exact) {
-    auto of = [&](auto d) { constexpr int X = decltype(d)::value; return NT == 1 ? exact ? tree_cfg<KT, X, 1, true>::WGS : tree_cfg<KT, X, 1, false>::WGS : exact ? tree_cfg<KT, X, 2, true>::WGS : tree_cfg<KT, X, 2, false>::WGS; };
-    return D == 256 ? of(std::integral_constant<int, 256>{}) : D == 128 ? of(std::integral_constant<int, 128>{}) : of(std::integral_constant<int, 64>{});
+// f(cache type, D, NT, EXACT), each as a constant
+template <typename F> int for_build(uint32_t type, int D, int NT, bool exact, F && f) {
+    auto e = [&](auto kt, auto d, auto nt) { return exact ? f(kt, d, nt, std::true_type{}) : f(kt, d, nt, std::false_type{}); };
+    auto n = [&](auto kt, auto d) { return NT == 0 ? e(kt, d, std::integral_constant<int, 0>{}) : NT == 1 ? e(kt, d, std::integral_constant<int, 1>{}) : e(kt, d, std::integral_constant<int, 2>{}); };
+    auto dd = [&](auto kt) { return D == 256 ? n(kt, std::integral_constant<int, 256>{}) : D == 128 ? n(kt, std::integral_constant<int, 128>{}) : n(kt, std::integral_constant<int, 64>{}); };
+    return type == P1A_KV_F16 ? dd(std::integral_constant<uint32_t, P1A_KV_F16>{}) : type == P1A_KV_Q8_0 ? dd(std::integral_constant<uint32_t, P1A_KV_Q8_0>{}) : dd(std::integral_constant<uint32_t, P1A_KV_Q4_0>{});
 }
 
 // the most items of `unit` that the sequences' rows times `mul` can make (as find_item counts them)
@@ -658,16 +1069,20 @@ long long item_bound(const rows_view & R, int mul, int unit) {
 tree_plan plan_tree(const p1a_kv & c, const rows_view & R, int Hq, int max_n, bool exact, int cus) {
     tree_plan pl{};
     const int GQA = Hq / c.Hkv;
-    pl.NT = (long long) R.max_rows * GQA <= 16 ? 1 : 2;
-    const shape sh = shape_of(R.max_rows, GQA, 16 * pl.NT);
-    pl.max_groups = sh.groups;
+    const long long cols = (long long) R.max_rows * GQA;
+    pl.NT = cols <= 16 ? 1 : cols <= 32 ? 2 : 0;
+    pl.max_groups = pl.NT ? 1 : groups_of(R.max_rows, GQA, 32, NW).groups;
     pl.nks = 1;
-    const long long groups = (long long) R.n_seq * sh.groups;
+    const long long groups = (long long) R.n_seq * pl.max_groups;
     pl.runs = (int) groups;
-    const int wgs = c.type == P1A_KV_F16 ? wgs_kt<P1A_KV_F16>(c.D, pl.NT, exact) : c.type == P1A_KV_Q8_0 ? wgs_kt<P1A_KV_Q8_0>(c.D, pl.NT, exact) : wgs_kt<P1A_KV_Q4_0>(c.D, pl.NT, exact);
+    const int wgs = for_build(c.type, c.D, pl.NT, exact, [](auto kt, auto d, auto nt, auto ex) {
+        if constexpr (nt.value != 0) return few_cfg<kt.value, d.value, nt.value, ex.value>::WGS;
+        else return team_cfg<kt.value, d.value, ex.value>::WGS;
+    });
+    const int step = pl.NT ? 32 * NW : for_build(c.type, c.D, 0, exact, [](auto kt, auto d, auto, auto ex) { return team_cfg<kt.value, d.value, ex.value>::BN; });
     const long long slots = (long long) std::max(cus, 1) * wgs, units = groups * c.Hkv;
     const long long keys = R.window == INT32_MAX ? max_n : std::min<long long>(max_n, (long long) R.window + R.max_rows + R.n_sink);
-    const long long nt = std::max<long long>(((keys + 31) / 32 + sh.ks - 1) / sh.ks, 1);
+    const long long nt = std::max<long long>((keys + step - 1) / step, 1);
     const size_t rows = (size_t) R.T * Hq, row_bytes = (size_t) c.D * 4 + 8;
     const long long runs = std::min(std::max(slots / c.Hkv, 1LL), groups * nt), per = (groups * nt + runs - 1) / runs;
     const long long most = std::min({64LL, runs, nt + 1, (128LL << 20) / (long long) (rows * row_bytes)});
@@ -708,10 +1123,9 @@ int launch_tree(const p1a_kv & c, const chunk_args & a, const uint32_t * mask, i
             P.part_ml = (float *) ((char *) first + pl.bytes_n);
         }
     }
-    const int rc = c.type == P1A_KV_F16 ? launch_kt<P1A_KV_F16>(P, c.D, pl.NT, exact, (unsigned) grid, s)
-                 : c.type == P1A_KV_Q8_0 ? launch_kt<P1A_KV_Q8_0>(P, c.D, pl.NT, exact, (unsigned) grid, s) : launch_kt<P1A_KV_Q4_0>(P, c.D, pl.NT, exact, (unsigned) grid, s);
+    const int rc = for_build(c.type, c.D, pl.NT, exact, [&](auto kt, auto d, auto nt, auto ex) { return launch_cfg<kt.value, d.value, nt.value, ex.value>(P, (unsigned) grid, s); });
     if (rc != P1A_OK || P.nks == 1) return rc;
-    const tree_merge_params M{a.R, P.part_o, P.part_ml, a.gate, a.out, a.lse, a.Hq, P.GQA, c.D, P.nks, a.out_bf16, 16 * pl.NT, pl.max_groups, P.part_n};
+    const tree_merge_params M{a.R, P.part_o, P.part_ml, a.gate, a.out, a.lse, a.Hq, P.GQA, c.D, P.nks, a.out_bf16, pl.NT ? 16 * pl.NT : 32, pl.NT ? 1 : NW, pl.max_groups, P.part_n};
     tree_merge_k<<<(unsigned) item_bound(a.R, a.Hq, NTHR / (c.D / 4)), NTHR, 0, s>>>(M);
     return launched();
 }
