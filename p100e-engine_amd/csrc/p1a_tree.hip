@@ -202,6 +202,8 @@ __device__ __forceinline__ sight sight_of(const tree_params & P, const seq_view 
     return v;
 }
 
+// (the hardware's exponential and reciprocal: within 4 2^-24 of the gate, where the other roundings of f32 results are 2^-22)
+__device__ __forceinline__ float tree_gate(float g) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -LOG2E)); }
 // Four results of a row from its sums relative to M: a partial (piece >= 0) or what the call is to give
 __device__ __forceinline__ void finish(const tree_params & P, size_t row, int d, int D, int piece, f4 acc, float M, float l) {
     if (piece >= 0) {
@@ -214,7 +216,7 @@ __device__ __forceinline__ void finish(const tree_params & P, size_t row, int d,
     if (P.gate) {
         const f4 gt = *reinterpret_cast<const f4 *>(P.gate + row * D + d);
 #pragma unroll
-        for (int y = 0; y < 4; ++y) v[y] *= gate_of(gt[y]);
+        for (int y = 0; y < 4; ++y) v[y] *= tree_gate(gt[y]);
     }
     put4(P.out, P.out_bf16, row * D + d, v);
 }
@@ -448,7 +450,7 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int j = 16 * x + e;             // (and 4 g)
-                        s[x][n][e] = (j <= hi && (j > lo || j < sk)) || (bits >> j & 1) ? s[x][n][e] : MINUS_INF;
+                        s[x][n][e] = ((j <= hi) & ((j > lo) | (j < sk))) | (int) (bits >> j & 1) ? s[x][n][e] : MINUS_INF;
                     }
             }
         }
@@ -702,17 +704,18 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     const int32_t * const ptab = P.pg.pt ? P.pg.pt + f.table : nullptr;
     const bool paged16 = P.pg.psh >= 4;
     auto tile_of = [&](int i) { return sp.tile(min(i, tb - 1)); };   // (past the last: that one once more, unused)
+    auto tile_of_item = [&](int e) { return tile_of(ta + max(e - (my_v ? 1 : 0), 0)); };   // (items: below)
     auto pos_of = [&](int tile) { return seen_in_group<BN>(sp, tile * BN, tile * BN + 16 * grp, tile * BN + 16 * grp + G::key(lane)); };
-    // (one page for the wave's 16 keys: through the scalar cache, beside the counter that tiles are waited for by)
-    auto page_of = [&](int tile) {
-        int page = 0;
-        if (ptab) {
-            if (paged16) page = sload_i32(ptab + (__builtin_amdgcn_readfirstlane(pos_of(tile)) >> P.pg.psh));
-            else {
-                page = ptab[pos_of(tile) >> P.pg.psh];
-                asm volatile("" : "+v"(page));
-            }
-        }
+    // Pages of 16 positions and more: one page for the wave's 16 keys of a tile, and lane l holds that of item 64 n + l - a load every 64 items, so that none has to be waited for
+    // while tiles are on their way. Smaller ones: a load for every item, and a wait for it.
+    auto pages_from = [&](int e0) {
+        const int tile = tile_of_item(e0 + lane), kb = tile * BN + 16 * grp;
+        return ptab && paged16 ? ptab[seen_in_group<BN>(sp, tile * BN, kb, kb) >> P.pg.psh] : 0;
+    };
+    auto page_of = [&](int e, int pages) {
+        if (paged16 || !ptab) return __builtin_amdgcn_readlane(pages, e & 63);
+        int page = ptab[pos_of(tile_of_item(e)) >> P.pg.psh];
+        asm volatile("" : "+v"(page));
         return page;
     };
     auto row_of = [&](int tile, int page) {
@@ -784,7 +787,7 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int j = mfma_row(i, 0);                     // (and 4 g)
-            s[i] = (j <= hi && (j > lo || j < sk)) || (bits >> j & 1) ? s[i] : MINUS_INF;
+            s[i] = ((j <= hi) & ((j > lo) | (j < sk))) | (int) (bits >> j & 1) ? s[i] : MINUS_INF;
         }
     };
     float top = -MINUS_INF;
@@ -800,12 +803,14 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     // ---- what a wave brings: of item e K of tile e or V of tile e - 1. Item e is asked for at step e - 4 and in LDS at the end of step e - 2 ----
     typename G::raw raw[2];
     auto to_of = [&](int e) { return (my_v ? v_place + (e + C::PLACES - 1) % C::PLACES * T_B : k_place + e % C::PLACES * T_B) + grp * G_B; };
-    int page = 0;                                             // of the item that is asked for next
+    int pages = 0;
     size_t row = 0;
-    auto tile_of_item = [&](int e) { return tile_of(ta + max(e - (my_v ? 1 : 0), 0)); };
-    auto next_row = [&](int e) {                              // item e's row; the page of the one behind it
-        row = row_of(tile_of_item(e), page);
-        page = page_of(tile_of_item(e + 1));
+    auto next_row = [&](int e) {
+        if (!(e & 63)) {
+            pages = pages_from(e);
+            asm volatile("" : "+v"(pages));                    // (waited for here: behind the branch every item would wait)
+        }
+        row = row_of(tile_of_item(e), page_of(e, pages));
     };
     auto load = [&](auto y, int e, typename G::raw & r) __attribute__((always_inline)) { G::template piece<y>(r, from + row, to_of(e), lane); };
     auto part = [&](auto y, int e, const typename G::raw & r) __attribute__((always_inline)) { if constexpr (!F16) PT::template store<y>(r, to_of(e), lane); };
@@ -903,7 +908,6 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     };
     auto put = [&](int e, const typename G::raw & r) __attribute__((always_inline)) { each<PT::N>([&](auto y) __attribute__((always_inline)) { part(y, e, r); }); };
     if (ta < tb) {
-        page = page_of(tile_of_item(0));
         ask(0, raw[0]);
         ask(1, raw[1]);
         if constexpr (F16) {
@@ -942,12 +946,13 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
             if constexpr (!F16) ask(i + 4, r);
             arrived(std::integral_constant<int, 2>{});
         };
-        for (int i = 0;;) {
+        // (in pairs, the last one by itself: with a way out between the two the compiler waits at the top for what was asked for last)
+        int i = 0;
+        for (; ta + i + 1 < tb; i += 2) {
             turn(i, sa, sb, raw[0]);
-            if (++i + ta == tb) break;
-            turn(i, sb, sa, raw[1]);
-            if (++i + ta == tb) break;
+            turn(i + 1, sb, sa, raw[1]);
         }
+        if (ta + i < tb) turn(i, sa, sb, raw[0]);
         if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");   // (nothing is on its way to LDS when the next group begins)
     }
 
@@ -1023,7 +1028,7 @@ __global__ void __launch_bounds__(NTHR) tree_merge_k(const tree_merge_params P) 
     if (P.gate) {
         const f4 gt = *reinterpret_cast<const f4 *>(P.gate + e);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] *= gate_of(gt[i]);
+        for (int i = 0; i < 4; ++i) v[i] *= tree_gate(gt[i]);
     }
     put4(P.out, P.out_bf16, e, v);
 }
