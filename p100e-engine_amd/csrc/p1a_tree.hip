@@ -36,8 +36,10 @@ struct tree_params : chunk_params {
 };
 
 // ---- runs of steps of equal length over the groups of all sequences (lane i of a wave counts for sequence s0 + i) ----
-// BN: keys of a tile; TPS: tiles of a step; BC: columns of a block; WAVES: blocks of a group
-template <int BN, int TPS, int BC, int WAVES> struct tree_runs {
+// BN: keys of a tile; TPS: tiles of a step; BC: columns of a block; WAVES: blocks of a group. A group counts SETUP steps more than it has: what it takes to find it, to ask for its first
+// tiles and q and to write its results (24 sequences of 3 ... 64 nodes over 500 ... 8000 keys: workgroups with many short groups were still at work for 34 us when half of all had ended)
+template <int BN, int TPS, int BC, int WAVES, int SETUP_> struct tree_runs {
+    static constexpr int SETUP = SETUP_;
     struct of_lane { int first, pos0, table, rows, per_group, steps; };
     of_lane first64;
     int first, end, per;
@@ -51,7 +53,7 @@ template <int BN, int TPS, int BC, int WAVES> struct tree_runs {
         r.pos0 = v.pos0;
         r.rows = v.count;
         if (v.count > 0) {
-            r.per_group = max((span_of_rows(R, v).nt + TPS - 1) / TPS, 1);
+            r.per_group = SETUP + max((span_of_rows(R, v).nt + TPS - 1) / TPS, 1);
             r.steps = r.per_group * groups_of(v.count, GQA, BC, WAVES).groups;
         }
         return r;
@@ -72,7 +74,13 @@ template <int BN, int TPS, int BC, int WAVES> struct tree_runs {
         end = min(first + per, n);
         return first < end;
     }
-    // whose step `at` is: sequence, group, the group's first step, its steps. False: nobody's (row0 or pos0 were written since begin())
+    // What of a group's steps, as found, is in this run: from .. to - 1 (counted without SETUP; nothing: to <= 0), which of its pieces that is and how many there are
+    struct share { int from, to, piece, pieces; };
+    template <class F> __device__ __forceinline__ share share_of(const F & f, int at, int run) const {
+        const int lo = f.first + SETUP, run0 = lo / per;
+        return share{max(at - lo, 0), min(end, f.first + f.steps) - lo, run - run0, (f.first + f.steps - 1) / per - run0 + 1};
+    }
+    // whose step `at` is: sequence, group, the group's first step, its steps (SETUP among them). False: nobody's (row0 or pos0 were written since begin())
     struct found { int seq, group, first, steps, table; seq_view v; };
     __device__ __forceinline__ bool find(const rows_view & R, const kv_view & pg, int GQA, int at, int lane, found & f) const {
         int base = 0;
@@ -230,7 +238,7 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
     using K = typename std::conditional<F16 || CODES, keys16<KT, D>, keysd<KT, D>>::type;
     using G = group<KT, D, CODES ? 0 : 1>;
     constexpr int NB = D / 32, NDT = D / 16, NQ = EXACT ? 2 : 1, PL_B = plane_bytes(D);
-    using runs_t = tree_runs<32, NW, 16 * NT, 1>;
+    using runs_t = tree_runs<32, NW, 16 * NT, 1, 4>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -260,18 +268,21 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
     if (P.nks > 1) {
         if (!steps.find(P.R, P.pg, P.GQA, at_step, lane, f)) return;
     } else {                                                  // a sequence each
-        f.seq = run; f.group = 0; f.first = 0; f.steps = 1 << 26;
+        f.seq = run; f.group = 0; f.first = 0; f.steps = 1;
         f.v = seq_of<true>(P.R, f.seq);
         f.table = P.pg.pt && P.pg.rtab ? sload_i32(P.pg.rtab + f.seq) : 0;
         if (f.v.count < 1) return;
     }
     const seq_view & sv = f.v;
-    const int run0 = f.first / steps.per, pieces = P.nks > 1 ? (f.first + f.steps - 1) / steps.per - run0 + 1 : 1, piece = P.nks > 1 ? run - run0 : 0;
+    typename runs_t::share due{0, 1 << 26, 0, 1};
+    if (P.nks > 1) due = steps.share_of(f, at_step, run);
+    at_step = f.first + f.steps;
+    if (due.to <= 0) continue;
+    const int pieces = due.pieces, piece = due.piece;
     const int R = min(sv.count * P.GQA, 16 * NT);
     auto row_index = [&](int r) { const int t = tok_of(r); return (size_t) (sv.first + t) * P.Hq + (size_t) hk * P.GQA + (r - t * P.GQA); };
     const span sp = runs_t::span_of_rows(P.R, sv);
-    const int ta = (at_step - f.first) * NW, tb = P.nks > 1 ? min((min(steps.end, f.first + f.steps) - f.first) * NW, sp.nt) : sp.nt;
-    at_step = f.first + f.steps;
+    const int ta = due.from * NW, tb = min(due.to * NW, sp.nt);
     // positions that all rows see
     const bool odd = sv.pos0 < 0 || sv.pos0 + sv.count > P.R.n_ctx;
     const int all_hi = odd ? -1 : sv.pos0 - 1, all_lo = P.R.window == INT32_MAX ? 0 : sp.pmax - P.R.window + 1;
@@ -308,7 +319,21 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
         }
     };
 
-    // page-table entries are asked for a tile ahead of the rows, which come a tile ahead of their products
+    // ---- q, the first tile, Q^T: columns 16 n + c. (Page-table entries are asked for a tile ahead of the rows, which come a tile ahead of their products) ----
+    f4 qx[NT][NB][2];
+    auto dim_of = [&](int b, int e) { if constexpr (F16 || CODES) return 32 * b + K::dims(g, e); else return K::dim(b, g, e); };
+    auto fetch_q = [&](auto as_bf16) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const size_t row = row_index(min(16 * n + c, R - 1)) * D;
+#pragma unroll
+            for (int b = 0; b < NB; ++b)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) qx[n][b][e] = q4_at(P.q, as_bf16, row + dim_of(b, e));
+        }
+    };
+    if (P.q_bf16) fetch_q(std::true_type{});
+    else fetch_q(std::false_type{});
     int i = ta + wave;
     auto tile_of = [&](int i) { return sp.tile(min(i, tb - 1)); };   // (past the last: that one once more, unused)
     key_rows::pages pg;
@@ -319,8 +344,6 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
         ask_v(at, 0);
         ask_k(at);
     }
-
-    // ---- Q^T: columns 16 n + c ----
     constexpr int NQR = C::QL ? 1 : NQ;                       // halves in registers
     h8 qf[NT][NQR][NB];
     char * const ql = lds + NW * C::WAVE_B + lane * 16;
@@ -328,39 +351,21 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
     float factor[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const size_t row = row_index(min(16 * n + c, R - 1));
-        h8 qq[NQ][NB];
-        if constexpr (F16 || CODES) factor[n] = ldexpf(P.factor, q_columns<KT, D, NQ>(P.q, P.q_bf16, row, P.sign, g, qq));
-        else {
-            f4 x[NB][2];
-            float most = 0.f;
-            auto fetch = [&](auto as_bf16) {
+        float most = 0.f;
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) x[b][e] = q4_at(P.q, as_bf16, row * D + K::dim(b, g, e));
-            };
-            if (P.q_bf16) fetch(std::true_type{});
-            else fetch(std::false_type{});
-#pragma unroll
-            for (int b = 0; b < NB; ++b)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[b][e >> 2][e & 3]));
-            const int ex = row_exponent(max_swap32(max_swap16(most)));
-            factor[n] = ldexpf(P.factor, ex);
-            const float by = ldexpf(P.sign, -ex);
-#pragma unroll
-            for (int b = 0; b < NB; ++b) {
-                h8 r[NQ];
-                halves<NQ>([&](int e) { return x[b][e >> 2][e & 3]; }, [&](int) { return by; }, r);
-                qq[0][b] = r[0];
-            }
-        }
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(qx[n][b][e >> 2][e & 3]));
+        const int ex = row_exponent(max_swap32(max_swap16(most)));
+        factor[n] = ldexpf(P.factor, ex);
+        const float by = ldexpf(P.sign, -ex);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+            h8 r[NQ];
+            halves<NQ>([&](int e) { return qx[n][b][e >> 2][e & 3]; }, [&](int) { return by; }, r);
 #pragma unroll
-            for (int k = 0; k < NQR; ++k) qf[n][k][b] = qq[k][b];
-            if constexpr (C::QL) *reinterpret_cast<h8 *>(ql + (n * NB + b) * 1024) = qq[NQ - 1][b];
+            for (int k = 0; k < NQR; ++k) qf[n][k][b] = r[k];
+            if constexpr (C::QL) *reinterpret_cast<h8 *>(ql + (n * NB + b) * 1024) = r[NQ - 1];
         }
         __builtin_amdgcn_sched_barrier(0);
     }
@@ -650,7 +655,7 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     constexpr bool F16 = C::F16;
     constexpr int BN = C::BN, G_B = C::G_B, T_B = C::T_B, PL_B = plane_bytes(D), NPL = C::NPL;
     constexpr int NKS = D / 16, NDT = D / 32, NQ = EXACT ? 2 : 1, PF_K = NPL == 2 ? 1 : EXACT ? 2 : 4, PF_V = NPL == 2 ? 1 : EXACT ? 2 : 3;
-    using runs_t = tree_runs<BN, 1, 32, NW>;
+    using runs_t = tree_runs<BN, 1, 32, NW, 6>;
     extern __shared__ __attribute__((aligned(16))) char lds[];
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -680,7 +685,7 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     if (P.nks > 1) {
         if (!steps.find(P.R, P.pg, P.GQA, at_step, lane, f)) return;
     } else {                                                  // a group each
-        f.seq = run / P.max_groups; f.group = run - f.seq * P.max_groups; f.first = 0; f.steps = 1 << 26;
+        f.seq = run / P.max_groups; f.group = run - f.seq * P.max_groups; f.first = 0; f.steps = 1;
         f.v = seq_of<true>(P.R, f.seq);
         f.table = P.pg.pt && P.pg.rtab ? sload_i32(P.pg.rtab + f.seq) : 0;
         if (f.v.count < 1) return;
@@ -688,13 +693,16 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     const seq_view & sv = f.v;
     const group_of sh = groups_of(sv.count, P.GQA, 32, NW);
     if (P.nks == 1 && f.group >= sh.groups) return;
-    const int run0 = f.first / steps.per, pieces = P.nks > 1 ? (f.first + f.steps - 1) / steps.per - run0 + 1 : 1, piece = P.nks > 1 ? run - run0 : 0;
+    typename runs_t::share due{0, 1 << 26, 0, 1};
+    if (P.nks > 1) due = steps.share_of(f, at_step, run);
+    at_step = f.first + f.steps;
+    if (due.to <= 0) continue;
+    const int pieces = due.pieces, piece = due.piece;
     const int col0 = (f.group * sh.bpg + wave) * 32, ncols = wave < sh.bpg ? min(sh.cols - col0, 32) : 0;   // this wave's columns (none: it brings keys only)
     const int my_col = ncols > 0 ? col0 + min(c, ncols - 1) : 0, my_tok = tok_of(my_col);
     const size_t my_row = (size_t) (sv.first + my_tok) * P.Hq + (size_t) hk * P.GQA + (my_col - my_tok * P.GQA);
     const span sp = runs_t::span_of_rows(P.R, sv);
-    const int ta = at_step - f.first, tb = P.nks > 1 ? min(min(steps.end, f.first + f.steps) - f.first, sp.nt) : sp.nt;
-    at_step = f.first + f.steps;
+    const int ta = due.from, tb = min(due.to, sp.nt);
     // positions that all rows see
     const bool odd = sv.pos0 < 0 || sv.pos0 + sv.count > P.R.n_ctx;
     const int all_hi = odd ? -1 : sv.pos0 - 1, all_lo = P.R.window == INT32_MAX ? 0 : sp.pmax - P.R.window + 1;
@@ -712,42 +720,34 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
         const int tile = tile_of_item(e0 + lane), kb = tile * BN + 16 * grp;
         return ptab && paged16 ? ptab[seen_in_group<BN>(sp, tile * BN, kb, kb) >> P.pg.psh] : 0;
     };
-    auto page_of = [&](int e, int pages) {
-        if (paged16 || !ptab) return __builtin_amdgcn_readlane(pages, e & 63);
-        int page = ptab[pos_of(tile_of_item(e)) >> P.pg.psh];
-        asm volatile("" : "+v"(page));
-        return page;
-    };
-    auto row_of = [&](int tile, int page) {
-        const int j = pos_of(tile);
-        return head_off + (ptab ? (size_t) page * P.pg.pstride + (size_t) (j & ((1 << P.pg.psh) - 1)) * P.pg.rowb : (size_t) j * P.pg.rowb);
-    };
 
     // ---- Q^T operands: lane (column c, half g) holds dims 16 ks + 8 g .. + 7 ----
     h8 qf[NQ][NKS];
     float factor = P.factor;
-    auto load_q = [&] {
-        f4 x[NKS][2];
-        float most = 0.f;
+    f4 qx[NKS][2];
+    auto fetch_q = [&] {
         auto fetch = [&](auto as_bf16) {
 #pragma unroll
             for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) x[ks][e] = q4_at(P.q, as_bf16, my_row * D + 16 * ks + 8 * g + 4 * e);
+                for (int e = 0; e < 2; ++e) qx[ks][e] = q4_at(P.q, as_bf16, my_row * D + 16 * ks + 8 * g + 4 * e);
         };
         if (P.q_bf16) fetch(std::true_type{});
         else fetch(std::false_type{});
+    };
+    auto take_q = [&] {
+        float most = 0.f;
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(x[ks][e >> 2][e & 3]));
+            for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(qx[ks][e >> 2][e & 3]));
         const int ex = row_exponent(max_swap32(most));
         factor = ldexpf(factor, ex);
         const float by = ldexpf(P.sign, -ex);
 #pragma unroll
         for (int ks = 0; ks < NKS; ++ks) {
             h8 r[NQ];
-            halves<NQ>([&](int e) { return x[ks][e >> 2][e & 3]; }, [&](int) { return by; }, r);
+            halves<NQ>([&](int e) { return qx[ks][e >> 2][e & 3]; }, [&](int) { return by; }, r);
 #pragma unroll
             for (int k = 0; k < NQ; ++k) {
                 qf[k][ks] = r[k];
@@ -758,12 +758,14 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     };
 
     f16x o[NDT];
-#pragma unroll
-    for (int dt = 0; dt < NDT; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
     float ref = MINUS_INF, l = 0.f, mx = MINUS_INF;           // mx: the column's largest score of the tile in hand
 
+    auto clear = [&] {
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+    };
     const k_frag kf(lane, G_B);
     const v_frag vf(lane);
     // (a place in LDS as a number the compiler does not see through - offsets from it fit the instructions, those from the start do not)
@@ -805,12 +807,28 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     auto to_of = [&](int e) { return (my_v ? v_place + (e + C::PLACES - 1) % C::PLACES * T_B : k_place + e % C::PLACES * T_B) + grp * G_B; };
     int pages = 0;
     size_t row = 0;
+    const int key_off = G::key(lane) * (int) P.pg.rowb;
     auto next_row = [&](int e) {
         if (!(e & 63)) {
             pages = pages_from(e);
             asm volatile("" : "+v"(pages));                    // (waited for here: behind the branch every item would wait)
         }
-        row = row_of(tile_of_item(e), page_of(e, pages));
+        const int tile = tile_of_item(e), kb = tile * BN + 16 * grp;
+        if (paged16 || !ptab) {                               // where the first of the 16 rows is, the same for all lanes, and how far behind it a lane's own
+            int a = kb, off = key_off;
+            if (!(kb + 15 <= sp.pmax && (kb >= sp.lo || kb + 15 < sp.ns))) {
+                const int j = pos_of(tile);
+                a = __builtin_amdgcn_readfirstlane(j);
+                off = (j - a) * (int) P.pg.rowb;
+            }
+            const size_t at = ptab ? (size_t) __builtin_amdgcn_readlane(pages, e & 63) * P.pg.pstride + (size_t) (a & ((1 << P.pg.psh) - 1)) * P.pg.rowb : (size_t) a * P.pg.rowb;
+            row = head_off + at + (ptrdiff_t) off;
+        } else {
+            const int j = pos_of(tile);
+            int page = ptab[j >> P.pg.psh];
+            asm volatile("" : "+v"(page));
+            row = head_off + (size_t) page * P.pg.pstride + (size_t) (j & ((1 << P.pg.psh) - 1)) * P.pg.rowb;
+        }
     };
     auto load = [&](auto y, int e, typename G::raw & r) __attribute__((always_inline)) { G::template piece<y>(r, from + row, to_of(e), lane); };
     auto part = [&](auto y, int e, const typename G::raw & r) __attribute__((always_inline)) { if constexpr (!F16) PT::template store<y>(r, to_of(e), lane); };
@@ -907,6 +925,7 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
         each<G::PIECES>([&](auto y) __attribute__((always_inline)) { load(y, e, r); });
     };
     auto put = [&](int e, const typename G::raw & r) __attribute__((always_inline)) { each<PT::N>([&](auto y) __attribute__((always_inline)) { part(y, e, r); }); };
+    fetch_q();
     if (ta < tb) {
         ask(0, raw[0]);
         ask(1, raw[1]);
@@ -914,12 +933,13 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
             ask(2, raw[0]);
             ask(3, raw[1]);
         }
-        load_q();
+        take_q();
         if constexpr (!F16) {
             put(0, raw[0]);
             ask(2, raw[0]);
         }
         arrived(std::integral_constant<int, 3>{});
+        clear();
         f16x sa, sb;
         if (ncols > 0) {
             const char * const kp = hidden(0);
@@ -954,7 +974,7 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
         }
         if (ta + i < tb) turn(i, sa, sb, raw[0]);
         if constexpr (F16) asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");   // (nothing is on its way to LDS when the next group begins)
-    }
+    } else clear();
 
     // ---- results: lane (column c, half g) holds dims 32 dt + 8 (i / 4) + 4 g + i % 4 ----
     {
@@ -1087,11 +1107,11 @@ tree_plan plan_tree(const p1a_kv & c, const rows_view & R, int Hq, int max_n, bo
     const int step = pl.NT ? 32 * NW : for_build(c.type, c.D, 0, exact, [](auto kt, auto d, auto, auto ex) { return team_cfg<kt.value, d.value, ex.value>::BN; });
     const long long slots = (long long) std::max(cus, 1) * wgs, units = groups * c.Hkv;
     const long long keys = R.window == INT32_MAX ? max_n : std::min<long long>(max_n, (long long) R.window + R.max_rows + R.n_sink);
-    const long long nt = std::max<long long>((keys + step - 1) / step, 1);
+    const long long nt = std::max<long long>((keys + step - 1) / step, 1) + (pl.NT ? 4 : 6);   // (set-up among them: SETUP of the kernels' runs)
     const size_t rows = (size_t) R.T * Hq, row_bytes = (size_t) c.D * 4 + 8;
     const long long runs = std::min(std::max(slots / c.Hkv, 1LL), groups * nt), per = (groups * nt + runs - 1) / runs;
     const long long most = std::min({64LL, runs, nt + 1, (128LL << 20) / (long long) (rows * row_bytes)});
-    if (most > 1 && (units + slots - 1) / slots * (nt + 3) > std::max(per, (nt + most - 2) / (most - 1)) + 8) {
+    if (most > 1 && (units + slots - 1) / slots * nt > std::max(per, (nt + most - 2) / (most - 1)) + 8) {
         pl.runs = (int) runs;
         pl.nks = (int) most;
         pl.bytes_n = ((size_t) groups * 4 + 255) & ~(size_t) 255;
