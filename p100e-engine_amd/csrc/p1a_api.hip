@@ -589,7 +589,7 @@ int p1a_tree_verify(const void * target, int target_type, size_t ld_target, cons
 size_t p1a_tree_verify_scratch_bytes(const p1a_rows * rows, int V, int flags) {
     rows_view R;
     if (tree_rows_ok(rows, "p1a_tree_verify_scratch_bytes", false, R) != P1A_OK || !rows->n_seq || V < 1 || V > 1 << 20) return 0;
-    return plan_verify(R, V, !(flags & P1A_VERIFY_PROBS)).bytes;
+    return plan_verify(R, V, !(flags & P1A_VERIFY_PROBS), true).bytes;
 }
 
 int p1a_tree_commit(const p1a_kv * layers, int n_layers, const p1a_rows * rows, const int32_t * n_accept, const int32_t * path, int ld_path, void * stream) {

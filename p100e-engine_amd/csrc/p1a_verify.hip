@@ -5,11 +5,16 @@
 // outcome does not depend on how the walk came there: all nodes decide at once, in as many rounds as a node has children, and the walk follows what they decided.
 //   stats_k   logits: every row in stretches of 4096 values, a workgroup each: the largest, where it is, the sum of exp((l - largest) / temp)
 //   decide_k  a workgroup per sequence: every node tests its first child (without a draft: all of them, as a rejection takes one known weight out); the walk
-//   sums_k    further children of nodes that the walk can still reach: the sum of max(p - a q, 0) a stretch; the last workgroup of a sequence decides on
-//   pick_k    the last node's row: sums a stretch; the last workgroup of a sequence finds the stretch where the running sum passes u, and the value in it
-// Sums, exponentials and comparisons are made in 64 bits: with 32 one draw in some hundreds would take the neighbouring token. exp2 is a Taylor polynomial (11
-// terms on |x ln 2| <= 0.347: 7e-15 of the value), 19 64-bit instructions a value: 24 M logits 12 us on the vector units, 20 from memory - both at once.
-// A sum's order is fixed by its place, so the same call gives the same tokens.
+//   sums_k    a launch for each further child of a node: nodes that the walk may still reach take the last round's sum, test a child, and sum what a rejection leaves
+//   left_k    the last node's row: what is left, a stretch a workgroup
+//   pick_k    a workgroup per sequence: the stretch where the running sum passes u, and the value in it (logits without a draft: at decide_k's end, as
+//             stats_k has summed every stretch and only those with a rejected token are summed again)
+// stats_k is bound by the memory that it reads (160 rows of 151936 f32 logits: 23 us, 4.2 TB/s), the others by their chains of dependent loads (5 ... 14 us each).
+// A kernel's end is what makes its sums known: with workgroups that count themselves and a last one that goes on, each had to make its writes visible to the other
+// XCDs' caches, and 32 chains over 151936 logits took 112 us instead of 57.
+// Sums, exponentials and comparisons are made in 64 bits: with 32 one draw in some hundreds would take the neighbouring token. 2^x comes from a table of 256 powers
+// and three terms (2e-13 of the value: a draw in 10^7), 12 64-bit instructions a value; the table is a constant of the program, since making it in every workgroup
+// took 5 us of each kernel. A sum's order is fixed by its place, so the same call gives the same tokens.
 #include "p1a_tiles.hpp"
 
 #include <algorithm>
@@ -36,45 +41,70 @@ struct verify_params {
     double * row_z;        // [T] logits: 1 / the row's sum
     float * row_max;       // [T] the row's largest
     int * row_arg;         // [T] where it is
-    double * node_a, * node_gone;                             // [T]
-    int * node_child;      // [T] the child under test
-    int * node_state;      // [T] accepted child, NONE, or WAITS for its sum
-    double * sums;         // [T][stretches] of a round, then [n_seq][stretches][2] of the last row
-    int * due, * here;     // [n_seq] workgroups that a round has for the sequence; that have come
+    // per node, two of each (a round reads one and writes the other)
+    double * node_a[2], * node_gone[2];
+    int * node_child[2];   // the child under test
+    int * node_state[2];   // accepted child, NONE, or WAITS for its sum
+    double * sums[2];      // [T][stretches] of a round; sums[0] then [n_seq][stretches] of the last row
+    int16_t * sibling;     // [T] next child of the same parent
+    int * waiting;         // [T] a sequence's nodes that wait, from its first row on
+    int * n_waiting;       // [n_seq]
     int * last_row;        // [n_seq] the row that the token is drawn from (-1: none)
     double * last_a;       // [n_seq]
 };
 enum { NONE = -1, WAITS = -2 };
 
-// 2^x for x <= 0
-__device__ __forceinline__ double exp2_64(double x) {
-    x = fmax(x, -1100.0);                                     // (below 2^-1074: 0)
-    const double n = __builtin_rint(x), f = (x - n) * 0.6931471805599453094;
-    double p = 2.50521083854417188e-8;                        // 1 / 11!, 1 / 10! ...
-    p = fma(p, f, 2.75573192239858907e-7);
-    p = fma(p, f, 2.75573192239858907e-6);
-    p = fma(p, f, 2.48015873015873016e-5);
-    p = fma(p, f, 1.98412698412698413e-4);
-    p = fma(p, f, 1.38888888888888889e-3);
-    p = fma(p, f, 8.33333333333333333e-3);
-    p = fma(p, f, 4.16666666666666667e-2);
-    p = fma(p, f, 1.66666666666666667e-1);
-    p = fma(p, f, 0.5);
-    p = fma(p, f, 1.0);
-    p = fma(p, f, 1.0);
-    return ldexp(p, (int) n);
+// ---- 2^x for x <= 0 ----
+// 2^x = 2^n 2^(k / 256) 2^f: a power from a table in LDS, and 1 + f ln 2 + ... for |f| <= 1 / 512 - up to the third power 1.4e-13 of the value
+struct powers { double of[256]; };
+constexpr powers powers_of_2() {                              // 2^(k / 256) = exp(k ln 2 / 256), 18 terms of the series in Horner's form
+    powers t{};
+    for (int k = 0; k < 256; ++k) {
+        const double f = k * (0.6931471805599453094 / 256);
+        double p = 1.0;
+        for (int i = 18; i >= 1; --i) p = 1.0 + f / i * p;
+        t.of[k] = p;
+    }
+    return t;
 }
-constexpr double LOG2E_64 = 1.4426950408889634074;
+__device__ const powers POWERS = powers_of_2();
+__device__ __forceinline__ void fill(powers & t) {
+    t.of[threadIdx.x] = POWERS.of[threadIdx.x];
+    __syncthreads();
+}
+// (x: 256 times the exponent. A NaN: 0)
+__device__ __forceinline__ double exp2_256(double x, const powers & t) {
+    x = fmax(x, -281600.0);                                   // (below 2^-1074: 0)
+    const double n = __builtin_rint(x), f = x - n;
+    const int k = (int) n;
+    constexpr double L = 0.6931471805599453094 / 256;
+    return ldexp(t.of[k & 255] * fma(fma(fma(f, L * L * L / 6, L * L / 2), f, L), f, 1.0), k >> 8);
+}
+constexpr double LOG2E_256 = 256 * 1.4426950408889634074;
 
-// weight of a logit beside the largest one: by = log2 e / temp
-__device__ __forceinline__ double logit_weight(float l, float most, double by) {
-    return l == most ? 1.0 : l > MINUS_INF ? exp2_64(((double) l - (double) most) * by) : 0.0;   // (a NaN: 0; finite beside an infinite one: 2^-inf)
-}
-// the scale of a sequence's logits; below 0: the largest one, with certainty
+__device__ __forceinline__ double probability(float q) { return q > 0.f ? (double) q : 0.0; }   // (a NaN: 0)
+// What logits weigh beside the largest of them, `most`, times z: by = 256 log2 e / temp (below 0: the one at `arg`, with certainty)
+struct softmax {
+    double by, z;
+    float most;
+    int arg;
+    __device__ __forceinline__ softmax(double by_, float most_, int arg_, double z_) : by(by_), z(z_), most(most_), arg(arg_) {}
+    // (what is decided once for a row stands outside of its values: f(how) with how(l, j) the weight of value j, l)
+    template <class F> __device__ __forceinline__ void with(const powers & t, F && f) const {
+        const float m = most;
+        const double b = by, c = most, s = z;
+        const int g = arg;
+        if (by < 0.0) f([=](float, int j) { return j == g ? 1.0 : 0.0; });
+        else if (m == MINUS_INF) f([](float, int) { return 0.0; });
+        else if (m == -MINUS_INF) f([=](float l, int) { return l == m ? s : 0.0; });   // (infinite ones share everything)
+        else f([=, &t](float l, int) { return exp2_256(((double) l - c) * b, t) * s; });   // (the difference first: a product with a small temperature rounds by whole powers)
+    }
+};
+// 256 log2 e / temp of a sequence's logits; below 0: the largest one, with certainty
 __device__ __forceinline__ double by_of(const verify_params & P, int seq) {
-    if (!P.temp) return LOG2E_64;
+    if (!P.temp) return LOG2E_256;
     const float t = P.temp[seq];
-    return t > 0.f ? LOG2E_64 / (double) t : -1.0;
+    return t > 0.f ? LOG2E_256 / (double) t : -1.0;
 }
 __device__ __forceinline__ float value_at(const char * p, size_t i, bool bf16) {
     typedef const __attribute__((address_space(1))) uint16_t * g16;
@@ -87,31 +117,48 @@ struct places {
     bool bf16;
     __device__ __forceinline__ int of(int e) const { return bf16 ? j0 + (e >> 3) * (VTHR * 8) + tid * 8 + (e & 7) : j0 + (e >> 2) * (VTHR * 4) + tid * 4 + (e & 3); }
 };
-// Both types leave the values in the order of `at` (that of the target's type)
+// (Both types leave the values in the order of `at`, that of the target's type; `none` behind the row's end. A type is asked for once, not for each value.)
+template <class At> __device__ __forceinline__ void load_each(float (&x)[PER], const char * row, bool bf16, At && at, int V, float none) {
+    auto all = [&](auto type) {
+#pragma unroll
+        for (int e = 0; e < PER; ++e) x[e] = value_at(row, min(at(e), V - 1), type.value);
+    };
+    if (bf16) all(std::true_type{});
+    else all(std::false_type{});
+#pragma unroll
+    for (int e = 0; e < PER; ++e) x[e] = at(e) < V ? x[e] : none;
+}
+template <int N> __device__ __forceinline__ void load_words(float * x, gbytes p, std::true_type) {      // N values of bf16, 8 a load
+#pragma unroll
+    for (int k = 0; k < N / 8; ++k) {
+        const u4 w = gload<u4_a2>(p + 16 * k);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[8 * k + e] = __builtin_bit_cast(float, e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    }
+}
+template <int N> __device__ __forceinline__ void load_words(float * x, gbytes p, std::false_type) {     // of f32, 4 a load
+#pragma unroll
+    for (int k = 0; k < N / 4; ++k) {
+        const u4 w = gload<u4_a4>(p + 16 * k);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { const uint32_t v = w[e]; x[4 * k + e] = __builtin_bit_cast(float, v); }   // (of an element itself the compiler casts the first)
+    }
+}
 __device__ __forceinline__ void load16(float (&x)[PER], const char * row, bool bf16, const places & at, int V, float none) {
-    if (at.j0 + STRETCH <= V && bf16 == at.bf16) {
-        if (bf16) {
+    if (at.j0 + STRETCH > V || bf16 != at.bf16) load_each(x, row, bf16, [&](int e) { return at.of(e); }, V, none);
+    else if (bf16) {
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const u4 w = gload<u4_a2>((gbytes) row + 2 * (size_t) at.of(8 * k));
+        for (int k = 0; k < 2; ++k) load_words<8>(x + 8 * k, (gbytes) row + 2 * (size_t) at.of(8 * k), std::true_type{});
+    } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[8 * k + e] = __builtin_bit_cast(float, e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
-            }
-        } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const u4 w = gload<u4_a4>((gbytes) row + 4 * (size_t) at.of(4 * k));
-#pragma unroll
-                for (int e = 0; e < 4; ++e) { const uint32_t v = w[e]; x[4 * k + e] = __builtin_bit_cast(float, v); }   // (of an element itself the compiler casts the first)
-            }
-        }
-        return;
+        for (int k = 0; k < 4; ++k) load_words<4>(x + 4 * k, (gbytes) row + 4 * (size_t) at.of(4 * k), std::false_type{});
     }
-#pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        const int j = at.of(e);
-        x[e] = j < V ? value_at(row, j, bf16) : none;
-    }
+}
+// the same of values j0 .. on end
+__device__ __forceinline__ void load_run(float (&x)[PER], const char * row, bool bf16, int j0, int V, float none) {
+    if (j0 + PER > V) load_each(x, row, bf16, [&](int e) { return j0 + e; }, V, none);
+    else if (bf16) load_words<PER>(x, (gbytes) row + 2 * (size_t) j0, std::true_type{});
+    else load_words<PER>(x, (gbytes) row + 4 * (size_t) j0, std::false_type{});
 }
 
 // sums over the workgroup, the same in every thread (lanes by an xor butterfly, waves in order)
@@ -148,6 +195,7 @@ __global__ void __launch_bounds__(VTHR) stats_k(const verify_params P) {
     __shared__ float wm[VTHR / 64];
     __shared__ int wi[VTHR / 64];
     __shared__ double ws[VTHR / 64];
+    __shared__ powers pw;
     const int t = blockIdx.x / P.stretches, z = blockIdx.x - t * P.stretches, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     float x[PER];
     const places at{z * STRETCH, tid, P.target_bf16 != 0};
@@ -155,30 +203,37 @@ __global__ void __launch_bounds__(VTHR) stats_k(const verify_params P) {
     const int seq = seq_of_row(P.R, t);
     if (seq < 0) return;
     const double by = by_of(P, seq);
+    fill(pw);
     float m = MINUS_INF;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) m = fmaxf(m, x[e]);         // (NaN: not looked at)
+    m = wave_max(m);
     int arg = INT32_MAX;
+    if (by < 0.0) {                                           // the lowest place of the largest
 #pragma unroll
-    for (int e = 0; e < PER; ++e) if (x[e] > m) { m = x[e]; arg = at.of(e); }      // (a thread's places ascend)
+        for (int e = PER - 1; e >= 0; --e) arg = x[e] == m ? at.of(e) : arg;
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const float om = __shfl_xor(m, d);
-        const int oi = __shfl_xor(arg, d);
-        if (om > m || (om == m && oi < arg)) { m = om; arg = oi; }
+        for (int d = 1; d < 64; d <<= 1) arg = min(arg, __shfl_xor(arg, d));
     }
     if (lane == 0) { wm[wave] = m; wi[wave] = arg; }
     __syncthreads();
     m = wm[0]; arg = wi[0];
 #pragma unroll
-    for (int w = 1; w < VTHR / 64; ++w) if (wm[w] > m || (wm[w] == m && wi[w] < arg)) { m = wm[w]; arg = wi[w]; }
+    for (int w = 1; w < VTHR / 64; ++w) {
+        arg = wm[w] > m ? wi[w] : wm[w] == m ? min(arg, wi[w]) : arg;
+        m = fmaxf(m, wm[w]);
+    }
     double s = 0.0;
     if (by >= 0.0) {
+        softmax(by, m, 0, 1.0).with(pw, [&](auto weight) {
 #pragma unroll
-        for (int e = 0; e < PER; ++e) s += logit_weight(x[e], m, by);
+            for (int e = 0; e < PER; ++e) s += weight(x[e], 0);
+        });
         s = group_sum(s, ws);
     }
     if (tid == 0) {
         const size_t i = (size_t) t * P.stretches + z;
-        P.st_sum[i] = m > MINUS_INF ? s : 0.0;
+        P.st_sum[i] = s;
         P.st_max[i] = m;
         P.st_arg[i] = arg;
     }
@@ -190,326 +245,154 @@ struct tree_lds {
     int token[NODES];
     int state[NODES];
     bool again[NODES];                                        // an elder sibling has the same token
-    int waiting;
+    float most[NODES];                                        // of the nodes' rows: the largest logit, where it is, 1 / the sum
+    int arg[NODES];
+    double z[NODES];
+    int waiting, length;
 };
 
-// p at token x of a row
-__device__ __forceinline__ double target_at(const verify_params & P, int seq, int row, int x) {
-    const float l = value_at(P.target, (size_t) row * P.ld_target + x, P.target_bf16);
-    if (!P.logits) return l > 0.f ? (double) l : 0.0;
-    const double by = by_of(P, seq);
-    if (by < 0.0) return x == P.row_arg[row] ? 1.0 : 0.0;
-    const float most = P.row_max[row];
-    return most > MINUS_INF ? logit_weight(l, most, by) * P.row_z[row] : 0.0;
+// A rejection of the child with the draft's probability q, of `mass`: what a and gone become. False: nothing is left to test another child with
+__device__ __forceinline__ bool reject(const verify_params & P, double mass, double q, double & a, double & gone) {
+    const double rest = 1.0 - gone;
+    if (!(rest > 0.0)) return false;
+    a += mass / rest;
+    if (P.distinct) gone += q;
+    return mass > 0.0 && 1.0 - gone > 0.0;                    // (no mass: nothing changes from here on and nobody is accepted; nothing to draw from: passed over)
 }
-__device__ __forceinline__ double draft_at(const verify_params & P, int row, int x) {
-    const float q = value_at(P.draft, (size_t) row * P.ld_draft + x, P.draft_bf16);
-    return q > 0.f ? (double) q : 0.0;
+__device__ __forceinline__ bool accept(double u, double mass, double p, double q, double a, double gone) { return u * (q / (1.0 - gone)) * mass < fmax(p - a * q, 0.0); }
+
+// f(weight) for a row: weight(l, j) of its value j, l
+template <class F> __device__ __forceinline__ void with_row(const verify_params & P, int seq, int row, const powers & pw, F && f) {
+    if (!P.logits) f([](float l, int) { return probability(l); });
+    else softmax(by_of(P, seq), P.row_max[row], P.row_arg[row], P.row_z[row]).with(pw, f);
 }
 
-// One round for sequence `seq`: nodes that wait have their sums. All threads of the workgroup call.
-__device__ void decide(const verify_params & P, int seq, bool begin, tree_lds & T) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const seq_view v = seq_of<true>(P.R, seq);
-    const int n = min(v.count, NODES);
-    if (n < 1) {
-        if (tid == 0) { P.n_accept[seq] = 0; P.next[seq] = -1; P.last_row[seq] = -1; P.due[seq] = 0; P.here[seq] = 0; }
-        for (int k = tid; k < P.ld_path; k += VTHR) P.path[(size_t) seq * P.ld_path + k] = -1;
-        return;
-    }
-    for (int i = tid; i < n; i += VTHR) {
-        const int x = P.token[v.first + i], p = P.parent ? P.parent[v.first + i] : i - 1;
-        T.token[i] = x;
-        T.up[i] = (int16_t) (i > 0 && p >= 0 && p < i && x >= 0 && x < P.V ? p : -1);
-        T.first[i] = -1;
-        T.state[i] = begin ? NONE : P.node_state[v.first + i];
-    }
-    if (tid == 0) T.waiting = 0;
-    __syncthreads();
-    // (a child's elder siblings: the nearest one's `sibling` it is; how many there are, against max_children)
-    for (int i = tid; i < n; i += VTHR) {
-        const int p = T.up[i];
-        const int x = T.token[i];
-        int elder = -1, k = 0;
-        bool again = false;
-        if (p >= 0)
-            for (int j = p + 1; j < i; ++j) if (T.up[j] == p) { elder = j; ++k; again |= T.token[j] == x; }
-        T.again[i] = again;
-        if (p >= 0 && (!P.draft || k < P.max_children)) {
-            if (elder < 0) T.first[p] = (int16_t) i;
-            else T.sibling[elder] = (int16_t) i;
-        }
-        int younger = -1;                                     // (the last one, or the last that is looked at, has none)
-        if (p >= 0 && (!P.draft || k + 1 < P.max_children))
-            for (int j = i + 1; j < n; ++j) if (T.up[j] == p) { younger = j; break; }
-        if (younger < 0) T.sibling[i] = -1;
-    }
-    __syncthreads();
-    // ---- rows' sums (logits), or sums of what is left at nodes that wait: a wave a row ----
-    for (int i = wave; i < n; i += VTHR / 64) {
-        const int row = v.first + i;
-        if (begin) {
-            if (!P.logits) continue;
-            const size_t at = (size_t) row * P.stretches;
-            float m = MINUS_INF;
-            int arg = INT32_MAX;
-            for (int z = lane; z < P.stretches; z += 64) { const float x = P.st_max[at + z]; if (x > m) { m = x; arg = P.st_arg[at + z]; } }
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const float om = __shfl_xor(m, d);
-                const int oi = __shfl_xor(arg, d);
-                if (om > m || (om == m && oi < arg)) { m = om; arg = oi; }
-            }
-            const double by = by_of(P, seq);
-            double s = 0.0;
-            if (by >= 0.0 && m > MINUS_INF)
-                for (int z = lane; z < P.stretches; z += 64) s += P.st_sum[at + z] * logit_weight(P.st_max[at + z], m, by);
-            s = wave_sum(s);
-            if (lane == 0) {
-                P.row_max[row] = m;
-                P.row_arg[row] = m > MINUS_INF ? arg : -1;
-                P.row_z[row] = s > 0.0 ? 1.0 / s : 0.0;
-            }
-        } else if (T.state[i] == WAITS) {
-            double s = 0.0;
-            for (int z = lane; z < P.stretches; z += 64) s += P.sums[(size_t) row * P.stretches + z];
-            s = wave_sum(s);
-            if (lane == 0) P.sums[(size_t) row * P.stretches] = s;
-        }
-    }
-    __threadfence_block();
-    __syncthreads();
-    // ---- every node tests ----
-    for (int i = tid; i < n; i += VTHR) {
-        const int row = v.first + i;
-        if (!begin && T.state[i] != WAITS) continue;
-        int c = begin ? T.first[i] : P.node_child[row], state = NONE;
-        double a = begin ? 0.0 : P.node_a[row], gone = begin ? 0.0 : P.node_gone[row], mass = begin ? 1.0 : P.sums[(size_t) row * P.stretches];
-        while (c >= 0) {
-            const int x = T.token[c];
-            const double u = (double) P.u[v.first + c], p = target_at(P, seq, row, x);
-            if (P.draft) {
-                const double q = draft_at(P, row, x), rest = 1.0 - gone;
-                const bool any = rest > 0.0;                  // (nothing left to draw from: passed over)
-                if (any && u * (q / rest) * mass < fmax(p - a * q, 0.0)) { state = c; break; }
-                c = T.sibling[c];
-                if (!any) continue;
-                a += mass / rest;
-                if (P.distinct) gone += q;
-                if (c < 0) break;
-                if (mass > 0.0) { state = WAITS; break; }     // (mass 0: nothing changes from here on, nobody is accepted)
-            } else {
-                const double left = T.again[c] ? 0.0 : p;     // (a token that was taken out already)
-                if (u * mass < left) { state = c; break; }
-                mass -= left;
-                c = T.sibling[c];
-            }
-        }
-        T.state[i] = state;
-        P.node_a[row] = a;
-        P.node_gone[row] = gone;
-        P.node_child[row] = c;
-    }
-    __syncthreads();
-    // ---- nodes that wait and can still be reached: every one above lets the walk through, or waits itself and has not tested the child yet ----
-    for (int i = tid; i < n; i += VTHR) {
-        int state = T.state[i];
-        if (state == WAITS) {
-            bool reach = true;
-            int j = i;
-            for (int p = T.up[j]; p >= 0 && reach; j = p, p = T.up[j]) {
-                const int sp = T.state[p];
-                reach = sp == j || (sp == WAITS && j >= P.node_child[v.first + p]);
-            }
-            if (reach && j == 0) atomicAdd(&T.waiting, 1);
-            else state = NONE;                                // (never asked again)
-        }
-        P.node_state[v.first + i] = state;
-    }
-    __syncthreads();
-    const int waiting = T.waiting;
-    __syncthreads();
-    if (tid == 0) {
-        P.due[seq] = waiting * P.stretches;
-        P.here[seq] = 0;
-    }
-    // ---- the walk ----
-    if (waiting == 0) {
-        if (tid == 0) {
-            int at = 0, k = 0;
-            for (int c = T.state[0]; c >= 0; c = T.state[at]) {
-                if (k < P.ld_path) P.path[(size_t) seq * P.ld_path + k] = c;
-                ++k;
-                at = c;
-            }
-            P.n_accept[seq] = k;
-            P.last_row[seq] = v.first + at;
-            P.last_a[seq] = P.node_a[v.first + at];
-            T.waiting = k;
-        }
-        __syncthreads();
-        for (int k = T.waiting + tid; k < P.ld_path; k += VTHR) P.path[(size_t) seq * P.ld_path + k] = -1;
-    }
-}
-
-__global__ void __launch_bounds__(VTHR) decide_k(const verify_params P) {
-    __shared__ tree_lds T;
-    decide(P, blockIdx.x, true, T);
-}
-
-// what the values of a row weigh
-struct row_of {
-    bool logits, certain;
-    float most;
-    int arg;
-    double by, z;
-    __device__ __forceinline__ row_of(const verify_params & P, int seq, int row) {
-        logits = P.logits;
-        by = logits ? by_of(P, seq) : 0.0;
-        certain = logits && by < 0.0;
-        most = logits ? P.row_max[row] : 0.f;
-        arg = logits ? P.row_arg[row] : -1;
-        z = logits ? P.row_z[row] : 1.0;
-    }
-    __device__ __forceinline__ double weight(float l, int j) const {
-        if (!logits) return l > 0.f ? (double) l : 0.0;
-        if (certain) return j == arg ? 1.0 : 0.0;
-        return most > MINUS_INF ? logit_weight(l, most, by) * z : 0.0;
-    }
+// ---- the last row of a sequence ----
+struct last_lds {
+    double ws[VTHR / 64], scan[VTHR];
+    uint32_t out[STRETCH / 32];                               // values of a stretch that are taken out
+    uint32_t touched[256 / 32];                               // stretches that have some
+    int last, found;
 };
-
-// true in the workgroup that comes last of `due` for the sequence; what the others wrote is there for it
-__device__ __forceinline__ bool comes_last(int * here, int due, int * lds) {
-    if (threadIdx.x == 0) {
-        __threadfence();
-        const int was = atomicAdd(here, 1);
-        __threadfence();
-        *lds = was == due - 1;
+// without a draft every child of the last node was rejected: f(token) for each
+template <class F> __device__ __forceinline__ void rejected(const verify_params & P, const seq_view & v, int me, F && f) {
+    if (P.draft) return;
+    for (int i = me + 1 + (int) threadIdx.x; i < min(v.count, NODES); i += VTHR) {
+        const int x = P.token[v.first + i];
+        if (x >= 0 && x < P.V && (P.parent ? P.parent[v.first + i] : i - 1) == me) f(x);
     }
-    __syncthreads();
-    return *lds != 0;
 }
-
-__global__ void __launch_bounds__(VTHR) sums_k(const verify_params P) {
-    __shared__ tree_lds T;
-    __shared__ double ws[VTHR / 64];
-    __shared__ int last;
-    const int t = blockIdx.x / P.stretches, z = blockIdx.x - t * P.stretches, tid = threadIdx.x;
-    const int seq = seq_of_row(P.R, t);
-    if (seq < 0 || P.node_state[t] != WAITS) return;
-    const double a = P.node_a[t];
-    const row_of row(P, seq, t);
+__device__ __forceinline__ void take_out(const verify_params & P, const seq_view & v, int me, int j0, last_lds & T) {
+    for (int i = threadIdx.x; i < STRETCH / 32; i += VTHR) T.out[i] = 0;
+    __syncthreads();
+    rejected(P, v, me, [&](int x) { if (x >= j0 && x < j0 + STRETCH) atomicOr(&T.out[(x - j0) >> 5], 1u << ((x - j0) & 31)); });
+    __syncthreads();
+}
+// what is left of a stretch (some), or all of it
+__device__ __forceinline__ double sum_of(const verify_params & P, int seq, const seq_view & v, int t, double a, int z, bool some, const powers & pw, last_lds & T) {
     float x[PER], y[PER];
-    const places at{z * STRETCH, tid, P.target_bf16 != 0};
+    const places at{z * STRETCH, (int) threadIdx.x, P.target_bf16 != 0};
+    const bool draft = some && P.draft && a > 0.0;
     load16(x, P.target + (size_t) t * P.ld_target * (P.target_bf16 ? 2 : 4), P.target_bf16, at, P.V, MINUS_INF);
-    load16(y, P.draft + (size_t) t * P.ld_draft * (P.draft_bf16 ? 2 : 4), P.draft_bf16, at, P.V, 0.f);
+    if (draft) load16(y, P.draft + (size_t) t * P.ld_draft * (P.draft_bf16 ? 2 : 4), P.draft_bf16, at, P.V, 0.f);
+    if (some && !P.draft) take_out(P, v, t - v.first, z * STRETCH, T);
     double s = 0.0;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) s += fmax(row.weight(x[e], at.of(e)) - a * (y[e] > 0.f ? (double) y[e] : 0.0), 0.0);
-    s = group_sum(s, ws);
-    if (tid == 0) P.sums[(size_t) t * P.stretches + z] = s;
-    if (comes_last(P.here + seq, P.due[seq], &last)) decide(P, seq, false, T);
-}
-
-__global__ void __launch_bounds__(VTHR) pick_k(const verify_params P) {
-    __shared__ double ws[VTHR / 64];
-    __shared__ double scan[VTHR];
-    __shared__ uint32_t out[STRETCH / 32];                    // values of a stretch that are taken out
-    __shared__ int last, found;
-    const int seq = blockIdx.x / P.stretches, z = blockIdx.x - seq * P.stretches, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int t = P.last_row[seq];
-    if (t < 0) return;
-    const double a = P.last_a[seq];
-    const seq_view v = seq_of<true>(P.R, seq);
-    const int n = min(v.count, NODES), me = t - v.first;
-    const row_of row(P, seq, t);
-    const bool draft = P.draft && a > 0.0;
-    // (without a draft every child of the last node was rejected)
-    auto take_out = [&](int j0) {
-        for (int i = tid; i < STRETCH / 32; i += VTHR) out[i] = 0;
-        __syncthreads();
-        if (!P.draft)
-            for (int i = me + 1 + tid; i < n; i += VTHR) {
-                const int x = P.token[v.first + i] - j0;
-                if (x >= 0 && x < STRETCH && (P.parent ? P.parent[v.first + i] : i - 1) == me) atomicOr(&out[x >> 5], 1u << (x & 31));
-            }
-        __syncthreads();
-    };
-    take_out(z * STRETCH);
-    const char * const tr = P.target + (size_t) t * P.ld_target * (P.target_bf16 ? 2 : 4), * const dr = P.draft + (size_t) t * P.ld_draft * (P.draft_bf16 ? 2 : 4);
-    {
-        float x[PER], y[PER];
-        const places at{z * STRETCH, tid, P.target_bf16 != 0};
-        load16(x, tr, P.target_bf16, at, P.V, MINUS_INF);
-        if (draft) load16(y, dr, P.draft_bf16, at, P.V, 0.f);
-        double left = 0.0, all = 0.0;
+    with_row(P, seq, t, pw, [&](auto weight) {
 #pragma unroll
         for (int e = 0; e < PER; ++e) {
             const int j = at.of(e), i = j - z * STRETCH;
-            const double p = row.weight(x[e], j);
-            all += p;
-            left += draft ? fmax(p - a * (y[e] > 0.f ? (double) y[e] : 0.0), 0.0) : out[i >> 5] >> (i & 31) & 1 ? 0.0 : p;
+            const double p = weight(x[e], j);
+            s += draft ? fmax(p - a * probability(y[e]), 0.0) : some && !P.draft && (T.out[i >> 5] >> (i & 31) & 1) ? 0.0 : p;
         }
-        left = group_sum(left, ws);
-        all = group_sum(all, ws);
-        if (tid == 0) {
-            double * const to = P.sums + 2 * ((size_t) seq * P.stretches + z);
-            to[0] = left;
-            to[1] = all;
-        }
-    }
-    if (!comes_last(P.here + seq, P.stretches, &last)) return;
+    });
+    return group_sum(s, T.ws);
+}
+
+__global__ void __launch_bounds__(VTHR) left_k(const verify_params P) {
+    __shared__ powers pw;
+    __shared__ last_lds T;
+    const int seq = blockIdx.x / P.stretches, z = blockIdx.x - seq * P.stretches;
+    const int t = P.last_row[seq];
+    if (t < 0) return;
+    if (P.logits) fill(pw);
+    const double s = sum_of(P, seq, seq_of<true>(P.R, seq), t, P.last_a[seq], z, true, pw, T);
+    if (threadIdx.x == 0) P.sums[0][(size_t) seq * P.stretches + z] = s;
+}
+
+// The token behind the last node's row t. known: the sums of its stretches are in sums[0]; otherwise (logits, no draft) in st_sum, but for those that something is taken out of
+__device__ __forceinline__ void pick(const verify_params & P, int seq, const seq_view & v, int t, double a, bool known, const powers & pw, last_lds & T) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // ---- the stretch: one a thread (there are 256 at most) ----
-    const double * const from = P.sums + 2 * (size_t) seq * P.stretches;
-    const double mine = tid < P.stretches ? from[2 * tid] : 0.0, whole = tid < P.stretches ? from[2 * tid + 1] : 0.0;
-    const bool some = group_sum(mine, ws) > 0.0;              // (nothing left: from p)
+    double mine = 0.0;
+    if (known) mine = tid < P.stretches ? P.sums[0][(size_t) seq * P.stretches + tid] : 0.0;
+    else {
+        const double by = by_of(P, seq);
+        const size_t at = (size_t) t * P.stretches;
+        if (tid < P.stretches) {
+            if (by < 0.0) mine = P.row_arg[t] >= 0 && P.row_arg[t] / STRETCH == tid ? 1.0 : 0.0;
+            else softmax(by, P.row_max[t], 0, P.row_z[t]).with(pw, [&](auto weight) { mine = P.st_sum[at + tid] * weight(P.st_max[at + tid], 0); });
+        }
+        if (tid < 256 / 32) T.touched[tid] = 0;
+        __syncthreads();
+        rejected(P, v, t - v.first, [&](int x) { atomicOr(&T.touched[(x / STRETCH) >> 5], 1u << (x / STRETCH & 31)); });
+        __syncthreads();
+        for (int w = 0; w < 256 / 32; ++w)
+            for (uint32_t bits = T.touched[w]; bits; bits &= bits - 1) {
+                const int z = 32 * w + __builtin_ctz(bits);
+                const double s = sum_of(P, seq, v, t, a, z, true, pw, T);
+                if (tid == z) mine = s;
+            }
+    }
+    bool some = group_sum(mine, T.ws) > 0.0;
+    if (!some)                                                // nothing left: from p
+        for (int z = 0; z < P.stretches; ++z) {
+            const double s = sum_of(P, seq, v, t, a, z, false, pw, T);
+            if (tid == z) mine = s;
+        }
     auto running = [&](double x) {                            // sums over the threads up to this one
         __syncthreads();
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) { const double y = __shfl_up(x, d); if (lane >= d) x += y; }
-        if (lane == 63) ws[wave] = x;
+        if (lane == 63) T.ws[wave] = x;
         __syncthreads();
-        for (int w = 0; w < wave; ++w) x += ws[w];
+        for (int w = 0; w < wave; ++w) x += T.ws[w];
         return x;
     };
-    const double w = some ? mine : whole, upto = running(w);
-    scan[tid] = upto;
-    if (tid == 0) found = INT32_MAX;
+    const double upto = running(mine), u = (double) P.u_next[seq];
+    T.scan[tid] = upto;
+    if (tid == 0) { T.found = INT32_MAX; T.last = -1; }
     __syncthreads();
-    const double total = scan[VTHR - 1];
+    const double total = T.scan[VTHR - 1], goal = u * total;
     if (!(total > 0.0)) {
         if (tid == 0) P.next[seq] = -1;
         return;
     }
-    const double goal = (double) P.u_next[seq] * total;
-    if (upto > goal && w > 0.0) atomicMin(&found, tid);
-    __syncthreads();
-    if (found == INT32_MAX) {                                 // (u of 1 and above: the last that weighs anything)
-        __syncthreads();
-        if (tid == 0) found = -1;
-        __syncthreads();
-        if (w > 0.0) atomicMax(&found, tid);
-        __syncthreads();
+    if (mine > 0.0) {
+        if (upto > goal) atomicMin(&T.found, tid);
+        atomicMax(&T.last, tid);
     }
-    const int zf = found;
-    const double before = zf ? scan[zf - 1] : 0.0;
     __syncthreads();
-    take_out(zf * STRETCH);
+    const int zf = T.found != INT32_MAX ? T.found : T.last;   // (u of 1 and above: the last that weighs anything)
+    const double before = zf ? T.scan[zf - 1] : 0.0;
     // ---- the value: 16 on end a thread ----
+    const bool draft = some && P.draft && a > 0.0;
+    float x[PER], y[PER];
+    load_run(x, P.target + (size_t) t * P.ld_target * (P.target_bf16 ? 2 : 4), P.target_bf16, zf * STRETCH + tid * PER, P.V, MINUS_INF);
+    if (draft) load_run(y, P.draft + (size_t) t * P.ld_draft * (P.draft_bf16 ? 2 : 4), P.draft_bf16, zf * STRETCH + tid * PER, P.V, 0.f);
+    take_out(P, v, t - v.first, zf * STRETCH, T);
     double p[PER], sum = 0.0;
+    with_row(P, seq, t, pw, [&](auto weight) {
 #pragma unroll
-    for (int e = 0; e < PER; ++e) {
-        const int i = tid * PER + e, j = zf * STRETCH + i;
-        p[e] = 0.0;
-        if (j < P.V) {
-            p[e] = row.weight(value_at(tr, j, P.target_bf16), j);
-            if (some && draft) { const float q = value_at(dr, j, P.draft_bf16); p[e] = fmax(p[e] - a * (q > 0.f ? (double) q : 0.0), 0.0); }
-            else if (some && (out[i >> 5] >> (i & 31) & 1)) p[e] = 0.0;
+        for (int e = 0; e < PER; ++e) {
+            const int i = tid * PER + e;
+            p[e] = weight(x[e], zf * STRETCH + i);
+            if (draft) p[e] = fmax(p[e] - a * probability(y[e]), 0.0);
+            else if (some && (T.out[i >> 5] >> (i & 31) & 1)) p[e] = 0.0;
+            sum += p[e];
         }
-        sum += p[e];
-    }
+    });
     double at = before + running(sum) - sum;
-    if (tid == 0) { found = INT32_MAX; last = -1; }
+    if (tid == 0) { T.found = INT32_MAX; T.last = -1; }
     __syncthreads();
     int pass = INT32_MAX, any = -1;
 #pragma unroll
@@ -520,15 +403,235 @@ __global__ void __launch_bounds__(VTHR) pick_k(const verify_params P) {
             if (at > goal) pass = min(pass, any);
         }
     }
-    if (pass != INT32_MAX) atomicMin(&found, pass);
-    if (any >= 0) atomicMax(&last, any);
+    if (pass != INT32_MAX) atomicMin(&T.found, pass);
+    if (any >= 0) atomicMax(&T.last, any);
     __syncthreads();
-    if (tid == 0) P.next[seq] = found != INT32_MAX ? found : last;   // (the stretch's own sum rounded above this one: its last)
+    if (tid == 0) P.next[seq] = T.found != INT32_MAX ? T.found : T.last;   // (the stretch's own sum rounded above this one: its last)
+}
+__global__ void __launch_bounds__(VTHR) pick_k(const verify_params P) {
+    __shared__ powers pw;
+    __shared__ last_lds T;
+    const int seq = blockIdx.x, t = P.last_row[seq];
+    if (t < 0) return;
+    if (P.logits) fill(pw);
+    pick(P, seq, seq_of<true>(P.R, seq), t, P.last_a[seq], true, pw, T);
+}
+
+// round: -1 at first; or the round whose sums are to be taken. walk: the path is known behind this one; and_pick: and so are the sums of all rows
+__global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int round, bool walk, bool and_pick) {
+    __shared__ tree_lds T;
+    __shared__ last_lds U;
+    __shared__ powers pw;
+    const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const seq_view v = seq_of<true>(P.R, seq);
+    const int n = min(v.count, NODES);
+    if (n < 1) {
+        if (tid == 0) { P.n_accept[seq] = 0; P.next[seq] = -1; P.last_row[seq] = -1; P.n_waiting[seq] = 0; }
+        for (int k = tid; k < P.ld_path; k += VTHR) P.path[(size_t) seq * P.ld_path + k] = -1;
+        return;
+    }
+    if (P.logits) fill(pw);
+    if (round < 0) {
+        const double by = P.logits ? by_of(P, seq) : 0.0;
+        for (int i = tid; i < n; i += VTHR) {
+            const int x = P.token[v.first + i], p = P.parent ? P.parent[v.first + i] : i - 1;
+            T.token[i] = x;
+            T.up[i] = (int16_t) (i > 0 && p >= 0 && p < i && x >= 0 && x < P.V ? p : -1);
+            T.first[i] = -1;
+        }
+        if (tid == 0) T.waiting = 0;
+        __syncthreads();
+        // ---- a thread a node: what its row and its parent's hold of its token; its elder siblings ----
+        for (int i = tid; i < n; i += VTHR) {
+            const int p = T.up[i], x = T.token[i];
+            int elder = -1, k = 0, younger = -1;
+            bool again = false;
+            if (p >= 0) {
+                for (int j = p + 1; j < i; ++j) if (T.up[j] == p) { elder = j; ++k; again |= T.token[j] == x; }
+                if (!P.draft || k + 1 < P.max_children)       // (the last one, or the last that is looked at, has none)
+                    for (int j = i + 1; j < n; ++j) if (T.up[j] == p) { younger = j; break; }
+                if (elder < 0) T.first[p] = (int16_t) i;
+            }
+            T.again[i] = again;
+            T.sibling[i] = (int16_t) younger;
+            P.sibling[v.first + i] = (int16_t) younger;
+        }
+        // ---- logits: a wave a row: the sum of its stretches ----
+        if (P.logits)
+            for (int i = wave; i < n; i += VTHR / 64) {
+                const size_t at = (size_t) (v.first + i) * P.stretches;
+                float m = MINUS_INF;
+                int arg = INT32_MAX;
+                for (int z = lane; z < P.stretches; z += 64) { const float x = P.st_max[at + z]; if (x > m) { m = x; arg = P.st_arg[at + z]; } }
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) {
+                    const float om = __shfl_xor(m, d);
+                    const int oi = __shfl_xor(arg, d);
+                    if (om > m || (om == m && oi < arg)) { m = om; arg = oi; }
+                }
+                double s = 0.0;
+                if (by >= 0.0 && m > MINUS_INF)
+                    for (int z = lane; z < P.stretches; z += 64) { double w = 0.0; softmax(by, m, 0, 1.0).with(pw, [&](auto weight) { w = weight(P.st_max[at + z], 0); }); s += P.st_sum[at + z] * w; }
+                s = wave_sum(s);
+                if (lane == 0) {
+                    T.most[i] = P.row_max[v.first + i] = m;
+                    T.arg[i] = P.row_arg[v.first + i] = m > MINUS_INF ? arg : -1;
+                    T.z[i] = P.row_z[v.first + i] = s > 0.0 ? 1.0 / s : 0.0;
+                }
+            }
+        __syncthreads();
+        // ---- every node tests ----
+        for (int i = tid; i < n; i += VTHR) {
+            const int row = v.first + i;
+            int c = T.first[i], state = NONE;
+            double a = 0.0, gone = 0.0, mass = 1.0;
+            while (c >= 0) {
+                const int x = T.token[c];
+                const double u = (double) P.u[v.first + c];
+                const float l = value_at(P.target, (size_t) row * P.ld_target + x, P.target_bf16);
+                double p = probability(l);
+                if (P.logits) softmax(by, T.most[i], T.arg[i], T.z[i]).with(pw, [&](auto weight) { p = weight(l, x); });
+                if (P.draft) {
+                    const double q = probability(value_at(P.draft, (size_t) row * P.ld_draft + x, P.draft_bf16));
+                    if (accept(u, 1.0, p, q, 0.0, 0.0)) { state = c; break; }
+                    c = T.sibling[c];
+                    if (reject(P, 1.0, q, a, gone) && c >= 0) state = WAITS;
+                    break;
+                }
+                const double left = T.again[c] ? 0.0 : p;     // (a token that was taken out already)
+                if (u * mass < left) { state = c; break; }
+                mass -= left;
+                c = T.sibling[c];
+            }
+            T.state[i] = state;
+            P.node_a[0][row] = a;
+            P.node_gone[0][row] = gone;
+            P.node_child[0][row] = T.first[i] = (int16_t) c;
+            P.node_state[0][row] = state;
+        }
+        __syncthreads();
+        // ---- nodes that wait and can still be reached: every one above lets the walk through, or waits itself and has not tested the child yet ----
+        for (int i = tid; i < n; i += VTHR) {
+            if (T.state[i] != WAITS) continue;
+            bool reach = true;
+            int j = i;
+            for (int p = T.up[j]; p >= 0 && reach; j = p, p = T.up[j]) {
+                const int sp = T.state[p];
+                reach = sp == j || (sp == WAITS && j >= T.first[p]);
+            }
+            if (reach && j == 0) P.waiting[v.first + atomicAdd(&T.waiting, 1)] = i;   // (in any order: each has its own sums)
+        }
+        __syncthreads();
+        if (tid == 0) P.n_waiting[seq] = T.waiting;
+    } else {
+        const int in = round & 1;
+        for (int i = tid; i < n; i += VTHR) T.state[i] = P.node_state[0][v.first + i];
+        __syncthreads();
+        // ---- nodes that waited: a wave each, with the last round's sum ----
+        const int m = P.n_waiting[seq];
+        for (int w = wave; w < m; w += VTHR / 64) {
+            const int i = P.waiting[v.first + w], row = v.first + i;
+            int state = P.node_state[in][row];
+            double a = P.node_a[in][row];
+            if (state == WAITS) {
+                double mass = 0.0;
+                for (int z = lane; z < P.stretches; z += 64) mass += P.sums[in][(size_t) row * P.stretches + z];
+                mass = wave_sum(mass);
+                const int c = P.node_child[in][row], x = P.token[v.first + c];
+                double gone = P.node_gone[in][row];
+                double p = 0.0;
+                with_row(P, seq, row, pw, [&](auto weight) { p = weight(value_at(P.target, (size_t) row * P.ld_target + x, P.target_bf16), x); });
+                const double q = probability(value_at(P.draft, (size_t) row * P.ld_draft + x, P.draft_bf16));
+                if (accept((double) P.u[v.first + c], mass, p, q, a, gone)) state = c;
+                else {
+                    reject(P, mass, q, a, gone);
+                    state = NONE;
+                }
+            }
+            if (lane == 0) {
+                T.state[i] = state;
+                P.node_a[0][row] = a;
+            }
+        }
+        __threadfence_block();
+        __syncthreads();
+    }
+    if (!walk) return;
+    // ---- the walk ----
+    if (tid == 0) {
+        int at = 0, k = 0;
+        for (int c = T.state[0]; c >= 0; c = T.state[at]) {
+            if (k < P.ld_path) P.path[(size_t) seq * P.ld_path + k] = c;
+            ++k;
+            at = c;
+        }
+        P.n_accept[seq] = k;
+        P.last_row[seq] = v.first + at;
+        P.last_a[seq] = P.node_a[0][v.first + at];
+        T.length = k;
+        T.waiting = at;
+    }
+    __syncthreads();
+    for (int k = T.length + tid; k < P.ld_path; k += VTHR) P.path[(size_t) seq * P.ld_path + k] = -1;
+    if (and_pick) pick(P, seq, v, v.first + T.waiting, 0.0, false, pw, U);
+}
+
+// Round k: a node that waits takes the sum of round k - 1 and tests its child with it (every workgroup of the node does, the first writes it down); if that is rejected and there is
+// another one, the sum of what is left now. SLOTS nodes of a sequence at a time.
+constexpr int SLOTS = 4;
+__global__ void __launch_bounds__(VTHR) sums_k(const verify_params P, int k) {
+    __shared__ double ws[VTHR / 64];
+    __shared__ powers pw;
+    const int z = blockIdx.x % P.stretches, b = blockIdx.x / P.stretches, slot = b % SLOTS, seq = b / SLOTS, tid = threadIdx.x, lane = tid & 63;
+    const int m = P.n_waiting[seq];
+    if (slot >= m) return;
+    const int in = k & 1, first = seq_of<true>(P.R, seq).first;
+    if (P.logits) fill(pw);
+    for (int w = slot; w < m; w += SLOTS) {
+        const int t = first + P.waiting[first + w];
+        int state = P.node_state[in][t], c = P.node_child[in][t];
+        double a = P.node_a[in][t], gone = P.node_gone[in][t];
+        float x[PER], y[PER];
+        const places at{z * STRETCH, tid, P.target_bf16 != 0};
+        if (state == WAITS) {
+            load16(x, P.target + (size_t) t * P.ld_target * (P.target_bf16 ? 2 : 4), P.target_bf16, at, P.V, MINUS_INF);
+            load16(y, P.draft + (size_t) t * P.ld_draft * (P.draft_bf16 ? 2 : 4), P.draft_bf16, at, P.V, 0.f);
+            if (k) {
+                double mass = 0.0;                            // (every wave for itself, all alike)
+                for (int i = lane; i < P.stretches; i += 64) mass += P.sums[in][(size_t) t * P.stretches + i];
+                mass = wave_sum(mass);
+                const int token = P.token[first + c];
+                const float l = value_at(P.target, (size_t) t * P.ld_target + token, P.target_bf16);
+                const double q = probability(value_at(P.draft, (size_t) t * P.ld_draft + token, P.draft_bf16));
+                double p = 0.0;
+                with_row(P, seq, t, pw, [&](auto weight) { p = weight(l, token); });
+                if (accept((double) P.u[first + c], mass, p, q, a, gone)) state = c;
+                else {
+                    c = P.sibling[first + c];
+                    if (!reject(P, mass, q, a, gone) || c < 0) state = NONE;
+                }
+            }
+        }
+        if (z == 0 && tid == 0) {
+            P.node_state[in ^ 1][t] = state;
+            P.node_child[in ^ 1][t] = c;
+            P.node_a[in ^ 1][t] = a;
+            P.node_gone[in ^ 1][t] = gone;
+        }
+        if (state != WAITS) continue;
+        double s = 0.0;
+        with_row(P, seq, t, pw, [&](auto weight) {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) s += fmax(weight(x[e], at.of(e)) - a * probability(y[e]), 0.0);
+        });
+        s = group_sum(s, ws);
+        if (tid == 0) P.sums[in ^ 1][(size_t) t * P.stretches + z] = s;
+    }
 }
 
 }   // namespace
 
-verify_plan plan_verify(const rows_view & R, int V, bool logits) {
+verify_plan plan_verify(const rows_view & R, int V, bool logits, bool draft) {
     verify_plan pl{};
     pl.stretches = std::max((V + STRETCH - 1) / STRETCH, 1);
     const size_t T = R.T, S = R.n_seq, z = pl.stretches;
@@ -540,21 +643,21 @@ verify_plan plan_verify(const rows_view & R, int V, bool logits) {
     put(3, T * 8);
     put(4, T * 4);
     put(5, T * 4);
-    put(6, T * 8);
-    put(7, T * 8);
-    put(8, T * 4);
-    put(9, T * 4);
-    put(10, std::max(T, 2 * S) * z * 8);
-    put(11, S * 4);
-    put(12, S * 4);
-    put(13, S * 4);
-    put(14, S * 8);
+    for (int i = 6; i < 10; ++i) put(i, T * 8);               // node_a, node_gone
+    for (int i = 10; i < 14; ++i) put(i, T * 4);              // node_child, node_state
+    put(14, std::max(draft ? T : 0, S) * z * 8);          // sums
+    put(15, draft ? T * z * 8 : 0);
+    put(16, T * 2);
+    put(17, T * 4);
+    put(18, S * 4);
+    put(19, S * 4);
+    put(20, S * 8);
     pl.bytes = at;
     return pl;
 }
 
 int launch_verify(const verify_args & a, hipStream_t s) {
-    const verify_plan pl = plan_verify(a.R, a.V, a.logits);
+    const verify_plan pl = plan_verify(a.R, a.V, a.logits, a.draft != nullptr);
     char * at = (char *) a.scratch;
     if (!at || ((uintptr_t) at & 255) || a.scratch_bytes < pl.bytes) {
         float * big, * small;
@@ -569,14 +672,23 @@ int launch_verify(const verify_args & a, hipStream_t s) {
     P.target_bf16 = a.target_bf16; P.draft_bf16 = a.draft_bf16; P.logits = a.logits; P.distinct = a.distinct;
     P.st_sum = (double *) (at + pl.at[0]); P.st_max = (float *) (at + pl.at[1]); P.st_arg = (int *) (at + pl.at[2]);
     P.row_z = (double *) (at + pl.at[3]); P.row_max = (float *) (at + pl.at[4]); P.row_arg = (int *) (at + pl.at[5]);
-    P.node_a = (double *) (at + pl.at[6]); P.node_gone = (double *) (at + pl.at[7]); P.node_child = (int *) (at + pl.at[8]); P.node_state = (int *) (at + pl.at[9]);
-    P.sums = (double *) (at + pl.at[10]); P.due = (int *) (at + pl.at[11]); P.here = (int *) (at + pl.at[12]); P.last_row = (int *) (at + pl.at[13]); P.last_a = (double *) (at + pl.at[14]);
-    const unsigned rows = (unsigned) a.R.T * (unsigned) pl.stretches;
-    if (a.logits && a.R.T) stats_k<<<rows, VTHR, 0, s>>>(P);
-    decide_k<<<a.R.n_seq, VTHR, 0, s>>>(P);
-    if (a.draft && a.R.T)
-        for (int k = 1; k < std::min(P.max_children, a.R.max_rows - 1); ++k) sums_k<<<rows, VTHR, 0, s>>>(P);
-    if (a.R.T) pick_k<<<(unsigned) a.R.n_seq * pl.stretches, VTHR, 0, s>>>(P);
+    for (int i = 0; i < 2; ++i) {
+        P.node_a[i] = (double *) (at + pl.at[6 + i]); P.node_gone[i] = (double *) (at + pl.at[8 + i]);
+        P.node_child[i] = (int *) (at + pl.at[10 + i]); P.node_state[i] = (int *) (at + pl.at[12 + i]);
+        P.sums[i] = (double *) (at + pl.at[14 + i]);
+    }
+    P.sibling = (int16_t *) (at + pl.at[16]); P.waiting = (int *) (at + pl.at[17]); P.n_waiting = (int *) (at + pl.at[18]); P.last_row = (int *) (at + pl.at[19]); P.last_a = (double *) (at + pl.at[20]);
+    // rounds: children behind the first that a node may have
+    const int rounds = a.draft ? std::max(std::min(P.max_children, a.R.max_rows - 1) - 1, 0) : 0;
+    if (a.logits && a.R.T) stats_k<<<(unsigned) a.R.T * (unsigned) pl.stretches, VTHR, 0, s>>>(P);
+    const bool at_once = a.logits && !a.draft;                // (stats_k has summed every row, and a rejection takes one value out)
+    decide_k<<<a.R.n_seq, VTHR, 0, s>>>(P, -1, rounds == 0, at_once);
+    for (int k = 0; k < rounds; ++k) sums_k<<<(unsigned) a.R.n_seq * SLOTS * pl.stretches, VTHR, 0, s>>>(P, k);
+    if (rounds) decide_k<<<a.R.n_seq, VTHR, 0, s>>>(P, rounds, true, false);
+    if (a.R.T && !at_once) {
+        left_k<<<(unsigned) a.R.n_seq * pl.stretches, VTHR, 0, s>>>(P);
+        pick_k<<<a.R.n_seq, VTHR, 0, s>>>(P);
+    }
     return launched();
 }
 
