@@ -40,21 +40,25 @@ struct tree_params : chunk_params {
 // tiles and q and to write its results (24 sequences of 3 ... 64 nodes over 500 ... 8000 keys: workgroups with many short groups were still at work for 34 us when half of all had ended)
 template <int BN, int TPS, int BC, int WAVES, int SETUP_> struct tree_runs {
     static constexpr int SETUP = SETUP_;
-    struct of_lane { int first, pos0, table, rows, per_group, steps; };
+    // (shape: rows, up to P1A_TREE_NODES, and groups in one register - lanes keep all of this while they work)
+    struct of_lane {
+        int first, pos0, table, shape, per_group;
+        __device__ __forceinline__ int steps() const { return per_group * (shape >> 11); }
+    };
+    static_assert(P1A_TREE_NODES < 1 << 11);
     of_lane first64;
     int first, end, per;
     static __device__ __forceinline__ span span_of_rows(const rows_view & R, const seq_view & v) { return span_of<BN>(R, v.pos0, v.pos0 + v.count - 1); }
     static __device__ __forceinline__ of_lane look(const rows_view & R, const kv_view & pg, int GQA, int s) {
-        of_lane r{0, 0, 0, 0, 0, 0};
+        of_lane r{0, 0, 0, 0, 0};
         if (s >= R.n_seq) return r;
         const seq_view v = seq_of(R, s);
         r.table = pg.pt && pg.rtab ? pg.rtab[s] : 0;
         r.first = v.first;
         r.pos0 = v.pos0;
-        r.rows = v.count;
         if (v.count > 0) {
             r.per_group = SETUP + max((span_of_rows(R, v).nt + TPS - 1) / TPS, 1);
-            r.steps = r.per_group * groups_of(v.count, GQA, BC, WAVES).groups;
+            r.shape = v.count | groups_of(v.count, GQA, BC, WAVES).groups << 11;
         }
         return r;
     }
@@ -65,7 +69,7 @@ template <int BN, int TPS, int BC, int WAVES, int SETUP_> struct tree_runs {
         int n = 0, most = 0;
         for (int s0 = 0; s0 < R.n_seq; s0 += 64) {
             const of_lane x = s0 ? look(R, pg, GQA, s0 + lane) : first64;
-            n += __builtin_amdgcn_readlane(lanes_up_to(x.steps), 63);
+            n += __builtin_amdgcn_readlane(lanes_up_to(x.steps()), 63);
             most = max(most, x.per_group);
         }
         most = rfl((int) wave_max((float) most));             // (a group has 2^25 steps at most: the f32 next to it, 1 off in 2^24, only moves the cut)
@@ -86,17 +90,17 @@ template <int BN, int TPS, int BC, int WAVES, int SETUP_> struct tree_runs {
         int base = 0;
         for (int s0 = 0; s0 < R.n_seq; s0 += 64) {
             const of_lane x = s0 ? look(R, pg, GQA, s0 + lane) : first64;
-            const int u = base + lanes_up_to(x.steps);
+            const int u = base + lanes_up_to(x.steps());
             const unsigned long long behind = __ballot(u > at);
             if (behind) {
                 const int l = __builtin_ctzll(behind);
                 f.seq = s0 + l;
                 f.steps = __builtin_amdgcn_readlane(x.per_group, l);
-                const int start = __builtin_amdgcn_readlane(u, l) - __builtin_amdgcn_readlane(x.steps, l);
+                const int shape = __builtin_amdgcn_readlane(x.shape, l), start = __builtin_amdgcn_readlane(u, l) - f.steps * (shape >> 11);
                 f.group = (at - start) / f.steps;
                 f.first = start + f.group * f.steps;
                 f.v.first = __builtin_amdgcn_readlane(x.first, l);
-                f.v.count = __builtin_amdgcn_readlane(x.rows, l);
+                f.v.count = shape & 2047;
                 f.v.pos0 = __builtin_amdgcn_readlane(x.pos0, l);
                 f.table = __builtin_amdgcn_readlane(x.table, l);
                 return true;
@@ -592,7 +596,8 @@ template <uint32_t KT, int D, bool EXACT> struct team_cfg {
     static constexpr int NPL = group_planes(KT, EXACT), BN = 32, NG = BN / 16, G_B = NPL * plane_bytes(D), T_B = NG * G_B;   // T_B: K or V of a tile
     // Tiles are asked for four steps ahead. f16 goes to LDS by itself: places for four; the others wait in registers, two deep, and LDS holds two
     static constexpr int PLACES = F16 ? 4 : 2;
-    static constexpr int LDS = 2 * PLACES * T_B;
+    static constexpr int PAST = 2 * PLACES * T_B;             // (behind the tiles: what the lanes know of the sequences)
+    static constexpr int LDS = PAST + 64 * sizeof(typename tree_runs<BN, 1, 32, NW, 6>::of_lane);
     static constexpr int WGS = D <= 128 ? 2 : 1;
 };
 
@@ -665,7 +670,12 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     steps.first = 0;
     steps.end = 1;
     steps.per = 1 << 30;
-    if (P0.nks > 1 && !steps.begin(P0.R, P0.pg, P0.GQA, run, runs, P0.nks)) return;
+    auto * const seqs = (typename runs_t::of_lane *) (lds + C::PAST);
+    if (P0.nks > 1) {
+        if (!steps.begin(P0.R, P0.pg, P0.GQA, run, runs, P0.nks)) return;
+        if (wave == 0) seqs[threadIdx.x] = steps.first64;    // (kept in registers it would take five of those that a group's work needs)
+        __syncthreads();
+    }
     const size_t head_off = (size_t) hk * head_bytes(KT, D);
     // wave w brings group w % 2 of every tile's K (waves 0 and 1) or V
     const int grp = wave & 1;
@@ -683,6 +693,7 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     const int lane = tid & 63, c = lane & 31, g = lane >> 5;
     typename runs_t::found f;
     if (P.nks > 1) {
+        steps.first64 = seqs[lane];
         if (!steps.find(P.R, P.pg, P.GQA, at_step, lane, f)) return;
     } else {                                                  // a group each
         f.seq = run / P.max_groups; f.group = run - f.seq * P.max_groups; f.first = 0; f.steps = 1;
@@ -782,8 +793,14 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
         if constexpr (EXACT) s = mfma32(a[0], qf[NQ - 1][ks], s);
         if constexpr (NPL == 2) s = mfma32(a[NPL - 1], qf[0][ks], s);
     };
+    // (what only the ends need is worked out there once more: kept, it would hold registers all the way)
+    auto again = [&](int x) {
+        asm volatile("" : "+v"(x));
+        return x;
+    };
     auto mask = [&](f16x & s, int k0) {
-        const sight v = sight_of(P, sv, my_tok, k0);
+        const int me = again(lane), g = me >> 5;
+        const sight v = sight_of(P, sv, tok_of(col0 + min(me & 31, ncols - 1)), k0);
         const int hi = v.hi - 4 * g, lo = v.lo - 4 * g, sk = v.sk - 4 * g;
         const uint32_t bits = v.bits >> (4 * g);
 #pragma unroll
@@ -807,7 +824,6 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     auto to_of = [&](int e) { return (my_v ? v_place + (e + C::PLACES - 1) % C::PLACES * T_B : k_place + e % C::PLACES * T_B) + grp * G_B; };
     int pages = 0;
     size_t row = 0;
-    const int key_off = G::key(lane) * (int) P.pg.rowb;
     auto next_row = [&](int e) {
         if (!(e & 63)) {
             pages = pages_from(e);
@@ -815,7 +831,7 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
         }
         const int tile = tile_of_item(e), kb = tile * BN + 16 * grp;
         if (paged16 || !ptab) {                               // where the first of the 16 rows is, the same for all lanes, and how far behind it a lane's own
-            int a = kb, off = key_off;
+            int a = kb, off = G::key(again(lane)) * (int) P.pg.rowb;
             if (!(kb + 15 <= sp.pmax && (kb >= sp.lo || kb + 15 < sp.ns))) {
                 const int j = pos_of(tile);
                 a = __builtin_amdgcn_readfirstlane(j);
@@ -980,7 +996,10 @@ __global__ void __launch_bounds__(NTHR, (team_cfg<KT, D, EXACT>::WGS)) team_k(co
     {
     const tree_params & P = read_again();
     l += __shfl_xor(l, 32);
+    const int me = again(lane), c = me & 31, g = me >> 5;
     if (c < ncols) {
+        const int col = col0 + c, tok = tok_of(col);
+        const size_t my_row = (size_t) (sv.first + tok) * P.Hq + (size_t) hk * P.GQA + (col - tok * P.GQA);
 #pragma unroll
         for (int dt = 0; dt < NDT; ++dt)
 #pragma unroll
