@@ -9,9 +9,10 @@
 //   left_k    the last node's row: what is left, a stretch a workgroup
 //   pick_k    a workgroup per sequence: the stretch where the running sum passes u, and the value in it (logits without a draft: at decide_k's end, as
 //             stats_k has summed every stretch and only those with a rejected token are summed again)
-// stats_k is bound by the memory that it reads (160 rows of 151936 f32 logits: 23 us, 4.2 TB/s), the others by their chains of dependent loads (5 ... 14 us each).
+// stats_k and left_k are bound by the memory that they read (160 rows of 151936 f32 logits: 23 us, 4.2 TB/s; what is left in 32 of them and the draft's: 11 us, 3.6 TB/s), the
+// others by chains of dependent loads (decide_k 8 us, a round of sums_k 6, pick_k 6 ... 8): what does not depend on one another is asked for at once.
 // A kernel's end is what makes its sums known: with workgroups that count themselves and a last one that goes on, each had to make its writes visible to the other
-// XCDs' caches, and 32 chains over 151936 logits took 112 us instead of 57.
+// XCDs' caches, and 32 chains over 151936 logits took 112 us instead of 48.
 // Sums, exponentials and comparisons are made in 64 bits: with 32 one draw in some hundreds would take the neighbouring token. 2^x comes from a table of 256 powers
 // and three terms (2e-13 of the value: a draw in 10^7), 12 64-bit instructions a value; the table is a constant of the program, since making it in every workgroup
 // took 5 us of each kernel. A sum's order is fixed by its place, so the same call gives the same tokens.
@@ -161,11 +162,26 @@ __device__ __forceinline__ void load_run(float (&x)[PER], const char * row, bool
     else load_words<PER>(x, (gbytes) row + 4 * (size_t) j0, std::false_type{});
 }
 
-// sums over the workgroup, the same in every thread (lanes by an xor butterfly, waves in order)
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) x += __shfl_xor(x, d);
+// sums over the lanes up to this one, over the wave and over the workgroup (those the same in every thread). Lanes are moved by vector instructions: through LDS the
+// six steps of a sum took half a microsecond
+template <int CTRL, int ROWS> __device__ __forceinline__ double moved(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t l = __builtin_amdgcn_update_dpp(0, (int) (uint32_t) u, CTRL, ROWS, 0xf, false), h = __builtin_amdgcn_update_dpp(0, (int) (u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t) h << 32 | l);
+}
+__device__ __forceinline__ double sum_up_to(double x) {
+    x += moved<0x111, 0xf>(x);                                // lanes 1, 2, 4, 8 below, of the row of 16
+    x += moved<0x112, 0xf>(x);
+    x += moved<0x114, 0xf>(x);
+    x += moved<0x118, 0xf>(x);
+    x += moved<0x142, 0xa>(x);                                // the row before's last, for rows 1 and 3
+    x += moved<0x143, 0xc>(x);                                // lane 31, for rows 2 and 3
     return x;
+}
+__device__ __forceinline__ double wave_sum(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, sum_up_to(x));
+    const uint32_t l = __builtin_amdgcn_readlane((int) (uint32_t) u, 63), h = __builtin_amdgcn_readlane((int) (u >> 32), 63);
+    return __builtin_bit_cast(double, (uint64_t) h << 32 | l);
 }
 __device__ __forceinline__ double group_sum(double x, double * lds) {
     x = wave_sum(x);
@@ -241,10 +257,12 @@ __global__ void __launch_bounds__(VTHR) stats_k(const verify_params P) {
 
 // ---- what a workgroup knows about its sequence while it decides ----
 struct tree_lds {
-    int16_t up[NODES], first[NODES], sibling[NODES];          // parent, first child, next child of the same parent: of nodes whose token there is
-    int token[NODES];
+    int16_t up[NODES];                                        // parent, of nodes whose token there is
+    int first[NODES];                                         // first child (none: NODES); then the child under test
+    int sibling[NODES], token[NODES];                         // next child of the same parent
     int state[NODES];
     bool again[NODES];                                        // an elder sibling has the same token
+    float value[NODES], q[NODES], u[NODES];                   // what the parent's rows hold of the token; its number
     float most[NODES];                                        // of the nodes' rows: the largest logit, where it is, 1 / the sum
     int arg[NODES];
     double z[NODES];
@@ -272,7 +290,7 @@ struct last_lds {
     double ws[VTHR / 64], scan[VTHR];
     uint32_t out[STRETCH / 32];                               // values of a stretch that are taken out
     uint32_t touched[256 / 32];                               // stretches that have some
-    int last, found;
+    int first[VTHR / 64], last[VTHR / 64];
 };
 // without a draft every child of the last node was rejected: f(token) for each
 template <class F> __device__ __forceinline__ void rejected(const verify_params & P, const seq_view & v, int me, F && f) {
@@ -319,13 +337,12 @@ __global__ void __launch_bounds__(VTHR) left_k(const verify_params P) {
     if (threadIdx.x == 0) P.sums[0][(size_t) seq * P.stretches + z] = s;
 }
 
-// The token behind the last node's row t. known: the sums of its stretches are in sums[0]; otherwise (logits, no draft) in st_sum, but for those that something is taken out of
-__device__ __forceinline__ void pick(const verify_params & P, int seq, const seq_view & v, int t, double a, bool known, const powers & pw, last_lds & T) {
+// The token behind the last node's row t, with the number u. known: `mine` is the sum of stretch number tid; otherwise (logits, no draft) they are in st_sum, but for those that
+// something is taken out of
+__device__ __forceinline__ void pick(const verify_params & P, int seq, const seq_view & v, int t, double a, bool known, double mine, double u, const powers & pw, last_lds & T) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // ---- the stretch: one a thread (there are 256 at most) ----
-    double mine = 0.0;
-    if (known) mine = tid < P.stretches ? P.sums[0][(size_t) seq * P.stretches + tid] : 0.0;
-    else {
+    if (!known) {
         const double by = by_of(P, seq);
         const size_t at = (size_t) t * P.stretches;
         if (tid < P.stretches) {
@@ -351,28 +368,34 @@ __device__ __forceinline__ void pick(const verify_params & P, int seq, const seq
         }
     auto running = [&](double x) {                            // sums over the threads up to this one
         __syncthreads();
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) { const double y = __shfl_up(x, d); if (lane >= d) x += y; }
+        x = sum_up_to(x);
         if (lane == 63) T.ws[wave] = x;
         __syncthreads();
         for (int w = 0; w < wave; ++w) x += T.ws[w];
         return x;
     };
-    const double upto = running(mine), u = (double) P.u_next[seq];
+    const double upto = running(mine);
     T.scan[tid] = upto;
-    if (tid == 0) { T.found = INT32_MAX; T.last = -1; }
     __syncthreads();
     const double total = T.scan[VTHR - 1], goal = u * total;
     if (!(total > 0.0)) {
         if (tid == 0) P.next[seq] = -1;
         return;
     }
-    if (mine > 0.0) {
-        if (upto > goal) atomicMin(&T.found, tid);
-        atomicMax(&T.last, tid);
-    }
-    __syncthreads();
-    const int zf = T.found != INT32_MAX ? T.found : T.last;   // (u of 1 and above: the last that weighs anything)
+    // the lowest thread that has passed the goal with `a`, or, if none has, the last one that has `b` at all (all of 256 threads on one address in LDS took 3 us)
+    auto first_or_last = [&](bool pass, int a, int b) {
+        const unsigned long long ps = __ballot(pass), as = __ballot(b >= 0);
+        const int f = __builtin_amdgcn_readlane(a, ps ? __builtin_ctzll(ps) : 0), z = __builtin_amdgcn_readlane(b, as ? 63 - __builtin_clzll(as) : 0);
+        if (lane == 0) { T.first[wave] = ps ? f : -1; T.last[wave] = as ? z : -1; }
+        __syncthreads();
+        int r = -1;
+#pragma unroll
+        for (int w = 0; w < VTHR / 64; ++w) r = r < 0 ? T.first[w] : r;
+#pragma unroll
+        for (int w = VTHR / 64 - 1; w >= 0; --w) r = r < 0 ? T.last[w] : r;
+        return r;
+    };
+    const int zf = first_or_last(mine > 0.0 && upto > goal, tid, mine > 0.0 ? tid : -1);   // (u of 1 and above: the last that weighs anything)
     const double before = zf ? T.scan[zf - 1] : 0.0;
     // ---- the value: 16 on end a thread ----
     const bool draft = some && P.draft && a > 0.0;
@@ -392,29 +415,27 @@ __device__ __forceinline__ void pick(const verify_params & P, int seq, const seq
         }
     });
     double at = before + running(sum) - sum;
-    if (tid == 0) { T.found = INT32_MAX; T.last = -1; }
-    __syncthreads();
-    int pass = INT32_MAX, any = -1;
+    int pass = -1, any = -1;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         at += p[e];
         if (p[e] > 0.0) {
             any = zf * STRETCH + tid * PER + e;
-            if (at > goal) pass = min(pass, any);
+            if (at > goal && pass < 0) pass = any;
         }
     }
-    if (pass != INT32_MAX) atomicMin(&T.found, pass);
-    if (any >= 0) atomicMax(&T.last, any);
-    __syncthreads();
-    if (tid == 0) P.next[seq] = T.found != INT32_MAX ? T.found : T.last;   // (the stretch's own sum rounded above this one: its last)
+    const int token = first_or_last(pass >= 0, pass, any);    // (none has passed: the stretch's own sum was rounded above this one)
+    if (tid == 0) P.next[seq] = token;
 }
 __global__ void __launch_bounds__(VTHR) pick_k(const verify_params P) {
     __shared__ powers pw;
     __shared__ last_lds T;
     const int seq = blockIdx.x, t = P.last_row[seq];
+    // (asked for together with t)
+    const double mine = (int) threadIdx.x < P.stretches ? P.sums[0][(size_t) seq * P.stretches + threadIdx.x] : 0.0, a = P.last_a[seq], u = (double) P.u_next[seq];
     if (t < 0) return;
     if (P.logits) fill(pw);
-    pick(P, seq, seq_of<true>(P.R, seq), t, P.last_a[seq], true, pw, T);
+    pick(P, seq, seq_of<true>(P.R, seq), t, a, true, mine, u, pw, T);
 }
 
 // round: -1 at first; or the round whose sums are to be taken. walk: the path is known behind this one; and_pick: and so are the sums of all rows
@@ -425,6 +446,7 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
     const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const seq_view v = seq_of<true>(P.R, seq);
     const int n = min(v.count, NODES);
+    const double u_next = and_pick ? (double) P.u_next[seq] : 0.0;
     if (n < 1) {
         if (tid == 0) { P.n_accept[seq] = 0; P.next[seq] = -1; P.last_row[seq] = -1; P.n_waiting[seq] = 0; }
         for (int k = tid; k < P.ld_path; k += VTHR) P.path[(size_t) seq * P.ld_path + k] = -1;
@@ -435,44 +457,38 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
         const double by = P.logits ? by_of(P, seq) : 0.0;
         for (int i = tid; i < n; i += VTHR) {
             const int x = P.token[v.first + i], p = P.parent ? P.parent[v.first + i] : i - 1;
+            const bool is = i > 0 && p >= 0 && p < i && x >= 0 && x < P.V;
             T.token[i] = x;
-            T.up[i] = (int16_t) (i > 0 && p >= 0 && p < i && x >= 0 && x < P.V ? p : -1);
-            T.first[i] = -1;
+            T.up[i] = (int16_t) (is ? p : -1);
+            T.first[i] = NODES;
+            T.sibling[i] = -1;
+            T.again[i] = false;
+            T.u[i] = P.u[v.first + i];
+            if (is) {
+                T.value[i] = value_at(P.target, (size_t) (v.first + p) * P.ld_target + x, P.target_bf16);
+                if (P.draft) T.q[i] = value_at(P.draft, (size_t) (v.first + p) * P.ld_draft + x, P.draft_bf16);
+            }
         }
         if (tid == 0) T.waiting = 0;
-        __syncthreads();
-        // ---- a thread a node: what its row and its parent's hold of its token; its elder siblings ----
-        for (int i = tid; i < n; i += VTHR) {
-            const int p = T.up[i], x = T.token[i];
-            int elder = -1, k = 0, younger = -1;
-            bool again = false;
-            if (p >= 0) {
-                for (int j = p + 1; j < i; ++j) if (T.up[j] == p) { elder = j; ++k; again |= T.token[j] == x; }
-                if (!P.draft || k + 1 < P.max_children)       // (the last one, or the last that is looked at, has none)
-                    for (int j = i + 1; j < n; ++j) if (T.up[j] == p) { younger = j; break; }
-                if (elder < 0) T.first[p] = (int16_t) i;
-            }
-            T.again[i] = again;
-            T.sibling[i] = (int16_t) younger;
-            P.sibling[v.first + i] = (int16_t) younger;
-        }
         // ---- logits: a wave a row: the sum of its stretches ----
         if (P.logits)
             for (int i = wave; i < n; i += VTHR / 64) {
                 const size_t at = (size_t) (v.first + i) * P.stretches;
                 float m = MINUS_INF;
+                for (int z = lane; z < P.stretches; z += 64) m = fmaxf(m, P.st_max[at + z]);
+                m = wave_max(m);
                 int arg = INT32_MAX;
-                for (int z = lane; z < P.stretches; z += 64) { const float x = P.st_max[at + z]; if (x > m) { m = x; arg = P.st_arg[at + z]; } }
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) {
-                    const float om = __shfl_xor(m, d);
-                    const int oi = __shfl_xor(arg, d);
-                    if (om > m || (om == m && oi < arg)) { m = om; arg = oi; }
-                }
                 double s = 0.0;
-                if (by >= 0.0 && m > MINUS_INF)
-                    for (int z = lane; z < P.stretches; z += 64) { double w = 0.0; softmax(by, m, 0, 1.0).with(pw, [&](auto weight) { w = weight(P.st_max[at + z], 0); }); s += P.st_sum[at + z] * w; }
-                s = wave_sum(s);
+                if (by < 0.0) {
+                    for (int z = lane; z < P.stretches; z += 64) arg = P.st_max[at + z] == m ? min(arg, P.st_arg[at + z]) : arg;
+#pragma unroll
+                    for (int d = 1; d < 64; d <<= 1) arg = min(arg, __shfl_xor(arg, d));
+                } else if (m > MINUS_INF) {
+                    softmax(by, m, 0, 1.0).with(pw, [&](auto weight) {
+                        for (int z = lane; z < P.stretches; z += 64) s += P.st_sum[at + z] * weight(P.st_max[at + z], 0);
+                    });
+                    s = wave_sum(s);
+                }
                 if (lane == 0) {
                     T.most[i] = P.row_max[v.first + i] = m;
                     T.arg[i] = P.row_arg[v.first + i] = m > MINUS_INF ? arg : -1;
@@ -480,19 +496,42 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
                 }
             }
         __syncthreads();
+        // ---- children of a node in their order: each looks for the nearest elder one, but for the first ----
+        if (P.parent) {
+            for (int i = tid; i < n; i += VTHR) if (T.up[i] >= 0) atomicMin(&T.first[T.up[i]], i);
+            __syncthreads();
+            for (int i = tid; i < n; i += VTHR) {
+                const int p = T.up[i];
+                if (p < 0 || T.first[p] == i) continue;
+                int j = i - 1;
+                while (T.up[j] != p) --j;
+                T.sibling[j] = i;
+            }
+            __syncthreads();
+            if (!P.draft) {
+                for (int i = tid; i < n; i += VTHR)
+                    if (T.up[i] >= 0) for (int j = T.first[T.up[i]]; j != i && !T.again[i]; j = T.sibling[j]) T.again[i] = T.token[j] == T.token[i];
+            } else
+                for (int i = tid; i < n; i += VTHR) {         // (what no round is left for is not looked at: the list ends)
+                    int j = T.first[i];
+                    for (int k = 1; k < P.max_children && j >= 0 && j < NODES; ++k) j = T.sibling[j];
+                    if (j >= 0 && j < NODES) T.sibling[j] = -1;
+                }
+            __syncthreads();
+        } else
+            for (int i = tid; i < n; i += VTHR) T.first[i] = i + 1 < n && T.up[i + 1] == i ? i + 1 : NODES;
+        for (int i = tid; i < n; i += VTHR) P.sibling[v.first + i] = (int16_t) T.sibling[i];
         // ---- every node tests ----
         for (int i = tid; i < n; i += VTHR) {
             const int row = v.first + i;
-            int c = T.first[i], state = NONE;
+            int c = T.first[i] < NODES ? T.first[i] : -1, state = NONE;
             double a = 0.0, gone = 0.0, mass = 1.0;
             while (c >= 0) {
-                const int x = T.token[c];
-                const double u = (double) P.u[v.first + c];
-                const float l = value_at(P.target, (size_t) row * P.ld_target + x, P.target_bf16);
-                double p = probability(l);
-                if (P.logits) softmax(by, T.most[i], T.arg[i], T.z[i]).with(pw, [&](auto weight) { p = weight(l, x); });
+                const double u = (double) T.u[c];
+                double p = probability(T.value[c]);
+                if (P.logits) softmax(by, T.most[i], T.arg[i], T.z[i]).with(pw, [&](auto weight) { p = weight(T.value[c], T.token[c]); });
                 if (P.draft) {
-                    const double q = probability(value_at(P.draft, (size_t) row * P.ld_draft + x, P.draft_bf16));
+                    const double q = probability(T.q[c]);
                     if (accept(u, 1.0, p, q, 0.0, 0.0)) { state = c; break; }
                     c = T.sibling[c];
                     if (reject(P, 1.0, q, a, gone) && c >= 0) state = WAITS;
@@ -506,7 +545,7 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
             T.state[i] = state;
             P.node_a[0][row] = a;
             P.node_gone[0][row] = gone;
-            P.node_child[0][row] = T.first[i] = (int16_t) c;
+            P.node_child[0][row] = T.first[i] = c;
             P.node_state[0][row] = state;
         }
         __syncthreads();
@@ -573,7 +612,7 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
     }
     __syncthreads();
     for (int k = T.length + tid; k < P.ld_path; k += VTHR) P.path[(size_t) seq * P.ld_path + k] = -1;
-    if (and_pick) pick(P, seq, v, v.first + T.waiting, 0.0, false, pw, U);
+    if (and_pick) pick(P, seq, v, v.first + T.waiting, 0.0, false, 0.0, u_next, pw, U);
 }
 
 // Round k: a node that waits takes the sum of round k - 1 and tests its child with it (every workgroup of the node does, the first writes it down); if that is rejected and there is
