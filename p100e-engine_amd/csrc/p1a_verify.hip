@@ -279,6 +279,10 @@ __device__ __forceinline__ bool reject(const verify_params & P, double mass, dou
 }
 __device__ __forceinline__ bool accept(double u, double mass, double p, double q, double a, double gone) { return u * (q / (1.0 - gone)) * mass < fmax(p - a * q, 0.0); }
 
+// What one kernel reads of another's nodes stays in the call's rows even where two sequences of row0 share some, and each leaves its own there
+__device__ __forceinline__ int row_in(const verify_params & P, int row) { return min(max(row, 0), P.R.T - 1); }
+__device__ __forceinline__ int token_in(const verify_params & P, int row) { return min(max(P.token[row_in(P, row)], 0), P.V - 1); }
+
 // f(weight) for a row: weight(l, j) of its value j, l
 template <class F> __device__ __forceinline__ void with_row(const verify_params & P, int seq, int row, const powers & pw, F && f) {
     if (!P.logits) f([](float l, int) { return probability(l); });
@@ -569,19 +573,19 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
         // ---- nodes that waited: a wave each, with the last round's sum ----
         const int m = P.n_waiting[seq];
         for (int w = wave; w < m; w += VTHR / 64) {
-            const int i = P.waiting[v.first + w], row = v.first + i;
+            const int i = min(P.waiting[row_in(P, v.first + w)], n - 1), row = v.first + i;
             int state = P.node_state[in][row];
             double a = P.node_a[in][row];
             if (state == WAITS) {
                 double mass = 0.0;
                 for (int z = lane; z < P.stretches; z += 64) mass += P.sums[in][(size_t) row * P.stretches + z];
                 mass = wave_sum(mass);
-                const int c = P.node_child[in][row], x = P.token[v.first + c];
+                const int c = P.node_child[in][row], x = token_in(P, v.first + c);
                 double gone = P.node_gone[in][row];
                 double p = 0.0;
                 with_row(P, seq, row, pw, [&](auto weight) { p = weight(value_at(P.target, (size_t) row * P.ld_target + x, P.target_bf16), x); });
                 const double q = probability(value_at(P.draft, (size_t) row * P.ld_draft + x, P.draft_bf16));
-                if (accept((double) P.u[v.first + c], mass, p, q, a, gone)) state = c;
+                if (accept((double) P.u[row_in(P, v.first + c)], mass, p, q, a, gone)) state = c;
                 else {
                     reject(P, mass, q, a, gone);
                     state = NONE;
@@ -599,7 +603,7 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
     // ---- the walk ----
     if (tid == 0) {
         int at = 0, k = 0;
-        for (int c = T.state[0]; c >= 0; c = T.state[at]) {
+        for (int c = T.state[0]; c > at && c < n; c = T.state[at]) {
             if (k < P.ld_path) P.path[(size_t) seq * P.ld_path + k] = c;
             ++k;
             at = c;
@@ -627,7 +631,7 @@ __global__ void __launch_bounds__(VTHR) sums_k(const verify_params P, int k) {
     const int in = k & 1, first = seq_of<true>(P.R, seq).first;
     if (P.logits) fill(pw);
     for (int w = slot; w < m; w += SLOTS) {
-        const int t = first + P.waiting[first + w];
+        const int t = row_in(P, first + P.waiting[row_in(P, first + w)]);
         int state = P.node_state[in][t], c = P.node_child[in][t];
         double a = P.node_a[in][t], gone = P.node_gone[in][t];
         float x[PER], y[PER];
@@ -639,14 +643,14 @@ __global__ void __launch_bounds__(VTHR) sums_k(const verify_params P, int k) {
                 double mass = 0.0;                            // (every wave for itself, all alike)
                 for (int i = lane; i < P.stretches; i += 64) mass += P.sums[in][(size_t) t * P.stretches + i];
                 mass = wave_sum(mass);
-                const int token = P.token[first + c];
+                const int token = token_in(P, first + c);
                 const float l = value_at(P.target, (size_t) t * P.ld_target + token, P.target_bf16);
                 const double q = probability(value_at(P.draft, (size_t) t * P.ld_draft + token, P.draft_bf16));
                 double p = 0.0;
                 with_row(P, seq, t, pw, [&](auto weight) { p = weight(l, token); });
-                if (accept((double) P.u[first + c], mass, p, q, a, gone)) state = c;
+                if (accept((double) P.u[row_in(P, first + c)], mass, p, q, a, gone)) state = c;
                 else {
-                    c = P.sibling[first + c];
+                    c = P.sibling[row_in(P, first + c)];
                     if (!reject(P, mass, q, a, gone) || c < 0) state = NONE;
                 }
             }

@@ -486,6 +486,24 @@ def test_verify_scratch_and_repeats(p1a):
             assert np.array_equal(a, c)
 
 
+def test_verify_sequences_that_share_rows(p1a):
+    """row0 that does not ascend: two sequences hold some of the same rows - nobody's results, but numbers of nodes and tokens that there are, and an end"""
+    for seed in range(6):
+        b = Batch(70 + seed, [12, 12, 12, 12], 9000, 4, draft="distinct", noise=2.0)
+        rows = p1a.Rows(48, n_seq=5, row0=dev(np.array([0, 24, 12, 40, 30, 48], np.int32)), max_rows=48)
+        held = [24, 0, 28, 0, 18]
+        n, nxt = (torch.full((5,), 77, dtype=torch.int32, device="cuda") for _ in range(2))
+        path = torch.full((5, 48), 77, dtype=torch.int32, device="cuda")
+        p1a.tree_verify(b.rows_on_gpu(b.target, torch.float32), dev(b.token), rows, dev(b.u), dev(np.resize(b.u_next, 5)), n, path, nxt, parent=dev(np.array(sum(b.parents, []), np.int32)),
+                        draft=b.rows_on_gpu(b.draft, torch.float32), max_children=4, distinct=True)
+        torch.cuda.synchronize()
+        for s, count in enumerate(held):
+            k = int(n[s])
+            got = path[s].tolist()
+            assert 0 <= k < max(count, 1) and got[k:] == [-1] * (48 - k) and all(0 < i < count for i in got[:k]) and got[:k] == sorted(set(got[:k]))
+            assert 0 <= int(nxt[s]) < 9000 if count else int(nxt[s]) == -1
+
+
 @pytest.mark.parametrize("how", ["none", "iid", "distinct"])
 def test_verify_keeps_the_target_s_distribution(p1a, how):
     """the first token behind node 0 has the target's distribution, whatever was drafted: 40000 trees of three children"""
