@@ -83,6 +83,19 @@ def _calls():
     return _call
 
 
+_tree = None
+
+
+def _trees():
+    """The same module with the entry points of drafted trees (apart, since their checks of tensors need torch's types)."""
+    global _tree
+    import torch
+    L, m = lib(), _calls()
+    m.bind_trees(*(ctypes.cast(getattr(L, n), ctypes.c_void_p).value for n in ("p1a_tree_rows", "p1a_tree_commit")), _of, torch.int32)
+    _tree = m
+    return _tree
+
+
 def lib():
     """Load libp1a_attn.so (built by __graft_entry__.build() / csrc/Makefile). Raises if it is missing."""
     global _lib
@@ -417,7 +430,7 @@ class Rows:
         if pos0 is not None:
             pos0 = pos0.data_ptr() if pos0.dtype is _I32 and pos0.numel() >= n_seq and pos0.is_contiguous() else _of(pos0, False, n_seq, "pos0")
         self._st = p1a_rows(T, n_seq, max_rows, max_n, row0, pos0, p0, window, n_sink)
-        self._ref = ctypes.byref(self._st)
+        self._ref, self._at = ctypes.byref(self._st), ctypes.addressof(self._st)
 
 
 _row_types = {}
@@ -516,12 +529,7 @@ def kv_compact(c, keep, mass=None, mass_out=None):
 def tree_rows(parent, rows, mask, pos=None, slot=None):
     """From the parents of drafted trees' nodes (parent int32 [T]): which nodes a row sees, mask int32 [T][words] (a bit each), its rotary position and its cache
     slot, int32 [T] each or None."""
-    T, words = rows.T, mask.shape[-1]
-    if pos is not None:
-        pos = _of(pos, False, T, "pos")
-    if slot is not None:
-        slot = _of(slot, False, T, "slot")
-    rc = (_lib or lib()).p1a_tree_rows(_of(parent, False, T, "parent"), rows._ref, _of(mask, False, T * words, "mask"), words, pos, slot, _stream())
+    rc = (_tree if _tree is not None and _tree is _call else _trees()).tree_rows(parent, rows, mask, pos, slot)
     if rc:
         _check(rc, "tree_rows")
 
@@ -596,8 +604,7 @@ def tree_commit(layers, rows, n_accept, path):
     """Moves the accepted nodes' rows of K and V behind node 0's, in every layer: n_accept int32 [n_seq], path int32 [n_seq][..] as tree_verify leaves them."""
     if not isinstance(layers, Layers):
         layers = Layers(layers)
-    width = path.shape[-1]
-    rc = (_lib or lib()).p1a_tree_commit(layers._at, layers.n, rows._ref, _of(n_accept, False, rows.n_seq, "n_accept"), _of(path, False, rows.n_seq * width, "path"), width, _stream())
+    rc = (_tree if _tree is not None and _tree is _call else _trees()).tree_commit(layers._at, layers.n, rows, n_accept, path)
     if rc:
         _check(rc, "tree_commit")
 

@@ -4,6 +4,8 @@
 // come here instead; arguments are taken as ctypes takes them (whole numbers cut to 32 bits, floats, ctypes numbers of the parameter's
 // type, what _as_parameter_ stands for, None for a null pointer, anything with data_ptr() as a device pointer), and the GIL is released around the call. One token of 4 heads of 64, prep and decode from Python:
 // 18.1 us with ctypes, 15.6 so (7.7 of them the C calls, 3.5 the caller's own indexing); two layers of 24 / 4 heads of 96 34.4 -> 29.2.
+// The small calls around a drafted tree, a launch of 2 ... 5 us each, come here too, with their checks of tensors: masks of
+// a tree's nodes 6.8 -> 6.2 us, an accepted path moved 7.3 -> 6.8 (2.7 of them the launch, 1.3 the caller's Rows).
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -14,7 +16,7 @@
 
 namespace {
 
-PyObject * s_data_ptr, * s_struct, * s_value, * s_as_parameter, * s_field[11];
+PyObject * s_data_ptr, * s_struct, * s_value, * s_as_parameter, * s_field[11], * s_dtype, * s_numel, * s_is_contiguous, * s_size, * s_T, * s_n_seq, * s_at, * last_dim;
 const char * const FIELDS[11] = {"type", "n_ctx", "Hkv", "D", "k", "v", "pt", "rtab", "psh", "pstride", "_pt_off"};
 enum { INT, UINT, SIZE, FLOAT, POINTER, DESC, NCLASS };
 
@@ -26,6 +28,10 @@ struct calls {
     decltype(&p1a_attn_prefill) f_prefill;
     decltype(&p1a_kv_append) f_append;
     PyObject * kv_class, * stream_of;
+    // the same of drafted trees, set by bind_trees(): what checks a tensor and says what is wrong with it, and torch's int32
+    decltype(&p1a_tree_rows) f_rows;
+    decltype(&p1a_tree_commit) f_commit;
+    PyObject * check, * int32;
     PyObject * classes[NCLASS];   // ctypes' c_int, c_uint32, c_size_t, c_float, c_void_p, and the descriptor's Structure
 
     // (each reader does nothing once an error is set, so that the callers test for one at the end)
@@ -131,6 +137,34 @@ struct calls {
         for (PyObject * x : f) Py_XDECREF(x);
         return !PyErr_Occurred();
     }
+    long long number(PyObject * r) {                          // of a call or an attribute, which it takes
+        const long long n = r ? PyLong_AsLongLong(r) : 0;
+        Py_XDECREF(r);
+        return n;
+    }
+    long long attribute(PyObject * o, PyObject * name) { return PyErr_Occurred() ? 0 : number(PyObject_GetAttr(o, name)); }
+    long long last_size(PyObject * t) { return PyErr_Occurred() ? 0 : number(PyObject_CallMethodOneArg(t, s_size, last_dim)); }
+    // the address of a tensor of at least `least` numbers on end, of torch's int32; None: null. What is not right about one the binding says
+    void * ints(PyObject * t, long long least, const char * what) {
+        if (PyErr_Occurred() || t == Py_None) return nullptr;
+        PyObject * type = PyObject_GetAttr(t, s_dtype);
+        if (!type) return nullptr;
+        bool right = type == int32;
+        Py_DECREF(type);
+        if (right) right = number(PyObject_CallMethodNoArgs(t, s_numel)) >= least && !PyErr_Occurred();
+        if (right) {
+            PyObject * r = PyObject_CallMethodNoArgs(t, s_is_contiguous);
+            right = r == Py_True;
+            Py_XDECREF(r);
+        }
+        if (PyErr_Occurred()) return nullptr;
+        if (right) return data_ptr(t);
+        PyObject * r = PyObject_CallFunction(check, "OOLs", t, Py_False, least, what);
+        if (!r) return nullptr;
+        void * p = address(r);
+        Py_DECREF(r);
+        return p;
+    }
     void * stream() {
         if (PyErr_Occurred()) return nullptr;
         PyObject * r = PyObject_CallNoArgs(stream_of);
@@ -145,9 +179,9 @@ bool takes(Py_ssize_t n, Py_ssize_t want) {
     if (n != want) PyErr_Format(PyExc_TypeError, "%zd arguments expected, %zd given", want, n);
     return n == want;
 }
-bool bound(const calls & C) {
-    if (!C.f_append) PyErr_SetString(PyExc_RuntimeError, "bind() comes first");
-    return C.f_append;
+bool bound(const calls & C, bool too = true) {
+    if (!C.f_append || !too) PyErr_SetString(PyExc_RuntimeError, "bind() comes first");
+    return C.f_append && too;
 }
 #define P1A_CALL(expr) do { if (PyErr_Occurred()) return nullptr; int rc_; Py_BEGIN_ALLOW_THREADS rc_ = (expr); Py_END_ALLOW_THREADS return PyLong_FromLong(rc_); } while (0)
 
@@ -211,6 +245,40 @@ PyObject * append(PyObject * self, PyObject * const * a, Py_ssize_t n) {
     void * s = C.stream();
     P1A_CALL(C.f_append(&kv, k, v, p0, p0_dev, pos, T, s));
 }
+// (parent, rows, mask, pos, slot)
+PyObject * tree_rows(PyObject * self, PyObject * const * a, Py_ssize_t n) {
+    calls & C = *(calls *) PyModule_GetState(self);
+    if (!takes(n, 5) || !bound(C, C.f_rows)) return nullptr;
+    const long long T = C.attribute(a[1], s_T), words = C.last_size(a[2]);
+    int32_t * pos = (int32_t *) C.ints(a[3], T, "pos"), * slot = (int32_t *) C.ints(a[4], T, "slot"), * parent = (int32_t *) C.ints(a[0], T, "parent");
+    const p1a_rows * rows = (const p1a_rows *) (uintptr_t) C.attribute(a[1], s_at);
+    uint32_t * mask = (uint32_t *) C.ints(a[2], T * words, "mask");
+    void * s = C.stream();
+    P1A_CALL(C.f_rows(parent, rows, mask, (int) words, pos, slot, s));
+}
+// (the layers' descriptors, how many they are, rows, n_accept, path)
+PyObject * tree_commit(PyObject * self, PyObject * const * a, Py_ssize_t n) {
+    calls & C = *(calls *) PyModule_GetState(self);
+    if (!takes(n, 5) || !bound(C, C.f_commit)) return nullptr;
+    const p1a_kv * layers = (const p1a_kv *) C.address(a[0]);
+    const int count = C.as_int(a[1]);
+    const long long n_seq = C.attribute(a[2], s_n_seq), width = C.last_size(a[4]);
+    const p1a_rows * rows = (const p1a_rows *) (uintptr_t) C.attribute(a[2], s_at);
+    const int32_t * n_accept = (const int32_t *) C.ints(a[3], n_seq, "n_accept"), * path = (const int32_t *) C.ints(a[4], n_seq * width, "path");
+    void * s = C.stream();
+    P1A_CALL(C.f_commit(layers, count, rows, n_accept, path, (int) width, s));
+}
+// (addresses of p1a_tree_rows, p1a_tree_commit; the binding's check of a tensor; torch.int32)
+PyObject * bind_trees(PyObject * self, PyObject * const * a, Py_ssize_t n) {
+    calls & C = *(calls *) PyModule_GetState(self);
+    if (!takes(n, 4)) return nullptr;
+    C.f_rows = (decltype(C.f_rows)) C.address(a[0]);
+    C.f_commit = (decltype(C.f_commit)) C.address(a[1]);
+    if (PyErr_Occurred()) return nullptr;
+    Py_INCREF(a[2]); Py_XSETREF(C.check, a[2]);
+    Py_INCREF(a[3]); Py_XSETREF(C.int32, a[3]);
+    Py_RETURN_NONE;
+}
 // (addresses of p1a_attn_prep, p1a_attn_decode_a16, p1a_attn_prefill, p1a_kv_append; the cache class; the current stream's handle; the
 // ctypes classes)
 PyObject * bind(PyObject * self, PyObject * const * a, Py_ssize_t n) {
@@ -230,26 +298,30 @@ PyObject * bind(PyObject * self, PyObject * const * a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"bind", (PyCFunction) (void (*)(void)) bind, METH_FASTCALL, nullptr}, {"prep", (PyCFunction) (void (*)(void)) prep, METH_FASTCALL, nullptr},
     {"decode", (PyCFunction) (void (*)(void)) decode, METH_FASTCALL, nullptr}, {"prefill", (PyCFunction) (void (*)(void)) prefill, METH_FASTCALL, nullptr},
-    {"append", (PyCFunction) (void (*)(void)) append, METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
+    {"append", (PyCFunction) (void (*)(void)) append, METH_FASTCALL, nullptr}, {"bind_trees", (PyCFunction) (void (*)(void)) bind_trees, METH_FASTCALL, nullptr},
+    {"tree_rows", (PyCFunction) (void (*)(void)) tree_rows, METH_FASTCALL, nullptr}, {"tree_commit", (PyCFunction) (void (*)(void)) tree_commit, METH_FASTCALL, nullptr}, {nullptr, nullptr, 0, nullptr}};
 int setup(PyObject *) {
     if (s_data_ptr) return 0;
     s_struct = PyUnicode_InternFromString("struct");
     s_value = PyUnicode_InternFromString("value");
     s_as_parameter = PyUnicode_InternFromString("_as_parameter_");
     for (int i = 0; i < 11; ++i) s_field[i] = PyUnicode_InternFromString(FIELDS[i]);
+    s_dtype = PyUnicode_InternFromString("dtype"); s_numel = PyUnicode_InternFromString("numel"); s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
+    s_size = PyUnicode_InternFromString("size"); s_T = PyUnicode_InternFromString("T"); s_n_seq = PyUnicode_InternFromString("n_seq"); s_at = PyUnicode_InternFromString("_at");
+    last_dim = PyLong_FromLong(-1);
     s_data_ptr = PyUnicode_InternFromString("data_ptr");
     return PyErr_Occurred() ? -1 : 0;
 }
 int traverse(PyObject * self, visitproc visit, void * arg) {
     if (calls * C = (calls *) PyModule_GetState(self)) {
-        Py_VISIT(C->kv_class); Py_VISIT(C->stream_of);
+        Py_VISIT(C->kv_class); Py_VISIT(C->stream_of); Py_VISIT(C->check); Py_VISIT(C->int32);
         for (PyObject * x : C->classes) Py_VISIT(x);
     }
     return 0;
 }
 int clear(PyObject * self) {
     if (calls * C = (calls *) PyModule_GetState(self)) {
-        Py_CLEAR(C->kv_class); Py_CLEAR(C->stream_of);
+        Py_CLEAR(C->kv_class); Py_CLEAR(C->stream_of); Py_CLEAR(C->check); Py_CLEAR(C->int32);
         for (PyObject * & x : C->classes) Py_CLEAR(x);
     }
     return 0;

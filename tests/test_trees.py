@@ -108,6 +108,50 @@ def test_binding_refuses():
         p1a.attn_tree(q.float()[:7], b.KVDesc(cache()), q.float(), r, i.view(8, 1), 4, 0.1)
 
 
+def test_native_calls_hand_over_what_they_are_given(monkeypatch):
+    """the calls that come through the native module: every argument at its place in the C call, tensors looked at first; and after the module was loaded anew"""
+    torch = pytest.importorskip("torch")
+    b = importlib.import_module("p100e-engine_amd.binding")
+    got = []
+
+    def stand_in(*types):
+        return ctypes.CFUNCTYPE(ctypes.c_int, *types)(lambda *a: got.append(a) or -7)
+    VP, I = ctypes.c_void_p, ctypes.c_int
+    kept = [stand_in(VP, VP, VP, I, VP, VP, VP), stand_in(VP, I, VP, VP, VP, I, VP)]
+    for again in range(2):
+        got.clear()
+        if again:
+            b._call = None
+        m = b._trees()
+        m.bind(*(ctypes.cast(getattr(b.lib(), n), VP).value for n in ("p1a_attn_prep", "p1a_attn_decode_a16", "p1a_attn_prefill", "p1a_kv_append")), b.KVCache, lambda: 0x7770,
+               ctypes.c_int, ctypes.c_uint32, ctypes.c_size_t, ctypes.c_float, VP, b.p1a_kv)
+        m.bind_trees(*(ctypes.cast(f, VP).value for f in kept), b._of, torch.int32)
+        try:
+            r = b.Rows(6, n_seq=2, p0=3)
+            parent, mask, pos, slot = (torch.zeros(n, dtype=torch.int32) for n in (6, 12, 6, 6))
+            mask = mask.view(6, 2)
+            layers = b.Layers([b.KVCache(1, 64, 1, 64, 0x1000, 0x2000)] * 3)
+            path = torch.zeros(2, 5, dtype=torch.int32)
+            for f in (lambda: b.tree_rows(parent, r, mask, pos, slot), lambda: b.tree_rows(parent, r, mask), lambda: b.tree_commit(layers, r, pos, path)):
+                with pytest.raises(b.P1AError, match="-7"):
+                    f()
+            assert got == [(parent.data_ptr(), r._at, mask.data_ptr(), 2, pos.data_ptr(), slot.data_ptr(), 0x7770), (parent.data_ptr(), r._at, mask.data_ptr(), 2, None, None, 0x7770),
+                           (layers._at, 3, r._at, pos.data_ptr(), path.data_ptr(), 5, 0x7770)]
+            for f in (lambda: b.tree_rows(parent[:5], r, mask), lambda: b.tree_rows(parent.long(), r, mask), lambda: b.tree_rows(parent, r, mask[:, :1]), lambda: b.tree_rows(parent, r, mask, pos[::2]),
+                      lambda: b.tree_commit(layers, r, pos[:1], path), lambda: b.tree_commit(layers, r, pos, path.float()), lambda: b.tree_commit(layers, r, pos, path[:, :3])):
+                with pytest.raises(b.P1AError, match="on end"):
+                    f()
+            for f in (lambda: b.tree_rows(parent, None, mask), lambda: b.tree_rows(parent, r, None), lambda: b.tree_rows(3, r, mask), lambda: m.tree_rows(parent, r, mask, pos)):
+                with pytest.raises((AttributeError, TypeError)):
+                    f()
+            assert len(got) == 3
+        finally:
+            b._call = b._tree = None                           # (the library's own entry points again)
+    with pytest.raises(RuntimeError, match="bind"):
+        b._calls().tree_rows(parent, r, mask, None, None)
+    b._trees()
+
+
 def test_scratch():
     L = p1a.lib()
     one = L.p1a_attn_tree_scratch_bytes(ctypes.byref(cache(n_ctx=32768)), ctypes.byref(rows(T=16, n_seq=1, max_rows=16)), 24, 1)
