@@ -17,7 +17,7 @@
 namespace p1a {
 namespace {
 
-constexpr int NW = 4, NTHR = NW * 64, PC = 8;                 // waves; columns folded at a time
+constexpr int NW = 4, NTHR = NW * 64;                         // waves
 constexpr int COLS = 32 * NW;                                 // columns of a group of team_k
 
 struct group_of { int cols, blocks, groups, bpg; };           // a sequence's columns under a kv head, blocks of BC of them, groups of at most `waves` blocks, a group's blocks
@@ -174,7 +174,8 @@ template <uint32_t KT, int D, int NT, bool EXACT> struct few_cfg {
     static_assert(D == 256 || 2 * NW * (WAVE_B + QL_B / NW + ML_B / NW) <= 160 * 1024, "two workgroups' LDS");
     static constexpr int ML_AT = ML_OVER ? V_B : NW * WAVE_B + QL_B, LDS = NW * WAVE_B + QL_B + (ML_OVER ? 0 : ML_B);
     static constexpr int WGS = D == 256 ? 1 : 2;              // workgroups of a compute unit
-    static_assert(PC * (D + 4) * 4 <= V_B, "folded columns fit where V was");
+    static constexpr int PC = 16 * (D + 4) * 4 <= V_B ? 16 : 8;   // columns folded at a time, where V was
+    static_assert(PC * (D + 4) * 4 <= V_B);
 };
 
 // bits `at` .. `at + 31` of a row's mask (at: from -31 on; what is not there is 0)
@@ -338,6 +339,9 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
     };
     if (P.q_bf16) fetch_q(std::true_type{});
     else fetch_q(std::false_type{});
+    uint32_t warm[NT];                                        // (the rows' masks come to the cache with q; the tiles that ask for them are the last ones)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) warm[n] = P.mask[(size_t) (sv.first + tok_of(min(16 * n + c, R - 1))) * P.words];
     int i = ta + wave;
     auto tile_of = [&](int i) { return sp.tile(min(i, tb - 1)); };   // (past the last: that one once more, unused)
     key_rows::pages pg;
@@ -371,6 +375,7 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
             for (int k = 0; k < NQR; ++k) qf[n][k][b] = r[k];
             if constexpr (C::QL) *reinterpret_cast<h8 *>(ql + (n * NB + b) * 1024) = r[NQ - 1];
         }
+        asm volatile("" :: "v"(warm[n]));
         __builtin_amdgcn_sched_barrier(0);
     }
 
@@ -536,7 +541,7 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
         l[n] += __shfl_xor(l[n], 16);
         l[n] += __shfl_xor(l[n], 32);
     }
-    // ---- fold the waves, in their order, eight columns at a time ----
+    // ---- fold the waves, in their order, PC columns at a time ----
     auto ml = [&](int w, int which, int col) -> float & { return reinterpret_cast<float *>(lds + C::ML_AT)[(w * 2 + which) * 16 * NT + col]; };
     if constexpr (C::ML_OVER) __syncthreads();                // (until the first wave has done with its scales)
     if (g == 0) {
@@ -548,11 +553,11 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int half = 0; half < 16; half += PC) {
+        for (int half = 0; half < 16; half += C::PC) {
             const int h0 = 16 * n + half;
             if (h0 >= R) break;
             if (h0) __syncthreads();
-            if (c >= half && c < half + PC) {
+            if (c >= half && c < half + C::PC) {
 #pragma unroll
                 for (int dt = 0; dt < NDT; ++dt) {
                     f4 v = o[n][dt];
@@ -564,7 +569,7 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
                 }
             }
             __syncthreads();
-            for (int t = tid; t < (min(h0 + PC, R) - h0) * D4; t += NTHR) {
+            for (int t = tid; t < (min(h0 + C::PC, R) - h0) * D4; t += NTHR) {
                 const int cc = t / D4, d = 4 * (t - cc * D4), col = h0 + cc;
                 float m[NW], lw[NW], M = MINUS_INF, lt = 0.f;
                 f4 x[NW], acc = {0.f, 0.f, 0.f, 0.f};
