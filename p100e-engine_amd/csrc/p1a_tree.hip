@@ -9,6 +9,12 @@
 // each, a quantized value times its scale; where results are f32 (EXACT) q and P are two halves and quantized K and V two planes (team_k) or whole numbers whose
 // scales multiply fp32 results (K) or P (V; few_k), as in p1a_chunk.hip and p1a_step.hip.
 // Only the last tiles hold nodes of the tree: there a column's 32 bits of its mask are shifted out of two words.
+// What bounds it, on one MI355X (team_k alone): one wave a SIMD with heads of 256, whose accumulators and q fill the registers. 63 nodes over 32768 keys (24 / 4 heads of 256,
+// q8_0, bf16 results): 89 us, a tile of 32 keys in 1.7 us = 356 instructions and 32 products of 33 clocks, some 9 clocks an instruction, 30 % of them waiting; 16 sequences of
+// 4 ... 16 nodes over 300 ... 32768 keys with f32 results: 165 us, 2.2 us a tile, 1.4 of them the 96 products of a wave whose columns are all there. With heads of 128 two
+// workgroups share a compute unit: 24 sequences of 3 ... 64 nodes over 500 ... 8000 keys (32 / 8 heads, f16) 75 us, 3.8 TB/s. Built and not kept: two waves a SIMD that share
+// columns, each with half of O (20 % slower: both make all of S), loads from LDS asked for further ahead with two planes (8 %), results through LDS to whole lines (11 %), a
+// merge by four threads for one (24 sequences: 25 us for 9), eight waves for a sequence alone (nothing).
 #include "p1a_tiles.hpp"
 
 #include <algorithm>
@@ -596,6 +602,9 @@ __global__ void __launch_bounds__(NTHR, (few_cfg<KT, D, NT, EXACT>::WGS)) few_k(
 }
 
 // ---- more columns: waves that share tiles ----
+// K or V of a tile is brought by two waves each, 16 keys a wave, and lies in LDS as f16 (two planes where results are exact): converted once for all columns. Products take it
+// as their first operand, so that a column is a lane's own: its maximum and sum need one exchange with the other half of the wave. A step holds P of a tile beside the
+// products S^T of the next one, and O^T beside that one's maximum; parts of what is put into LDS stand between products.
 template <uint32_t KT, int D, bool EXACT> struct team_cfg {
     static constexpr bool F16 = KT == P1A_KV_F16;
     static constexpr int NPL = group_planes(KT, EXACT), BN = 32, NG = BN / 16, G_B = NPL * plane_bytes(D), T_B = NG * G_B;   // T_B: K or V of a tile
