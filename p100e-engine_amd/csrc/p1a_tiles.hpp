@@ -615,7 +615,7 @@ struct verify_args {
     bool target_bf16, draft_bf16, logits, distinct;
     void * scratch; size_t scratch_bytes;
 };
-struct verify_plan { int stretches; size_t at[21], bytes; };   // stretches of a row; where the parts of the scratch begin (p1a_verify.hip), and all of it
+struct verify_plan { int stretches; size_t at[16], bytes; };   // stretches of a row; where the parts of the scratch begin (p1a_verify.hip), and all of it
 verify_plan plan_verify(const rows_view & R, int V, bool logits, bool draft);
 int launch_verify(const verify_args & a, hipStream_t s);
 int launch_evict_select(const float * mass, int ld, int n_seq, int Hkv, const int32_t * n_dev, int n, int budget, int n_sink, int n_recent, int32_t * keep, hipStream_t s);

@@ -26,6 +26,14 @@ namespace {
 constexpr int VTHR = 256, PER = 16, STRETCH = VTHR * PER;     // values of a thread, of a workgroup
 constexpr int NODES = P1A_TREE_NODES;
 
+// A node that waits for its sum, all in one place: what a round asks for first
+struct alignas(16) pending {
+    double a, gone;
+    int node, child, state, token;                            // the child under test, its token and its number
+    float u;
+    int next, unused[2];                                      // the child behind it (-1: none)
+};
+
 struct verify_params {
     const char * target, * draft;
     size_t ld_target, ld_draft;                               // in values
@@ -42,13 +50,11 @@ struct verify_params {
     double * row_z;        // [T] logits: 1 / the row's sum
     float * row_max;       // [T] the row's largest
     int * row_arg;         // [T] where it is
-    // per node, two of each (a round reads one and writes the other)
-    double * node_a[2], * node_gone[2];
-    int * node_child[2];   // the child under test
-    int * node_state[2];   // accepted child, NONE, or WAITS for its sum
+    double * node_a;       // [T]
+    int * node_state;      // [T] accepted child, NONE, or WAITS for its sum
+    pending * wait[2];     // [T] a sequence's nodes that wait, from its first row on: two of them (a round reads one and writes the other)
     double * sums[2];      // [T][stretches] of a round; sums[0] then [n_seq][stretches] of the last row
     int16_t * sibling;     // [T] next child of the same parent
-    int * waiting;         // [T] a sequence's nodes that wait, from its first row on
     int * n_waiting;       // [n_seq]
     int * last_row;        // [n_seq] the row that the token is drawn from (-1: none)
     double * last_a;       // [n_seq]
@@ -265,7 +271,7 @@ struct tree_lds {
     float value[NODES], q[NODES], u[NODES];                   // what the parent's rows hold of the token; its number
     float most[NODES];                                        // of the nodes' rows: the largest logit, where it is, 1 / the sum
     int arg[NODES];
-    double z[NODES];
+    double z[NODES], gone[NODES];
     int waiting, length;
 };
 
@@ -281,7 +287,6 @@ __device__ __forceinline__ bool accept(double u, double mass, double p, double q
 
 // What one kernel reads of another's nodes stays in the call's rows even where two sequences of row0 share some, and each leaves its own there
 __device__ __forceinline__ int row_in(const verify_params & P, int row) { return min(max(row, 0), P.R.T - 1); }
-__device__ __forceinline__ int token_in(const verify_params & P, int row) { return min(max(P.token[row_in(P, row)], 0), P.V - 1); }
 
 // f(weight) for a row: weight(l, j) of its value j, l
 template <class F> __device__ __forceinline__ void with_row(const verify_params & P, int seq, int row, const powers & pw, F && f) {
@@ -547,10 +552,10 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
                 c = T.sibling[c];
             }
             T.state[i] = state;
-            P.node_a[0][row] = a;
-            P.node_gone[0][row] = gone;
-            P.node_child[0][row] = T.first[i] = c;
-            P.node_state[0][row] = state;
+            P.node_a[row] = a;
+            P.node_state[row] = state;
+            T.gone[i] = gone;
+            T.first[i] = c;
         }
         __syncthreads();
         // ---- nodes that wait and can still be reached: every one above lets the walk through, or waits itself and has not tested the child yet ----
@@ -562,30 +567,34 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
                 const int sp = T.state[p];
                 reach = sp == j || (sp == WAITS && j >= T.first[p]);
             }
-            if (reach && j == 0) P.waiting[v.first + atomicAdd(&T.waiting, 1)] = i;   // (in any order: each has its own sums)
+            if (reach && j == 0) {                            // (in any order: each has its own sums; a behind one rejection is 1)
+                const int c = T.first[i];
+                P.wait[0][v.first + atomicAdd(&T.waiting, 1)] = pending{1.0, T.gone[i], i, c, WAITS, T.token[c], T.u[c], T.sibling[c], {0, 0}};
+            }
         }
         __syncthreads();
         if (tid == 0) P.n_waiting[seq] = T.waiting;
     } else {
         const int in = round & 1;
-        for (int i = tid; i < n; i += VTHR) T.state[i] = P.node_state[0][v.first + i];
+        for (int i = tid; i < n; i += VTHR) T.state[i] = P.node_state[v.first + i];
         __syncthreads();
         // ---- nodes that waited: a wave each, with the last round's sum ----
         const int m = P.n_waiting[seq];
         for (int w = wave; w < m; w += VTHR / 64) {
-            const int i = min(P.waiting[row_in(P, v.first + w)], n - 1), row = v.first + i;
-            int state = P.node_state[in][row];
-            double a = P.node_a[in][row];
+            const pending o = P.wait[in][row_in(P, v.first + w)];
+            const int i = min(max(o.node, 0), n - 1), row = v.first + i;
+            int state = o.state;
+            double a = o.a;
             if (state == WAITS) {
                 double mass = 0.0;
                 for (int z = lane; z < P.stretches; z += 64) mass += P.sums[in][(size_t) row * P.stretches + z];
-                mass = wave_sum(mass);
-                const int c = P.node_child[in][row], x = token_in(P, v.first + c);
-                double gone = P.node_gone[in][row];
-                double p = 0.0;
-                with_row(P, seq, row, pw, [&](auto weight) { p = weight(value_at(P.target, (size_t) row * P.ld_target + x, P.target_bf16), x); });
+                const int x = min(max(o.token, 0), P.V - 1);
+                const float l = value_at(P.target, (size_t) row * P.ld_target + x, P.target_bf16);
                 const double q = probability(value_at(P.draft, (size_t) row * P.ld_draft + x, P.draft_bf16));
-                if (accept((double) P.u[row_in(P, v.first + c)], mass, p, q, a, gone)) state = c;
+                mass = wave_sum(mass);
+                double gone = o.gone, p = 0.0;
+                with_row(P, seq, row, pw, [&](auto weight) { p = weight(l, x); });
+                if (accept((double) o.u, mass, p, q, a, gone)) state = o.child;
                 else {
                     reject(P, mass, q, a, gone);
                     state = NONE;
@@ -593,7 +602,7 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
             }
             if (lane == 0) {
                 T.state[i] = state;
-                P.node_a[0][row] = a;
+                P.node_a[row] = a;
             }
         }
         __threadfence_block();
@@ -610,7 +619,7 @@ __global__ void __launch_bounds__(VTHR) decide_k(const verify_params P, int roun
         }
         P.n_accept[seq] = k;
         P.last_row[seq] = v.first + at;
-        P.last_a[seq] = P.node_a[0][v.first + at];
+        P.last_a[seq] = P.node_a[v.first + at];
         T.length = k;
         T.waiting = at;
     }
@@ -631,37 +640,36 @@ __global__ void __launch_bounds__(VTHR) sums_k(const verify_params P, int k) {
     const int in = k & 1, first = seq_of<true>(P.R, seq).first;
     if (P.logits) fill(pw);
     for (int w = slot; w < m; w += SLOTS) {
-        const int t = row_in(P, first + P.waiting[row_in(P, first + w)]);
-        int state = P.node_state[in][t], c = P.node_child[in][t];
-        double a = P.node_a[in][t], gone = P.node_gone[in][t];
+        pending o = P.wait[in][row_in(P, first + w)];
+        const int t = row_in(P, first + o.node);
         float x[PER], y[PER];
         const places at{z * STRETCH, tid, P.target_bf16 != 0};
-        if (state == WAITS) {
+        if (o.state == WAITS) {
             load16(x, P.target + (size_t) t * P.ld_target * (P.target_bf16 ? 2 : 4), P.target_bf16, at, P.V, MINUS_INF);
             load16(y, P.draft + (size_t) t * P.ld_draft * (P.draft_bf16 ? 2 : 4), P.draft_bf16, at, P.V, 0.f);
             if (k) {
+                const int token = min(max(o.token, 0), P.V - 1), behind = row_in(P, first + o.next);
+                const float l = value_at(P.target, (size_t) t * P.ld_target + token, P.target_bf16), u = P.u[behind];
+                const double q = probability(value_at(P.draft, (size_t) t * P.ld_draft + token, P.draft_bf16));
+                const int then = P.token[behind], next = P.sibling[behind];
                 double mass = 0.0;                            // (every wave for itself, all alike)
                 for (int i = lane; i < P.stretches; i += 64) mass += P.sums[in][(size_t) t * P.stretches + i];
                 mass = wave_sum(mass);
-                const int token = token_in(P, first + c);
-                const float l = value_at(P.target, (size_t) t * P.ld_target + token, P.target_bf16);
-                const double q = probability(value_at(P.draft, (size_t) t * P.ld_draft + token, P.draft_bf16));
                 double p = 0.0;
                 with_row(P, seq, t, pw, [&](auto weight) { p = weight(l, token); });
-                if (accept((double) P.u[row_in(P, first + c)], mass, p, q, a, gone)) state = c;
+                if (accept((double) o.u, mass, p, q, o.a, o.gone)) o.state = o.child;
                 else {
-                    c = P.sibling[row_in(P, first + c)];
-                    if (!reject(P, mass, q, a, gone) || c < 0) state = NONE;
+                    if (!reject(P, mass, q, o.a, o.gone) || o.next < 0) o.state = NONE;
+                    o.child = o.next;
+                    o.token = then;
+                    o.u = u;
+                    o.next = next;
                 }
             }
         }
-        if (z == 0 && tid == 0) {
-            P.node_state[in ^ 1][t] = state;
-            P.node_child[in ^ 1][t] = c;
-            P.node_a[in ^ 1][t] = a;
-            P.node_gone[in ^ 1][t] = gone;
-        }
-        if (state != WAITS) continue;
+        if (z == 0 && tid == 0) P.wait[in ^ 1][row_in(P, first + w)] = o;
+        if (o.state != WAITS) continue;
+        const double a = o.a;
         double s = 0.0;
         with_row(P, seq, t, pw, [&](auto weight) {
 #pragma unroll
@@ -686,15 +694,16 @@ verify_plan plan_verify(const rows_view & R, int V, bool logits, bool draft) {
     put(3, T * 8);
     put(4, T * 4);
     put(5, T * 4);
-    for (int i = 6; i < 10; ++i) put(i, T * 8);               // node_a, node_gone
-    for (int i = 10; i < 14; ++i) put(i, T * 4);              // node_child, node_state
-    put(14, std::max(draft ? T : 0, S) * z * 8);          // sums
-    put(15, draft ? T * z * 8 : 0);
-    put(16, T * 2);
-    put(17, T * 4);
-    put(18, S * 4);
-    put(19, S * 4);
-    put(20, S * 8);
+    put(6, T * 8);                                            // node_a, node_state
+    put(7, T * 4);
+    put(8, draft ? T * sizeof(pending) : 0);
+    put(9, draft ? T * sizeof(pending) : 0);
+    put(10, std::max(draft ? T : 0, S) * z * 8);              // sums
+    put(11, draft ? T * z * 8 : 0);
+    put(12, T * 2);
+    put(13, S * 4);
+    put(14, S * 4);
+    put(15, S * 8);
     pl.bytes = at;
     return pl;
 }
@@ -715,12 +724,9 @@ int launch_verify(const verify_args & a, hipStream_t s) {
     P.target_bf16 = a.target_bf16; P.draft_bf16 = a.draft_bf16; P.logits = a.logits; P.distinct = a.distinct;
     P.st_sum = (double *) (at + pl.at[0]); P.st_max = (float *) (at + pl.at[1]); P.st_arg = (int *) (at + pl.at[2]);
     P.row_z = (double *) (at + pl.at[3]); P.row_max = (float *) (at + pl.at[4]); P.row_arg = (int *) (at + pl.at[5]);
-    for (int i = 0; i < 2; ++i) {
-        P.node_a[i] = (double *) (at + pl.at[6 + i]); P.node_gone[i] = (double *) (at + pl.at[8 + i]);
-        P.node_child[i] = (int *) (at + pl.at[10 + i]); P.node_state[i] = (int *) (at + pl.at[12 + i]);
-        P.sums[i] = (double *) (at + pl.at[14 + i]);
-    }
-    P.sibling = (int16_t *) (at + pl.at[16]); P.waiting = (int *) (at + pl.at[17]); P.n_waiting = (int *) (at + pl.at[18]); P.last_row = (int *) (at + pl.at[19]); P.last_a = (double *) (at + pl.at[20]);
+    P.node_a = (double *) (at + pl.at[6]); P.node_state = (int *) (at + pl.at[7]);
+    for (int i = 0; i < 2; ++i) { P.wait[i] = (pending *) (at + pl.at[8 + i]); P.sums[i] = (double *) (at + pl.at[10 + i]); }
+    P.sibling = (int16_t *) (at + pl.at[12]); P.n_waiting = (int *) (at + pl.at[13]); P.last_row = (int *) (at + pl.at[14]); P.last_a = (double *) (at + pl.at[15]);
     // rounds: children behind the first that a node may have
     const int rounds = a.draft ? std::max(std::min(P.max_children, a.R.max_rows - 1) - 1, 0) : 0;
     if (a.logits && a.R.T) stats_k<<<(unsigned) a.R.T * (unsigned) pl.stretches, VTHR, 0, s>>>(P);
