@@ -430,7 +430,7 @@ class Rows:
         if pos0 is not None:
             pos0 = pos0.data_ptr() if pos0.dtype is _I32 and pos0.numel() >= n_seq and pos0.is_contiguous() else _of(pos0, False, n_seq, "pos0")
         self._st = p1a_rows(T, n_seq, max_rows, max_n, row0, pos0, p0, window, n_sink)
-        self._ref, self._at = ctypes.byref(self._st), ctypes.addressof(self._st)
+        self._ref = ctypes.byref(self._st)
 
 
 _row_types = {}

@@ -16,7 +16,7 @@
 
 namespace {
 
-PyObject * s_data_ptr, * s_struct, * s_value, * s_as_parameter, * s_field[11], * s_dtype, * s_numel, * s_is_contiguous, * s_size, * s_T, * s_n_seq, * s_at, * last_dim;
+PyObject * s_data_ptr, * s_struct, * s_value, * s_as_parameter, * s_field[11], * s_dtype, * s_numel, * s_is_contiguous, * s_size, * s_T, * s_n_seq, * s_st, * last_dim;
 const char * const FIELDS[11] = {"type", "n_ctx", "Hkv", "D", "k", "v", "pt", "rtab", "psh", "pstride", "_pt_off"};
 enum { INT, UINT, SIZE, FLOAT, POINTER, DESC, NCLASS };
 
@@ -143,6 +143,18 @@ struct calls {
         return n;
     }
     long long attribute(PyObject * o, PyObject * name) { return PyErr_Occurred() ? 0 : number(PyObject_GetAttr(o, name)); }
+    // the p1a_rows of a Rows
+    void rows_of(PyObject * o, p1a_rows & rows) {
+        PyObject * st = PyErr_Occurred() ? nullptr : PyObject_GetAttr(o, s_st);
+        if (!st) return;
+        Py_buffer b;
+        if (PyObject_GetBuffer(st, &b, PyBUF_SIMPLE) == 0) {
+            if (b.len == (Py_ssize_t) sizeof rows) memcpy(&rows, b.buf, sizeof rows);
+            else PyErr_SetString(PyExc_TypeError, "no p1a_rows");
+            PyBuffer_Release(&b);
+        }
+        Py_DECREF(st);
+    }
     long long last_size(PyObject * t) { return PyErr_Occurred() ? 0 : number(PyObject_CallMethodOneArg(t, s_size, last_dim)); }
     // the address of a tensor of at least `least` numbers on end, of torch's int32; None: null. What is not right about one the binding says
     void * ints(PyObject * t, long long least, const char * what) {
@@ -251,10 +263,11 @@ PyObject * tree_rows(PyObject * self, PyObject * const * a, Py_ssize_t n) {
     if (!takes(n, 5) || !bound(C, C.f_rows)) return nullptr;
     const long long T = C.attribute(a[1], s_T), words = C.last_size(a[2]);
     int32_t * pos = (int32_t *) C.ints(a[3], T, "pos"), * slot = (int32_t *) C.ints(a[4], T, "slot"), * parent = (int32_t *) C.ints(a[0], T, "parent");
-    const p1a_rows * rows = (const p1a_rows *) (uintptr_t) C.attribute(a[1], s_at);
+    p1a_rows rows;
+    C.rows_of(a[1], rows);
     uint32_t * mask = (uint32_t *) C.ints(a[2], T * words, "mask");
     void * s = C.stream();
-    P1A_CALL(C.f_rows(parent, rows, mask, (int) words, pos, slot, s));
+    P1A_CALL(C.f_rows(parent, &rows, mask, (int) words, pos, slot, s));
 }
 // (the layers' descriptors, how many they are, rows, n_accept, path)
 PyObject * tree_commit(PyObject * self, PyObject * const * a, Py_ssize_t n) {
@@ -263,10 +276,11 @@ PyObject * tree_commit(PyObject * self, PyObject * const * a, Py_ssize_t n) {
     const p1a_kv * layers = (const p1a_kv *) C.address(a[0]);
     const int count = C.as_int(a[1]);
     const long long n_seq = C.attribute(a[2], s_n_seq), width = C.last_size(a[4]);
-    const p1a_rows * rows = (const p1a_rows *) (uintptr_t) C.attribute(a[2], s_at);
+    p1a_rows rows;
+    C.rows_of(a[2], rows);
     const int32_t * n_accept = (const int32_t *) C.ints(a[3], n_seq, "n_accept"), * path = (const int32_t *) C.ints(a[4], n_seq * width, "path");
     void * s = C.stream();
-    P1A_CALL(C.f_commit(layers, count, rows, n_accept, path, (int) width, s));
+    P1A_CALL(C.f_commit(layers, count, &rows, n_accept, path, (int) width, s));
 }
 // (addresses of p1a_tree_rows, p1a_tree_commit; the binding's check of a tensor; torch.int32)
 PyObject * bind_trees(PyObject * self, PyObject * const * a, Py_ssize_t n) {
@@ -307,7 +321,7 @@ int setup(PyObject *) {
     s_as_parameter = PyUnicode_InternFromString("_as_parameter_");
     for (int i = 0; i < 11; ++i) s_field[i] = PyUnicode_InternFromString(FIELDS[i]);
     s_dtype = PyUnicode_InternFromString("dtype"); s_numel = PyUnicode_InternFromString("numel"); s_is_contiguous = PyUnicode_InternFromString("is_contiguous");
-    s_size = PyUnicode_InternFromString("size"); s_T = PyUnicode_InternFromString("T"); s_n_seq = PyUnicode_InternFromString("n_seq"); s_at = PyUnicode_InternFromString("_at");
+    s_size = PyUnicode_InternFromString("size"); s_T = PyUnicode_InternFromString("T"); s_n_seq = PyUnicode_InternFromString("n_seq"); s_st = PyUnicode_InternFromString("_st");
     last_dim = PyLong_FromLong(-1);
     s_data_ptr = PyUnicode_InternFromString("data_ptr");
     return PyErr_Occurred() ? -1 : 0;

@@ -115,9 +115,10 @@ def test_native_calls_hand_over_what_they_are_given(monkeypatch):
     got = []
 
     def stand_in(*types):
-        return ctypes.CFUNCTYPE(ctypes.c_int, *types)(lambda *a: got.append(a) or -7)
+        return ctypes.CFUNCTYPE(ctypes.c_int, *types)(lambda *a: got.append(tuple(bytes(x.contents) if isinstance(x, R) else x for x in a)) or -7)
     VP, I = ctypes.c_void_p, ctypes.c_int
-    kept = [stand_in(VP, VP, VP, I, VP, VP, VP), stand_in(VP, I, VP, VP, VP, I, VP)]
+    R = ctypes.POINTER(b.p1a_rows)
+    kept = [stand_in(VP, R, VP, I, VP, VP, VP), stand_in(VP, I, R, VP, VP, I, VP)]
     for again in range(2):
         got.clear()
         if again:
@@ -135,8 +136,9 @@ def test_native_calls_hand_over_what_they_are_given(monkeypatch):
             for f in (lambda: b.tree_rows(parent, r, mask, pos, slot), lambda: b.tree_rows(parent, r, mask), lambda: b.tree_commit(layers, r, pos, path)):
                 with pytest.raises(b.P1AError, match="-7"):
                     f()
-            assert got == [(parent.data_ptr(), r._at, mask.data_ptr(), 2, pos.data_ptr(), slot.data_ptr(), 0x7770), (parent.data_ptr(), r._at, mask.data_ptr(), 2, None, None, 0x7770),
-                           (layers._at, 3, r._at, pos.data_ptr(), path.data_ptr(), 5, 0x7770)]
+            at = bytes(r._st)
+            assert got == [(parent.data_ptr(), at, mask.data_ptr(), 2, pos.data_ptr(), slot.data_ptr(), 0x7770), (parent.data_ptr(), at, mask.data_ptr(), 2, None, None, 0x7770),
+                           (layers._at, 3, at, pos.data_ptr(), path.data_ptr(), 5, 0x7770)]
             for f in (lambda: b.tree_rows(parent[:5], r, mask), lambda: b.tree_rows(parent.long(), r, mask), lambda: b.tree_rows(parent, r, mask[:, :1]), lambda: b.tree_rows(parent, r, mask, pos[::2]),
                       lambda: b.tree_commit(layers, r, pos[:1], path), lambda: b.tree_commit(layers, r, pos, path.float()), lambda: b.tree_commit(layers, r, pos, path[:, :3])):
                 with pytest.raises(b.P1AError, match="on end"):
