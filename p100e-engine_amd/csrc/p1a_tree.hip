@@ -214,7 +214,7 @@ __device__ __forceinline__ sight sight_of(const tree_params & P, const seq_view 
         v.sk = P.R.n_sink - k0;
     }
     if (live && at > -32) {
-        const int left = sv.count - at;                       // nodes that are there
+        const int left = min(sv.count, P.R.n_ctx - sv.pos0) - at;   // nodes that are there, in slots that are
         v.bits = mask_bits(row, P.words, at);
         v.bits = left >= 32 ? v.bits : left > 0 ? v.bits & ((1u << left) - 1) : 0;
     }
