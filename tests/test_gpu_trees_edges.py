@@ -1,15 +1,18 @@
 """Calls on drafted trees at the ends of what their documentation allows, each against its formula in 64 bits. Tolerances of attention are those of test_gpu_trees.py."""
 import numpy as np
 import pytest
+import torch
 
 import _inputs as I
 import _oracle as O
-from _bounded import Cache
+from _bounded import Cache, rows_exact, seen
+from _gpu import dev
 from test_gpu_trees import Call
 
 pytestmark = pytest.mark.gpu
 
 KVS = {"f16": O.KV_F16, "q8_0": O.KV_Q8_0, "q4_0": O.KV_Q4_0}
+REL = 1e-5
 
 
 @pytest.mark.parametrize("Hq", [1, 12])                         # (20 columns: waves with keys of their own; 240: waves that share them)
@@ -29,3 +32,42 @@ def test_masks_that_name_slots_past_the_cache(p1a, kv, Hq):
             for see in (some, every):
                 Call(p1a, flat, Hq, [20], [90], window, n_sink, see=see[:1]).check(p1a, out_bf16, lse=not out_bf16)
                 Call(p1a, paged, Hq, [20, 20], [40, 47], window, n_sink, see=see, junk=True, words=2).check(p1a, out_bf16, lse=not out_bf16)
+
+
+@pytest.mark.parametrize("window", [(1 << 31) - 2, (1 << 31) - 7, (1 << 30) + 5, 1200])
+@pytest.mark.parametrize("kv", list(KVS))
+def test_windows_that_reach_past_everything(p1a, kv, window):
+    """... hide nothing, whatever 32 bits hold of them: trees, chunks of few rows and of many, weight per position"""
+    for D, Hq, count in ((64, 4, 3), (128, 12, 40)):
+        cache = Cache(p1a, KVS[kv], 1, D, 4, [33 + count], 94)
+        Call(p1a, cache, Hq, [count], [33], window, 2).check(p1a)
+        chain = Call(p1a, cache, Hq, [count], [33], see=[np.tril(np.ones((count, count), bool))])
+        want, lse = chain.run(p1a)
+        n = 33 + count
+        rows = p1a.Rows(count, pos0=chain.dpos, window=window, n_sink=2)
+        out, z, mass = torch.empty_like(chain.q), torch.empty(count, Hq, device="cuda"), torch.zeros(1, 1, n, device="cuda")
+        p1a.attn_chunk(chain.q, cache.kv, out, rows, Hq, chain.scale, lse=z)
+        assert np.linalg.norm(out.cpu().numpy() - want) <= 2 * REL * np.linalg.norm(want)
+        p1a.attn_mass(chain.q, cache.kv, z, mass, rows, Hq, chain.scale)
+        weight = rows_exact(chain.q64, cache.heads("k", 0, n), cache.heads("v", 0, n), seen(33 + np.arange(count), n, 0, 0), chain.scale)[2].sum((0, 1))
+        assert np.linalg.norm(mass.cpu().numpy()[0, 0] - weight) <= REL * np.linalg.norm(weight)
+
+
+@pytest.mark.parametrize("count", [4, 40])
+def test_gates_far_from_zero(p1a, count):
+    """each gated result beside the one without a gate. The exponential and the reciprocal are 2^-23 of themselves off, the sum and the product 2^-24; g log2 e is rounded by 2^-24 of
+    itself and log2 e by 0.22 2^-24, which moves the exponential by 1.22 |g| 2^-24 and the gate by that times 1 - gate"""
+    g = I.rng(95)
+    cache = Cache(p1a, O.KV_F16, 1, 64, 4, [300], 96)
+    call = Call(p1a, cache, 6, [count], [260])
+    plain, _ = call.run(p1a)
+    for most in (1, 10, 30, 80):
+        gate = (most * (2 * g.random((count, 6 * 64)) - 1)).astype(np.float32)
+        call.dgate = dev(gate)
+        got, _ = call.run(p1a)
+        sigma = 1 / (1 + np.exp(-gate.astype(np.float64)))
+        want, off = plain * sigma.reshape(plain.shape), ((6.01 + 1.22 * np.abs(gate) * (1 - sigma)) * 2.0 ** -24).reshape(plain.shape)
+        assert (np.abs(got - want) <= off * np.abs(want)).all(), (most, float((np.abs(got - want) / (off * np.abs(want))).max()))
+    call.dgate = dev(np.where(np.arange(6 * 64) % 2, np.inf, -np.inf).astype(np.float32) * np.ones((count, 1), np.float32))
+    got, _ = call.run(p1a)
+    assert np.array_equal(got.reshape(count, -1)[:, 1::2], plain.reshape(count, -1)[:, 1::2]) and (got.reshape(count, -1)[:, ::2] == 0).all()
