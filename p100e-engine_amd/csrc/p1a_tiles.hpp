@@ -595,6 +595,7 @@ struct mass_args {
 struct mass_plan { int few, runs, blocks, splits, pld; size_t bytes; };   // (few as in chunk_plan; pld: positions of a partial row; bytes of scratch)
 mass_plan plan_mass(const p1a_kv & c, const rows_view & R, int Hq, int max_n, int ld, int cus);
 int launch_mass(const p1a_kv & c, const mass_args & a, hipStream_t s);
+constexpr long long MOST_GROUPS = (1LL << 32) / 256 - 1;     // workgroups of 256 threads that one launch holds
 struct tree_plan {
     int NT, max_groups;                // tiles of 16 columns of a wave; groups of waves' columns that a sequence may have
     int nks, runs;                     // as in chunk_params

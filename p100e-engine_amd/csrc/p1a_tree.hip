@@ -1168,7 +1168,7 @@ int launch_tree(const p1a_kv & c, const chunk_args & a, const uint32_t * mask, i
     const bool exact = !a.out_bf16 || a.lse;
     const tree_plan pl = plan_tree(c, a.R, a.Hq, a.max_n, exact, cu_count());
     const long long steps = (((long long) c.n_ctx + 31) / 32 + 1) * pl.max_groups * a.R.n_seq, grid = (pl.runs + 7LL) / 8 * 8 * c.Hkv;
-    if (steps > 1 << 30 || grid > 0x7fffffffLL) { set_error("p1a_attn_tree: too many positions and nodes for one call"); return P1A_E_SHAPE; }
+    if (steps > 1 << 30 || grid > MOST_GROUPS) { set_error("p1a_attn_tree: too many positions and nodes for one call (%lld steps, %lld workgroups)", steps, grid); return P1A_E_SHAPE; }
     P.nks = pl.nks; P.runs = pl.runs; P.max_groups = pl.max_groups;
     P.part_o = P.part_ml = nullptr; P.part_n = nullptr;
     if (P.nks > 1) {

@@ -710,6 +710,10 @@ verify_plan plan_verify(const rows_view & R, int V, bool logits, bool draft) {
 
 int launch_verify(const verify_args & a, hipStream_t s) {
     const verify_plan pl = plan_verify(a.R, a.V, a.logits, a.draft != nullptr);
+    // rounds: children behind the first that a node may have
+    const int rounds = a.draft ? std::max(std::min(a.parent ? a.max_children : 1, a.R.max_rows - 1) - 1, 0) : 0;
+    const long long most = std::max(a.logits ? (long long) a.R.T * pl.stretches : 0, (long long) a.R.n_seq * pl.stretches * (rounds ? SLOTS : 1));
+    if (most > MOST_GROUPS) { set_error("p1a_tree_verify: unsupported shape (T=%d n_seq=%d V=%d: %lld workgroups)", a.R.T, a.R.n_seq, a.V, most); return P1A_E_SHAPE; }
     char * at = (char *) a.scratch;
     if (!at || ((uintptr_t) at & 255) || a.scratch_bytes < pl.bytes) {
         float * big, * small;
@@ -727,8 +731,6 @@ int launch_verify(const verify_args & a, hipStream_t s) {
     P.node_a = (double *) (at + pl.at[6]); P.node_state = (int *) (at + pl.at[7]);
     for (int i = 0; i < 2; ++i) { P.wait[i] = (pending *) (at + pl.at[8 + i]); P.sums[i] = (double *) (at + pl.at[10 + i]); }
     P.sibling = (int16_t *) (at + pl.at[12]); P.n_waiting = (int *) (at + pl.at[13]); P.last_row = (int *) (at + pl.at[14]); P.last_a = (double *) (at + pl.at[15]);
-    // rounds: children behind the first that a node may have
-    const int rounds = a.draft ? std::max(std::min(P.max_children, a.R.max_rows - 1) - 1, 0) : 0;
     if (a.logits && a.R.T) stats_k<<<(unsigned) a.R.T * (unsigned) pl.stretches, VTHR, 0, s>>>(P);
     const bool at_once = a.logits && !a.draft;                // (stats_k has summed every row, and a rejection takes one value out)
     decide_k<<<a.R.n_seq, VTHR, 0, s>>>(P, -1, rounds == 0, at_once);
