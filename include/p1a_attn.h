@@ -349,7 +349,8 @@ size_t p1a_attn_tree_scratch_bytes(const p1a_kv *c, const p1a_rows *rows, int Hq
  *   n_accept [n_seq]: accepted tokens; path [n_seq][ld_path]: their nodes in order, -1 behind them (ld_path >= 1; what does not fit is left out, n_accept counts it); next [n_seq]: the token behind
  *     them, -1 where its row has no weight at all or the sequence no rows.
  * row0 as ever; pos0 and the rest of p1a_rows are not looked at. V up to 2^20, rows 16-byte aligned when ld and V allow it and aligned to their type otherwise, T up to 2^20, and with
- * z = V / 4096, rounded up, T * z (logits), n_seq * z and (children in rounds, from the second on) 4 n_seq * z below 2^24.
+ * z = V / 4096, rounded up, T * z (logits), n_seq * z and (children in rounds, from the second on) 4 n_seq * z below 2^24. T == 0: target, draft, token, u and parent may be NULL, as what has T
+ * rows may in all these calls.
  * Scratch (sums of stretches of rows, p1a_tree_verify_scratch_bytes) under the rules of p1a_attn_chunk. The same bits every time.
  */
 #define P1A_VERIFY_PROBS    1

@@ -529,7 +529,7 @@ int p1a_tree_rows(const int32_t * parent, const p1a_rows * rows, uint32_t * mask
     rows_view R;
     const int rc = tree_rows_ok(rows, who, true, R);
     if (rc != P1A_OK) return rc;
-    if (!parent || !mask || words < 0) { set_error("%s: null parent / mask or negative words", who); return P1A_E_ARG; }
+    if ((rows->T && (!parent || !mask)) || words < 0) { set_error("%s: null parent / mask or negative words", who); return P1A_E_ARG; }   // (no rows: tensors without memory)
     if ((long long) words * 32 < R.max_rows || words > P1A_TREE_NODES / 32) { set_error("%s: %d words for trees of %d nodes", who, words, R.max_rows); return P1A_E_SHAPE; }
     if (((uintptr_t) parent | (uintptr_t) mask | (uintptr_t) pos | (uintptr_t) slot) & 3) { set_error("%s: pointers must be 4-byte aligned", who); return P1A_E_SHAPE; }
     if (!rows->T || !rows->n_seq) return P1A_OK;
@@ -542,7 +542,7 @@ int p1a_attn_tree(const void * q, int q_type, const p1a_kv * c, void * out, int 
     chunk_args a;
     const int rc = rows_ok(c, rows, Hq, who, a.R, a.max_n);
     if (rc != P1A_OK) return rc;
-    if (!q || !out || !mask || words < 0) { set_error("%s: null q / out / mask or negative words", who); return P1A_E_ARG; }
+    if ((rows->T && (!q || !out || !mask)) || words < 0) { set_error("%s: null q / out / mask or negative words", who); return P1A_E_ARG; }
     if (!rows_type_ok(q_type, who) || !rows_type_ok(out_type, who)) return P1A_E_ARG;
     if (((uintptr_t) q | (uintptr_t) out | (uintptr_t) gate) & 15 || ((uintptr_t) lse | (uintptr_t) mask) & 3) { set_error("%s: q/out/gate must be 16-byte aligned, lse and mask 4-byte", who); return P1A_E_SHAPE; }
     if (a.R.max_rows > P1A_TREE_NODES || (long long) words * 32 < a.R.max_rows || words > P1A_TREE_NODES / 32) { set_error("%s: %d words for trees of %d nodes (up to %d)", who, words, a.R.max_rows, P1A_TREE_NODES); return P1A_E_SHAPE; }
@@ -568,7 +568,7 @@ int p1a_tree_verify(const void * target, int target_type, size_t ld_target, cons
     verify_args a;
     const int rc = tree_rows_ok(rows, who, false, a.R);
     if (rc != P1A_OK) return rc;
-    if (!target || !token || !u || !u_next || !n_accept || !path || !next || ld_path < 1 || V < 1 || flags & ~(P1A_VERIFY_PROBS | P1A_VERIFY_DISTINCT) || (draft && parent && max_children < 1)) {
+    if ((rows->T && (!target || !token || !u)) || !u_next || !n_accept || !path || !next || ld_path < 1 || V < 1 || flags & ~(P1A_VERIFY_PROBS | P1A_VERIFY_DISTINCT) || (draft && parent && max_children < 1)) {
         set_error("%s: null argument, unknown flag, or a count below 1 (ld_path=%d V=%d max_children=%d)", who, ld_path, V, max_children);
         return P1A_E_ARG;
     }

@@ -71,3 +71,17 @@ def test_gates_far_from_zero(p1a, count):
     call.dgate = dev(np.where(np.arange(6 * 64) % 2, np.inf, -np.inf).astype(np.float32) * np.ones((count, 1), np.float32))
     got, _ = call.run(p1a)
     assert np.array_equal(got.reshape(count, -1)[:, 1::2], plain.reshape(count, -1)[:, 1::2]) and (got.reshape(count, -1)[:, ::2] == 0).all()
+
+
+def test_a_step_without_rows(p1a):
+    """no row of any sequence: nothing accepted, no token"""
+    cache, i = Cache(p1a, O.KV_F16, 1, 64, 4, [30], 97), torch.empty(0, 1, dtype=torch.int32, device="cuda")
+    q = torch.empty(0, 4, 64, device="cuda")
+    p1a.tree_rows(i.flatten(), p1a.Rows(0), i, pos=i.flatten(), slot=i.flatten())
+    p1a.attn_tree(q, cache.kv, q.clone(), p1a.Rows(0), i, 4, 0.125, lse=torch.empty(0, 4, device="cuda"))
+    for draft in (None, torch.empty(0, 50, device="cuda")):
+        rows = p1a.Rows(0, n_seq=3, row0=dev(np.zeros(4, np.int32)))
+        i, f = torch.empty(0, dtype=torch.int32, device="cuda"), torch.empty(0, device="cuda")
+        n, nxt, path = (torch.full((3, w), 77, dtype=torch.int32, device="cuda") for w in (1, 1, 4))
+        p1a.tree_verify(torch.empty(0, 50, device="cuda"), i, rows, f, torch.rand(3, device="cuda"), n, path, nxt, parent=i, draft=draft, max_children=3)
+        assert (n == 0).all() and (nxt == -1).all() and (path == -1).all()

@@ -1,9 +1,9 @@
-"""Calls on drafted trees whose sizes leave what a launch can hold are refused before anything is launched (no GPU)."""
+"""Calls on drafted trees whose sizes leave what a launch can hold are refused before anything is launched; steps without rows are not (no GPU)."""
 import ctypes
 import importlib
 
 from test_bounded import SHAPE, cache, rows
-from test_trees import tree, verify
+from test_trees import tree, tree_rows, verify
 
 p1a = importlib.import_module("p100e-engine_amd")
 
@@ -20,3 +20,9 @@ def test_verifications_that_a_launch_does_not_hold():
 def test_attention_that_a_launch_does_not_hold():
     assert tree(kv=cache(n_ctx=256, Hkv=512, pstride=512 * 512 << 8), r=rows(T=1000, n_seq=8192, max_rows=1000), words=32, Hq=32768) == SHAPE
     assert b"workgroups" in p1a.lib().p1a_last_error()
+
+
+def test_a_step_without_rows():
+    """... whose tensors have no memory"""
+    r = rows(T=0)
+    assert tree(r=r, q=None, out=None, mask=None) == 0 and tree_rows(r=r, parent=None, mask=None, pos=None, slot=None) == 0
