@@ -85,3 +85,20 @@ def test_a_step_without_rows(p1a):
         n, nxt, path = (torch.full((3, w), 77, dtype=torch.int32, device="cuda") for w in (1, 1, 4))
         p1a.tree_verify(torch.empty(0, 50, device="cuda"), i, rows, f, torch.rand(3, device="cuda"), n, path, nxt, parent=i, draft=draft, max_children=3)
         assert (n == 0).all() and (nxt == -1).all() and (path == -1).all()
+
+
+@pytest.mark.parametrize("kv", list(KVS))
+def test_a_chain_behind_a_window_shorter_than_itself(p1a, kv):
+    """the window cuts what is in front of the tree, never the path: rows whose window reaches back to the tree's first node give what attn_chunk gives, the others see more than a chunk's"""
+    counts, lens, window, n_sink = [23, 40], [200, 60], 9, 2
+    cache = Cache(p1a, KVS[kv], 2, 64, 4, lens, 98)
+    call = Call(p1a, cache, 4, counts, [n - c for n, c in zip(lens, counts)], window, n_sink, see=[np.tril(np.ones((n, n), bool)) for n in counts])
+    got = call.check(p1a)
+    out = torch.empty(call.T, 4, 64, device="cuda")
+    p1a.attn_chunk(call.q, cache.kv, out, call.rows, 4, call.scale)
+    out = out.cpu().numpy()
+    for s, c in enumerate(counts):
+        a, b = call.first[s], call.first[s] + window
+        assert np.linalg.norm(out[a:b] - got[a:b]) <= 2 * REL * np.linalg.norm(got[a:b])
+        far = slice(b, call.first[s] + c)
+        assert (np.abs(out[far] - got[far]).max((1, 2)) > 1e-3).all()
