@@ -308,7 +308,8 @@ int p1a_kv_compact(const p1a_kv *c, const int32_t *keep, int n_seq, int budget, 
  * Per sequence a step has nodes: node 0 is the last token that is certain, node i > 0 a drafted token with a parent among nodes 0 .. i - 1; a chain is the tree
  * where i's parent is i - 1. Node i of sequence s is row row0[s] + i of p1a_rows and stands in cache slot pos0[s] + i, its rotary position is pos0[s] + its depth. A
  * step: p1a_tree_rows; per layer p1a_attn_prep_mrope (sect = s0 = 1: cache rows from `slot`, rotary positions from `pos`) and p1a_attn_tree; p1a_tree_verify on the rows'
- * logits; p1a_tree_commit, after which the sequence holds pos0[s] + 1 + n_accept[s] positions. A sequence has at most P1A_TREE_NODES nodes (rows->max_rows says how
+ * logits; p1a_tree_commit, after which the sequence holds pos0[s] + 1 + n_accept[s] positions - where ld_path holds its whole path: what does not fit is not moved. The pages of all
+ * nodes' slots below n_ctx have to be there when the step begins, whatever the masks name. A sequence has at most P1A_TREE_NODES nodes (rows->max_rows says how
  * many it may have here); rows of no sequence are left as they are.
  */
 #define P1A_TREE_NODES 1024
@@ -323,13 +324,13 @@ int p1a_tree_rows(const int32_t *parent, const p1a_rows *rows, uint32_t *mask, i
 /*
  * Attention of the nodes' rows over the cache, which holds their own K and V in their slots: as p1a_attn_chunk, but row i of sequence s sees the positions j < pos0[s] - with
  * a window those with j > p - window or j < n_sink, p = pos0[s] + the nodes of its mask - 1 (pos0[s] for an empty one) - and of its tree the slots pos0[s] + b whose bit b is set
- * in mask [T][words], whatever the window. Any mask may be given; bits of nodes that the sequence does not have are not looked at, 32 words >= rows->max_rows. A row
+ * in mask [T][words], whatever the window. Any mask may be given - one that leaves out nodes above a row moves its window back by as many -; bits of nodes that the sequence does not have are not looked at, 32 words >= rows->max_rows. A row
  * that sees nothing, or whose slot is negative or not below n_ctx, has the result 0 and the log-sum-exp -inf.
  * Types, precision, alignment, limits, scratch and capture as for p1a_attn_chunk (partials: 128 MB at most); from one node to P1A_TREE_NODES.
  */
 int p1a_attn_tree(const void *q, int q_type, const p1a_kv *c, void *out, int out_type, const float *gate, float *lse, const p1a_rows *rows,
                   const uint32_t *mask, int words, int Hq, float scale, void *scratch, size_t scratch_bytes, void *stream);
-/* bytes of partials such a call has (0: none); f32: whether it has f32 results (out or lse) */
+/* bytes of partials such a call has (0: none); f32: whether it has f32 results (out or lse) - the same bytes for both at present */
 size_t p1a_attn_tree_scratch_bytes(const p1a_kv *c, const p1a_rows *rows, int Hq, int f32);
 
 /*
@@ -345,6 +346,7 @@ size_t p1a_attn_tree_scratch_bytes(const p1a_kv *c, const p1a_rows *rows, int Hq
  *     probability too); infinite logits share everything.
  *   draft [T] rows of V probabilities, ld_draft apart (0: V), of draft_type; rows of nodes without children are not read.
  *   token [T] int32; a node whose token is not in 0 .. V - 1 is passed over. parent [T] as above, or NULL: chains.
+ *   Children are asked in ascending order, which has to be the one they were drawn in. Children that were chosen and not drawn (the k likeliest tokens) go without a draft.
  *   max_children: the most children of a node that are looked at with a draft (>= 1; parent == NULL: 1 whatever it is); further ones are passed over. It costs a launch each.
  *   n_accept [n_seq]: accepted tokens; path [n_seq][ld_path]: their nodes in order, -1 behind them (ld_path >= 1; what does not fit is left out, n_accept counts it); next [n_seq]: the token behind
  *     them, -1 where its row has no weight at all or the sequence no rows.

@@ -556,7 +556,7 @@ def attn_tree(q, c, out, rows, mask, Hq, scale, gate=None, lse=None, scratch=Non
 
 
 def tree_scratch_bytes(c, rows, Hq, f32=True):
-    """bytes of partials of an attn_tree call; f32: out is float32, or lse is asked for"""
+    """bytes of partials of an attn_tree call; f32: out is float32, or lse is asked for (the same bytes for both at present)"""
     return int(lib().p1a_attn_tree_scratch_bytes(ctypes.byref(c.struct()), rows._ref, Hq, 1 if f32 else 0))
 
 
@@ -570,8 +570,8 @@ def _weights(t, T, what):
 def tree_verify(target, token, rows, u, u_next, n_accept, path, next, parent=None, draft=None, temp=None, logits=True, max_children=1, distinct=False, scratch=None):
     """Which drafted tokens stand, and the token behind them: target [T][V] logits (of temperatures temp [n_seq]; 0: the largest one) or, with logits=False,
     probabilities, draft [T][V] probabilities or None, float32 or bfloat16; token, parent int32 [T] (parent None: chains), u float32 [T] and u_next [n_seq] in
-    [0, 1). Writes n_accept [n_seq], path [n_seq][..] and next [n_seq], int32. max_children: children of a node that are looked at with a draft; distinct:
-    siblings were drawn without replacement."""
+    [0, 1). Writes n_accept [n_seq], path [n_seq][..] and next [n_seq], int32. max_children: children of a node that are looked at with a draft, in ascending
+    order - one unless told otherwise, whatever the tree has; distinct: siblings were drawn without replacement."""
     T, S = rows.T, rows.n_seq
     tp, tt, tld = _weights(target, T, "target")
     V, width = target.shape[1], path.shape[-1]
