@@ -102,3 +102,77 @@ def test_a_chain_behind_a_window_shorter_than_itself(p1a, kv):
         assert np.linalg.norm(out[a:b] - got[a:b]) <= 2 * REL * np.linalg.norm(got[a:b])
         far = slice(b, call.first[s] + c)
         assert (np.abs(out[far] - got[far]).max((1, 2)) > 1e-3).all()
+
+
+@pytest.mark.parametrize("kv", list(KVS))
+def test_rounded_results_with_their_log_sum_exp(p1a, kv):
+    """bf16 results beside an f32 log-sum-exp, whole and split: the results of f32 rounded once, the same log-sum-exp"""
+    for D, Hq, lens, counts in ((64, 4, [300, 40], [3, 2]), (256, 12, [900, 70], [30, 8]), (128, 6, [5000], [4])):
+        cache = Cache(p1a, KVS[kv], 2, D, 4, lens, 99)
+        call = Call(p1a, cache, Hq, counts, [n - c for n, c in zip(lens, counts)], gate=True)
+        got, lse = call.run(p1a)
+        short, z = call.run(p1a, out_bf16=True)
+        assert np.array_equal(z, lse) and np.array_equal(short, torch.from_numpy(got).to(torch.bfloat16).double().numpy())
+
+
+@pytest.mark.parametrize("Hq, lens", [(2, [900, 60]), (12, [900, 60]), (12, [9000, 60])])
+def test_sequences_longer_than_max_rows(p1a, Hq, lens):
+    """rows past the first max_rows of a sequence are left as they are, and nobody sees them: masks, attention and verification as of trees that end there"""
+    cache, counts, most, V = Cache(p1a, O.KV_Q8_0, 1, 64, 6, lens, 100), [13, 5], 7, 60
+    pos0 = [n - 13 for n in lens]
+    whole = Call(p1a, cache, Hq, counts, pos0)
+    cut = Call(p1a, cache, Hq, [most, 5], pos0, see=[m[:most, :most] for m in whole.see])
+    rows = p1a.Rows(18, n_seq=2, row0=whole.row0, pos0=whole.dpos, max_rows=most)
+    out, lse = torch.full_like(whole.q, 77), torch.full((18, Hq), 77.0, device="cuda")
+    p1a.attn_tree(whole.q, cache.kv, out, rows, whole.mask, Hq, whole.scale, lse=lse)
+    assert (out[most:13] == 77).all() and (lse[most:13] == 77).all()
+    keep = [*range(most), *range(13, 18)]
+    cut.q = whole.q[keep].contiguous()
+    want = torch.empty(most + 5, Hq, 64, device="cuda")
+    p1a.attn_tree(cut.q, cache.kv, want, cut.rows, cut.mask, Hq, whole.scale)
+    assert torch.equal(out[keep], want)
+    parent = dev(np.array([*range(-1, 12), *range(-1, 4)], np.int32))
+    mask, pos, slot = (torch.full((18, w), 77, dtype=torch.int32, device="cuda") for w in (1, 1, 1))
+    p1a.tree_rows(parent, rows, mask, pos=pos, slot=slot)
+    assert all((t[most:13] == 77).all() and (t[:most] != 77).all() for t in (mask, pos, slot))
+    assert pos[:most, 0].tolist() == list(range(pos0[0], pos0[0] + most)) and (mask[:, 0][keep] == dev(np.array([(2 << i) - 1 for i in [*range(most), *range(5)]], np.int32))).all()
+    n, nxt = (torch.empty(2, dtype=torch.int32, device="cuda") for _ in range(2))
+    path = torch.empty(2, 12, dtype=torch.int32, device="cuda")
+    target = torch.zeros(18, V, device="cuda")
+    token = torch.arange(18, dtype=torch.int32, device="cuda")
+    target[torch.arange(17), token[1:].long()] = 50             # (every draft is what the target says)
+    p1a.tree_verify(target, token, rows, torch.rand(18, device="cuda"), torch.rand(2, device="cuda"), n, path, nxt, parent=parent)
+    assert n.tolist() == [most - 1, 4] and path[0].tolist() == [*range(1, most)] + [-1] * (13 - most) and nxt[0] == most
+
+
+def test_thousands_of_sequences(p1a):
+    counts = [(s * 5) % 4 for s in range(3000)]
+    lens = [20 + (s * 13) % 40 for s in range(3000)]
+    cache = Cache(p1a, O.KV_F16, 1, 64, 4, lens, 101)
+    Call(p1a, cache, 4, counts, [n - c for n, c in zip(lens, counts)]).check(p1a)
+
+
+def test_masks_of_one_sequence_from_the_host(p1a):
+    """the position of the only sequence is the host's; no positions and no slots asked for, or one of them"""
+    parent = dev(np.array([-1, 0, 0, 2], np.int32))
+    mask, at = torch.zeros(4, 2, dtype=torch.int32, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    p1a.tree_rows(parent, p1a.Rows(4, p0=70), mask)
+    assert mask[:, 0].tolist() == [1, 3, 5, 13] and mask[:, 1].tolist() == [0] * 4
+    p1a.tree_rows(parent, p1a.Rows(4, p0=70), mask, slot=at)
+    assert at.tolist() == [70, 71, 72, 73]
+    p1a.tree_rows(parent, p1a.Rows(4, p0=70), mask, pos=at)
+    assert at.tolist() == [70, 71, 71, 72]
+
+
+def test_commit_in_as_many_layers_as_a_call_takes(p1a):
+    """128 layers; and a second commit of the same path, which moves what it finds"""
+    layers, g = 128, torch.Generator("cuda").manual_seed(1)
+    k, v = (torch.randint(0, 255, (layers, 20, 2 * 128), generator=g, dtype=torch.uint8, device="cuda") for _ in range(2))
+    kv = [p1a.KVCache(1, 20, 2, 64, a.data_ptr(), b.data_ptr()) for a, b in zip(k, v)]
+    rows, n, path = p1a.Rows(9, p0=8), dev(np.array([3], np.int32)), dev(np.array([[2, 5, 8]], np.int32))
+    for _ in range(2):
+        want = [t.clone() for t in (k, v)]
+        for t in want:
+            t[:, 9:12] = t[:, [10, 13, 16]].clone()
+        p1a.tree_commit(kv, rows, n, path)
+        assert torch.equal(k, want[0]) and torch.equal(v, want[1])
