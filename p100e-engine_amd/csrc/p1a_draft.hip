@@ -1,6 +1,6 @@
 // Drafted trees, the two ends of a step: masks, rotary positions and slots from parents (p1a_tree_rows), and the accepted path moved behind node 0 in every
-// layer (p1a_tree_commit). Both move next to nothing; what they cost is a launch and as many round trips to memory as depend on each other: 2.0 us for eight nodes, 4.2 for 64
-// sequences of 256; 3.7 us for one sequence's path in 16 layers, 4.9 for 32 sequences' (9.7 MB, 2 TB/s).
+// layer (p1a_tree_commit). Both move next to nothing; what they cost is a launch and as many round trips to memory as depend on each other: 1.8 us for eight nodes, 4.0 for 64
+// sequences of 33 ... 256; 3.4 us for one sequence's path in 16 layers, 4.6 for 32 sequences' (9.7 MB, 2.1 TB/s).
 #include "p1a_tiles.hpp"
 
 #include <algorithm>
