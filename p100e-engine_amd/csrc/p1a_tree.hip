@@ -13,7 +13,7 @@
 // whose accumulators and q fill the registers. 63 nodes over 32768 keys (24 / 4 heads of 256, q8_0, bf16 results): 88 us, a tile of 32 keys in 1.7 us = 356 instructions and 32
 // products of 32 clocks, some 9 clocks an instruction, 29 % of the waves' time waiting; 16 sequences of 4 ... 16 nodes over 300 ... 32768 keys with f32 results: 163 us, 2.2 us a tile, 1.4 of
 // them the 96 products of a wave whose columns are all there, 45 % waiting. With heads of 128 two workgroups share a compute unit: 24 sequences of 3 ... 64 nodes over
-// 500 ... 8000 keys (32 / 8 heads, f16) 70 us, 4.0 TB/s, 45 % waiting. Where all of it is few_k: 16 sequences of 1 ... 5 nodes over 300 ... 32768 keys (24 / 4 of 256) 108 us
+// 500 ... 8000 keys (32 / 8 heads, f16) 70 us with the same inputs again, 83 and 3.4 TB/s with others, 45 % waiting. Where all of it is few_k: 16 sequences of 1 ... 5 nodes over 300 ... 32768 keys (24 / 4 of 256) 108 us
 // (f16, 4.6 TB/s), 101 (q8_0, f32 results), 66 (q8_0, bf16). Built and not kept: two waves a SIMD that share
 // columns, each with half of O (20 % slower: both make all of S), loads from LDS asked for further ahead with two planes (8 %), results through LDS to whole lines (11 %), a
 // merge by four threads for one (24 sequences: 25 us for 9), eight waves for a sequence alone (nothing).
